@@ -57,6 +57,10 @@ int zs_abi_version(void);
 #define ZS_LAYOUT_SPEC_BATCH 2
 #define ZS_LAYOUT_LANE_STREAM 3
 #define ZS_LAYOUT_HALLUC_REPORT 4
+#define ZS_LAYOUT_BEAM 5
+#define ZS_LAYOUT_BEAM_STATE 6
+#define ZS_LAYOUT_TEACHER 7
+#define ZS_LAYOUT_DISTILL 8
 int zs_struct_layout(int which, size_t* size, size_t* offsets, size_t cap);
 
 /* Context on HIP device `device`, with scratch sized for batches of up to
@@ -377,6 +381,164 @@ typedef struct zs_lane_stream {
  * one context must be issued in order on one stream. m <= max_rows. */
 int zs_lane_step(zs_ctx* ctx, const float* d_logits, uint32_t m, uint32_t V, uint64_t ld,
                  const zs_lane_stream* h_streams, uint32_t* d_out, int* path, void* stream);
+
+/* ---- logits of three types ----------------------------------------------
+ * Beam search and distillation read rows of fp32, fp16 or bf16 logits; a row
+ * may start at any element (base aligned to its type, any ld >= V), V <=
+ * ZS_HEAD_MAX_VOCAB. None has a counterpart in the reference, which decodes
+ * one hypothesis per request and trains nothing. Their scratch is the
+ * caller's (d_work, 256-byte aligned, *_work bytes; no contents expected): a
+ * call holds no memory of the context, so calls may overlap on any streams as
+ * long as each has its own scratch. Nothing is allocated, copied from the
+ * host or synchronised: the calls can be captured into a HIP graph. */
+#define ZS_F32 0u
+#define ZS_F16 1u
+#define ZS_BF16 2u
+#define ZS_HEAD_MAX_VOCAB 1048576u
+
+/* ---- beam search -----------------------------------------------------------
+ * One step for `groups` requests of `width` beams, row = group * width + beam.
+ * Candidates are the pairs (beam, id):
+ *     s(b, v) = scores[b] + x~[b][v] - ln sum_u exp(x~[b][u])     (f32, rounded once)
+ * over the row's masked logits x~ (ids whose allow bit is 0 and NaN count as
+ * -inf, +inf as the largest f32; no candidates at -inf, nor of a beam whose
+ * score is not finite: its row is not read). They are taken in the order
+ * (s descending, beam ascending, x~ descending, id ascending):
+ *   - an EOS id among the first `width` finishes: it enters the pool of the
+ *     request's best `width` hypotheses with s / (steps + 1)^length_penalty,
+ *     behind equal ones; an EOS id further on is dropped;
+ *   - the first `width` other ids are the next beams.
+ * The request is done when the pool is full and (with ZS_BEAM_EARLY, at once;
+ * else) its worst is at least the best next beam's s / (steps + 1)^length_penalty,
+ * or when no next beam is left. A request that was done stays as it is: no
+ * row of it is read, its next beams are absent.
+ * Absent next beams have parent -1, token -1 and score -inf; absent pool
+ * entries score -inf, length 0, parent -1 and token -1. Pool entries name
+ * their tokens by (length, parent beam at that step, EOS id): the tokens are
+ * followed back through the (parent, token) of the steps. */
+#define ZS_BEAM_MAX_WIDTH 32
+#define ZS_BEAM_MAX_ROWS 1048576   /* groups * width */
+#define ZS_BEAM_MAX_EOS 8
+#define ZS_BEAM_EARLY 1u
+typedef struct zs_beam {
+    uint32_t groups, width, V, dtype;
+    uint64_t ld;
+    const void* d_logits;             /* [groups*width][ld] */
+    const uint32_t* d_allow_bits;     /* [groups*width][allow_words] or NULL */
+    uint32_t allow_words;             /* >= ceil(V/32) */
+    uint32_t n_eos;
+    uint32_t eos[ZS_BEAM_MAX_EOS];    /* distinct; ids >= V never occur */
+    float length_penalty;
+    uint32_t flags;                   /* 0 or ZS_BEAM_EARLY */
+    const float* d_scores;            /* [groups*width] */
+    /* the pool and the request's state before the step ... */
+    const float* d_fin_score;         /* [groups][width], best first */
+    const int32_t* d_fin_length;
+    const int32_t* d_fin_parent;
+    const int32_t* d_fin_token;
+    const int32_t* d_steps;           /* [groups] tokens so far */
+    const int32_t* d_done;            /* [groups] */
+    /* ... and after it; each may be the array before it itself */
+    float* d_fin_score_out;
+    int32_t* d_fin_length_out;
+    int32_t* d_fin_parent_out;
+    int32_t* d_fin_token_out;
+    int32_t* d_steps_out;
+    int32_t* d_done_out;
+    /* the next beams, best first */
+    int32_t* d_parent;                /* [groups*width] beam of the group, or -1 */
+    int32_t* d_token;                 /* [groups*width] */
+    float* d_score;                   /* [groups*width]; may be d_scores */
+    void* d_work;
+    uint64_t work_bytes;
+} zs_beam;
+int zs_beam_select_work(uint32_t groups, uint32_t width, uint32_t V, uint32_t n_eos, uint64_t* bytes);
+int zs_beam_select(zs_ctx* ctx, const zs_beam* args, void* stream);
+
+/* The beams' states follow their parents: for every state array, row
+ * group * width + b becomes what row group * width + parent[b] was. In place,
+ * all arrays in as few launches as they need (ZS_REORDER_BATCH arrays each);
+ * rows whose parent is their own beam, negative or >= width stay. A row of an
+ * array is n_outer * n_inner blocks of `bytes` bytes, block (o, i) of row r
+ * at base + o * outer_stride + r * row_stride + i * inner_stride (bytes);
+ * blocks of different rows, or of different arrays, must not overlap. */
+#define ZS_REORDER_BATCH 48
+typedef struct zs_beam_state {
+    void* d_base;
+    uint64_t row_stride, outer_stride, inner_stride, bytes;
+    uint32_t n_outer, n_inner;
+} zs_beam_state;
+int zs_beam_reorder(zs_ctx* ctx, uint32_t groups, uint32_t width, const int32_t* d_parent,
+                    const zs_beam_state* h_states, uint32_t n_states, void* stream);
+
+/* ---- a teacher's top log-probabilities -------------------------------------
+ * Per row the K largest logits (value descending, id ascending; NaN counts as
+ * -inf, +inf as the largest f32), as ids and logp = ln softmax(x / T) over the
+ * whole row; absent entries (fewer than K above -inf) have id 0xffffffff and
+ * logp -inf. lse = ln sum exp(x / T), -inf for a row of none. K <= V. */
+#define ZS_TEACHER_KMAX 128
+typedef struct zs_teacher {
+    uint32_t N, V, K, dtype;
+    uint64_t ld;
+    const void* d_logits;             /* [N][ld] */
+    float temperature;                /* > 0, finite */
+    uint32_t pad;
+    uint32_t* d_ids;                  /* [N][K] */
+    float* d_logp;                    /* [N][K] */
+    float* d_lse;                     /* [N] */
+    void* d_work;
+    uint64_t work_bytes;
+} zs_teacher;
+int zs_teacher_topk_work(uint32_t N, uint32_t V, uint32_t K, uint64_t* bytes);
+int zs_teacher_topk(zs_ctx* ctx, const zs_teacher* args, void* stream);
+
+/* ---- distillation from a teacher's list -------------------------------------
+ * Row r has the student's logits x, a teacher's list (ids, logp; entries with
+ * an id >= V or logp -inf are absent; an id listed twice counts twice) and
+ * optionally a label. With z = x / T, q = softmax(z) and p = exp(logp):
+ *   without ZS_DISTILL_TAIL  p is divided by its sum over the list and
+ *       KL = sum_k p_k (ln p_k - ln q_k)                 (0 for an empty list)
+ *   with it the ids outside the list are one more outcome: p_t = max(0, 1 -
+ *       sum_k p_k), q_t = sum of q outside the list, KL += p_t (ln p_t - ln q_t)
+ *   CE = -ln softmax(x)[label]                            (d_labels given)
+ *   loss[r] = kl_weight * KL + ce_weight * CE
+ * A row whose label is ignore_index has loss 0 and gradient 0, and is not
+ * read; a label outside [0, V) otherwise gives NaN. NaN and infinities of x
+ * are not looked for: they come out as the formulas have them.
+ *   zs_distill_loss       writes d_loss and d_stats: the row's maximum m,
+ *       sum exp((x - m) / T), sum exp(x - m) and sum outside the list of
+ *       exp((x - m) / T); the third is the second's value where CE is not
+ *       taken or T = 1, the fourth 0 without the tail, all 0 for ignored rows
+ *   zs_distill_grad       reads d_stats and writes d_grad = row_grad[r] *
+ *       d loss[r] / d x, rounded once to the logits' type; d_grad may be
+ *       d_logits itself (ld_grad = ld)
+ *   zs_distill_loss_grad  both in one call (d_stats is not used)
+ * row_grad_stride 0 reads one value for all rows (a broadcast gradient). */
+#define ZS_DISTILL_KMAX 128
+#define ZS_DISTILL_TAIL 1u
+typedef struct zs_distill {
+    uint32_t N, V, K, dtype;
+    uint64_t ld;
+    const void* d_logits;             /* [N][ld] */
+    const uint32_t* d_ids;            /* [N][K] */
+    const float* d_logp;              /* [N][K] */
+    const int64_t* d_labels;          /* [N] or NULL */
+    int64_t ignore_index;
+    float temperature, kl_weight, ce_weight;
+    uint32_t flags;                   /* 0 or ZS_DISTILL_TAIL */
+    float* d_loss;                    /* [N] */
+    float* d_stats;                   /* [N][4], 16-byte aligned */
+    const float* d_row_grad;          /* [N] at row_grad_stride */
+    uint64_t row_grad_stride;
+    void* d_grad;                     /* [N][ld_grad], the logits' type */
+    uint64_t ld_grad;
+    void* d_work;
+    uint64_t work_bytes;
+} zs_distill;
+int zs_distill_work(uint32_t N, uint32_t V, uint64_t* bytes);
+int zs_distill_loss(zs_ctx* ctx, const zs_distill* args, void* stream);
+int zs_distill_grad(zs_ctx* ctx, const zs_distill* args, void* stream);
+int zs_distill_loss_grad(zs_ctx* ctx, const zs_distill* args, void* stream);
 
 /* ---- profiling ----------------------------------------------------------
  * When enabled, zs_sample and zs_spec_verify record a HIP event around their

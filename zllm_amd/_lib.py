@@ -99,6 +99,44 @@ class HallucReport(C.Structure):
                 ("risky_fraction", C.c_float), ("peak_token", C.c_int64), ("n_tokens", C.c_uint64)]
 
 
+class Beam(C.Structure):
+    _fields_ = [
+        ("groups", C.c_uint32), ("width", C.c_uint32), ("V", C.c_uint32), ("dtype", C.c_uint32), ("ld", C.c_uint64),
+        ("d_logits", C.c_void_p), ("d_allow_bits", C.c_void_p), ("allow_words", C.c_uint32), ("n_eos", C.c_uint32),
+        ("eos", C.c_uint32 * 8), ("length_penalty", C.c_float), ("flags", C.c_uint32),
+        ("d_scores", C.c_void_p), ("d_fin_score", C.c_void_p), ("d_fin_length", C.c_void_p),
+        ("d_fin_parent", C.c_void_p), ("d_fin_token", C.c_void_p), ("d_steps", C.c_void_p), ("d_done", C.c_void_p),
+        ("d_fin_score_out", C.c_void_p), ("d_fin_length_out", C.c_void_p), ("d_fin_parent_out", C.c_void_p),
+        ("d_fin_token_out", C.c_void_p), ("d_steps_out", C.c_void_p), ("d_done_out", C.c_void_p),
+        ("d_parent", C.c_void_p), ("d_token", C.c_void_p), ("d_score", C.c_void_p),
+        ("d_work", C.c_void_p), ("work_bytes", C.c_uint64),
+    ]
+
+
+class BeamStateDesc(C.Structure):
+    _fields_ = [("d_base", C.c_void_p), ("row_stride", C.c_uint64), ("outer_stride", C.c_uint64),
+                ("inner_stride", C.c_uint64), ("bytes", C.c_uint64), ("n_outer", C.c_uint32), ("n_inner", C.c_uint32)]
+
+
+class Teacher(C.Structure):
+    _fields_ = [
+        ("N", C.c_uint32), ("V", C.c_uint32), ("K", C.c_uint32), ("dtype", C.c_uint32), ("ld", C.c_uint64),
+        ("d_logits", C.c_void_p), ("temperature", C.c_float), ("pad", C.c_uint32), ("d_ids", C.c_void_p),
+        ("d_logp", C.c_void_p), ("d_lse", C.c_void_p), ("d_work", C.c_void_p), ("work_bytes", C.c_uint64),
+    ]
+
+
+class Distill(C.Structure):
+    _fields_ = [
+        ("N", C.c_uint32), ("V", C.c_uint32), ("K", C.c_uint32), ("dtype", C.c_uint32), ("ld", C.c_uint64),
+        ("d_logits", C.c_void_p), ("d_ids", C.c_void_p), ("d_logp", C.c_void_p), ("d_labels", C.c_void_p),
+        ("ignore_index", C.c_int64), ("temperature", C.c_float), ("kl_weight", C.c_float), ("ce_weight", C.c_float),
+        ("flags", C.c_uint32), ("d_loss", C.c_void_p), ("d_stats", C.c_void_p), ("d_row_grad", C.c_void_p),
+        ("row_grad_stride", C.c_uint64), ("d_grad", C.c_void_p), ("ld_grad", C.c_uint64), ("d_work", C.c_void_p),
+        ("work_bytes", C.c_uint64),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/zs.h declares
 SIGNATURES = {
     "zs_abi_version": (C.c_int, []),
@@ -160,6 +198,16 @@ SIGNATURES = {
     "zs_logprobs_json": (C.c_int, [C.c_int, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p,
                                    C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_char_p, C.c_size_t,
                                    C.POINTER(C.c_size_t)]),
+    "zs_beam_select_work": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_uint64)]),
+    "zs_beam_select": (C.c_int, [C.c_void_p, C.POINTER(Beam), C.c_void_p]),
+    "zs_beam_reorder": (C.c_int, [C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p, C.POINTER(BeamStateDesc),
+                                  C.c_uint32, C.c_void_p]),
+    "zs_teacher_topk_work": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_uint64)]),
+    "zs_teacher_topk": (C.c_int, [C.c_void_p, C.POINTER(Teacher), C.c_void_p]),
+    "zs_distill_work": (C.c_int, [C.c_uint32, C.c_uint32, C.POINTER(C.c_uint64)]),
+    "zs_distill_loss": (C.c_int, [C.c_void_p, C.POINTER(Distill), C.c_void_p]),
+    "zs_distill_grad": (C.c_int, [C.c_void_p, C.POINTER(Distill), C.c_void_p]),
+    "zs_distill_loss_grad": (C.c_int, [C.c_void_p, C.POINTER(Distill), C.c_void_p]),
     "zs_tool_call_envelope_regex": (C.c_int, [C.POINTER(C.c_char_p), C.POINTER(C.c_char_p), C.c_uint32, C.c_char_p,
                                               C.c_size_t, C.POINTER(C.c_size_t), C.c_char_p, C.c_size_t]),
 }
@@ -168,7 +216,8 @@ SIGNATURES = {
 ABI_VERSION = 2
 
 # zs_struct_layout ids (ZS_LAYOUT_*) of the Structures above
-LAYOUTS = {0: Batch, 1: RowParams, 2: SpecBatch, 3: LaneStream, 4: HallucReport}
+LAYOUTS = {0: Batch, 1: RowParams, 2: SpecBatch, 3: LaneStream, 4: HallucReport, 5: Beam, 6: BeamStateDesc,
+           7: Teacher, 8: Distill}
 
 
 def layout_mismatches(lib_):

@@ -11,6 +11,9 @@
 #include <map>
 #include <vector>
 #include "zs_internal.h"
+#include "zs_head_args.h"
+#include "zs_beam.h"
+#include "zs_distill.h"
 
 // launchers (zs_sample.hip, zs_dfa.hip)
 extern "C" int zs_sample_launch(zs_ctx* ctx, const zs_batch* bt, hipStream_t stream);
@@ -93,6 +96,33 @@ extern "C" int zs_struct_layout(int which, size_t* size, size_t* offsets, size_t
         ZS_OFF(zs_halluc_report, risk_score), ZS_OFF(zs_halluc_report, mean_entropy),
         ZS_OFF(zs_halluc_report, normalized_entropy), ZS_OFF(zs_halluc_report, risky_fraction),
         ZS_OFF(zs_halluc_report, peak_token), ZS_OFF(zs_halluc_report, n_tokens)};
+    static const size_t beam[] = {
+        ZS_OFF(zs_beam, groups), ZS_OFF(zs_beam, width), ZS_OFF(zs_beam, V), ZS_OFF(zs_beam, dtype),
+        ZS_OFF(zs_beam, ld), ZS_OFF(zs_beam, d_logits), ZS_OFF(zs_beam, d_allow_bits), ZS_OFF(zs_beam, allow_words),
+        ZS_OFF(zs_beam, n_eos), ZS_OFF(zs_beam, eos), ZS_OFF(zs_beam, length_penalty), ZS_OFF(zs_beam, flags),
+        ZS_OFF(zs_beam, d_scores), ZS_OFF(zs_beam, d_fin_score), ZS_OFF(zs_beam, d_fin_length),
+        ZS_OFF(zs_beam, d_fin_parent), ZS_OFF(zs_beam, d_fin_token), ZS_OFF(zs_beam, d_steps), ZS_OFF(zs_beam, d_done),
+        ZS_OFF(zs_beam, d_fin_score_out), ZS_OFF(zs_beam, d_fin_length_out), ZS_OFF(zs_beam, d_fin_parent_out),
+        ZS_OFF(zs_beam, d_fin_token_out), ZS_OFF(zs_beam, d_steps_out), ZS_OFF(zs_beam, d_done_out),
+        ZS_OFF(zs_beam, d_parent), ZS_OFF(zs_beam, d_token), ZS_OFF(zs_beam, d_score), ZS_OFF(zs_beam, d_work),
+        ZS_OFF(zs_beam, work_bytes)};
+    static const size_t bstate[] = {
+        ZS_OFF(zs_beam_state, d_base), ZS_OFF(zs_beam_state, row_stride), ZS_OFF(zs_beam_state, outer_stride),
+        ZS_OFF(zs_beam_state, inner_stride), ZS_OFF(zs_beam_state, bytes), ZS_OFF(zs_beam_state, n_outer),
+        ZS_OFF(zs_beam_state, n_inner)};
+    static const size_t teach[] = {
+        ZS_OFF(zs_teacher, N), ZS_OFF(zs_teacher, V), ZS_OFF(zs_teacher, K), ZS_OFF(zs_teacher, dtype),
+        ZS_OFF(zs_teacher, ld), ZS_OFF(zs_teacher, d_logits), ZS_OFF(zs_teacher, temperature), ZS_OFF(zs_teacher, pad),
+        ZS_OFF(zs_teacher, d_ids), ZS_OFF(zs_teacher, d_logp), ZS_OFF(zs_teacher, d_lse), ZS_OFF(zs_teacher, d_work),
+        ZS_OFF(zs_teacher, work_bytes)};
+    static const size_t dist[] = {
+        ZS_OFF(zs_distill, N), ZS_OFF(zs_distill, V), ZS_OFF(zs_distill, K), ZS_OFF(zs_distill, dtype),
+        ZS_OFF(zs_distill, ld), ZS_OFF(zs_distill, d_logits), ZS_OFF(zs_distill, d_ids), ZS_OFF(zs_distill, d_logp),
+        ZS_OFF(zs_distill, d_labels), ZS_OFF(zs_distill, ignore_index), ZS_OFF(zs_distill, temperature),
+        ZS_OFF(zs_distill, kl_weight), ZS_OFF(zs_distill, ce_weight), ZS_OFF(zs_distill, flags),
+        ZS_OFF(zs_distill, d_loss), ZS_OFF(zs_distill, d_stats), ZS_OFF(zs_distill, d_row_grad),
+        ZS_OFF(zs_distill, row_grad_stride), ZS_OFF(zs_distill, d_grad), ZS_OFF(zs_distill, ld_grad),
+        ZS_OFF(zs_distill, d_work), ZS_OFF(zs_distill, work_bytes)};
     const size_t* f;
     size_t n, sz;
     switch (which) {
@@ -101,6 +131,10 @@ extern "C" int zs_struct_layout(int which, size_t* size, size_t* offsets, size_t
         case ZS_LAYOUT_SPEC_BATCH: f = spec; n = sizeof(spec) / sizeof(size_t); sz = sizeof(zs_spec_batch); break;
         case ZS_LAYOUT_LANE_STREAM: f = lane; n = sizeof(lane) / sizeof(size_t); sz = sizeof(zs_lane_stream); break;
         case ZS_LAYOUT_HALLUC_REPORT: f = rep; n = sizeof(rep) / sizeof(size_t); sz = sizeof(zs_halluc_report); break;
+        case ZS_LAYOUT_BEAM: f = beam; n = sizeof(beam) / sizeof(size_t); sz = sizeof(zs_beam); break;
+        case ZS_LAYOUT_BEAM_STATE: f = bstate; n = sizeof(bstate) / sizeof(size_t); sz = sizeof(zs_beam_state); break;
+        case ZS_LAYOUT_TEACHER: f = teach; n = sizeof(teach) / sizeof(size_t); sz = sizeof(zs_teacher); break;
+        case ZS_LAYOUT_DISTILL: f = dist; n = sizeof(dist) / sizeof(size_t); sz = sizeof(zs_distill); break;
         default: return ZS_EINVAL;
     }
     if (size) *size = sz;
@@ -1044,4 +1078,213 @@ extern "C" int zs_lane_step(zs_ctx* ctx, const float* d_logits, uint32_t m, uint
     }
     zs_device_guard_end(ctx, prev);
     return rc ? zs_set_error(ctx, rc, "zs_lane_step: %s", hipGetErrorString(hipGetLastError())) : ZS_OK;
+}
+
+// ---------------------------------------------------------------------------
+// beam search and distillation: rows of three types, the caller's scratch
+// ---------------------------------------------------------------------------
+static int rows_check(zs_ctx* ctx, uint32_t V, uint32_t dtype, uint64_t ld, const void* logits, const char* who) {
+    if (dtype > ZS_BF16) return zs_set_error(ctx, ZS_EINVAL, "%s: unknown dtype %u", who, dtype);
+    if (V == 0 || V > ZS_HEAD_MAX_VOCAB)
+        return zs_set_error(ctx, ZS_ELIMIT, "%s: V=%u outside 1..%u", who, V, ZS_HEAD_MAX_VOCAB);
+    if (!logits) return zs_set_error(ctx, ZS_EINVAL, "%s: null logits", who);
+    if (ld < V) return zs_set_error(ctx, ZS_EINVAL, "%s: ld < V", who);
+    if ((uintptr_t)logits & (dtype == ZS_F32 ? 3u : 1u))
+        return zs_set_error(ctx, ZS_EINVAL, "%s: logits not aligned to their type", who);
+    return ZS_OK;
+}
+static int work_check(zs_ctx* ctx, const void* work, uint64_t have, uint64_t need, const char* who) {
+    if (!need) return ZS_OK;
+    if (!work || ((uintptr_t)work & 255u)) return zs_set_error(ctx, ZS_EINVAL, "%s: d_work null or not 256-byte aligned", who);
+    if (have < need)
+        return zs_set_error(ctx, ZS_EINVAL, "%s: work_bytes=%llu, %llu needed", who, (unsigned long long)have, (unsigned long long)need);
+    return ZS_OK;
+}
+
+extern "C" int zs_beam_select_work(uint32_t groups, uint32_t width, uint32_t V, uint32_t n_eos, uint64_t* bytes) {
+    if (!bytes || width == 0 || width > ZS_BEAM_MAX_WIDTH || n_eos > ZS_BEAM_MAX_EOS || V == 0 || V > ZS_HEAD_MAX_VOCAB ||
+        (uint64_t)groups * width > ZS_BEAM_MAX_ROWS)
+        return ZS_EINVAL;
+    *bytes = hd_work_bytes((uint64_t)groups * width, V, width + n_eos, true);
+    return ZS_OK;
+}
+
+extern "C" int zs_beam_select(zs_ctx* ctx, const zs_beam* b, void* stream) {
+    const char* who = "zs_beam_select";
+    if (!ctx || !b) return zs_set_error(ctx, ZS_EINVAL, "%s: null argument", who);
+    if (b->width == 0 || b->width > ZS_BEAM_MAX_WIDTH)
+        return zs_set_error(ctx, ZS_ELIMIT, "%s: width=%u outside 1..%d", who, b->width, ZS_BEAM_MAX_WIDTH);
+    if (b->n_eos > ZS_BEAM_MAX_EOS) return zs_set_error(ctx, ZS_ELIMIT, "%s: n_eos=%u > %d", who, b->n_eos, ZS_BEAM_MAX_EOS);
+    const uint64_t R = (uint64_t)b->groups * b->width;
+    if (R > ZS_BEAM_MAX_ROWS) return zs_set_error(ctx, ZS_ELIMIT, "%s: %llu rows > %d", who, (unsigned long long)R, ZS_BEAM_MAX_ROWS);
+    if (b->flags & ~(uint32_t)ZS_BEAM_EARLY) return zs_set_error(ctx, ZS_EINVAL, "%s: unknown flags %#x", who, b->flags);
+    if (!(b->length_penalty - b->length_penalty == 0.0f)) return zs_set_error(ctx, ZS_EINVAL, "%s: length_penalty not finite", who);
+    if (R == 0) return ZS_OK;
+    int rc = rows_check(ctx, b->V, b->dtype, b->ld, b->d_logits, who);
+    if (rc) return rc;
+    if (!b->d_scores || !b->d_fin_score || !b->d_fin_length || !b->d_fin_parent || !b->d_fin_token || !b->d_steps ||
+        !b->d_done || !b->d_fin_score_out || !b->d_fin_length_out || !b->d_fin_parent_out || !b->d_fin_token_out ||
+        !b->d_steps_out || !b->d_done_out || !b->d_parent || !b->d_token || !b->d_score)
+        return zs_set_error(ctx, ZS_EINVAL, "%s: null required pointer", who);
+    if (b->d_allow_bits && b->allow_words < (b->V + 31) / 32)
+        return zs_set_error(ctx, ZS_EINVAL, "%s: allow_words < ceil(V/32)", who);
+    uint64_t need = 0;
+    (void)zs_beam_select_work(b->groups, b->width, b->V, b->n_eos, &need);
+    if ((rc = work_check(ctx, b->d_work, b->work_bytes, need, who))) return rc;
+    hd_args h{};
+    h.logits = b->d_logits; h.ld = b->ld; h.R = R; h.V = b->V; h.K = b->width + b->n_eos;
+    h.c = (float)1.44269504088896340736; h.inv_t = 1.0;
+    h.allow = b->d_allow_bits; h.allow_words = b->allow_words;
+    h.scores = b->d_scores; h.done = b->d_done; h.width = b->width;
+    hd_work(h, b->d_work, true);
+    bm_args m{};
+    m.width = b->width; m.K = h.K; m.n_eos = b->n_eos; m.early = b->flags & ZS_BEAM_EARLY;
+    for (uint32_t i = 0; i < b->n_eos; i++) m.eos[i] = b->eos[i];
+    m.length_penalty = b->length_penalty;
+    m.scores = b->d_scores; m.list = h.list; m.lse = h.lse;
+    m.fin_score = b->d_fin_score; m.fin_length = b->d_fin_length; m.fin_parent = b->d_fin_parent; m.fin_token = b->d_fin_token;
+    m.steps = b->d_steps; m.done = b->d_done;
+    m.fin_score_o = b->d_fin_score_out; m.fin_length_o = b->d_fin_length_out; m.fin_parent_o = b->d_fin_parent_out;
+    m.fin_token_o = b->d_fin_token_out; m.steps_o = b->d_steps_out; m.done_o = b->d_done_out;
+    m.parent = b->d_parent; m.token = b->d_token; m.score_o = b->d_score;
+    const int prev = zs_device_guard_begin(ctx);
+    rc = hd_head_launch(h, b->dtype, (hipStream_t)stream);
+    if (!rc) rc = bm_merge_launch(m, b->groups, (hipStream_t)stream);
+    zs_device_guard_end(ctx, prev);
+    return rc ? zs_set_error(ctx, ZS_EHIP, "%s: launch failed", who) : ZS_OK;
+}
+
+extern "C" int zs_beam_reorder(zs_ctx* ctx, uint32_t groups, uint32_t width, const int32_t* d_parent,
+                               const zs_beam_state* states, uint32_t n, void* stream) {
+    const char* who = "zs_beam_reorder";
+    if (!ctx || (n && !states) || !d_parent) return zs_set_error(ctx, ZS_EINVAL, "%s: null argument", who);
+    if (width == 0 || width > ZS_BEAM_MAX_WIDTH)
+        return zs_set_error(ctx, ZS_ELIMIT, "%s: width=%u outside 1..%d", who, width, ZS_BEAM_MAX_WIDTH);
+    if ((uint64_t)groups * width > ZS_BEAM_MAX_ROWS)
+        return zs_set_error(ctx, ZS_ELIMIT, "%s: more than %d rows", who, ZS_BEAM_MAX_ROWS);
+    for (uint32_t i = 0; i < n; i++) {
+        const zs_beam_state& s = states[i];
+        if (!s.bytes || !s.n_outer || !s.n_inner) continue;
+        if (!s.d_base) return zs_set_error(ctx, ZS_EINVAL, "%s: state %u: null base", who, i);
+        if (s.row_stride == 0 || (s.n_outer > 1 && s.outer_stride == 0) || (s.n_inner > 1 && s.inner_stride == 0))
+            return zs_set_error(ctx, ZS_EINVAL, "%s: state %u: blocks overlap (stride 0)", who, i);
+    }
+    if (groups == 0 || width == 1) return ZS_OK;   // a single beam has itself for a parent
+    const int prev = zs_device_guard_begin(ctx);
+    int rc = 0;
+    for (uint32_t i0 = 0; i0 < n && !rc; i0 += ZS_REORDER_BATCH) {
+        ro_args a{};
+        a.parent = d_parent;
+        a.width = width;
+        uint32_t blocks = 0;
+        for (uint32_t i = i0; i < n && i < i0 + ZS_REORDER_BATCH; i++) {
+            const zs_beam_state& s = states[i];
+            if (!s.bytes || !s.n_outer || !s.n_inner) continue;
+            const uint64_t bits = (uint64_t)(uintptr_t)s.d_base | s.row_stride | s.bytes | (s.n_outer > 1 ? s.outer_stride : 0) |
+                                  (s.n_inner > 1 ? s.inner_stride : 0);
+            bm_state& o = a.s[a.n++];
+            o.unit = bits & 1 ? 1 : bits & 2 ? 2 : bits & 12 ? 4 : 16;
+            o.base = (char*)s.d_base;
+            o.row_stride = s.row_stride;
+            o.outer_stride = s.outer_stride;
+            o.inner_stride = s.inner_stride;
+            o.cols = s.bytes / o.unit;
+            o.n_inner = s.n_inner;
+            o.total = o.cols * s.n_inner * s.n_outer;
+            o.first = blocks;
+            o.blocks = ro_blocks(o.total, groups);
+            blocks += o.blocks;
+        }
+        if (a.n) rc = ro_launch(a, blocks, groups, (hipStream_t)stream);
+    }
+    zs_device_guard_end(ctx, prev);
+    return rc ? zs_set_error(ctx, ZS_EHIP, "%s: launch failed", who) : ZS_OK;
+}
+
+extern "C" int zs_teacher_topk_work(uint32_t N, uint32_t V, uint32_t K, uint64_t* bytes) {
+    if (!bytes || K == 0 || K > ZS_TEACHER_KMAX || V == 0 || V > ZS_HEAD_MAX_VOCAB || K > V) return ZS_EINVAL;
+    *bytes = hd_work_bytes(N, V, K, false);
+    return ZS_OK;
+}
+
+extern "C" int zs_teacher_topk(zs_ctx* ctx, const zs_teacher* b, void* stream) {
+    const char* who = "zs_teacher_topk";
+    if (!ctx || !b) return zs_set_error(ctx, ZS_EINVAL, "%s: null argument", who);
+    if (b->K == 0 || b->K > ZS_TEACHER_KMAX || b->K > b->V)
+        return zs_set_error(ctx, ZS_ELIMIT, "%s: K=%u outside 1..min(V, %d)", who, b->K, ZS_TEACHER_KMAX);
+    if (!(b->temperature > 0.0f) || !(b->temperature <= 3.4e38f))
+        return zs_set_error(ctx, ZS_EINVAL, "%s: temperature must be positive and finite", who);
+    if (b->N == 0) return ZS_OK;
+    int rc = rows_check(ctx, b->V, b->dtype, b->ld, b->d_logits, who);
+    if (rc) return rc;
+    if (!b->d_ids || !b->d_logp || !b->d_lse) return zs_set_error(ctx, ZS_EINVAL, "%s: null output", who);
+    uint64_t need = 0;
+    (void)zs_teacher_topk_work(b->N, b->V, b->K, &need);
+    if ((rc = work_check(ctx, b->d_work, b->work_bytes, need, who))) return rc;
+    hd_args h{};
+    h.logits = b->d_logits; h.ld = b->ld; h.R = b->N; h.V = b->V; h.K = b->K;
+    h.inv_t = 1.0 / (double)b->temperature;
+    h.c = (float)(1.44269504088896340736 * h.inv_t);
+    h.ids = b->d_ids; h.logp = b->d_logp; h.lse_out = b->d_lse;
+    hd_work(h, b->d_work, false);
+    const int prev = zs_device_guard_begin(ctx);
+    rc = hd_head_launch(h, b->dtype, (hipStream_t)stream);
+    zs_device_guard_end(ctx, prev);
+    return rc ? zs_set_error(ctx, ZS_EHIP, "%s: launch failed", who) : ZS_OK;
+}
+
+extern "C" int zs_distill_work(uint32_t N, uint32_t V, uint64_t* bytes) {
+    if (!bytes || V == 0 || V > ZS_HEAD_MAX_VOCAB) return ZS_EINVAL;
+    *bytes = ds_work_bytes(N, V);
+    return ZS_OK;
+}
+
+static int distill_call(zs_ctx* ctx, const zs_distill* b, int what, const char* who, void* stream) {
+    if (!ctx || !b) return zs_set_error(ctx, ZS_EINVAL, "%s: null argument", who);
+    if (b->K == 0 || b->K > ZS_DISTILL_KMAX)
+        return zs_set_error(ctx, ZS_ELIMIT, "%s: K=%u outside 1..%d", who, b->K, ZS_DISTILL_KMAX);
+    if (b->flags & ~(uint32_t)ZS_DISTILL_TAIL) return zs_set_error(ctx, ZS_EINVAL, "%s: unknown flags %#x", who, b->flags);
+    if (!(b->temperature > 0.0f) || !(b->temperature <= 3.4e38f))
+        return zs_set_error(ctx, ZS_EINVAL, "%s: temperature must be positive and finite", who);
+    if (!(b->kl_weight - b->kl_weight == 0.0f) || !(b->ce_weight - b->ce_weight == 0.0f))
+        return zs_set_error(ctx, ZS_EINVAL, "%s: weights must be finite", who);
+    if (b->N == 0) return ZS_OK;
+    int rc = rows_check(ctx, b->V, b->dtype, b->ld, b->d_logits, who);
+    if (rc) return rc;
+    if (!b->d_ids || !b->d_logp || ((what & DS_LOSS) && !b->d_loss) || (what == DS_GRAD && !b->d_stats) ||
+        (what == DS_LOSS && !b->d_stats) || ((what & DS_GRAD) && (!b->d_grad || !b->d_row_grad)))
+        return zs_set_error(ctx, ZS_EINVAL, "%s: null required pointer", who);
+    if (what != (DS_LOSS | DS_GRAD) && ((uintptr_t)b->d_stats & 15u))
+        return zs_set_error(ctx, ZS_EINVAL, "%s: d_stats not 16-byte aligned", who);
+    if ((what & DS_GRAD) && (b->ld_grad < b->V || ((uintptr_t)b->d_grad & (b->dtype == ZS_F32 ? 3u : 1u))))
+        return zs_set_error(ctx, ZS_EINVAL, "%s: ld_grad < V or d_grad not aligned to its type", who);
+    if ((what & DS_GRAD) && b->d_grad == b->d_logits && b->ld_grad != b->ld)
+        return zs_set_error(ctx, ZS_EINVAL, "%s: a gradient in place needs ld_grad == ld", who);
+    if ((rc = work_check(ctx, b->d_work, b->work_bytes, ds_work_bytes(b->N, b->V), who))) return rc;
+    ds_args a{};
+    a.logits = b->d_logits; a.ld = b->ld; a.N = b->N; a.V = b->V; a.K = b->K;
+    a.ids = b->d_ids; a.logp = b->d_logp; a.labels = b->d_labels; a.ignore = b->ignore_index;
+    a.inv_t = 1.0 / (double)b->temperature;
+    a.c = (float)(1.44269504088896340736 * a.inv_t);
+    a.kl = b->kl_weight; a.ce = b->ce_weight;
+    a.tail = b->flags & ZS_DISTILL_TAIL;
+    a.two = b->d_labels && b->ce_weight != 0.0f && b->temperature != 1.0f;
+    a.loss = b->d_loss;
+    a.stats = what == (DS_LOSS | DS_GRAD) ? nullptr : b->d_stats;
+    a.row_grad = b->d_row_grad; a.row_grad_stride = b->row_grad_stride;
+    a.grad = b->d_grad; a.ld_grad = b->ld_grad;
+    a.work = (float*)b->d_work;
+    const int prev = zs_device_guard_begin(ctx);
+    rc = ds_launch(a, b->dtype, what, (hipStream_t)stream);
+    zs_device_guard_end(ctx, prev);
+    return rc ? zs_set_error(ctx, ZS_EHIP, "%s: launch failed", who) : ZS_OK;
+}
+extern "C" int zs_distill_loss(zs_ctx* ctx, const zs_distill* args, void* stream) {
+    return distill_call(ctx, args, DS_LOSS, "zs_distill_loss", stream);
+}
+extern "C" int zs_distill_grad(zs_ctx* ctx, const zs_distill* args, void* stream) {
+    return distill_call(ctx, args, DS_GRAD, "zs_distill_grad", stream);
+}
+extern "C" int zs_distill_loss_grad(zs_ctx* ctx, const zs_distill* args, void* stream) {
+    return distill_call(ctx, args, DS_LOSS | DS_GRAD, "zs_distill_loss_grad", stream);
 }

@@ -1,0 +1,134 @@
+// zs_head.h -- rows of logits in any of the three types, from any element on:
+// what beam search (zs_beam.hip), the teacher's lists (zs_head.hip) and
+// distillation (zs_distill.hip) read rows through.
+#pragma once
+#include <hip/hip_runtime.h>
+#include "zs_internal.h"
+#include "zs_dev.h"
+#include "zs_head_args.h"
+
+// A row is read as 16-byte vectors of E elements. It may start at any element
+// of its type: vectors are counted from the 16-byte boundary at or below the
+// row's first element, and the ids of vector j are j * E - shift + q. Only the
+// first and the last vector can hold ids outside the row; those two are read
+// element by element, so that nothing outside the row is touched.
+template <int DT> struct hd_elem;
+template <> struct hd_elem<ZS_F32> { typedef float T; static constexpr int E = 4; };
+template <> struct hd_elem<ZS_F16> { typedef _Float16 T; static constexpr int E = 8; };
+template <> struct hd_elem<ZS_BF16> { typedef uint16_t T; static constexpr int E = 8; };
+
+__device__ __forceinline__ float hd_float(float v) { return v; }
+__device__ __forceinline__ float hd_float(_Float16 v) { return (float)v; }
+__device__ __forceinline__ float hd_float(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+
+template <int DT>
+__device__ __forceinline__ void hd_unpack(const uint4& v, float (&x)[hd_elem<DT>::E]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (DT == ZS_F32) {
+            x[i] = __uint_as_float(w[i]);
+        } else if constexpr (DT == ZS_BF16) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+            const h2 h = __builtin_bit_cast(h2, w[i]);
+            x[2 * i] = (float)h[0];
+            x[2 * i + 1] = (float)h[1];
+        }
+    }
+}
+// Rounded to nearest even; what the type cannot hold becomes infinite.
+template <int DT>
+__device__ __forceinline__ uint32_t hd_pack2(float a, float b) {
+    if constexpr (DT == ZS_BF16) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        const b2 v = {(__bf16)a, (__bf16)b};
+        return __builtin_bit_cast(uint32_t, v);
+    } else {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        const h2 v = {(_Float16)a, (_Float16)b};
+        return __builtin_bit_cast(uint32_t, v);
+    }
+}
+
+template <int DT>
+struct hd_row {
+    typedef typename hd_elem<DT>::T T;
+    static constexpr int E = hd_elem<DT>::E;
+    const T* row;
+    uint32_t shift, V, nvec;
+    __device__ __forceinline__ hd_row(const void* base, uint64_t ld, uint64_t r, uint32_t V_) {
+        row = reinterpret_cast<const T*>(base) + r * ld;
+        V = V_;
+        shift = (uint32_t)((uintptr_t)row & 15u) / (uint32_t)sizeof(T);
+        nvec = (V + shift + E - 1u) / E;
+    }
+    __device__ __forceinline__ int id0(uint32_t j) const { return (int)(j * E) - (int)shift; }
+    __device__ __forceinline__ bool inside(uint32_t j) const { const int i = id0(j); return i >= 0 && (uint32_t)i + E <= V; }
+    __device__ __forceinline__ uint4 load(uint32_t j) const { return zs_gload(reinterpret_cast<const uint4*>(row + id0(j))); }
+    __device__ __forceinline__ float at(uint32_t id) const { return hd_float(zs_gload(row + id)); }
+    // the vector's values; `none` where it has no id of the row
+    __device__ __forceinline__ void get(uint32_t j, float (&x)[E], float none) const {
+        if (inside(j)) {
+            hd_unpack<DT>(load(j), x);
+            return;
+        }
+        const int i = id0(j);
+#pragma unroll
+        for (int q = 0; q < E; q++) x[q] = i + q >= 0 && (uint32_t)(i + q) < V ? at((uint32_t)(i + q)) : none;
+    }
+};
+
+// The allow bits of ids i .. i + E - 1 (bit q: id i + q); i may be negative
+// and past V, where the bits are unspecified (such ids are no ids of the row).
+template <int E>
+__device__ __forceinline__ uint32_t hd_allow(const uint32_t* words, uint32_t nwords, int i) {
+    const uint32_t p = (uint32_t)max(i, 0), w = p >> 5, s = p & 31u;
+    if (w >= nwords) return 0u;
+    uint64_t two = zs_gload(words + w);
+    if (s + E > 32u && w + 1u < nwords) two |= (uint64_t)zs_gload(words + w + 1u) << 32;
+    const uint32_t b = (uint32_t)(two >> s);
+    return i < 0 ? b << (uint32_t)(-i) : b;
+}
+
+// The sum of E values as a tree: a running sum that holds the largest term
+// takes one rounding per vector, not one per value (rows whose first value
+// has most of the mass lost 5e-7 of their sum to a chain of 300 values).
+template <int E>
+__device__ __forceinline__ float hd_sum(const float (&e)[E]) {
+    if constexpr (E == 4) return (e[0] + e[1]) + (e[2] + e[3]);
+    else return ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+}
+
+// A value as the heads of rows see it: NaN counts as -inf (nothing is known of
+// it), +inf as the largest number (an id that is certain; several share).
+__device__ __forceinline__ float hd_clean(float x) { return fminf(x == x ? x : -INFINITY, __FLT_MAX__); }
+// Order of the candidates: a larger key is a larger value, -0 and +0 are one
+// value; 0 is no candidate (-inf).
+__device__ __forceinline__ uint32_t hd_key(float x) { return x > -INFINITY ? zs_total_key(x + 0.0f) : 0u; }
+
+#define HD_LOG2E 1.44269504088896340736
+
+// ln sum exp(x / T) from sum = sum exp((x - m) / T); -inf for no mass
+__device__ __forceinline__ double hd_lse(float m, double inv_t, double sum) { return sum > 0.0 ? (double)m * inv_t + log(sum) : -INFINITY; }
+
+// Is row r's head wanted?
+__device__ __forceinline__ bool hd_live(const hd_args& a, uint64_t r) {
+    return !a.scores || (!a.done[r / a.width] && fabsf(a.scores[r]) <= __FLT_MAX__);
+}
+// Entry t of row r, e = ~key << 32 | id (~0: none); by threads t < K.
+__device__ __forceinline__ void hd_put(const hd_args& a, uint64_t r, uint32_t t, unsigned long long e, double lse) {
+    if (t >= a.K) return;
+    const bool some = e != ~0ull;
+    const float x = zs_key_to_float(~(uint32_t)(e >> 32));
+    if (a.ids) {
+        a.ids[r * a.K + t] = some ? (uint32_t)e : 0xffffffffu;
+        a.logp[r * a.K + t] = some ? (float)((double)x * a.inv_t - lse) : -INFINITY;
+        if (t == 0) a.lse_out[r] = (float)lse;
+    } else {
+        a.list[r * a.K + t] = some ? ((unsigned long long)zs_f2u(x) << 32) | (uint32_t)e : ~0ull;
+        if (t == 0) a.lse[r] = lse;
+    }
+}
