@@ -170,8 +170,8 @@ __global__ __launch_bounds__(DS_NT) void zs_k_distill_row(ds_args a, uint64_t r0
 }
 
 int ds_launch(const ds_args& a, uint32_t dtype, int what, hipStream_t stream) {
-    for (uint64_t r0 = 0; r0 < a.N; r0 += HD_ROWS) {
-        const dim3 grid((uint32_t)(a.N - r0 < HD_ROWS ? a.N - r0 : HD_ROWS));
+    for (uint64_t r0 = 0; r0 < a.N; r0 += HD_BLOCKS) {
+        const dim3 grid((uint32_t)(a.N - r0 < HD_BLOCKS ? a.N - r0 : HD_BLOCKS));
 #define DS_GO(DT)                                                                                                      \
     if (what == DS_LOSS) hipLaunchKernelGGL((zs_k_distill_row<DT, DS_LOSS>), grid, dim3(DS_NT), 0, stream, a, r0);     \
     else if (what == DS_GRAD) hipLaunchKernelGGL((zs_k_distill_row<DT, DS_GRAD>), grid, dim3(DS_NT), 0, stream, a, r0); \

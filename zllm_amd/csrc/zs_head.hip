@@ -1,140 +1,368 @@
 // zs_head.hip -- the head of a row of logits: its K largest values with their
 // ids and its log-normaliser, for a teacher's lists (zs_teacher_topk) and for
 // the beam step (zs_beam.hip).
+//
+// One pass over the logits (zs_k_head_scan, the whole GPU): every wave takes
+// 2048 values into registers, leaves the largest value of each group of 2^gs
+// of them and its own maximum m with sum exp((x - m) / T). Then one workgroup
+// a row (zs_k_head_pick): ln sum from the waves' records, and a key that at
+// least K groups reach, so that the K largest values lie in the groups whose
+// maximum reaches it, a few more than K, whose values are read again, listed
+// and sorted.
 #include "zs_head.h"
+#include "zs_select.h"
 
-#define HR_NT 512
+// ---------------------------------------------------------------------------
+// the pass
+// ---------------------------------------------------------------------------
+#define HS_NT 256
 
-// Adds into lds[256] the histogram of 8-bit digits and returns, by the whole
-// workgroup, the digit that holds the need-th key from above and what is
-// still needed inside it.
-template <int NT>
-__device__ __forceinline__ void hr_digit(const uint32_t* hist, uint32_t need, uint32_t* u) {
-    if (threadIdx.x < 64) {
-        const uint32_t t = threadIdx.x;
-        uint32_t c[4], loc = 0;
-#pragma unroll
-        for (int q = 0; q < 4; q++) { c[q] = hist[255u - 4u * t - (uint32_t)q]; loc += c[q]; }
-        const uint32_t inc = wave_incl_scan_u(loc);
-        uint32_t before = inc - loc;
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            if (before < need && need <= before + c[q]) { u[0] = 255u - 4u * t - (uint32_t)q; u[1] = need - before; }
-            before += c[q];
-        }
-    }
-    __syncthreads();
+// Maximum over lanes whose numbers differ in the bits FROM .. TO / 2.
+template <int FROM, int TO>
+__device__ __forceinline__ float hs_max(float v) {
+    if constexpr (FROM < TO) return hs_max<FROM * 2, TO>(fmaxf(v, zs_lane_xor<FROM>(v)));
+    else return v;
 }
 
-// One workgroup a row: the maximum, the sum, then a radix selection of the
-// K-th key over passes of the row.
+// LG: lanes of a group
+template <int DT, int LG, bool MASK>
+__global__ __launch_bounds__(HS_NT) void zs_k_head_scan(hd_args a, uint64_t r0) {
+    constexpr int E = hd_elem<DT>::E, U = HD_WAVE / 64 / E;
+    const uint64_t r = r0 + blockIdx.x / a.chunks;
+    const uint32_t chunk = blockIdx.x % a.chunks;
+    if (!hd_live(a, r)) return;
+    const hd_row<DT> row(a.logits, a.ld, r, a.V);
+    const uint32_t t = threadIdx.x, lane = (uint32_t)zs_lane();
+    const uint32_t first = chunk * (U * HS_NT), j0 = first + t;
+    if (first >= row.nvec) return;
+    float x[U][E];
+    if (row.inside(first) && row.inside(first + U * HS_NT - 1u)) {
+        uint4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) v[u] = row.load(j0 + (uint32_t)u * HS_NT);
+#pragma unroll
+        for (int u = 0; u < U; u++) hd_unpack<DT>(v[u], x[u]);
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t j = j0 + (uint32_t)u * HS_NT;
+            if (j < row.nvec) row.get(j, x[u], -INFINITY);
+            else
+#pragma unroll
+                for (int q = 0; q < E; q++) x[u][q] = -INFINITY;
+        }
+    }
+    if (MASK) {
+        const uint32_t* allow = a.allow + r * a.allow_words;
+        uint32_t b[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) b[u] = hd_allow<E>(allow, a.allow_words, row.id0(j0 + (uint32_t)u * HS_NT));
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int q = 0; q < E; q++) x[u][q] = b[u] >> q & 1u ? x[u][q] : -INFINITY;
+    }
+    float g[U], m;
+    auto maxima = [&]() {
+        m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float v = x[u][0];
+#pragma unroll
+            for (int q = 1; q < E; q++) v = fmaxf(v, x[u][q]);
+            g[u] = hs_max<1, LG>(v);
+            m = fmaxf(m, g[u]);
+        }
+        m = hs_max<LG, 64>(m);
+    };
+    maxima();
+    // 2^(x c - mc): one fma a value; mc's rounding is a factor of all of them
+    float mr = m > -INFINITY ? m : 0.0f, mc = mr * a.c, s = 0.0f;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        float e[E];
+#pragma unroll
+        for (int q = 0; q < E; q++) e[q] = __builtin_amdgcn_exp2f(fmaf(x[u][q], a.c, -mc));
+        s += hd_sum(e);
+    }
+    s = zs_wave_reduce(s, [](float p, float q) { return p + q; });
+    if (s < INFINITY && fabsf(mc) < INFINITY) {
+        s *= __builtin_amdgcn_exp2f(-fmaf(mr, a.c, -mc));
+    } else {
+        // NaN or +inf among the values, or a maximum whose exponent no float holds
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int q = 0; q < E; q++) x[u][q] = hd_clean(x[u][q]);
+        maxima();
+        mr = m > -INFINITY ? m : 0.0f;
+        s = 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float e[E];
+#pragma unroll
+            for (int q = 0; q < E; q++) e[q] = __builtin_amdgcn_exp2f((x[u][q] - mr) * a.c);
+            s += hd_sum(e);
+        }
+        s = zs_wave_reduce(s, [](float p, float q) { return p + q; });
+    }
+    if (lane == 0) a.rec[r * a.recs + chunk * (HS_NT / 64) + (uint32_t)zs_wid()] = make_float2(m, s);
+    // a group's lanes store their vectors' groups in turn
+    uint32_t* gmax = a.gmax + r * a.gstride;
+    constexpr int ST = LG < U ? LG : U;
+    const uint32_t i = lane & (uint32_t)(LG - 1);
+#pragma unroll
+    for (int u = 0; u < U; u += ST) {
+        float v = g[u];
+#pragma unroll
+        for (int k = 1; k < ST; k++) v = i == (uint32_t)k ? g[u + k] : v;
+        const uint32_t j = j0 + ((uint32_t)u + i) * HS_NT;
+        if (i < (uint32_t)ST && j - i < row.nvec) gmax[j / LG] = hd_key(v);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// the pick
+// ---------------------------------------------------------------------------
+#define HP_NT 256
+#define HP_GPT (HD_GROUPS / HP_NT)   // groups per thread at most
+#define HP_GL 256                    // listed groups at most (rows in no order: K + 20 to K + 80)
+#define HP_LIST 1024                 // listed values at most
+
+// Places of the set bits (place t + e * HP_NT for bit e) in ascending order.
+template <int E>
+__device__ __forceinline__ uint32_t hp_places(uint32_t bits, uint32_t* out, uint32_t* cnt) {
+    constexpr uint32_t NW = HP_NT / 64;
+    const uint32_t lane = (uint32_t)zs_lane(), wid = (uint32_t)zs_wid();
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const uint32_t n = (uint32_t)__popcll(__ballot(bits >> e & 1u));
+        if (lane == 0) cnt[(uint32_t)e * NW + wid] = n;
+    }
+    __syncthreads();
+    uint32_t run = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const unsigned long long m = __ballot(bits >> e & 1u);
+        uint32_t before = run;
+#pragma unroll
+        for (uint32_t w = 0; w < NW; w++) {
+            const uint32_t c = cnt[(uint32_t)e * NW + w];
+            before += w < wid ? c : 0u;
+            run += c;
+        }
+        if (bits >> e & 1u) out[before + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u))] =
+            threadIdx.x + (uint32_t)e * HP_NT;
+    }
+    __syncthreads();
+    return run;
+}
+
 template <int DT, bool MASK>
-__global__ __launch_bounds__(HR_NT) void zs_k_head_row(hd_args a, uint64_t r0) {
-    constexpr int E = hd_elem<DT>::E, NW = HR_NT / 64;
-    __shared__ unsigned long long list[HD_KMAX];
-    __shared__ uint32_t hist[256], u[4], shu[NW];
-    __shared__ float shf[NW];
-    __shared__ double shd[NW];
+__global__ __launch_bounds__(HP_NT) void zs_k_head_pick(hd_args a, uint64_t r0, uint32_t lgs) {
+    constexpr int E = hd_elem<DT>::E;
+    constexpr uint32_t NW = HP_NT / 64;
+    __shared__ unsigned long long list[HP_LIST];
+    __shared__ uint32_t gl[HP_GL], pl[ZS_TEACHER_KMAX];
+    __shared__ uint32_t hist[256], u[4], wthr[NW];
+    __shared__ double lse_s;
     const uint64_t r = r0 + blockIdx.x;
     if (!hd_live(a, r)) return;
     const hd_row<DT> row(a.logits, a.ld, r, a.V);
     const uint32_t* allow = MASK ? a.allow + r * a.allow_words : nullptr;
-    const uint32_t t = threadIdx.x;
-    auto values = [&](uint32_t j, float (&x)[E]) {
-        row.get(j, x, -INFINITY);
+    const uint32_t t = threadIdx.x, lane = (uint32_t)zs_lane(), wid = (uint32_t)zs_wid(), K = a.K;
+    const uint32_t ng = (row.nvec + (1u << lgs) - 1u) >> lgs;
+    const uint32_t* gm = a.gmax + r * a.gstride;
+    // thread t of wave w holds groups 4 lane + w + 256 e: the groups of a short
+    // row fall on all waves alike
+    uint32_t k[HP_GPT], tm = 0;
+#pragma unroll
+    for (int e = 0; e < HP_GPT; e++) {
+        const uint32_t g = NW * lane + wid + (uint32_t)e * HP_NT;
+        k[e] = (uint32_t)e * HP_NT < ng ? zs_gload(gm + min(g, ng - 1u)) : 0u;
+        if (g >= ng) k[e] = 0u;
+    }
+    if (wid == NW - 1u) {   // ln sum exp(x / T) of the row
+        const uint32_t recs = (row.nvec * E + HD_CHUNK - 1u) / HD_CHUNK * (HD_CHUNK / HD_WAVE);
+        const float2* rec = a.rec + r * a.recs;
+        float m = -INFINITY;
+        for (uint32_t i = lane; i < recs; i += 64u) m = fmaxf(m, rec[i].x);
+        m = wave_max_f(m);
+        double s = 0.0;
+        for (uint32_t i = lane; i < recs; i += 64u) {
+            const float2 v = rec[i];
+            if (v.x > -INFINITY) s += (double)v.y * exp(((double)v.x - (double)m) * a.inv_t);
+        }
+        s = wave_sum_d(s);
+        if (lane == 0) lse_s = hd_lse(m, a.inv_t, s);
+    }
+#pragma unroll
+    for (int e = 0; e < HP_GPT; e++) tm = max(tm, k[e]);
+    if (t < 4) u[t] = 0;
+    // theta: in every wave the ceil(K / waves)-th largest thread maximum; the
+    // smallest of them is reached by K groups (1: too few hold a candidate, all
+    // are listed then)
+    const uint32_t srt = wave_sort_u32(tm);
+    const uint32_t wt = zs_readlane_u(srt, 64u - (K + NW - 1u) / NW);
+    if (lane == 0) wthr[wid] = wt;
+    __syncthreads();
+    uint32_t theta = wthr[0];
+#pragma unroll
+    for (uint32_t w = 1; w < NW; w++) theta = min(theta, wthr[w]);
+    theta = max(theta, 1u);
+    uint32_t ngt = 0;
+#pragma unroll
+    for (int e = 0; e < HP_GPT; e++) ngt += k[e] >= theta ? 1u : 0u;
+    uint32_t p = ngt ? atomicAdd(&u[0], ngt) : 0u;
+#pragma unroll
+    for (int e = 0; e < HP_GPT; e++) {
+        if (k[e] < theta) continue;
+        if (p < HP_GL) gl[p] = NW * lane + wid + (uint32_t)e * HP_NT;
+        p++;
+    }
+    __syncthreads();
+    const uint32_t n_gl = u[0], lm = (1u << lgs) - 1u;
+    auto keys_of = [&](const float (&x)[E], uint32_t j, uint32_t (&kq)[E]) {
         uint32_t b = ~0u;
         if (MASK) b = hd_allow<E>(allow, a.allow_words, row.id0(j));
 #pragma unroll
-        for (int q = 0; q < E; q++) x[q] = (b >> q & 1u) ? hd_clean(x[q]) : -INFINITY;
+        for (int q = 0; q < E; q++) kq[q] = b >> q & 1u ? hd_key(hd_clean(x[q])) : 0u;
     };
-    float x[E], m = -INFINITY;
-    for (uint32_t j = t; j < row.nvec; j += HR_NT) {
-        values(j, x);
+    auto keys = [&](uint32_t j, uint32_t (&kq)[E]) {
+        float x[E];
+        row.get(j, x, -INFINITY);
+        keys_of(x, j, kq);
+    };
+    auto entry = [&](uint32_t key, uint32_t j, int q) {
+        return ((unsigned long long)(~key) << 32) | (uint32_t)(row.id0(j) + q);
+    };
+    if (n_gl <= HP_GL) {
+        const uint32_t nit = n_gl << lgs;
+        // four vectors a thread in flight; those at the row's ends, and all of
+        // a row that has no others, are read by `keys`
+        constexpr int NU = 4;
+        const bool wide = row.nvec >= 3u;
+        for (uint32_t i0 = 0; i0 < nit; i0 += NU * HP_NT) {
+            uint4 v[NU];
+            uint32_t jv[NU];
 #pragma unroll
-        for (int q = 0; q < E; q++) m = fmaxf(m, x[q]);
-    }
-    m = block_max_f<HR_NT>(m, shf);
-    const float mr = m > -INFINITY ? m : 0.0f;
-    float s = 0.0f;
-    for (uint32_t j = t; j < row.nvec; j += HR_NT) {
-        values(j, x);
+            for (int w = 0; w < NU; w++) {
+                const uint32_t i = i0 + t + (uint32_t)w * HP_NT;
+                jv[w] = i < nit ? (gl[i >> lgs] << lgs) + (i & lm) : row.nvec;
+                if (wide) v[w] = row.load(row.inside(jv[w]) ? jv[w] : 1u);
+            }
 #pragma unroll
-        for (int q = 0; q < E; q++) x[q] = __builtin_amdgcn_exp2f((x[q] - mr) * a.c);
-        s += hd_sum(x);
-    }
-    const double sum = block_sum_d<HR_NT>((double)s, shd);
-    const double lse = hd_lse(mr, a.inv_t, sum);
-    // the K-th key: its digits from the top, `need` of the keys equal so far
-    uint32_t mask = 0, key = 0, need = a.K, all = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (t < 256) hist[t] = 0;
-        __syncthreads();
-        for (uint32_t j = t; j < row.nvec; j += HR_NT) {
-            values(j, x);
+            for (int w = 0; w < NU; w++) {
+                const uint32_t j = jv[w];
+                uint32_t kq[E], n = 0;
+                if (wide && row.inside(j)) {
+                    float x[E];
+                    hd_unpack<DT>(v[w], x);
+                    keys_of(x, j, kq);
+                } else if (j < row.nvec) {
+                    keys(j, kq);
+                } else {
 #pragma unroll
-            for (int q = 0; q < E; q++) {
-                const uint32_t k = hd_key(x[q]);
-                if (k && (k & mask) == key) atomicAdd(&hist[k >> shift & 255u], 1u);
+                    for (int q = 0; q < E; q++) kq[q] = 0u;
+                }
+                // (one atomic a wave: one a lane is served lane by lane)
+                uint32_t p = 0;
+#pragma unroll
+                for (int q = 0; q < E; q++) {
+                    const unsigned long long m = __ballot(kq[q] >= theta);
+                    p = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, p));
+                    n += (uint32_t)__popcll(m);
+                }
+                if (!n) continue;
+                uint32_t p0 = 0;
+                if (lane == 0) p0 = atomicAdd(&u[1], n);
+                p += (uint32_t)__builtin_amdgcn_readfirstlane((int)p0);
+#pragma unroll
+                for (int q = 0; q < E; q++) {
+                    if (kq[q] < theta) continue;
+                    if (p < HP_LIST) list[p] = entry(kq[q], j, q);
+                    p++;
+                }
             }
         }
-        __syncthreads();
-        if (shift == 24) {
-            all = block_sum_u<HR_NT>(t < 256 ? hist[t] : 0u, shu);
-            if (all <= a.K) break;
-        }
-        hr_digit<HR_NT>(hist, need, u);
-        key |= u[0] << shift;
-        mask |= 0xffu << shift;
-        need = u[1];
-        __syncthreads();
-    }
-    // those above it in any order, those equal to it by id
-    if (t == 0) u[2] = 0;
-    const bool every = all <= a.K;
-    uint32_t taken = 0;
-    __syncthreads();
-    for (uint32_t j0 = 0; j0 < row.nvec; j0 += HR_NT) {
-        const uint32_t j = j0 + t;
-        uint32_t k[E], n = 0;
-        if (j < row.nvec) {
-            values(j, x);
-#pragma unroll
-            for (int q = 0; q < E; q++) { k[q] = hd_key(x[q]); n += !every && k[q] == key ? 1u : 0u; }
-        } else {
-#pragma unroll
-            for (int q = 0; q < E; q++) k[q] = 0u;
-        }
-        uint32_t tot = 0, at = 0;
-        if (!every) at = taken + block_excl_scan_u<HR_NT>(n, shu, &tot);
-        taken += tot;
-#pragma unroll
-        for (int q = 0; q < E; q++) {
-            const bool tie = !every && k[q] == key;
-            if (tie ? at < need : every ? k[q] != 0u : k[q] > key)
-                list[atomicAdd(&u[2], 1u)] = ((unsigned long long)(~k[q]) << 32) | (uint32_t)(row.id0(j) + q);
-            at += tie ? 1u : 0u;
-        }
     }
     __syncthreads();
-    const uint32_t n = u[2];
+    uint32_t n = u[1];
+    if (n_gl > HP_GL || n > HP_LIST) {
+        // Many groups or values reach theta (sorted rows, equal values). The
+        // first K values lie in the first K groups by (maximum descending,
+        // group ascending): K groups in front of another hold K values in front
+        // of any of its. The same holds of the groups' parts, down to single
+        // vectors: level by level, 16 parts of a group at most.
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < HP_GPT; e++) {   // (places in group order here)
+            const uint32_t g = t + (uint32_t)e * HP_NT;
+            k[e] = g < ng ? zs_gload(gm + g) : 0u;
+        }
+        uint32_t ngl = hp_places<HP_GPT>(zs_first<HP_NT, HP_GPT>(k, K, hist, u), gl, hist);
+        constexpr int NP = ZS_TEACHER_KMAX * 16 / HP_NT;
+        for (uint32_t lg = lgs; lg > 0;) {
+            const uint32_t lp = lg > 4u ? 4u : lg;
+            lg -= lp;
+            const uint32_t lm = (1u << lp) - 1u;
+            uint32_t pk[NP];
+#pragma unroll
+            for (int w = 0; w < NP; w++) {
+                const uint32_t i = t + (uint32_t)w * HP_NT;
+                pk[w] = 0u;
+                if (i >= ngl << lp) continue;
+                const uint32_t part = (gl[i >> lp] << lp) + (i & lm);
+                for (uint32_t j = part << lg; j < (part + 1u) << lg && j < row.nvec; j++) {
+                    uint32_t kq[E];
+                    keys(j, kq);
+#pragma unroll
+                    for (int q = 0; q < E; q++) pk[w] = max(pk[w], kq[q]);
+                }
+            }
+            ngl = hp_places<NP>(zs_first<HP_NT, NP>(pk, K, hist, u), pl, hist);
+            const uint32_t part = t < ngl ? (gl[pl[t] >> lp] << lp) + (pl[t] & lm) : 0u;
+            __syncthreads();
+            if (t < ngl) gl[t] = part;
+            __syncthreads();
+        }
+        if (t < ngl) {
+            uint32_t kq[E];
+            keys(gl[t], kq);
+#pragma unroll
+            for (int q = 0; q < E; q++) list[t * E + (uint32_t)q] = kq[q] ? entry(kq[q], gl[t], q) : ~0ull;
+        }
+        n = ngl * E;
+        __syncthreads();
+    }
+    static_assert(ZS_TEACHER_KMAX * 8 <= HP_LIST && ZS_TEACHER_KMAX <= HP_GL, "the first K groups and their vectors' values fit");
     uint32_t np2 = 64;
     while (np2 < n) np2 <<= 1;
-    if (t >= n && t < np2) list[t] = ~0ull;
+    for (uint32_t i = n + t; i < np2; i += HP_NT) list[i] = ~0ull;
     __syncthreads();
-    block_bitonic_u64<HR_NT>(list, (int)np2);
-    hd_put(a, r, t, t < n ? list[t] : ~0ull, lse);
+    if (np2 <= HP_NT) block_sort_reg_u64<HP_NT, 1>(list, np2);
+    else block_sort_reg_u64<HP_NT, HP_LIST / HP_NT>(list, np2);
+    hd_put(a, r, t, t < n ? list[t] : ~0ull, lse_s);
 }
 
 int hd_head_launch(const hd_args& a, uint32_t dtype, hipStream_t stream) {
-    for (uint64_t r0 = 0; r0 < a.R; r0 += HD_ROWS) {
-        const dim3 grid((uint32_t)(a.R - r0 < HD_ROWS ? a.R - r0 : HD_ROWS));
-#define HR_GO(DT)                                                                                                    \
-    if (a.allow) hipLaunchKernelGGL((zs_k_head_row<DT, true>), grid, dim3(HR_NT), 0, stream, a, r0);                 \
-    else hipLaunchKernelGGL((zs_k_head_row<DT, false>), grid, dim3(HR_NT), 0, stream, a, r0)
-        if (dtype == ZS_F32) { HR_GO(ZS_F32); }
-        else if (dtype == ZS_F16) { HR_GO(ZS_F16); }
-        else { HR_GO(ZS_BF16); }
-#undef HR_GO
+    const uint32_t gs = hd_group_shift(a.V, a.K), lgs = gs - (dtype == ZS_F32 ? 2u : 3u);
+    const uint64_t per = HD_BLOCKS / a.chunks;
+    for (uint64_t r0 = 0; r0 < a.R; r0 += per) {
+        const uint32_t n = (uint32_t)(a.R - r0 < per ? a.R - r0 : per);
+#define HS_GO(DT, LG)                                                                                                              \
+    if (a.allow) {                                                                                                                 \
+        hipLaunchKernelGGL((zs_k_head_scan<DT, LG, true>), dim3(n * a.chunks), dim3(HS_NT), 0, stream, a, r0);                     \
+        hipLaunchKernelGGL((zs_k_head_pick<DT, true>), dim3(n), dim3(HP_NT), 0, stream, a, r0, lgs);                               \
+    } else {                                                                                                                       \
+        hipLaunchKernelGGL((zs_k_head_scan<DT, LG, false>), dim3(n * a.chunks), dim3(HS_NT), 0, stream, a, r0);                    \
+        hipLaunchKernelGGL((zs_k_head_pick<DT, false>), dim3(n), dim3(HP_NT), 0, stream, a, r0, lgs);                              \
+    }
+#define HS_GS(DT, L4)                                                                                                              \
+    if (gs == 4) { HS_GO(DT, L4) } else if (gs == 6) { HS_GO(DT, L4 * 4) } else { HS_GO(DT, L4 * 16) }
+        if (dtype == ZS_F32) { HS_GS(ZS_F32, 4) }
+        else if (dtype == ZS_F16) { HS_GS(ZS_F16, 2) }
+        else { HS_GS(ZS_BF16, 2) }
     }
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }

@@ -5,7 +5,10 @@
 #include "zs_internal.h"
 
 #define HD_KMAX 128            // entries of a head at most
-#define HD_ROWS (1u << 20)     // rows per launch at most
+#define HD_WAVE 2048           // values of a row that a wave of the pass takes
+#define HD_CHUNK (4 * HD_WAVE) // and a workgroup
+#define HD_GROUPS 5120         // groups of a row at most (the pick holds their maxima in registers)
+#define HD_BLOCKS (1u << 22)   // workgroups per launch at most
 
 // The heads of R rows. For a teacher (d_ids) the list goes out as ids and
 // log-probabilities; for the beam step into `list` (bits of x~ << 32 | id,
@@ -24,6 +27,11 @@ struct hd_args {
     uint32_t width;
     unsigned long long* list;   // [R][K]
     double* lse;                // [R]
+    // the pass: group maxima and, per wave, (maximum, sum exp((x - maximum) / T))
+    uint32_t chunks;            // workgroups a row
+    uint32_t gstride, recs;     // groups and records a row
+    uint32_t* gmax;             // [R][gstride] keys
+    float2* rec;                // [R][recs]
     // teacher
     uint32_t* ids;
     float* logp;
@@ -31,18 +39,40 @@ struct hd_args {
 };
 int hd_head_launch(const hd_args& a, uint32_t dtype, hipStream_t stream);
 
-// The scratch of R rows: (beam) the lists and normalisers.
-inline uint64_t hd_pad(uint64_t n) { return (n + 255u) & ~(uint64_t)255u; }
-inline uint64_t hd_work_bytes(uint64_t R, uint32_t V, uint32_t K, bool beam) {
-    (void)V;
-    return beam ? hd_pad(R * K * 8u) + hd_pad(R * 8u) : 0u;
+// log2 of the values in a group: 64, or 16 where a row has few groups for the
+// list that is wanted (a threshold from group maxima is close only when there
+// are several times K of them), or 256 where 64 would make too many. 2048 rows
+// of 151936 bf16, K = 64: see zs_head.hip.
+inline uint32_t hd_group_shift(uint32_t V, uint32_t K) {
+    if ((V >> 6) + 2u > HD_GROUPS) return 8;
+    return (V >> 6) >= 8u * K || (V >> 4) + 2u > HD_GROUPS ? 6 : 4;
 }
-inline void hd_work(hd_args& a, void* work, bool beam) {
+// The scratch of R rows: the pass's and, for the beam step, the lists and
+// normalisers. A row's first value may lie up to 15 bytes behind a 16-byte
+// boundary, from which groups and chunks are counted: 7 values more.
+inline uint64_t hd_pad(uint64_t n) { return (n + 255u) & ~(uint64_t)255u; }
+inline uint64_t hd_work(hd_args& a, void* work, bool beam) {
     char* p = (char*)work;
+    const uint32_t gs = hd_group_shift(a.V, a.K);
+    a.chunks = (a.V + 7u + HD_CHUNK - 1u) / HD_CHUNK;
+    a.recs = a.chunks * (HD_CHUNK / HD_WAVE);
+    a.gstride = (a.V + 7u + (1u << gs) - 1u) >> gs;
+    a.gmax = (uint32_t*)p;
+    p += hd_pad(a.R * a.gstride * 4u);
+    a.rec = (float2*)p;
+    p += hd_pad(a.R * a.recs * 8u);
     if (beam) {
         a.list = (unsigned long long*)p;
         p += hd_pad(a.R * a.K * 8u);
         a.lse = (double*)p;
         p += hd_pad(a.R * 8u);
     }
+    return (uint64_t)(p - (char*)work);
+}
+inline uint64_t hd_work_bytes(uint64_t R, uint32_t V, uint32_t K, bool beam) {
+    hd_args a{};
+    a.R = R;
+    a.V = V;
+    a.K = K;
+    return hd_work(a, (void*)256, beam);
 }
