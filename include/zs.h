@@ -535,7 +535,7 @@ typedef struct zs_distill {
     void* d_work;
     uint64_t work_bytes;
 } zs_distill;
-int zs_distill_work(uint32_t N, uint32_t V, uint64_t* bytes);
+int zs_distill_work(uint32_t N, uint32_t V, uint32_t K, uint64_t* bytes);
 int zs_distill_loss(zs_ctx* ctx, const zs_distill* args, void* stream);
 int zs_distill_grad(zs_ctx* ctx, const zs_distill* args, void* stream);
 int zs_distill_loss_grad(zs_ctx* ctx, const zs_distill* args, void* stream);

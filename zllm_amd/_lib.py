@@ -204,7 +204,7 @@ SIGNATURES = {
                                   C.c_uint32, C.c_void_p]),
     "zs_teacher_topk_work": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_uint64)]),
     "zs_teacher_topk": (C.c_int, [C.c_void_p, C.POINTER(Teacher), C.c_void_p]),
-    "zs_distill_work": (C.c_int, [C.c_uint32, C.c_uint32, C.POINTER(C.c_uint64)]),
+    "zs_distill_work": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_uint64)]),
     "zs_distill_loss": (C.c_int, [C.c_void_p, C.POINTER(Distill), C.c_void_p]),
     "zs_distill_grad": (C.c_int, [C.c_void_p, C.POINTER(Distill), C.c_void_p]),
     "zs_distill_loss_grad": (C.c_int, [C.c_void_p, C.POINTER(Distill), C.c_void_p]),

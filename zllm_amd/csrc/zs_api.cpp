@@ -1233,9 +1233,11 @@ extern "C" int zs_teacher_topk(zs_ctx* ctx, const zs_teacher* b, void* stream) {
     return rc ? zs_set_error(ctx, ZS_EHIP, "%s: launch failed", who) : ZS_OK;
 }
 
-extern "C" int zs_distill_work(uint32_t N, uint32_t V, uint64_t* bytes) {
-    if (!bytes || V == 0 || V > ZS_HEAD_MAX_VOCAB) return ZS_EINVAL;
-    *bytes = ds_work_bytes(N, V);
+extern "C" int zs_distill_work(uint32_t N, uint32_t V, uint32_t K, uint64_t* bytes) {
+    if (!bytes || K == 0 || K > ZS_DISTILL_KMAX || V == 0 || V > ZS_HEAD_MAX_VOCAB) return ZS_EINVAL;
+    ds_args a{};
+    a.N = N; a.V = V; a.K = K;
+    *bytes = ds_work(a, (void*)256);
     return ZS_OK;
 }
 
@@ -1260,9 +1262,9 @@ static int distill_call(zs_ctx* ctx, const zs_distill* b, int what, const char* 
         return zs_set_error(ctx, ZS_EINVAL, "%s: ld_grad < V or d_grad not aligned to its type", who);
     if ((what & DS_GRAD) && b->d_grad == b->d_logits && b->ld_grad != b->ld)
         return zs_set_error(ctx, ZS_EINVAL, "%s: a gradient in place needs ld_grad == ld", who);
-    if ((rc = work_check(ctx, b->d_work, b->work_bytes, ds_work_bytes(b->N, b->V), who))) return rc;
     ds_args a{};
     a.logits = b->d_logits; a.ld = b->ld; a.N = b->N; a.V = b->V; a.K = b->K;
+    if ((rc = work_check(ctx, b->d_work, b->work_bytes, ds_work(a, b->d_work), who))) return rc;
     a.ids = b->d_ids; a.logp = b->d_logp; a.labels = b->d_labels; a.ignore = b->ignore_index;
     a.inv_t = 1.0 / (double)b->temperature;
     a.c = (float)(1.44269504088896340736 * a.inv_t);
@@ -1273,7 +1275,6 @@ static int distill_call(zs_ctx* ctx, const zs_distill* b, int what, const char* 
     a.stats = what == (DS_LOSS | DS_GRAD) ? nullptr : b->d_stats;
     a.row_grad = b->d_row_grad; a.row_grad_stride = b->row_grad_stride;
     a.grad = b->d_grad; a.ld_grad = b->ld_grad;
-    a.work = (float*)b->d_work;
     const int prev = zs_device_guard_begin(ctx);
     rc = ds_launch(a, b->dtype, what, (hipStream_t)stream);
     zs_device_guard_end(ctx, prev);

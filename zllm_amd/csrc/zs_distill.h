@@ -1,7 +1,14 @@
-// zs_distill.h -- kernel arguments of distillation from a teacher's list.
+// zs_distill.h -- kernel arguments of distillation from a teacher's list and the
+// layout of their scratch.
 #pragma once
 #include <hip/hip_runtime.h>
-#include "zs_internal.h"
+#include "zs_head_args.h"
+
+// What the gradient of a row goes by: y = e * (in the list ? fi : fo) + e1 * f1
+// - fp * p - fc * [the label], e = 2^(x c - mc), e1 the same at T = 1.
+struct ds_coef {
+    float m, mc, m1, fi, fo, f1, fp, fc;
+};
 
 struct ds_args {
     const void* logits;
@@ -22,14 +29,26 @@ struct ds_args {
     uint64_t row_grad_stride;
     void* grad;
     uint64_t ld_grad;
-    float* work;             // records
+    // scratch
+    uint32_t chunks, recs;   // workgroups and records a row
+    float4* rec;             // [N][recs] per wave: maximum, sums at T and at 1, the first outside the list
+    ds_coef* coef;           // [N]
+    float* p;                // [N][K] probabilities of the list, 0 for absent entries
 };
 #define DS_LOSS 1
 #define DS_GRAD 2
 int ds_launch(const ds_args& a, uint32_t dtype, int what, hipStream_t stream);
-// The scratch of N rows.
-inline uint64_t ds_work_bytes(uint64_t N, uint32_t V) {
-    (void)N;
-    (void)V;
-    return 0;
+
+// Chunks are counted from the 16-byte boundary at or below the row (7 values more).
+inline uint64_t ds_work(ds_args& a, void* work) {
+    char* p = (char*)work;
+    a.chunks = (a.V + 7u + HD_CHUNK - 1u) / HD_CHUNK;
+    a.recs = a.chunks * (HD_CHUNK / HD_WAVE);
+    a.rec = (float4*)p;
+    p += hd_pad(a.N * a.recs * sizeof(float4));
+    a.coef = (ds_coef*)p;
+    p += hd_pad(a.N * sizeof(ds_coef));
+    a.p = (float*)p;
+    p += hd_pad(a.N * a.K * sizeof(float));
+    return (uint64_t)(p - (char*)work);
 }

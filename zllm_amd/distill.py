@@ -101,7 +101,7 @@ def _grad_args(what, a, logits, row_grad, out):
 
 def _call(ctx, fn, what, a, dev):
     need = C.c_uint64()
-    _check(ctx.h, lib().zs_distill_work(a.N, a.V, C.byref(need)), "zs_distill_work")
+    _check(ctx.h, lib().zs_distill_work(a.N, a.V, a.K, C.byref(need)), "zs_distill_work")
     work = _work(need.value, dev)
     if work is not None:
         a.d_work, a.work_bytes = work.data_ptr(), need.value
