@@ -462,7 +462,7 @@ int zs_beam_select(zs_ctx* ctx, const zs_beam* args, void* stream);
  * array is n_outer * n_inner blocks of `bytes` bytes, block (o, i) of row r
  * at base + o * outer_stride + r * row_stride + i * inner_stride (bytes);
  * blocks of different rows, or of different arrays, must not overlap. */
-#define ZS_REORDER_BATCH 48
+#define ZS_REORDER_BATCH 40
 typedef struct zs_beam_state {
     void* d_base;
     uint64_t row_stride, outer_stride, inner_stride, bytes;

@@ -14,6 +14,10 @@
 
 #define DS_NT 256
 #define DS_K ZS_DISTILL_KMAX
+#ifndef DS_FUSED_ROWS
+#define DS_FUSED_ROWS 512
+#endif
+#define DS_FUSED_LDS 49152
 
 // A row that takes no part: its label is ignore_index.
 __device__ __forceinline__ bool ds_skip(const ds_args& a, uint64_t r) { return a.labels && zs_gload(a.labels + r) == a.ignore; }
@@ -26,7 +30,7 @@ __device__ __forceinline__ void ds_load(const hd_row<DT>& row, uint32_t first, f
     if (row.inside(first) && row.inside(first + U * DS_NT - 1u)) {
         uint4 v[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) v[u] = row.load(j0 + (uint32_t)u * DS_NT);
+        for (int u = 0; u < U; u++) v[u] = row.once(j0 + (uint32_t)u * DS_NT);
 #pragma unroll
         for (int u = 0; u < U; u++) hd_unpack<DT>(v[u], x[u]);
     } else {
@@ -117,6 +121,70 @@ __global__ __launch_bounds__(DS_NT) void zs_k_distill_scan(ds_args a, uint64_t r
 // ---------------------------------------------------------------------------
 // a row's end: the list's probabilities, the loss, the gradient's factors
 // ---------------------------------------------------------------------------
+// The list of a row, an entry a thread (t < K), and its probabilities.
+struct ds_entry {
+    uint32_t id;
+    bool there;
+    double p;       // normalised without the tail
+    double pt, P;   // the tail's, and of all outcomes (the same on every thread)
+};
+template <int NT>
+__device__ __forceinline__ ds_entry ds_list(const ds_args& a, uint64_t r, double* shd) {
+    ds_entry o;
+    o.id = 0xffffffffu;
+    o.there = false;
+    o.p = 0.0;
+    if (threadIdx.x < a.K) {
+        o.id = a.ids[r * a.K + threadIdx.x];
+        const float lk = a.logp[r * a.K + threadIdx.x];
+        o.there = o.id < a.V && lk != -INFINITY;
+        if (o.there) o.p = exp((double)lk);
+    }
+    const double psum = block_sum_d<NT>(o.p, shd);
+    o.pt = a.tail ? fmax(1.0 - psum, 0.0) : 0.0;
+    if (!a.tail && psum > 0.0) o.p /= psum;
+    o.P = a.tail ? psum + o.pt : (psum > 0.0 ? 1.0 : psum);
+    return o;
+}
+// The row's loss (and what the backward pass needs) from its maximum and
+// sums; xk: the entry's logit. Called by every thread.
+template <int NT>
+__device__ __forceinline__ void ds_loss(const ds_args& a, uint64_t r, const ds_entry& l, float xk, int64_t label, float xl,
+                                        double m, double S, double S1, double So, double* shd) {
+    double term = 0.0;
+    if (l.there && l.p != 0.0) term = l.p * (log(l.p) - (((double)xk - m) * a.inv_t - log(S)));   // (NaN stays)
+    term = block_sum_d<NT>(term, shd);
+    if (threadIdx.x) return;
+    if (l.pt > 0.0) term += l.pt * (log(l.pt) - (log(So) - log(S)));
+    double loss = (double)a.kl * term;
+    if (a.labels) loss += (double)a.ce * (log(S1) - ((double)xl - m));
+    a.loss[r] = (float)loss;
+    if (a.stats) *reinterpret_cast<float4*>(a.stats + r * 4) = make_float4((float)m, (float)S, (float)S1, (float)So);
+}
+// The gradient's factors.
+__device__ __forceinline__ ds_coef ds_factors(const ds_args& a, uint64_t r, const ds_entry& l, bool bad_label, double m, double S,
+                                              double S1, double So) {
+    const double g = bad_label ? (double)NAN : (double)a.row_grad[r * a.row_grad_stride];
+    const double kl = g * a.kl * a.inv_t, ce = a.labels ? g * a.ce : 0.0;
+    const float mf = (float)m, c1 = (float)HD_LOG2E;
+    // e = 2^(x c - mc) has mc's rounding for a factor (none where mc is no number: differences are taken)
+    const float mc = mf * a.c, m1 = mf * c1;
+    const double f = fabsf(mc) < INFINITY ? exp2(-(double)fmaf(mf, a.c, -mc)) : 1.0;
+    const double f1 = fabsf(m1) < INFINITY ? exp2(-(double)fmaf(mf, c1, -m1)) : 1.0;
+    const double one = a.labels ? ce / S1 : 0.0;
+    const double in = kl * l.P / S + (a.two ? 0.0 : one);
+    ds_coef k;
+    k.m = mf;
+    k.mc = mc;
+    k.m1 = m1;
+    k.fi = (float)(in * f);
+    k.fo = (float)((in - (a.tail && So > 0.0 ? kl * l.pt / So : 0.0)) * f);
+    k.f1 = (float)(one * f1);
+    k.fp = (float)kl;
+    k.fc = (float)ce;
+    return k;
+}
+
 #define DF_NT 128   // a thread for every entry of the list
 template <int DT, int WHAT>
 __global__ __launch_bounds__(DF_NT) void zs_k_distill_row(ds_args a, uint64_t r0) {
@@ -132,21 +200,10 @@ __global__ __launch_bounds__(DF_NT) void zs_k_distill_row(ds_args a, uint64_t r0
     }
     const hd_row<DT> row(a.logits, a.ld, r, a.V);
     const bool bad_label = a.labels && (label < 0 || label >= (int64_t)a.V);
-    double p = 0.0;
-    bool there = false;
-    float xk = 0.0f, xl = NAN;
-    if (t < a.K) {
-        const uint32_t id = a.ids[r * a.K + t];
-        const float lk = a.logp[r * a.K + t];
-        there = id < a.V && lk != -INFINITY;
-        if (there) {
-            p = exp((double)lk);
-            if (WHAT & DS_LOSS) xk = row.at(id);
-        }
-    }
-    if ((WHAT & DS_LOSS) && a.labels && !bad_label) xl = row.at((uint32_t)label);
+    const ds_entry l = ds_list<DF_NT>(a, r, shd);
     double m, S, S1, So;
     if (WHAT & DS_LOSS) {
+        const float xk = l.there ? row.at(l.id) : 0.0f, xl = a.labels && !bad_label ? row.at((uint32_t)label) : NAN;
         constexpr int E = hd_elem<DT>::E;
         const uint32_t recs = (row.nvec * E + HD_CHUNK - 1u) / HD_CHUNK * (HD_CHUNK / HD_WAVE);
         const float4* rec = a.rec + r * a.recs;
@@ -165,6 +222,7 @@ __global__ __launch_bounds__(DF_NT) void zs_k_distill_row(ds_args a, uint64_t r0
         if (!(m > -INFINITY)) S = NAN;   // a row of nothing has no distribution
         S1 = a.two ? block_sum_d<DF_NT>(S1, shd) : S;
         So = a.tail ? block_sum_d<DF_NT>(So, shd) : 0.0;
+        ds_loss<DF_NT>(a, r, l, xk, label, xl, m, S, S1, So, shd);
     } else {
         const float4 st = *reinterpret_cast<const float4*>(a.stats + r * 4);
         m = st.x;
@@ -172,45 +230,9 @@ __global__ __launch_bounds__(DF_NT) void zs_k_distill_row(ds_args a, uint64_t r0
         S1 = st.z;
         So = st.w;
     }
-    const double psum = block_sum_d<DF_NT>(p, shd);
-    const double pt = a.tail ? fmax(1.0 - psum, 0.0) : 0.0;
-    if (!a.tail && psum > 0.0) p /= psum;
-    const double P = a.tail ? psum + pt : (psum > 0.0 ? 1.0 : psum);
-    if (WHAT & DS_LOSS) {
-        double term = 0.0;
-        if (there && p != 0.0) term = p * (log(p) - (((double)xk - m) * a.inv_t - log(S)));   // (NaN stays)
-        term = block_sum_d<DF_NT>(term, shd);
-        if (t == 0) {
-            if (pt > 0.0) term += pt * (log(pt) - (log(So) - log(S)));
-            double loss = (double)a.kl * term;
-            if (a.labels) loss += (double)a.ce * (log(S1) - ((double)xl - m));
-            a.loss[r] = (float)loss;
-            if (a.stats) *reinterpret_cast<float4*>(a.stats + r * 4) = make_float4((float)m, (float)S, (float)S1, (float)So);
-        }
-    }
     if (WHAT & DS_GRAD) {
-        if (t < a.K) a.p[r * a.K + t] = (float)p;
-        if (t == 0) {
-            const double g = bad_label ? (double)NAN : (double)a.row_grad[r * a.row_grad_stride];
-            const double kl = g * a.kl * a.inv_t, ce = a.labels ? g * a.ce : 0.0;
-            const float mf = (float)m, c1 = (float)HD_LOG2E;
-            // e = 2^(x c - mc) has mc's rounding for a factor (none where mc is no number: differences are taken)
-            const float mc = mf * a.c, m1 = mf * c1;
-            const double f = fabsf(mc) < INFINITY ? exp2(-(double)fmaf(mf, a.c, -mc)) : 1.0;
-            const double f1 = fabsf(m1) < INFINITY ? exp2(-(double)fmaf(mf, c1, -m1)) : 1.0;
-            const double one = a.labels ? ce / S1 : 0.0;
-            const double in = kl * P / S + (a.two ? 0.0 : one);
-            ds_coef k;
-            k.m = mf;
-            k.mc = mc;
-            k.m1 = m1;
-            k.fi = (float)(in * f);
-            k.fo = (float)((in - (a.tail && So > 0.0 ? kl * pt / So : 0.0)) * f);
-            k.f1 = (float)(one * f1);
-            k.fp = (float)kl;
-            k.fc = (float)ce;
-            a.coef[r] = k;
-        }
+        if (t < a.K) a.p[r * a.K + t] = (float)l.p;
+        if (t == 0) a.coef[r] = ds_factors(a, r, l, bad_label, m, S, S1, So);
     }
 }
 
@@ -222,6 +244,29 @@ __device__ __forceinline__ void ds_store1(void* p, float y) {
     if constexpr (DT == ZS_F32) *(float*)p = y;
     else *(uint16_t*)p = (uint16_t)hd_pack2<DT>(y, 0.0f);
 }
+// e and e1 (times its factor) of one value
+template <bool TWO>
+__device__ __forceinline__ void ds_exps(const ds_args& a, const ds_coef& k, bool diff, bool diff1, float x, float& e, float& e1) {
+    const float c1 = (float)HD_LOG2E;
+    e = __builtin_amdgcn_exp2f(diff ? (x - k.m) * a.c : fmaf(x, a.c, -k.mc));
+    e1 = TWO ? __builtin_amdgcn_exp2f(diff1 ? (x - k.m) * c1 : fmaf(x, c1, -k.m1)) * k.f1 : 0.0f;
+}
+// A vector of the gradient to ids i0 .. i0 + E - 1 of the row.
+template <int DT>
+__device__ __forceinline__ void ds_store(typename hd_elem<DT>::T* grad, uint32_t V, bool whole, int i0, const float (&y)[hd_elem<DT>::E]) {
+    constexpr int E = hd_elem<DT>::E;
+    if (whole) {
+        uint4 v;
+        if constexpr (DT == ZS_F32) v = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+        else v = make_uint4(hd_pack2<DT>(y[0], y[1]), hd_pack2<DT>(y[2], y[3]), hd_pack2<DT>(y[E / 2], y[E / 2 + 1]), hd_pack2<DT>(y[E - 2], y[E - 1]));
+        *reinterpret_cast<uint4*>(grad + i0) = v;
+    } else {
+#pragma unroll
+        for (int q = 0; q < E; q++)
+            if ((uint32_t)(i0 + q) < V) ds_store1<DT>(grad + i0 + q, y[q]);
+    }
+}
+
 template <int DT, bool TWO>
 __global__ __launch_bounds__(DS_NT) void zs_k_distill_grad(ds_args a, uint64_t r0) {
     constexpr int E = hd_elem<DT>::E, U = HD_WAVE / 64 / E;
@@ -275,11 +320,7 @@ __global__ __launch_bounds__(DS_NT) void zs_k_distill_grad(ds_args a, uint64_t r
         for (int u = 0; u < U; u++) {
             float e[E], e1[E];
 #pragma unroll
-            for (int q = 0; q < E; q++) {
-                e[q] = __builtin_amdgcn_exp2f(diff ? (x[u][q] - k.m) * a.c : fmaf(x[u][q], a.c, -k.mc));
-                const float c1 = (float)HD_LOG2E;
-                e1[q] = TWO ? __builtin_amdgcn_exp2f(diff1 ? (x[u][q] - k.m) * c1 : fmaf(x[u][q], c1, -k.m1)) * k.f1 : 0.0f;
-            }
+            for (int q = 0; q < E; q++) ds_exps<TWO>(a, k, diff, diff1, x[u][q], e[q], e1[q]);
             if (reinterpret_cast<const uint8_t*>(mask)[u * DS_NT + t]) {
                 const int i0 = row.id0(first + t + (uint32_t)u * DS_NT);
                 uint32_t in = 0;
@@ -309,16 +350,212 @@ __global__ __launch_bounds__(DS_NT) void zs_k_distill_grad(ds_args a, uint64_t r
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const uint32_t j = first + t + (uint32_t)u * DS_NT;
-        const int i0 = row.id0(j);
-        if (aligned && row.inside(j)) {
-            uint4 v;
-            if constexpr (DT == ZS_F32) v = make_uint4(__float_as_uint(x[u][0]), __float_as_uint(x[u][1]), __float_as_uint(x[u][2]), __float_as_uint(x[u][3]));
-            else v = make_uint4(hd_pack2<DT>(x[u][0], x[u][1]), hd_pack2<DT>(x[u][2], x[u][3]), hd_pack2<DT>(x[u][E / 2], x[u][E / 2 + 1]), hd_pack2<DT>(x[u][E - 2], x[u][E - 1]));
-            *reinterpret_cast<uint4*>(grad + i0) = v;
+        ds_store<DT>(grad, a.V, aligned && row.inside(j), row.id0(j), x[u]);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// loss and gradient by one workgroup a row
+// ---------------------------------------------------------------------------
+#define FU_NT 512
+#define FU_HASH 256
+__device__ __forceinline__ uint32_t fu_slot(uint32_t id) { return id * 2654435761u >> 24; }
+
+// The row is read twice by the workgroup that holds it, the second time from
+// its end backwards: what was read last is in the L2 still, the rest in the
+// memory-side cache.
+template <int DT, bool TAIL, bool TWO>
+__global__ __launch_bounds__(FU_NT, 4) void zs_k_distill_fused(ds_args a, uint64_t r0) {
+    constexpr int E = hd_elem<DT>::E, U = 4, BV = U * FU_NT;   // vectors of a batch
+    typedef typename hd_elem<DT>::T T;
+    extern __shared__ uint32_t mask[];   // a byte a vector: its ids in the list (then the label's too)
+    __shared__ uint32_t hid[FU_HASH], lid[DS_K], dup;
+    __shared__ float hp[FU_HASH], lp[DS_K], shf[FU_NT / 64];
+    __shared__ double shd[FU_NT / 64];
+    __shared__ ds_coef coef;
+    const uint64_t r = r0 + blockIdx.x;
+    const uint32_t t = threadIdx.x;
+    const hd_row<DT> row(a.logits, a.ld, r, a.V);
+    T* grad = reinterpret_cast<T*>(a.grad) + r * a.ld_grad;
+    const bool aligned = (((uintptr_t)grad ^ (uintptr_t)row.row) & 15u) == 0;
+    const int64_t label = a.labels ? a.labels[r] : -1;
+    if (a.labels && label == a.ignore) {
+        if (t == 0) a.loss[r] = 0.0f;
+        const float zero[E] = {};
+        for (uint32_t j = t; j < row.nvec; j += FU_NT) ds_store<DT>(grad, a.V, aligned && row.inside(j), row.id0(j), zero);
+        return;
+    }
+    const bool bad_label = a.labels && (label < 0 || label >= (int64_t)a.V);
+    const uint32_t nb = (row.nvec + BV - 1u) / BV;
+    auto fetch = [&](uint32_t b, uint4 (&v)[U]) {
+        const uint32_t first = b * BV, j = first + t;
+        if (row.inside(first) && row.inside(first + BV - 1u)) {
+#pragma unroll
+            for (int u = 0; u < U; u++) v[u] = row.load(j + (uint32_t)u * FU_NT);
         } else {
 #pragma unroll
-            for (int q = 0; q < E; q++)
-                if (i0 + q >= 0 && (uint32_t)(i0 + q) < a.V) ds_store1<DT>(grad + i0 + q, x[u][q]);
+            for (int u = 0; u < U; u++) v[u] = row.raw(j + (uint32_t)u * FU_NT);
+        }
+    };
+    uint4 cur[U], nxt[U];
+    fetch(0, cur);
+    // the list: a byte a vector that holds entries, the entries by their ids
+    for (uint32_t i = t; i < (row.nvec + 3u) / 4u; i += FU_NT) mask[i] = 0;
+    if (t < FU_HASH) hid[t] = 0xffffffffu;
+    if (t == 0) dup = 0;
+    const ds_entry l = ds_list<FU_NT>(a, r, shd);   // (its barriers order the clearing)
+    const float xk = l.there ? row.at(l.id) : 0.0f, xl = a.labels && !bad_label ? row.at((uint32_t)label) : NAN;
+    uint32_t slot = FU_HASH;
+    if (t < a.K) {
+        lid[t] = l.there ? l.id : 0xffffffffu;
+        lp[t] = (float)l.p;
+    }
+    if (l.there) {
+        const uint32_t pos = l.id + row.shift, j = pos / E;
+        atomicOr(&mask[j / 4], 1u << (j % 4 * 8 + pos % E));
+        for (uint32_t s = fu_slot(l.id);; s = (s + 1u) % FU_HASH) {   // (half the slots stay free)
+            const uint32_t was = atomicCAS(&hid[s], 0xffffffffu, l.id);
+            if (was == 0xffffffffu) { slot = s; break; }
+            if (was == l.id) { dup = 1; break; }
+        }
+    }
+    __syncthreads();
+    if (slot < FU_HASH) {
+        float p = lp[t];
+        if (dup) {
+            p = 0.0f;
+            for (uint32_t k = 0; k < a.K; k++) p += lid[k] == l.id ? lp[k] : 0.0f;
+        }
+        hp[slot] = p;
+    }
+    const uint8_t* in_list = reinterpret_cast<const uint8_t*>(mask);
+    // first pass: a maximum and sums per thread, relative to 2^ref
+    const float c1 = (float)HD_LOG2E;
+    float m = -INFINITY, s = 0.0f, so = 0.0f, s1 = 0.0f;
+    for (uint32_t b = 0; b < nb; b++) {
+        if (b + 1u < nb) fetch(b + 1u, nxt);
+        float x[U][E], bm = m;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            hd_unpack<DT>(cur[u], x[u]);
+#pragma unroll
+            for (int q = 0; q < E; q++) bm = fmaxf(bm, x[u][q]);
+        }
+        const float mr = bm > -INFINITY ? bm : 0.0f, ref = mr * a.c, ref1 = mr * c1;
+        if (bm > m) {
+            const float f = m > -INFINITY ? __builtin_amdgcn_exp2f(m * a.c - ref) : 0.0f;
+            s *= f;
+            if (TAIL) so *= f;
+            if (TWO) s1 *= m > -INFINITY ? __builtin_amdgcn_exp2f(m * c1 - ref1) : 0.0f;
+            m = bm;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float e[E];
+            const uint32_t j = b * BV + t + (uint32_t)u * FU_NT;
+            if (TWO) {
+#pragma unroll
+                for (int q = 0; q < E; q++) e[q] = __builtin_amdgcn_exp2f(fmaf(x[u][q], c1, -ref1));
+                s1 += hd_sum(e);
+            }
+#pragma unroll
+            for (int q = 0; q < E; q++) e[q] = __builtin_amdgcn_exp2f(fmaf(x[u][q], a.c, -ref));
+            const float v = hd_sum(e);
+            s += v;
+            if (TAIL) {
+                const uint32_t in = j < row.nvec ? in_list[j] : 0u;
+                if (in) {
+#pragma unroll
+                    for (int q = 0; q < E; q++) e[q] = in >> q & 1u ? 0.0f : e[q];
+                    so += hd_sum(e);
+                } else {
+                    so += v;
+                }
+            }
+        }
+        if (b + 1u < nb) {
+#pragma unroll
+            for (int u = 0; u < U; u++) cur[u] = nxt[u];
+        }
+    }
+    const float M = block_max_f<FU_NT>(m, shf);
+    double S, S1, So;
+    const float Mr = M > -INFINITY ? M : 0.0f;
+    auto total = [&](float v, float c) {   // of sums relative to 2^(m c), to 2^(M c)
+        const float f = m > -INFINITY ? __builtin_amdgcn_exp2f(m * c - Mr * c) : 0.0f;
+        return block_sum_d<FU_NT>((double)(v * f), shd) * exp2(-(double)fmaf(Mr, c, -(Mr * c)));
+    };
+    if (fabsf(Mr * a.c) < INFINITY && fabsf(Mr * c1) < INFINITY) {
+        S = total(s, a.c);
+        S1 = TWO ? total(s1, c1) : S;
+        So = TAIL ? total(so, a.c) : 0.0;
+    } else {
+        // a maximum whose exponent no float holds: by differences, once more
+        double d = 0.0, d1 = 0.0, dout = 0.0;
+        for (uint32_t j = t; j < row.nvec; j += FU_NT) {
+            float x[E];
+            row.get(j, x, -INFINITY);
+#pragma unroll
+            for (int q = 0; q < E; q++) {
+                const float e = __builtin_amdgcn_exp2f((x[q] - M) * a.c);
+                d += e;
+                if (TWO) d1 += __builtin_amdgcn_exp2f((x[q] - M) * c1);
+                if (TAIL && !(in_list[j] >> q & 1u)) dout += e;
+            }
+        }
+        S = block_sum_d<FU_NT>(d, shd);
+        S1 = TWO ? block_sum_d<FU_NT>(d1, shd) : S;
+        So = TAIL ? block_sum_d<FU_NT>(dout, shd) : 0.0;
+    }
+    if (!(M > -INFINITY)) S = S1 = NAN;   // a row of nothing has no distribution
+    ds_loss<FU_NT>(a, r, l, xk, label, xl, (double)M, S, S1, So, shd);
+    if (t == 0) {
+        coef = ds_factors(a, r, l, bad_label, (double)M, S, S1, So);
+        if (label >= 0 && !bad_label) {
+            const uint32_t pos = (uint32_t)label + row.shift, j = pos / E;
+            mask[j / 4] |= 1u << (j % 4 * 8 + pos % E);
+        }
+    }
+    __syncthreads();
+    // second pass, from the batch at hand backwards
+    const ds_coef k = coef;
+    const bool diff = !(fabsf(k.mc) < INFINITY), diff1 = !(fabsf(k.m1) < INFINITY);
+    for (uint32_t b = nb; b-- > 0;) {
+        if (b) fetch(b - 1u, nxt);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t j = b * BV + t + (uint32_t)u * FU_NT;
+            float x[E], e[E], e1[E];
+            hd_unpack<DT>(cur[u], x);
+#pragma unroll
+            for (int q = 0; q < E; q++) ds_exps<TWO>(a, k, diff, diff1, x[q], e[q], e1[q]);
+            const int i0 = row.id0(j);
+            uint32_t in = j < row.nvec ? in_list[j] : 0u;
+            if (in) {
+#pragma unroll
+                for (int q = 0; q < E; q++) {
+                    const uint32_t id = (uint32_t)(i0 + q);
+                    float f = k.fo, sub = 0.0f;
+                    if (in >> q & 1u) {
+                        if ((int64_t)id == label) sub = k.fc;
+                        for (uint32_t h = fu_slot(id); hid[h] != 0xffffffffu; h = (h + 1u) % FU_HASH)
+                            if (hid[h] == id) {
+                                f = k.fi;
+                                sub += k.fp * hp[h];
+                                break;
+                            }
+                    }
+                    x[q] = e[q] * f + (e1[q] - sub);
+                }
+            } else {
+#pragma unroll
+                for (int q = 0; q < E; q++) x[q] = TWO ? e[q] * k.fo + e1[q] : e[q] * k.fo;
+            }
+            if (j < row.nvec) ds_store<DT>(grad, a.V, aligned && row.inside(j), i0, x);
+        }
+        if (b) {
+#pragma unroll
+            for (int u = 0; u < U; u++) cur[u] = nxt[u];
         }
     }
 }
@@ -326,6 +563,14 @@ __global__ __launch_bounds__(DS_NT) void zs_k_distill_grad(ds_args a, uint64_t r
 template <int DT>
 static void ds_go(const ds_args& a, int what, uint64_t r0, uint32_t n, hipStream_t stream) {
     const dim3 grid(n * a.chunks), wg(DS_NT);
+    const uint32_t lds = (a.V + 7u) / hd_elem<DT>::E + 4u & ~3u;   // a byte a vector
+    if (what == (DS_LOSS | DS_GRAD) && a.N >= DS_FUSED_ROWS && lds <= DS_FUSED_LDS) {
+        if (a.tail && a.two) hipLaunchKernelGGL((zs_k_distill_fused<DT, true, true>), dim3(n), dim3(FU_NT), lds, stream, a, r0);
+        else if (a.tail) hipLaunchKernelGGL((zs_k_distill_fused<DT, true, false>), dim3(n), dim3(FU_NT), lds, stream, a, r0);
+        else if (a.two) hipLaunchKernelGGL((zs_k_distill_fused<DT, false, true>), dim3(n), dim3(FU_NT), lds, stream, a, r0);
+        else hipLaunchKernelGGL((zs_k_distill_fused<DT, false, false>), dim3(n), dim3(FU_NT), lds, stream, a, r0);
+        return;
+    }
     if (what & DS_LOSS) {
         if (a.tail && a.two) hipLaunchKernelGGL((zs_k_distill_scan<DT, true, true>), grid, wg, 0, stream, a, r0);
         else if (a.tail) hipLaunchKernelGGL((zs_k_distill_scan<DT, true, false>), grid, wg, 0, stream, a, r0);

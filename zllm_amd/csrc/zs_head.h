@@ -67,7 +67,32 @@ struct hd_row {
     }
     __device__ __forceinline__ int id0(uint32_t j) const { return (int)(j * E) - (int)shift; }
     __device__ __forceinline__ bool inside(uint32_t j) const { const int i = id0(j); return i >= 0 && (uint32_t)i + E <= V; }
+    // one that is not read again (7.2 TB/s of a large read where plain loads reach 6.5)
+    __device__ __forceinline__ uint4 once(uint32_t j) const {
+        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+        const u4 v = __builtin_nontemporal_load((const __attribute__((address_space(1))) u4*)(row + id0(j)));
+        return make_uint4(v.x, v.y, v.z, v.w);
+    }
     __device__ __forceinline__ uint4 load(uint32_t j) const { return zs_gload(reinterpret_cast<const uint4*>(row + id0(j))); }
+    // the vector as it stands, -inf where it has no id of the row
+    __device__ __forceinline__ uint4 raw(uint32_t j) const {
+        if (inside(j)) return load(j);
+        uint32_t w[4];
+        const int i = id0(j);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if constexpr (DT == ZS_F32) {
+                w[k] = (uint32_t)(i + k) < V ? __float_as_uint(row[i + k]) : 0xff800000u;
+            } else {
+                constexpr uint32_t none = DT == ZS_F16 ? 0xfc00u : 0xff80u;
+                const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
+                const uint32_t lo = (uint32_t)(i + 2 * k) < V ? p[i + 2 * k] : none;
+                const uint32_t hi = (uint32_t)(i + 2 * k + 1) < V ? p[i + 2 * k + 1] : none;
+                w[k] = lo | hi << 16;
+            }
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
     __device__ __forceinline__ float at(uint32_t id) const { return hd_float(zs_gload(row + id)); }
     // the vector's values; `none` where it has no id of the row
     __device__ __forceinline__ void get(uint32_t j, float (&x)[E], float none) const {

@@ -39,7 +39,7 @@ __global__ __launch_bounds__(HS_NT) void zs_k_head_scan(hd_args a, uint64_t r0) 
     if (row.inside(first) && row.inside(first + U * HS_NT - 1u)) {
         uint4 v[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) v[u] = row.load(j0 + (uint32_t)u * HS_NT);
+        for (int u = 0; u < U; u++) v[u] = row.once(j0 + (uint32_t)u * HS_NT);
 #pragma unroll
         for (int u = 0; u < U; u++) hd_unpack<DT>(v[u], x[u]);
     } else {
@@ -185,14 +185,21 @@ __global__ __launch_bounds__(HP_NT) void zs_k_head_pick(hd_args a, uint64_t r0, 
     if (wid == NW - 1u) {   // ln sum exp(x / T) of the row
         const uint32_t recs = (row.nvec * E + HD_CHUNK - 1u) / HD_CHUNK * (HD_CHUNK / HD_WAVE);
         const float2* rec = a.rec + r * a.recs;
-        float m = -INFINITY;
-        for (uint32_t i = lane; i < recs; i += 64u) m = fmaxf(m, rec[i].x);
+        // (two a lane at once: rows of 262144 ids; longer ones take turns)
+        float2 v[2];
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+            const uint32_t i = lane + 64u * (uint32_t)w;
+            v[w] = i < recs ? rec[i] : make_float2(-INFINITY, 0.0f);
+        }
+        float m = fmaxf(v[0].x, v[1].x);
+        for (uint32_t i = lane + 128u; i < recs; i += 64u) m = fmaxf(m, rec[i].x);
         m = wave_max_f(m);
         double s = 0.0;
-        for (uint32_t i = lane; i < recs; i += 64u) {
-            const float2 v = rec[i];
-            if (v.x > -INFINITY) s += (double)v.y * exp(((double)v.x - (double)m) * a.inv_t);
-        }
+        auto add = [&](float2 o) { if (o.x > -INFINITY) s += (double)o.y * exp(((double)o.x - (double)m) * a.inv_t); };
+        add(v[0]);
+        add(v[1]);
+        for (uint32_t i = lane + 128u; i < recs; i += 64u) add(rec[i]);
         s = wave_sum_d(s);
         if (lane == 0) lse_s = hd_lse(m, a.inv_t, s);
     }
@@ -336,7 +343,23 @@ __global__ __launch_bounds__(HP_NT) void zs_k_head_pick(hd_args a, uint64_t r0, 
         __syncthreads();
     }
     static_assert(ZS_TEACHER_KMAX * 8 <= HP_LIST && ZS_TEACHER_KMAX <= HP_GL, "the first K groups and their vectors' values fit");
-    uint32_t np2 = 64;
+    if (n <= 128u) {
+        // an entry's place is the number of entries in front of it
+        if (t >= 128u) return;
+        const unsigned long long e = t < n ? list[t] : ~0ull;
+        uint32_t place = 0, i = 0;
+        for (; i + 4u <= n; i += 4u) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) place += list[i + (uint32_t)q] < e ? 1u : 0u;
+        }
+        for (; i < n; i++) place += list[i] < e ? 1u : 0u;
+        // entries of no candidate (~0 all) lie behind the others as they stand
+        if (e == ~0ull && t < n)
+            for (i = 0; i < t; i++) place += list[i] == ~0ull ? 1u : 0u;
+        hd_put(a, r, t < n ? place : t, e, lse_s);
+        return;
+    }
+    uint32_t np2 = 256;
     while (np2 < n) np2 <<= 1;
     for (uint32_t i = n + t; i < np2; i += HP_NT) list[i] = ~0ull;
     __syncthreads();
