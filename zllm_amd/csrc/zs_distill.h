@@ -5,9 +5,11 @@
 #include "zs_head_args.h"
 
 // What the gradient of a row goes by: y = e * (in the list ? fi : fo) + e1 * f1
-// - fp * p - fc * [the label], e = 2^(x c - mc), e1 the same at T = 1.
+// - fp * p - fc * [the label], e = 2^(x c - mc), e1 = 2^(x c1 - m1).
 struct ds_coef {
-    float m, mc, m1, fi, fo, f1, fp, fc;
+    float c, mc, c1, m1, fi, fo, f1, fp, fc;
+    uint32_t lone;   // the label, where the list does not have it (~0 else)
+    float pad[2];
 };
 
 struct ds_args {
@@ -33,7 +35,7 @@ struct ds_args {
     uint32_t chunks, recs;   // workgroups and records a row
     float4* rec;             // [N][recs] per wave: maximum, sums at T and at 1, the first outside the list
     ds_coef* coef;           // [N]
-    float* p;                // [N][K] probabilities of the list, 0 for absent entries
+    float* p;                // [N][K] probability of an entry's id (an id listed twice has both), -1 for absent entries
 };
 #define DS_LOSS 1
 #define DS_GRAD 2

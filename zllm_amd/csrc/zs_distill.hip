@@ -17,6 +17,7 @@
 #ifndef DS_FUSED_ROWS
 #define DS_FUSED_ROWS 512
 #endif
+#define DS_FUSED_VOCAB 4096
 #define DS_FUSED_LDS 49152
 
 // A row that takes no part: its label is ignore_index.
@@ -82,14 +83,14 @@ __global__ __launch_bounds__(DS_NT) void zs_k_distill_scan(ds_args a, uint64_t r
     const float mr = m > -INFINITY ? m : 0.0f;
     float s, s1 = 0.0f, so = 0.0f;
     // 2^(x c - mc): one fma a value; mc's rounding is a factor of all of them
-    auto sums = [&](float c, bool diff, float& s, float& so, bool list) {
-        const float mc = mr * c;
+    auto sums = [&](float c0, float& s, float& so, bool list) {
+        const float c = hd_factor(mr, c0), mc = mr * c;
         s = so = 0.0f;
 #pragma unroll
         for (int u = 0; u < U; u++) {
             float e[E];
 #pragma unroll
-            for (int q = 0; q < E; q++) e[q] = __builtin_amdgcn_exp2f(diff ? (x[u][q] - mr) * c : fmaf(x[u][q], c, -mc));
+            for (int q = 0; q < E; q++) e[q] = __builtin_amdgcn_exp2f(fmaf(x[u][q], c, -mc));
             const float v = hd_sum(e);
             s += v;
             if (TAIL && list) {
@@ -104,17 +105,13 @@ __global__ __launch_bounds__(DS_NT) void zs_k_distill_scan(ds_args a, uint64_t r
             }
         }
         const auto add = [](float p, float q) { return p + q; };
-        const float f = diff ? 1.0f : __builtin_amdgcn_exp2f(-fmaf(mr, c, -mc));
+        const float f = __builtin_amdgcn_exp2f(-fmaf(mr, c, -mc));
         s = zs_wave_reduce(s, add) * f;
         if (TAIL && list) so = zs_wave_reduce(so, add) * f;
     };
     float none;
-    if (fabsf(mr * a.c) < INFINITY) sums(a.c, false, s, so, true);
-    else sums(a.c, true, s, so, true);   // (an exponent that no float holds)
-    if (TWO) {
-        if (fabsf(mr * (float)HD_LOG2E) < INFINITY) sums((float)HD_LOG2E, false, s1, none, false);
-        else sums((float)HD_LOG2E, true, s1, none, false);
-    }
+    sums(a.c, s, so, true);
+    if (TWO) sums((float)HD_LOG2E, s1, none, false);
     if (zs_lane() == 0) a.rec[r * a.recs + chunk * (HD_CHUNK / HD_WAVE) + (uint32_t)zs_wid()] = make_float4(m, s, s1, so);
 }
 
@@ -146,6 +143,38 @@ __device__ __forceinline__ ds_entry ds_list(const ds_args& a, uint64_t r, double
     o.P = a.tail ? psum + o.pt : (psum > 0.0 ? 1.0 : psum);
     return o;
 }
+// The probability of the entry's id, of all entries that name it: what the
+// gradient takes off there. Called by every thread.
+#define DS_HASH 256   // twice the entries: a free slot is near
+struct ds_ids {
+    uint32_t slot[DS_HASH], ids[DS_K], dup;
+    float ps[DS_K];
+};
+template <int NT>
+__device__ __forceinline__ float ds_of_id(const ds_entry& l, uint32_t K, ds_ids& d) {
+    const uint32_t t = threadIdx.x;
+    for (uint32_t i = t; i < DS_HASH; i += NT) d.slot[i] = 0xffffffffu;
+    if (t == 0) d.dup = 0;
+    if (t < DS_K) {
+        d.ids[t] = l.there ? l.id : 0xffffffffu;
+        d.ps[t] = l.there ? (float)l.p : 0.0f;
+    }
+    __syncthreads();
+    if (l.there) {
+        for (uint32_t s = l.id * 2654435761u >> 24;; s = (s + 1u) % DS_HASH) {
+            const uint32_t was = atomicCAS(&d.slot[s], 0xffffffffu, l.id);
+            if (was == 0xffffffffu) break;
+            if (was == l.id) { d.dup = 1; break; }
+        }
+    }
+    __syncthreads();
+    float p = (float)l.p;
+    if (d.dup && l.there) {
+        p = 0.0f;
+        for (uint32_t k = 0; k < K; k++) p += d.ids[k] == l.id ? d.ps[k] : 0.0f;
+    }
+    return p;
+}
 // The row's loss (and what the backward pass needs) from its maximum and
 // sums; xk: the entry's logit. Called by every thread.
 template <int NT>
@@ -166,17 +195,16 @@ __device__ __forceinline__ ds_coef ds_factors(const ds_args& a, uint64_t r, cons
                                               double S1, double So) {
     const double g = bad_label ? (double)NAN : (double)a.row_grad[r * a.row_grad_stride];
     const double kl = g * a.kl * a.inv_t, ce = a.labels ? g * a.ce : 0.0;
-    const float mf = (float)m, c1 = (float)HD_LOG2E;
-    // e = 2^(x c - mc) has mc's rounding for a factor (none where mc is no number: differences are taken)
-    const float mc = mf * a.c, m1 = mf * c1;
-    const double f = fabsf(mc) < INFINITY ? exp2(-(double)fmaf(mf, a.c, -mc)) : 1.0;
-    const double f1 = fabsf(m1) < INFINITY ? exp2(-(double)fmaf(mf, c1, -m1)) : 1.0;
+    ds_coef k;
+    // e = 2^(x c - mc) has mc's rounding for a factor
+    const float mf = (float)m;
+    k.c = hd_factor(mf, a.c);
+    k.mc = mf * k.c;
+    k.c1 = hd_factor(mf, (float)HD_LOG2E);
+    k.m1 = mf * k.c1;
+    const double f = exp2(-(double)fmaf(mf, k.c, -k.mc)), f1 = exp2(-(double)fmaf(mf, k.c1, -k.m1));
     const double one = a.labels ? ce / S1 : 0.0;
     const double in = kl * l.P / S + (a.two ? 0.0 : one);
-    ds_coef k;
-    k.m = mf;
-    k.mc = mc;
-    k.m1 = m1;
     k.fi = (float)(in * f);
     k.fo = (float)((in - (a.tail && So > 0.0 ? kl * l.pt / So : 0.0)) * f);
     k.f1 = (float)(one * f1);
@@ -231,8 +259,15 @@ __global__ __launch_bounds__(DF_NT) void zs_k_distill_row(ds_args a, uint64_t r0
         So = st.w;
     }
     if (WHAT & DS_GRAD) {
-        if (t < a.K) a.p[r * a.K + t] = (float)l.p;
-        if (t == 0) a.coef[r] = ds_factors(a, r, l, bad_label, m, S, S1, So);
+        __shared__ ds_ids ids;
+        const float p = ds_of_id<DF_NT>(l, a.K, ids);
+        if (t < a.K) a.p[r * a.K + t] = l.there ? p : -1.0f;
+        const bool listed = __syncthreads_or(l.there && (int64_t)l.id == label);
+        if (t == 0) {
+            ds_coef k = ds_factors(a, r, l, bad_label, m, S, S1, So);
+            k.lone = label < 0 || bad_label || listed ? 0xffffffffu : (uint32_t)label;
+            a.coef[r] = k;
+        }
     }
 }
 
@@ -246,10 +281,9 @@ __device__ __forceinline__ void ds_store1(void* p, float y) {
 }
 // e and e1 (times its factor) of one value
 template <bool TWO>
-__device__ __forceinline__ void ds_exps(const ds_args& a, const ds_coef& k, bool diff, bool diff1, float x, float& e, float& e1) {
-    const float c1 = (float)HD_LOG2E;
-    e = __builtin_amdgcn_exp2f(diff ? (x - k.m) * a.c : fmaf(x, a.c, -k.mc));
-    e1 = TWO ? __builtin_amdgcn_exp2f(diff1 ? (x - k.m) * c1 : fmaf(x, c1, -k.m1)) * k.f1 : 0.0f;
+__device__ __forceinline__ void ds_exps(const ds_coef& k, float x, float& e, float& e1) {
+    e = __builtin_amdgcn_exp2f(fmaf(x, k.c, -k.mc));
+    e1 = TWO ? __builtin_amdgcn_exp2f(fmaf(x, k.c1, -k.m1)) * k.f1 : 0.0f;
 }
 // A vector of the gradient to ids i0 .. i0 + E - 1 of the row.
 template <int DT>
@@ -267,13 +301,24 @@ __device__ __forceinline__ void ds_store(typename hd_elem<DT>::T* grad, uint32_t
     }
 }
 
+// The gradient at an id of the list (p of it; fi) or at the label alone (fo).
+template <bool TWO>
+__device__ __forceinline__ float ds_at(const ds_coef& k, float x, bool listed, float p, bool label) {
+    float e, e1;
+    ds_exps<TWO>(k, x, e, e1);
+    return e * (listed ? k.fi : k.fo) + (e1 - ((listed ? k.fp * p : 0.0f) + (label ? k.fc : 0.0f)));
+}
+
+// Every id's gradient as one outside the list first; those of the list and the
+// label are written over it by the wave that wrote their vector, whose stores
+// arrive in order: no test per vector, and nothing is waited for.
 template <int DT, bool TWO>
 __global__ __launch_bounds__(DS_NT) void zs_k_distill_grad(ds_args a, uint64_t r0) {
     constexpr int E = hd_elem<DT>::E, U = HD_WAVE / 64 / E;
     typedef typename hd_elem<DT>::T T;
-    __shared__ uint32_t mask[U * DS_NT / 4];   // a byte a vector: its ids in the list, or the label
-    __shared__ uint32_t hid[DS_K], cnt[DS_K / 64];
-    __shared__ float hp[DS_K];
+    __shared__ uint32_t hid[DS_K + 1];
+    __shared__ float hy[DS_K + 1];
+    __shared__ uint32_t hits;
     const uint64_t r = r0 + blockIdx.x / a.chunks;
     const uint32_t chunk = blockIdx.x % a.chunks, t = threadIdx.x;
     const hd_row<DT> row(a.logits, a.ld, r, a.V);
@@ -281,66 +326,39 @@ __global__ __launch_bounds__(DS_NT) void zs_k_distill_grad(ds_args a, uint64_t r
     if (first >= row.nvec) return;
     T* grad = reinterpret_cast<T*>(a.grad) + r * a.ld_grad;
     const bool aligned = (((uintptr_t)grad ^ (uintptr_t)row.row) & 15u) == 0;
-    const bool skip = ds_skip(a, r);
-    const int64_t label = a.labels ? zs_gload(a.labels + r) : -1;
     float x[U][E];
+    const bool skip = ds_skip(a, r);
     if (!skip) {
+        const int64_t label = a.labels ? zs_gload(a.labels + r) : -1;
         uint32_t id = 0xffffffffu;
-        float p = 0.0f;
+        float p = -1.0f;
         if (t < a.K) {
             id = zs_gload(a.ids + r * a.K + t);
             p = zs_gload(a.p + r * a.K + t);
-            if (id < a.V && p == 0.0f && zs_gload(a.logp + r * a.K + t) == -INFINITY) id = 0xffffffffu;   // absent
         }
         const ds_coef k = a.coef[r];
         ds_load<DT, U>(row, first, x);
-#pragma unroll
-        for (int i = 0; i < U / 4; i++) mask[i * DS_NT + t] = 0;
-        // the chunk's entries, in the list's order
-        const uint32_t pos = id + row.shift, j = pos / E - first;
-        const bool hit = id < a.V && j < U * DS_NT;
-        const unsigned long long hm = __ballot(hit);
-        if (t < DS_K && zs_lane() == 0) cnt[zs_wid()] = (uint32_t)__popcll(hm);
+        if (t == 0) hits = 0;
+        // the chunk's entries (p is NaN where the list has one), and the label where they do not have it
+        const bool listed = t < a.K && p != -1.0f;
+        if (t == DS_K) id = k.lone;
+        const bool mine = (listed || t == DS_K) && id < a.V && (id + row.shift) / E - first < U * DS_NT;
+        const float xk = mine ? row.at(id) : 0.0f;
         __syncthreads();
-        if (hit) {
-            uint32_t at = zs_wid() ? cnt[0] : 0u;
-            at = __builtin_amdgcn_mbcnt_hi((uint32_t)(hm >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hm, at));
-            hid[at] = id;
-            hp[at] = k.fp * p;
-            atomicOr(&mask[j / 4], 1u << (j % 4 * 8 + pos % E));
-        }
-        if (t == DS_K && label >= 0 && label < (int64_t)a.V) {
-            const uint32_t lp = (uint32_t)label + row.shift, lj = lp / E - first;
-            if (lj < U * DS_NT) atomicOr(&mask[lj / 4], 1u << (lj % 4 * 8 + lp % E));
+        if (mine) {
+            const uint32_t h = atomicAdd(&hits, 1u);
+            hid[h] = id;
+            hy[h] = ds_at<TWO>(k, xk, listed, p, (int64_t)id == label);
         }
         __syncthreads();
-        const uint32_t hits = cnt[0] + cnt[1];
-        const bool diff = !(fabsf(k.mc) < INFINITY), diff1 = !(fabsf(k.m1) < INFINITY);
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            float e[E], e1[E];
+        for (int u = 0; u < U; u++)
 #pragma unroll
-            for (int q = 0; q < E; q++) ds_exps<TWO>(a, k, diff, diff1, x[u][q], e[q], e1[q]);
-            if (reinterpret_cast<const uint8_t*>(mask)[u * DS_NT + t]) {
-                const int i0 = row.id0(first + t + (uint32_t)u * DS_NT);
-                uint32_t in = 0;
-                float sub[E];
-#pragma unroll
-                for (int q = 0; q < E; q++) sub[q] = (int64_t)(i0 + q) == label ? k.fc : 0.0f;
-                for (uint32_t h = 0; h < hits; h++) {
-                    const int at = (int)hid[h] - i0;
-                    if (at < 0 || at >= E) continue;
-                    in |= 1u << at;
-#pragma unroll
-                    for (int q = 0; q < E; q++) sub[q] += q == at ? hp[h] : 0.0f;
-                }
-#pragma unroll
-                for (int q = 0; q < E; q++) x[u][q] = e[q] * (in >> q & 1u ? k.fi : k.fo) + (e1[q] - sub[q]);
-            } else {
-#pragma unroll
-                for (int q = 0; q < E; q++) x[u][q] = TWO ? e[q] * k.fo + e1[q] : e[q] * k.fo;
+            for (int q = 0; q < E; q++) {
+                float e, e1;
+                ds_exps<TWO>(k, x[u][q], e, e1);
+                x[u][q] = TWO ? e * k.fo + e1 : e * k.fo;
             }
-        }
     } else {
 #pragma unroll
         for (int u = 0; u < U; u++)
@@ -352,25 +370,28 @@ __global__ __launch_bounds__(DS_NT) void zs_k_distill_grad(ds_args a, uint64_t r
         const uint32_t j = first + t + (uint32_t)u * DS_NT;
         ds_store<DT>(grad, a.V, aligned && row.inside(j), row.id0(j), x[u]);
     }
+    if (skip) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (uint32_t h = (uint32_t)zs_lane(); h < hits; h += 64u)
+        if ((((hid[h] + row.shift) / E - first) % DS_NT >> 6) == (uint32_t)zs_wid()) ds_store1<DT>(grad + hid[h], hy[h]);
 }
 
 // ---------------------------------------------------------------------------
 // loss and gradient by one workgroup a row
 // ---------------------------------------------------------------------------
 #define FU_NT 512
-#define FU_HASH 256
-__device__ __forceinline__ uint32_t fu_slot(uint32_t id) { return id * 2654435761u >> 24; }
-
 // The row is read twice by the workgroup that holds it, the second time from
-// its end backwards: what was read last is in the L2 still, the rest in the
-// memory-side cache.
+// its end backwards. Loads run a batch ahead of their use; they are issued
+// without conditions (vectors at the row's ends are clamped to whole ones, the
+// ends themselves read apart), or the compiler waits for all of them at every
+// join of the branches.
 template <int DT, bool TAIL, bool TWO>
 __global__ __launch_bounds__(FU_NT, 4) void zs_k_distill_fused(ds_args a, uint64_t r0) {
     constexpr int E = hd_elem<DT>::E, U = 4, BV = U * FU_NT;   // vectors of a batch
     typedef typename hd_elem<DT>::T T;
-    extern __shared__ uint32_t mask[];   // a byte a vector: its ids in the list (then the label's too)
-    __shared__ uint32_t hid[FU_HASH], lid[DS_K], dup;
-    __shared__ float hp[FU_HASH], lp[DS_K], shf[FU_NT / 64];
+    extern __shared__ uint32_t mask[];   // (TAIL) a byte a vector, whole batches: its ids in the list
+    __shared__ uint32_t hid[DS_K + 1];
+    __shared__ float hy[DS_K + 1], shf[FU_NT / 64];
     __shared__ double shd[FU_NT / 64];
     __shared__ ds_coef coef;
     const uint64_t r = r0 + blockIdx.x;
@@ -387,184 +408,177 @@ __global__ __launch_bounds__(FU_NT, 4) void zs_k_distill_fused(ds_args a, uint64
     }
     const bool bad_label = a.labels && (label < 0 || label >= (int64_t)a.V);
     const uint32_t nb = (row.nvec + BV - 1u) / BV;
+    // whole vectors lo .. hi (rows of DS_FUSED_VOCAB ids have some); threads 0
+    // and 1 have the vectors before and behind them
+    const uint32_t lo = row.shift ? 1u : 0u, hi = (a.V + row.shift) / E - 1u;
+    const uint32_t edge = t == 0 ? 0u : row.nvec - 1u;
+    const bool has_edge = t < 2u && (t == 0 ? lo > 0u : hi + 1u < row.nvec);
     auto fetch = [&](uint32_t b, uint4 (&v)[U]) {
-        const uint32_t first = b * BV, j = first + t;
-        if (row.inside(first) && row.inside(first + BV - 1u)) {
 #pragma unroll
-            for (int u = 0; u < U; u++) v[u] = row.load(j + (uint32_t)u * FU_NT);
-        } else {
+        for (int u = 0; u < U; u++) v[u] = row.load(min(max(b * BV + t + (uint32_t)u * FU_NT, lo), hi));
+    };
+    auto unpack = [&](const uint4 (&v)[U], uint32_t b, float (&x)[U][E]) {
 #pragma unroll
-            for (int u = 0; u < U; u++) v[u] = row.raw(j + (uint32_t)u * FU_NT);
+        for (int u = 0; u < U; u++) hd_unpack<DT>(v[u], x[u]);
+        if (b * BV < lo || b * BV + BV - 1u > hi) {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const uint32_t j = b * BV + t + (uint32_t)u * FU_NT;
+#pragma unroll
+                for (int q = 0; q < E; q++) x[u][q] = j >= lo && j <= hi ? x[u][q] : -INFINITY;
+            }
         }
     };
     uint4 cur[U], nxt[U];
     fetch(0, cur);
-    // the list: a byte a vector that holds entries, the entries by their ids
-    for (uint32_t i = t; i < (row.nvec + 3u) / 4u; i += FU_NT) mask[i] = 0;
-    if (t < FU_HASH) hid[t] = 0xffffffffu;
-    if (t == 0) dup = 0;
+    if (TAIL)
+        for (uint32_t i = t; i < nb * (BV / 4); i += FU_NT) mask[i] = 0;
     const ds_entry l = ds_list<FU_NT>(a, r, shd);   // (its barriers order the clearing)
     const float xk = l.there ? row.at(l.id) : 0.0f, xl = a.labels && !bad_label ? row.at((uint32_t)label) : NAN;
-    uint32_t slot = FU_HASH;
-    if (t < a.K) {
-        lid[t] = l.there ? l.id : 0xffffffffu;
-        lp[t] = (float)l.p;
-    }
-    if (l.there) {
+    if (TAIL && l.there) {
         const uint32_t pos = l.id + row.shift, j = pos / E;
         atomicOr(&mask[j / 4], 1u << (j % 4 * 8 + pos % E));
-        for (uint32_t s = fu_slot(l.id);; s = (s + 1u) % FU_HASH) {   // (half the slots stay free)
-            const uint32_t was = atomicCAS(&hid[s], 0xffffffffu, l.id);
-            if (was == 0xffffffffu) { slot = s; break; }
-            if (was == l.id) { dup = 1; break; }
-        }
     }
-    __syncthreads();
-    if (slot < FU_HASH) {
-        float p = lp[t];
-        if (dup) {
-            p = 0.0f;
-            for (uint32_t k = 0; k < a.K; k++) p += lid[k] == l.id ? lp[k] : 0.0f;
-        }
-        hp[slot] = p;
-    }
+    __shared__ ds_ids ids;
+    const float pid = ds_of_id<FU_NT>(l, a.K, ids);
+    if (t < DS_K) hid[t] = l.there ? l.id : 0xffffffffu;
     const uint8_t* in_list = reinterpret_cast<const uint8_t*>(mask);
     // first pass: a maximum and sums per thread, relative to 2^ref
     const float c1 = (float)HD_LOG2E;
-    float m = -INFINITY, s = 0.0f, so = 0.0f, s1 = 0.0f;
-    for (uint32_t b = 0; b < nb; b++) {
-        if (b + 1u < nb) fetch(b + 1u, nxt);
-        float x[U][E], bm = m;
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            hd_unpack<DT>(cur[u], x[u]);
-#pragma unroll
-            for (int q = 0; q < E; q++) bm = fmaxf(bm, x[u][q]);
-        }
-        const float mr = bm > -INFINITY ? bm : 0.0f, ref = mr * a.c, ref1 = mr * c1;
+    float m = -INFINITY, s = 0.0f, so = 0.0f, s1 = 0.0f, c, ref, ct, ref1;
+    auto raise = [&](float bm) {   // to a maximum of at least bm
+        const float mr = bm > -INFINITY ? bm : 0.0f;
+        c = hd_factor(mr, a.c);
+        ref = mr * c;
+        ct = TWO ? hd_factor(mr, c1) : c;
+        ref1 = mr * ct;
         if (bm > m) {
-            const float f = m > -INFINITY ? __builtin_amdgcn_exp2f(m * a.c - ref) : 0.0f;
+            // (what came before a maximum whose factor is another has no mass beside it)
+            const float f = m > -INFINITY && c == a.c ? __builtin_amdgcn_exp2f(m * c - ref) : 0.0f;
             s *= f;
             if (TAIL) so *= f;
-            if (TWO) s1 *= m > -INFINITY ? __builtin_amdgcn_exp2f(m * c1 - ref1) : 0.0f;
+            if (TWO) s1 *= m > -INFINITY && ct == c1 ? __builtin_amdgcn_exp2f(m * ct - ref1) : 0.0f;
             m = bm;
         }
+    };
+    auto add = [&](const float (&x)[E], uint32_t in) {
+        float e[E];
+        if (TWO) {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            float e[E];
-            const uint32_t j = b * BV + t + (uint32_t)u * FU_NT;
-            if (TWO) {
+            for (int q = 0; q < E; q++) e[q] = __builtin_amdgcn_exp2f(fmaf(x[q], ct, -ref1));
+            s1 += hd_sum(e);
+        }
 #pragma unroll
-                for (int q = 0; q < E; q++) e[q] = __builtin_amdgcn_exp2f(fmaf(x[u][q], c1, -ref1));
-                s1 += hd_sum(e);
-            }
+        for (int q = 0; q < E; q++) e[q] = __builtin_amdgcn_exp2f(fmaf(x[q], c, -ref));
+        const float v = hd_sum(e);
+        s += v;
+        if (TAIL) {
+            if (in) {
 #pragma unroll
-            for (int q = 0; q < E; q++) e[q] = __builtin_amdgcn_exp2f(fmaf(x[u][q], a.c, -ref));
-            const float v = hd_sum(e);
-            s += v;
-            if (TAIL) {
-                const uint32_t in = j < row.nvec ? in_list[j] : 0u;
-                if (in) {
-#pragma unroll
-                    for (int q = 0; q < E; q++) e[q] = in >> q & 1u ? 0.0f : e[q];
-                    so += hd_sum(e);
-                } else {
-                    so += v;
-                }
+                for (int q = 0; q < E; q++) e[q] = in >> q & 1u ? 0.0f : e[q];
+                so += hd_sum(e);
+            } else {
+                so += v;
             }
         }
+    };
+    for (uint32_t b = 0; b < nb; b++) {
+        // (behind the last batch, the one that the second pass takes after it)
+        fetch(b + 1u < nb ? b + 1u : nb >= 2u ? nb - 2u : 0u, nxt);
+        float x[U][E], bm = m;
+        uint32_t in[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) in[u] = TAIL ? in_list[b * BV + t + (uint32_t)u * FU_NT] : 0u;
+        unpack(cur, b, x);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int q = 0; q < E; q++) bm = fmaxf(bm, x[u][q]);
+        raise(bm);
+#pragma unroll
+        for (int u = 0; u < U; u++) add(x[u], in[u]);
         if (b + 1u < nb) {
 #pragma unroll
             for (int u = 0; u < U; u++) cur[u] = nxt[u];
         }
     }
+    if (has_edge) {
+        float x[E], bm = m;
+        row.get(edge, x, -INFINITY);
+#pragma unroll
+        for (int q = 0; q < E; q++) bm = fmaxf(bm, x[q]);
+        raise(bm);
+        add(x, TAIL ? in_list[edge] : 0u);
+    }
     const float M = block_max_f<FU_NT>(m, shf);
     double S, S1, So;
     const float Mr = M > -INFINITY ? M : 0.0f;
-    auto total = [&](float v, float c) {   // of sums relative to 2^(m c), to 2^(M c)
-        const float f = m > -INFINITY ? __builtin_amdgcn_exp2f(m * c - Mr * c) : 0.0f;
+    auto total = [&](float v, float c0) {   // of sums relative to 2^(m c), to 2^(M c)
+        const float c = hd_factor(Mr, c0);
+        const float f = m == M ? 1.0f : m > -INFINITY && c == c0 ? __builtin_amdgcn_exp2f(m * c - Mr * c) : 0.0f;
         return block_sum_d<FU_NT>((double)(v * f), shd) * exp2(-(double)fmaf(Mr, c, -(Mr * c)));
     };
-    if (fabsf(Mr * a.c) < INFINITY && fabsf(Mr * c1) < INFINITY) {
-        S = total(s, a.c);
-        S1 = TWO ? total(s1, c1) : S;
-        So = TAIL ? total(so, a.c) : 0.0;
-    } else {
-        // a maximum whose exponent no float holds: by differences, once more
-        double d = 0.0, d1 = 0.0, dout = 0.0;
-        for (uint32_t j = t; j < row.nvec; j += FU_NT) {
-            float x[E];
-            row.get(j, x, -INFINITY);
-#pragma unroll
-            for (int q = 0; q < E; q++) {
-                const float e = __builtin_amdgcn_exp2f((x[q] - M) * a.c);
-                d += e;
-                if (TWO) d1 += __builtin_amdgcn_exp2f((x[q] - M) * c1);
-                if (TAIL && !(in_list[j] >> q & 1u)) dout += e;
-            }
-        }
-        S = block_sum_d<FU_NT>(d, shd);
-        S1 = TWO ? block_sum_d<FU_NT>(d1, shd) : S;
-        So = TAIL ? block_sum_d<FU_NT>(dout, shd) : 0.0;
-    }
+    S = total(s, a.c);
+    S1 = TWO ? total(s1, c1) : S;
+    So = TAIL ? total(so, a.c) : 0.0;
     if (!(M > -INFINITY)) S = S1 = NAN;   // a row of nothing has no distribution
     ds_loss<FU_NT>(a, r, l, xk, label, xl, (double)M, S, S1, So, shd);
+    const bool listed = __syncthreads_or(l.there && (int64_t)l.id == label);
     if (t == 0) {
         coef = ds_factors(a, r, l, bad_label, (double)M, S, S1, So);
-        if (label >= 0 && !bad_label) {
-            const uint32_t pos = (uint32_t)label + row.shift, j = pos / E;
-            mask[j / 4] |= 1u << (j % 4 * 8 + pos % E);
-        }
+        coef.lone = label < 0 || bad_label || listed ? 0xffffffffu : (uint32_t)label;
     }
     __syncthreads();
-    // second pass, from the batch at hand backwards
+    // second pass, from the batch at hand backwards: every id as one outside
+    // the list; the others are written over it as in zs_k_distill_grad
     const ds_coef k = coef;
-    const bool diff = !(fabsf(k.mc) < INFINITY), diff1 = !(fabsf(k.m1) < INFINITY);
+    if (t < DS_K) {
+        if (l.there) hy[t] = ds_at<TWO>(k, xk, true, pid, (int64_t)l.id == label);
+    } else if (t == DS_K) {
+        hid[DS_K] = k.lone;
+        hy[DS_K] = ds_at<TWO>(k, xl, false, 0.0f, true);
+    }
+    __syncthreads();
+    auto derive = [&](float (&x)[E]) {   // a vector's gradient in the place of its values
+#pragma unroll
+        for (int q = 0; q < E; q++) {
+            float e, e1;
+            ds_exps<TWO>(k, x[q], e, e1);
+            x[q] = TWO ? e * k.fo + e1 : e * k.fo;
+        }
+    };
     for (uint32_t b = nb; b-- > 0;) {
-        if (b) fetch(b - 1u, nxt);
+        float x[U][E];
+        unpack(cur, b, x);
+#pragma unroll
+        for (int u = 0; u < U; u++) cur[u] = nxt[u];
+        fetch(b >= 2u ? b - 2u : 0u, nxt);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const uint32_t j = b * BV + t + (uint32_t)u * FU_NT;
-            float x[E], e[E], e1[E];
-            hd_unpack<DT>(cur[u], x);
-#pragma unroll
-            for (int q = 0; q < E; q++) ds_exps<TWO>(a, k, diff, diff1, x[q], e[q], e1[q]);
-            const int i0 = row.id0(j);
-            uint32_t in = j < row.nvec ? in_list[j] : 0u;
-            if (in) {
-#pragma unroll
-                for (int q = 0; q < E; q++) {
-                    const uint32_t id = (uint32_t)(i0 + q);
-                    float f = k.fo, sub = 0.0f;
-                    if (in >> q & 1u) {
-                        if ((int64_t)id == label) sub = k.fc;
-                        for (uint32_t h = fu_slot(id); hid[h] != 0xffffffffu; h = (h + 1u) % FU_HASH)
-                            if (hid[h] == id) {
-                                f = k.fi;
-                                sub += k.fp * hp[h];
-                                break;
-                            }
-                    }
-                    x[q] = e[q] * f + (e1[q] - sub);
-                }
-            } else {
-#pragma unroll
-                for (int q = 0; q < E; q++) x[q] = TWO ? e[q] * k.fo + e1[q] : e[q] * k.fo;
-            }
-            if (j < row.nvec) ds_store<DT>(grad, a.V, aligned && row.inside(j), i0, x);
+            derive(x[u]);
+            if (j >= lo && j <= hi) ds_store<DT>(grad, a.V, aligned, row.id0(j), x[u]);
         }
-        if (b) {
-#pragma unroll
-            for (int u = 0; u < U; u++) cur[u] = nxt[u];
-        }
+    }
+    if (has_edge) {
+        float x[E];
+        row.get(edge, x, -INFINITY);
+        derive(x);
+        ds_store<DT>(grad, a.V, false, row.id0(edge), x);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (uint32_t h = (uint32_t)zs_lane(); h <= DS_K; h += 64u) {
+        const uint32_t id = hid[h], j = (id + row.shift) / E;
+        const uint32_t owner = j < lo || j > hi ? 0u : j % FU_NT >> 6;
+        if (id < a.V && owner == (uint32_t)zs_wid()) ds_store1<DT>(grad + id, hy[h]);
     }
 }
 
 template <int DT>
 static void ds_go(const ds_args& a, int what, uint64_t r0, uint32_t n, hipStream_t stream) {
     const dim3 grid(n * a.chunks), wg(DS_NT);
-    const uint32_t lds = (a.V + 7u) / hd_elem<DT>::E + 4u & ~3u;   // a byte a vector
-    if (what == (DS_LOSS | DS_GRAD) && a.N >= DS_FUSED_ROWS && lds <= DS_FUSED_LDS) {
+    const uint32_t lds = a.tail ? ((a.V + 7u) / hd_elem<DT>::E / (4u * FU_NT) + 1u) * (4u * FU_NT) : 0u;   // a byte a vector, whole batches
+    if (what == (DS_LOSS | DS_GRAD) && a.N >= DS_FUSED_ROWS && a.V >= DS_FUSED_VOCAB && lds <= DS_FUSED_LDS) {
         if (a.tail && a.two) hipLaunchKernelGGL((zs_k_distill_fused<DT, true, true>), dim3(n), dim3(FU_NT), lds, stream, a, r0);
         else if (a.tail) hipLaunchKernelGGL((zs_k_distill_fused<DT, true, false>), dim3(n), dim3(FU_NT), lds, stream, a, r0);
         else if (a.two) hipLaunchKernelGGL((zs_k_distill_fused<DT, false, true>), dim3(n), dim3(FU_NT), lds, stream, a, r0);

@@ -127,6 +127,12 @@ __device__ __forceinline__ float hd_sum(const float (&e)[E]) {
     else return ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
 }
 
+// The factor of the exponent for values of at most m: c, or, where m c is past
+// the floats, 2^-32. There the next float below m lies over 2^100 / c under it,
+// so that every value but m itself has no mass with either factor, and with a
+// power of two m's product is exact.
+__device__ __forceinline__ float hd_factor(float m, float c) { return fabsf(m * c) < INFINITY ? c : 0x1p-32f; }
+
 // A value as the heads of rows see it: NaN counts as -inf (nothing is known of
 // it), +inf as the largest number (an id that is certain; several share).
 __device__ __forceinline__ float hd_clean(float x) { return fminf(x == x ? x : -INFINITY, __FLT_MAX__); }

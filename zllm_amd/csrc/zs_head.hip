@@ -77,34 +77,27 @@ __global__ __launch_bounds__(HS_NT) void zs_k_head_scan(hd_args a, uint64_t r0) 
     };
     maxima();
     // 2^(x c - mc): one fma a value; mc's rounding is a factor of all of them
-    float mr = m > -INFINITY ? m : 0.0f, mc = mr * a.c, s = 0.0f;
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        float e[E];
-#pragma unroll
-        for (int q = 0; q < E; q++) e[q] = __builtin_amdgcn_exp2f(fmaf(x[u][q], a.c, -mc));
-        s += hd_sum(e);
-    }
-    s = zs_wave_reduce(s, [](float p, float q) { return p + q; });
-    if (s < INFINITY && fabsf(mc) < INFINITY) {
-        s *= __builtin_amdgcn_exp2f(-fmaf(mr, a.c, -mc));
-    } else {
-        // NaN or +inf among the values, or a maximum whose exponent no float holds
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int q = 0; q < E; q++) x[u][q] = hd_clean(x[u][q]);
-        maxima();
-        mr = m > -INFINITY ? m : 0.0f;
+    float s;
+    auto sum = [&]() {
+        const float mr = m > -INFINITY ? m : 0.0f, c = hd_factor(mr, a.c), mc = mr * c;
         s = 0.0f;
 #pragma unroll
         for (int u = 0; u < U; u++) {
             float e[E];
 #pragma unroll
-            for (int q = 0; q < E; q++) e[q] = __builtin_amdgcn_exp2f((x[u][q] - mr) * a.c);
+            for (int q = 0; q < E; q++) e[q] = __builtin_amdgcn_exp2f(fmaf(x[u][q], c, -mc));
             s += hd_sum(e);
         }
-        s = zs_wave_reduce(s, [](float p, float q) { return p + q; });
+        s = zs_wave_reduce(s, [](float p, float q) { return p + q; }) * __builtin_amdgcn_exp2f(-fmaf(mr, c, -mc));
+    };
+    sum();
+    if (!(s < INFINITY)) {   // NaN or +inf among the values
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int q = 0; q < E; q++) x[u][q] = hd_clean(x[u][q]);
+        maxima();
+        sum();
     }
     if (lane == 0) a.rec[r * a.recs + chunk * (HS_NT / 64) + (uint32_t)zs_wid()] = make_float2(m, s);
     // a group's lanes store their vectors' groups in turn
