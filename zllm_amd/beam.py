@@ -13,22 +13,36 @@ The reference decodes one hypothesis per request; there is no counterpart.
 torch holds the device memory and the stream; the computation is libzs's.
 """
 import ctypes as C
+import functools
+import struct
 from dataclasses import dataclass
 from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
 
-from ._lib import Beam, BeamStateDesc, lib
+from ._lib import Beam, BeamStateDesc, ZsError, lib
 from .engine import Context, _check
 
 MAX_WIDTH = 32
 MAX_EOS = 8
+MAX_VOCAB = 1 << 20
 ZS_BEAM_EARLY = 1
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
+# The arguments are packed to bytes: a step of 4 beams over 32000 ids takes
+# the host half as long as with the ctypes fields set one by one.
+_BEAM = struct.Struct("=4IQ2Q2I8IfI18Q")
+assert _BEAM.size == C.sizeof(Beam)
 
-def _rows(logits: torch.Tensor, what: str) -> torch.Tensor:
+
+def _stream(dev: torch.device) -> int:
+    """The current stream's handle (torch.cuda.current_stream makes an object
+    of it first, which takes as long as a launch)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _rows(logits: torch.Tensor, what: str) -> None:
     """Checks a [rows, V] tensor of logits: any of the three types, any row
     stride, the values of a row adjacent."""
     if logits.dim() != 2 or logits.dtype not in DTYPES:
@@ -37,7 +51,6 @@ def _rows(logits: torch.Tensor, what: str) -> torch.Tensor:
         raise ValueError(f"{what}: logits are on {logits.device}, not on a GPU")
     if logits.shape[1] > 1 and logits.stride(1) != 1:
         raise ValueError(f"{what}: the logits of a row are not adjacent")
-    return logits
 
 
 def _ld(t: torch.Tensor) -> int:
@@ -46,18 +59,33 @@ def _ld(t: torch.Tensor) -> int:
 
 
 def _like(t: torch.Tensor, shape, dtype, dev, what: str, name: str) -> torch.Tensor:
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != dev or not t.is_contiguous():
+    if t.shape != shape or t.dtype != dtype or t.device != dev or not t.is_contiguous():
         raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor {tuple(shape)} on {dev}")
     return t
 
 
-def _work(nbytes: int, dev) -> Optional[torch.Tensor]:
-    """Scratch of one call, from torch's allocator: it is the current
-    stream's, so calls on other streams never share it."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+def _work(nbytes: int, dev) -> Tuple[Optional[torch.Tensor], int]:
+    """Scratch of one call and its address, from torch's allocator: it is the
+    current stream's, so calls on other streams never share it."""
+    if not nbytes:
+        return None, 0
+    t = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    return t, t.data_ptr()
 
 
-@dataclass
+@functools.lru_cache(maxsize=1024)
+def _work_bytes(name: str, *sizes: int) -> int:
+    need = C.c_uint64()
+    rc = getattr(lib(), name)(*sizes, C.byref(need))
+    if rc:
+        raise ZsError(f"{name}{sizes} failed ({rc})")
+    return need.value
+
+
+_POOL = ("score", "length", "parent", "token", "steps", "done")
+
+
+@dataclass(frozen=True)
 class BeamPool:
     """Finished hypotheses of each request, best first ([groups, width]; absent
     ones score -inf), and the requests' state ([groups]). An entry's tokens
@@ -76,8 +104,17 @@ class BeamPool:
         return cls(torch.full((groups, width), -float("inf"), device=device), i(0, groups, width), i(-1, groups, width),
                    i(-1, groups, width), i(0, groups), i(0, groups))
 
+    def _pointers(self, G: int, W: int, dev, what: str):
+        if getattr(self, "_checked", None) != (G, W, dev):   # (the fields do not change)
+            for name in _POOL:
+                _like(getattr(self, name), (G,) if name in ("steps", "done") else (G, W),
+                      torch.float32 if name == "score" else torch.int32, dev, what, "pool." + name)
+            object.__setattr__(self, "_checked", (G, W, dev))
+        return (self.score.data_ptr(), self.length.data_ptr(), self.parent.data_ptr(), self.token.data_ptr(),
+                self.steps.data_ptr(), self.done.data_ptr())
 
-@dataclass
+
+@dataclass(frozen=True)
 class BeamStep:
     parents: torch.Tensor  # int32 [groups, width]: beam of the group, -1 for none
     tokens: torch.Tensor   # int32 [groups, width]
@@ -86,10 +123,12 @@ class BeamStep:
 
     @classmethod
     def alloc(cls, groups: int, width: int, device) -> "BeamStep":
-        f = torch.empty((2, groups, width), device=device).unbind(0)
+        f = torch.empty((2, groups, width), dtype=torch.float32, device=device).unbind(0)
         i = torch.empty((5, groups, width), dtype=torch.int32, device=device).unbind(0)
         g = torch.empty((2, groups), dtype=torch.int32, device=device).unbind(0)
-        return cls(i[0], i[1], f[0], BeamPool(f[1], i[2], i[3], i[4], g[0], g[1]))
+        pool = BeamPool(f[1], i[2], i[3], i[4], g[0], g[1])
+        object.__setattr__(pool, "_checked", (groups, width, device))
+        return cls(i[0], i[1], f[0], pool)
 
 
 def beam_select(ctx: Context, logits: torch.Tensor, scores: torch.Tensor, pool: BeamPool, eos: Sequence[int] = (),
@@ -109,40 +148,31 @@ def beam_select(ctx: Context, logits: torch.Tensor, scores: torch.Tensor, pool: 
     R, V = logits.shape
     if R != G * W:
         raise ValueError(f"{what}: {R} rows of logits for {G} groups of {W} beams")
-    eos = [int(e) for e in eos]
-    if len(eos) > MAX_EOS or any(not 0 <= e < 2 ** 32 for e in eos):
+    n_eos = len(eos)
+    if n_eos > MAX_EOS or any(not 0 <= e < 2 ** 32 for e in eos):
         raise ValueError(f"{what}: at most {MAX_EOS} EOS ids, not negative")
     _like(scores, (G, W), torch.float32, dev, what, "scores")
-    a = Beam()
-    a.groups, a.width, a.V, a.dtype, a.ld = G, W, V, DTYPES[logits.dtype], _ld(logits)
-    a.d_logits = logits.data_ptr()
+    allow, words = 0, 0
     if allow_bits is not None:
         if allow_bits.dim() != 2 or allow_bits.shape[0] != R or allow_bits.shape[1] * 32 < V:
             raise ValueError(f"{what}: allow_bits are [rows, ceil(V / 32)]")
-        _like(allow_bits, allow_bits.shape, torch.int32, dev, what, "allow_bits")
-        a.d_allow_bits, a.allow_words = allow_bits.data_ptr(), allow_bits.shape[1]
-    a.n_eos = len(eos)
-    for i, e in enumerate(eos):
-        a.eos[i] = e
-    a.length_penalty, a.flags = length_penalty, ZS_BEAM_EARLY if early_stopping else 0
+        allow, words = _like(allow_bits, allow_bits.shape, torch.int32, dev, what, "allow_bits").data_ptr(), \
+            allow_bits.shape[1]
     if out is None:
         out = BeamStep.alloc(G, W, dev)
-    a.d_scores = scores.data_ptr()
-    for p, tail in ((pool, ""), (out.pool, "_out")):
-        for name in ("score", "length", "parent", "token"):
-            t = _like(getattr(p, name), (G, W), torch.float32 if name == "score" else torch.int32, dev, what, "pool." + name)
-            setattr(a, "d_fin_" + name + tail, t.data_ptr())
-        for name in ("steps", "done"):
-            setattr(a, "d_" + name + tail, _like(getattr(p, name), (G,), torch.int32, dev, what, "pool." + name).data_ptr())
-    a.d_parent = _like(out.parents, (G, W), torch.int32, dev, what, "out.parents").data_ptr()
-    a.d_token = _like(out.tokens, (G, W), torch.int32, dev, what, "out.tokens").data_ptr()
-    a.d_score = _like(out.scores, (G, W), torch.float32, dev, what, "out.scores").data_ptr()
-    need = C.c_uint64()
-    _check(ctx.h, lib().zs_beam_select_work(G, W, V, len(eos), C.byref(need)), "zs_beam_select_work")
-    work = _work(need.value, dev)
-    if work is not None:
-        a.d_work, a.work_bytes = work.data_ptr(), need.value
-    _check(ctx.h, lib().zs_beam_select(ctx.h, C.byref(a), torch.cuda.current_stream(dev).cuda_stream), what)
+    else:
+        _like(out.parents, (G, W), torch.int32, dev, what, "out.parents")
+        _like(out.tokens, (G, W), torch.int32, dev, what, "out.tokens")
+        _like(out.scores, (G, W), torch.float32, dev, what, "out.scores")
+    nbytes = _work_bytes("zs_beam_select_work", G, W, V, n_eos) if 0 < G * W and 0 < V <= MAX_VOCAB else 0
+    work, at = _work(nbytes, dev)
+    raw = _BEAM.pack(G, W, V, DTYPES[logits.dtype], _ld(logits), logits.data_ptr(), allow, words, n_eos, *eos,
+                     *(0,) * (MAX_EOS - n_eos), length_penalty, ZS_BEAM_EARLY if early_stopping else 0, scores.data_ptr(),
+                     *pool._pointers(G, W, dev, what), *out.pool._pointers(G, W, dev, what), out.parents.data_ptr(),
+                     out.tokens.data_ptr(), out.scores.data_ptr(), at, nbytes)
+    rc = lib().zs_beam_select(ctx.h, C.byref(Beam.from_buffer_copy(raw)), _stream(dev))
+    if rc:
+        _check(ctx.h, rc, what)
     return out
 
 
@@ -207,8 +237,9 @@ def beam_reorder(ctx: Context, states: BeamStates, parents: torch.Tensor) -> Non
     dev = states.tensors[0].device
     _like(parents, (states.rows // states.width, states.width), torch.int32, dev, "beam_reorder", "parents")
     rc = lib().zs_beam_reorder(ctx.h, parents.shape[0], states.width, parents.data_ptr(), states.descs, states.n,
-                               torch.cuda.current_stream(dev).cuda_stream)
-    _check(ctx.h, rc, "beam_reorder")
+                               _stream(dev))
+    if rc:
+        _check(ctx.h, rc, "beam_reorder")
 
 
 @dataclass
@@ -226,7 +257,7 @@ class BeamSearch:
     def __init__(self, ctx: Context, groups: int, width: int, max_steps: int, eos: Sequence[int] = (),
                  length_penalty: float = 1.0, early_stopping: bool = False, device="cuda"):
         self.ctx, self.groups, self.width, self.max_steps = ctx, groups, width, max_steps
-        self.eos, self.length_penalty, self.early_stopping = tuple(eos), length_penalty, early_stopping
+        self.eos, self.length_penalty, self.early_stopping = tuple(int(e) for e in eos), length_penalty, early_stopping
         self.scores = torch.full((groups, width), -float("inf"), device=device)
         self.scores[:, 0] = 0.0
         self.pool = BeamPool.empty(groups, width, device)

@@ -10,17 +10,22 @@ counterpart. torch holds the device memory and the stream; the computation is
 libzs's.
 """
 import ctypes as C
+import struct
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
 
 from ._lib import Distill, Teacher, lib
-from .beam import DTYPES, _ld, _like, _rows, _work
+from .beam import DTYPES, MAX_VOCAB, _ld, _like, _rows, _stream, _work, _work_bytes
 from .engine import Context, _check
 
 MAX_TOP = 128
 ZS_DISTILL_TAIL = 1
+# the arguments are packed to bytes, as zllm_amd.beam's
+_TEACHER = struct.Struct("=4I2QfI5Q")
+_DISTILL = struct.Struct("=4IQ4Qq3fI8Q")
+assert _TEACHER.size == C.sizeof(Teacher) and _DISTILL.size == C.sizeof(Distill)
 
 
 def teacher_topk(ctx: Context, logits: torch.Tensor, K: int, temperature: float = 1.0
@@ -38,16 +43,13 @@ def teacher_topk(ctx: Context, logits: torch.Tensor, K: int, temperature: float 
     ids = torch.empty((N, K), dtype=torch.int32, device=dev)
     logp = torch.empty((N, K), dtype=torch.float32, device=dev)
     lse = torch.empty(N, dtype=torch.float32, device=dev)
-    a = Teacher()
-    a.N, a.V, a.K, a.dtype, a.ld = N, V, K, DTYPES[logits.dtype], _ld(logits)
-    a.d_logits, a.temperature = logits.data_ptr(), temperature
-    a.d_ids, a.d_logp, a.d_lse = ids.data_ptr(), logp.data_ptr(), lse.data_ptr()
-    need = C.c_uint64()
-    _check(ctx.h, lib().zs_teacher_topk_work(N, V, K, C.byref(need)), "zs_teacher_topk_work")
-    work = _work(need.value, dev)
-    if work is not None:
-        a.d_work, a.work_bytes = work.data_ptr(), need.value
-    _check(ctx.h, lib().zs_teacher_topk(ctx.h, C.byref(a), torch.cuda.current_stream(dev).cuda_stream), what)
+    nbytes = _work_bytes("zs_teacher_topk_work", N, V, K) if N and V <= MAX_VOCAB else 0
+    work, at = _work(nbytes, dev)
+    raw = _TEACHER.pack(N, V, K, DTYPES[logits.dtype], _ld(logits), logits.data_ptr(), temperature, 0, ids.data_ptr(),
+                        logp.data_ptr(), lse.data_ptr(), at, nbytes)
+    rc = lib().zs_teacher_topk(ctx.h, C.byref(Teacher.from_buffer_copy(raw)), _stream(dev))
+    if rc:
+        _check(ctx.h, rc, what)
     return ids, logp, lse
 
 
@@ -63,49 +65,44 @@ class DistillConfig:
     ignore_index: int = -100
 
 
-def _args(what, logits, ids, logp, cfg, labels) -> Distill:
+def _call(ctx, entry, what, logits, ids, logp, cfg, labels, loss=0, stats=0, row_grad=0, row_grad_stride=0, grad=0,
+          ld_grad=0):
     _rows(logits, what)
     N, V = logits.shape
     dev = logits.device
     if ids.dim() != 2 or ids.shape[0] != N or not 1 <= ids.shape[1] <= MAX_TOP:
         raise ValueError(f"{what}: ids are [N, K], K 1 to {MAX_TOP}")
-    a = Distill()
-    a.N, a.V, a.K, a.dtype, a.ld = N, V, ids.shape[1], DTYPES[logits.dtype], _ld(logits)
-    a.d_logits = logits.data_ptr()
-    a.d_ids = _like(ids, ids.shape, torch.int32, dev, what, "ids").data_ptr()
-    a.d_logp = _like(logp, ids.shape, torch.float32, dev, what, "logp").data_ptr()
-    if labels is not None:
-        a.d_labels = _like(labels, (N,), torch.int64, dev, what, "labels").data_ptr()
-    a.ignore_index = cfg.ignore_index
-    a.temperature, a.kl_weight, a.ce_weight = cfg.temperature, cfg.kl_weight, cfg.ce_weight
-    a.flags = ZS_DISTILL_TAIL if cfg.tail else 0
-    return a
+    K = ids.shape[1]
+    _like(ids, (N, K), torch.int32, dev, what, "ids")
+    _like(logp, (N, K), torch.float32, dev, what, "logp")
+    lab = 0 if labels is None else _like(labels, (N,), torch.int64, dev, what, "labels").data_ptr()
+    nbytes = _work_bytes("zs_distill_work", N, V, K) if N and 0 < V <= MAX_VOCAB else 0
+    work, at = _work(nbytes, dev)
+    raw = _DISTILL.pack(N, V, K, DTYPES[logits.dtype], _ld(logits), logits.data_ptr(), ids.data_ptr(), logp.data_ptr(),
+                        lab, cfg.ignore_index, cfg.temperature, cfg.kl_weight, cfg.ce_weight,
+                        ZS_DISTILL_TAIL if cfg.tail else 0, loss, stats, row_grad, row_grad_stride, grad, ld_grad, at,
+                        nbytes)
+    rc = getattr(lib(), entry)(ctx.h, C.byref(Distill.from_buffer_copy(raw)), _stream(dev))
+    if rc:
+        _check(ctx.h, rc, what)
 
 
-def _grad_args(what, a, logits, row_grad, out):
+def _grad(what, logits, row_grad, out):
+    """The gradient's arguments and its tensor."""
+    _rows(logits, what)
     N = logits.shape[0]
     dev = logits.device
     if row_grad.dtype != torch.float32 or row_grad.device != dev or row_grad.dim() > 1 or \
             (row_grad.dim() == 1 and row_grad.shape[0] != N):
         raise ValueError(f"{what}: row_grad is a float32 tensor [N] (or of no dimension: one value for all rows)")
-    a.d_row_grad = row_grad.data_ptr()
-    a.row_grad_stride = row_grad.stride(0) if row_grad.dim() else 0   # 0 too for a value expanded over the rows
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or \
             (out.shape[1] > 1 and out.stride(1) != 1) or (N > 1 and out.stride(0) < out.shape[1]):
         raise ValueError(f"{what}: out is like logits, the values of a row adjacent")
-    a.d_grad, a.ld_grad = out.data_ptr(), _ld(out)
-    return out
-
-
-def _call(ctx, fn, what, a, dev):
-    need = C.c_uint64()
-    _check(ctx.h, lib().zs_distill_work(a.N, a.V, a.K, C.byref(need)), "zs_distill_work")
-    work = _work(need.value, dev)
-    if work is not None:
-        a.d_work, a.work_bytes = work.data_ptr(), need.value
-    _check(ctx.h, fn(ctx.h, C.byref(a), torch.cuda.current_stream(dev).cuda_stream), what)
+    # (the stride is 0 too for a value expanded over the rows)
+    return dict(row_grad=row_grad.data_ptr(), row_grad_stride=row_grad.stride(0) if row_grad.dim() else 0,
+                grad=out.data_ptr(), ld_grad=_ld(out)), out
 
 
 def distill_loss(ctx: Context, logits: torch.Tensor, ids: torch.Tensor, logp: torch.Tensor, cfg: DistillConfig,
@@ -113,11 +110,10 @@ def distill_loss(ctx: Context, logits: torch.Tensor, ids: torch.Tensor, logp: to
     """Loss per row (float32 [N]) of the student's logits [N, V] against the
     teacher's list, and what the backward pass needs of the rows (float32
     [N, 4]). labels: int64 [N], cfg.ignore_index marks rows of no loss."""
-    a = _args("distill_loss", logits, ids, logp, cfg, labels)
-    loss = torch.empty(a.N, dtype=torch.float32, device=logits.device)
-    stats = torch.empty((a.N, 4), dtype=torch.float32, device=logits.device)
-    a.d_loss, a.d_stats = loss.data_ptr(), stats.data_ptr()
-    _call(ctx, lib().zs_distill_loss, "distill_loss", a, logits.device)
+    N = logits.shape[0]
+    loss = torch.empty(N, dtype=torch.float32, device=logits.device)
+    stats = torch.empty((N, 4), dtype=torch.float32, device=logits.device)
+    _call(ctx, "zs_distill_loss", "distill_loss", logits, ids, logp, cfg, labels, loss.data_ptr(), stats.data_ptr())
     return loss, stats
 
 
@@ -127,10 +123,9 @@ def distill_grad(ctx: Context, logits: torch.Tensor, ids: torch.Tensor, logp: to
     """Gradient of sum_r row_grad[r] * loss[r] by the logits, in their type;
     stats from distill_loss. out may be the logits themselves."""
     what = "distill_grad"
-    a = _args(what, logits, ids, logp, cfg, labels)
-    a.d_stats = _like(stats, (a.N, 4), torch.float32, logits.device, what, "stats").data_ptr()
-    out = _grad_args(what, a, logits, row_grad, out)
-    _call(ctx, lib().zs_distill_grad, what, a, logits.device)
+    kw, out = _grad(what, logits, row_grad, out)
+    st = _like(stats, (logits.shape[0], 4), torch.float32, logits.device, what, "stats").data_ptr()
+    _call(ctx, "zs_distill_grad", what, logits, ids, logp, cfg, labels, stats=st, **kw)
     return out
 
 
@@ -140,11 +135,9 @@ def distill_loss_grad(ctx: Context, logits: torch.Tensor, ids: torch.Tensor, log
     """distill_loss and distill_grad in one call, where the rows' weights are
     known before the loss (a mean over the rows: row_grad = 1 / N)."""
     what = "distill_loss_grad"
-    a = _args(what, logits, ids, logp, cfg, labels)
-    loss = torch.empty(a.N, dtype=torch.float32, device=logits.device)
-    a.d_loss = loss.data_ptr()
-    out = _grad_args(what, a, logits, row_grad, out)
-    _call(ctx, lib().zs_distill_loss_grad, what, a, logits.device)
+    kw, out = _grad(what, logits, row_grad, out)
+    loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
+    _call(ctx, "zs_distill_loss_grad", what, logits, ids, logp, cfg, labels, loss.data_ptr(), **kw)
     return loss, out
 
 
