@@ -1148,8 +1148,7 @@ extern "C" int zs_beam_select(zs_ctx* ctx, const zs_beam* b, void* stream) {
     m.fin_token_o = b->d_fin_token_out; m.steps_o = b->d_steps_out; m.done_o = b->d_done_out;
     m.parent = b->d_parent; m.token = b->d_token; m.score_o = b->d_score;
     const int prev = zs_device_guard_begin(ctx);
-    rc = hd_head_launch(h, b->dtype, (hipStream_t)stream);
-    if (!rc) rc = bm_merge_launch(m, b->groups, (hipStream_t)stream);
+    rc = hd_head_launch(h, &m, b->dtype, (hipStream_t)stream);
     zs_device_guard_end(ctx, prev);
     return rc ? zs_set_error(ctx, ZS_EHIP, "%s: launch failed", who) : ZS_OK;
 }
@@ -1230,7 +1229,7 @@ extern "C" int zs_teacher_topk(zs_ctx* ctx, const zs_teacher* b, void* stream) {
     h.ids = b->d_ids; h.logp = b->d_logp; h.lse_out = b->d_lse;
     hd_work(h, b->d_work, false);
     const int prev = zs_device_guard_begin(ctx);
-    rc = hd_head_launch(h, b->dtype, (hipStream_t)stream);
+    rc = hd_head_launch(h, nullptr, b->dtype, (hipStream_t)stream);
     zs_device_guard_end(ctx, prev);
     return rc ? zs_set_error(ctx, ZS_EHIP, "%s: launch failed", who) : ZS_OK;
 }

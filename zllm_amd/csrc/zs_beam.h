@@ -17,7 +17,6 @@ struct bm_args {
     int32_t *parent, *token;
     float* score_o;
 };
-int bm_merge_launch(const bm_args& a, uint32_t groups, hipStream_t stream);
 
 // One state array: `total` columns of `unit` bytes per row in blocks of `cols`.
 struct bm_state {
@@ -45,6 +44,6 @@ inline void ro_div(uint64_t d, uint32_t& mul, uint32_t& sh) {
 // Workgroups for `total` columns of a group's rows: a column per thread up to
 // about 32 workgroups a CU over all groups, loops past that.
 inline uint32_t ro_blocks(uint64_t total, uint32_t groups) {
-    const uint64_t want = (total + 255u) / 256u, most = 8192u / groups + 1u;
+    const uint64_t want = (total + 255u) / 256u, most = 32768u / groups + 1u;
     return (uint32_t)(want < most ? want : most);
 }

@@ -1,147 +1,7 @@
-// zs_beam.hip -- beam search: the step of a group of beams from the heads of
-// their rows (zs_head.hip), and the reordering of the beams' states.
-#include "zs_head.h"
+// zs_beam.hip -- beam search: the states of the beams follow their parents.
+// (The step itself ends in zs_head.hip's pick, with zs_beam_merge.h.)
+#include <hip/hip_runtime.h>
 #include "zs_beam.h"
-
-// ---------------------------------------------------------------------------
-// The step of one request by one wave, the lists read and scored by four. The
-// rows' heads are sorted, so the
-// candidates' order is a merge of at most 32 lists (held in LDS): lane b has the
-// score of beam b's next candidate, each turn takes the largest (the lowest
-// beam of equals). A row needs width + n_eos entries: its first `width` that do not
-// end are among them, and so is every EOS id among the first `width` overall.
-// ---------------------------------------------------------------------------
-__device__ __forceinline__ bool bm_is_eos(const bm_args& a, uint32_t id) {
-    bool e = false;
-#pragma unroll
-    for (uint32_t i = 0; i < ZS_BEAM_MAX_EOS; i++) e |= i < a.n_eos && a.eos[i] == id;
-    return e;
-}
-
-#define BM_NT 256
-__global__ __launch_bounds__(BM_NT) void zs_k_beam_merge(bm_args a) {
-    constexpr int NL = ZS_BEAM_MAX_WIDTH * (ZS_BEAM_MAX_WIDTH + ZS_BEAM_MAX_EOS) / BM_NT;   // entries a thread at most
-    __shared__ float cs_[ZS_BEAM_MAX_WIDTH * (ZS_BEAM_MAX_WIDTH + ZS_BEAM_MAX_EOS)];      // the lists' scores and ids
-    __shared__ uint32_t ci_[ZS_BEAM_MAX_WIDTH * (ZS_BEAM_MAX_WIDTH + ZS_BEAM_MAX_EOS)];
-    __shared__ float bs_[ZS_BEAM_MAX_WIDTH];
-    __shared__ double bl_[ZS_BEAM_MAX_WIDTH];
-    __shared__ float fin_s[ZS_BEAM_MAX_WIDTH];
-    __shared__ int fin_p[ZS_BEAM_MAX_WIDTH], fin_t[ZS_BEAM_MAX_WIDTH];
-    const uint32_t g = blockIdx.x, lane = threadIdx.x, W = a.width, K = a.K;
-    const size_t at = (size_t)g * W;
-    const bool beam = lane < W;
-    // all loads at once: what is not needed is dropped afterwards
-    const int was = a.done[g], steps = a.steps[g];
-    const float score = beam ? a.scores[at + lane] : -INFINITY;
-    const double lse = beam ? a.lse[at + lane] : 0.0;
-    unsigned long long e[NL];
-#pragma unroll
-    for (int k = 0; k < NL; k++) {
-        const uint32_t i = lane + (uint32_t)k * BM_NT;
-        e[k] = i < W * K ? a.list[at * K + i] : ~0ull;
-    }
-    // the pool as it was (threads below W)
-    float ps = beam ? a.fin_score[at + lane] : -INFINITY;
-    int pl = beam ? a.fin_length[at + lane] : 0, pp = beam ? a.fin_parent[at + lane] : -1, pt = beam ? a.fin_token[at + lane] : -1;
-    if (!(ps == ps)) ps = -INFINITY;
-    if (beam) {
-        // (beams that do not live left no list)
-        bs_[lane] = !was && fabsf(score) <= __FLT_MAX__ ? score : -INFINITY;
-        bl_[lane] = lse;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < NL; k++) {
-        const uint32_t i = lane + (uint32_t)k * BM_NT;
-        if (i >= W * K) break;
-        const uint32_t b = i / K;
-        const float bs = bs_[b];
-        const bool some = bs > -INFINITY && e[k] != ~0ull;
-        cs_[i] = some ? (float)((double)bs + ((double)zs_u2f((uint32_t)(e[k] >> 32)) - bl_[b])) : -INFINITY;
-        ci_[i] = (uint32_t)e[k] | (bm_is_eos(a, (uint32_t)e[k]) ? 0x80000000u : 0u);
-    }
-    __syncthreads();
-    if (lane >= 64u) return;
-    // the beam's next candidate and the one behind it
-    float s = -INFINITY, s2 = -INFINITY;
-    uint32_t id = 0, id2 = 0, next = 0;
-    auto ahead = [&]() {
-        const bool some = beam && next < K;
-        s2 = some ? cs_[lane * K + next] : -INFINITY;
-        id2 = some ? ci_[lane * K + next] : 0u;
-        next++;
-    };
-    ahead();
-    s = s2;
-    id = id2;
-    ahead();
-    int o_parent = -1, o_token = -1;
-    float o_score = -INFINITY;
-    uint32_t n_live = 0, n_fin = 0;
-    for (uint32_t rank = 0; n_live < W; rank++) {
-        const float cs = wave_max_f(s);
-        if (!(cs > -INFINITY)) break;
-        const uint32_t b = (uint32_t)__ffsll((long long)__ballot(s == cs)) - 1u;   // the lowest beam of equals
-        const uint32_t cid = zs_readlane_u(id, b);
-        if (cid >> 31) {   // EOS
-            if (rank < W) {
-                if (lane == 0) { fin_s[n_fin] = cs; fin_p[n_fin] = (int)b; fin_t[n_fin] = (int)(cid & 0x7fffffffu); }
-                n_fin++;
-            }
-        } else {
-            if (lane == n_live) { o_parent = (int)b; o_token = (int)cid; o_score = cs; }
-            n_live++;
-        }
-        if (lane == b) {
-            s = s2;
-            id = id2;
-            ahead();
-        }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");   // (one wave from here on)
-    // the pool and what finished, the pool first among equals: lane i's place
-    // is the number of lanes in front of it
-    const float len = (float)(steps + 1), norm = a.length_penalty == 1.0f ? len : a.length_penalty == 0.0f ? 1.0f : powf(len, a.length_penalty);
-    if (lane >= W && lane < W + n_fin && lane < 64u) {
-        const uint32_t i = lane - W;
-        ps = fin_s[i] / norm;
-        pl = steps + 1;
-        pp = fin_p[i];
-        pt = fin_t[i];
-    }
-    uint32_t place = 0;
-    for (uint32_t i = 0; i < W + n_fin; i++) {
-        const float o = zs_readlane_f(ps, i);
-        place += o > ps || (o == ps && i < lane) ? 1u : 0u;
-    }
-    const bool stays = lane < W + n_fin && place < W;
-    const unsigned long long worst_m = __ballot(stays && place == W - 1u);
-    const float worst = worst_m ? zs_readlane_f(ps, (uint32_t)__ffsll((long long)worst_m) - 1u) : -INFINITY;
-    const float best = zs_readlane_f(o_score, 0);
-    const bool full = worst > -INFINITY;
-    const bool done = n_live == 0 || (full && (a.early || worst >= best / norm));
-    if (stays) {
-        const bool some = ps > -INFINITY;
-        a.fin_score_o[at + place] = ps;
-        a.fin_length_o[at + place] = some ? pl : 0;
-        a.fin_parent_o[at + place] = some ? pp : -1;
-        a.fin_token_o[at + place] = some ? pt : -1;
-    }
-    if (beam) {
-        a.parent[at + lane] = o_parent;
-        a.token[at + lane] = o_token;
-        a.score_o[at + lane] = o_score;
-    }
-    if (lane == 0) {
-        a.steps_o[g] = was ? steps : steps + 1;
-        a.done_o[g] = was ? was : done ? 1 : 0;
-    }
-}
-
-int bm_merge_launch(const bm_args& a, uint32_t groups, hipStream_t stream) {
-    hipLaunchKernelGGL(zs_k_beam_merge, dim3(groups), dim3(BM_NT), 0, stream, a);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
-}
 
 // ---------------------------------------------------------------------------
 // Reordering in place. A thread owns one column (16, 4, 2 or 1 bytes at the same
@@ -150,6 +10,7 @@ int bm_merge_launch(const bm_args& a, uint32_t groups, hipStream_t stream) {
 // array needs no second copy.
 // ---------------------------------------------------------------------------
 #define RO_NT 256
+#define RO_GLOBAL __attribute__((address_space(1)))
 // n / d for n < 2^31, from ro_div's multiplier
 __device__ __forceinline__ uint32_t ro_quot(uint32_t n, uint32_t mul, uint32_t sh) { return sh >= 32u ? __umulhi(n, mul) >> (sh - 32u) : n; }
 
@@ -168,10 +29,10 @@ __device__ __forceinline__ void ro_column(const bm_state& s, uint64_t col, uint6
     T v[W];
 #pragma unroll
     for (int w = 0; w < W; w++)
-        if (parent[w] != w) v[w] = *reinterpret_cast<const T*>(base + (uint32_t)parent[w] * s.row_stride);
+        if (parent[w] != w) v[w] = __builtin_nontemporal_load((const RO_GLOBAL T*)(base + (uint32_t)parent[w] * s.row_stride));
 #pragma unroll
     for (int w = 0; w < W; w++)
-        if (parent[w] != w) *reinterpret_cast<T*>(base + (uint32_t)w * s.row_stride) = v[w];
+        if (parent[w] != w) __builtin_nontemporal_store(v[w], (RO_GLOBAL T*)(base + (uint32_t)w * s.row_stride));
 }
 
 template <int W>

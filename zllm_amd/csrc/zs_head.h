@@ -159,7 +159,9 @@ __device__ __forceinline__ void hd_put(const hd_args& a, uint64_t r, uint32_t t,
         a.logp[r * a.K + t] = some ? (float)((double)x * a.inv_t - lse) : -INFINITY;
         if (t == 0) a.lse_out[r] = (float)lse;
     } else {
-        a.list[r * a.K + t] = some ? ((unsigned long long)zs_f2u(x) << 32) | (uint32_t)e : ~0ull;
-        if (t == 0) a.lse[r] = lse;
+        // (past the L2, which other parts of the GPU do not share)
+        __hip_atomic_store(a.list + r * a.K + t, some ? ((unsigned long long)zs_f2u(x) << 32) | (uint32_t)e : ~0ull,
+                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (t == 0) __hip_atomic_store(a.lse + r, lse, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
 }

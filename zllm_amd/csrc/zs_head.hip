@@ -11,6 +11,7 @@
 // and sorted.
 #include "zs_head.h"
 #include "zs_select.h"
+#include "zs_beam_merge.h"
 
 // ---------------------------------------------------------------------------
 // the pass
@@ -30,6 +31,7 @@ __global__ __launch_bounds__(HS_NT) void zs_k_head_scan(hd_args a, uint64_t r0) 
     constexpr int E = hd_elem<DT>::E, U = HD_WAVE / 64 / E;
     const uint64_t r = r0 + blockIdx.x / a.chunks;
     const uint32_t chunk = blockIdx.x % a.chunks;
+    if (a.count && chunk == 0 && threadIdx.x == 0 && r % a.width == 0) a.count[r / a.width] = 0;
     if (!hd_live(a, r)) return;
     const hd_row<DT> row(a.logits, a.ld, r, a.V);
     const uint32_t t = threadIdx.x, lane = (uint32_t)zs_lane();
@@ -152,15 +154,13 @@ __device__ __forceinline__ uint32_t hp_places(uint32_t bits, uint32_t* out, uint
 }
 
 template <int DT, bool MASK>
-__global__ __launch_bounds__(HP_NT) void zs_k_head_pick(hd_args a, uint64_t r0, uint32_t lgs) {
+__device__ __forceinline__ void hp_pick(const hd_args& a, uint64_t r, uint32_t lgs) {
     constexpr int E = hd_elem<DT>::E;
     constexpr uint32_t NW = HP_NT / 64;
     __shared__ unsigned long long list[HP_LIST];
     __shared__ uint32_t gl[HP_GL], pl[ZS_TEACHER_KMAX];
     __shared__ uint32_t hist[256], u[4], wthr[NW];
     __shared__ double lse_s;
-    const uint64_t r = r0 + blockIdx.x;
-    if (!hd_live(a, r)) return;
     const hd_row<DT> row(a.logits, a.ld, r, a.V);
     const uint32_t* allow = MASK ? a.allow + r * a.allow_words : nullptr;
     const uint32_t t = threadIdx.x, lane = (uint32_t)zs_lane(), wid = (uint32_t)zs_wid(), K = a.K;
@@ -361,18 +361,41 @@ __global__ __launch_bounds__(HP_NT) void zs_k_head_pick(hd_args a, uint64_t r0, 
     hd_put(a, r, t, t < n ? list[t] : ~0ull, lse_s);
 }
 
-int hd_head_launch(const hd_args& a, uint32_t dtype, hipStream_t stream) {
+// BEAM: the workgroup that is the last of its request's takes the step.
+template <int DT, bool MASK, bool BEAM>
+__global__ __launch_bounds__(HP_NT) void zs_k_head_pick(hd_args a, bm_args m, uint64_t r0, uint32_t lgs) {
+    const uint64_t r = r0 + blockIdx.x;
+    if (hd_live(a, r)) hp_pick<DT, MASK>(a, r, lgs);
+    if (!BEAM) return;
+    __shared__ uint32_t last;
+    const uint32_t g = (uint32_t)(r / a.width);
+    // The list goes past the L2 (hd_put) and is waited for before the count; a
+    // release of the whole L2 by every workgroup took 3 times the pick's time
+    // (32 x 32 beams: 93 us instead of 32).
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
+    __syncthreads();
+    if (threadIdx.x == 0)
+        last = __hip_atomic_fetch_add(&a.count[g], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.width - 1u ? 1u : 0u;
+    __syncthreads();
+    if (!last) return;
+    bm_merge(m, g);
+}
+
+int hd_head_launch(const hd_args& a, const bm_args* m, uint32_t dtype, hipStream_t stream) {
     const uint32_t gs = hd_group_shift(a.V, a.K), lgs = gs - (dtype == ZS_F32 ? 2u : 3u);
     const uint64_t per = HD_BLOCKS / a.chunks;
     for (uint64_t r0 = 0; r0 < a.R; r0 += per) {
         const uint32_t n = (uint32_t)(a.R - r0 < per ? a.R - r0 : per);
+#define HP_GO(DT, MASK)                                                                                                            \
+    if (m) hipLaunchKernelGGL((zs_k_head_pick<DT, MASK, true>), dim3(n), dim3(HP_NT), 0, stream, a, *m, r0, lgs);                   \
+    else hipLaunchKernelGGL((zs_k_head_pick<DT, MASK, false>), dim3(n), dim3(HP_NT), 0, stream, a, bm_args{}, r0, lgs);
 #define HS_GO(DT, LG)                                                                                                              \
     if (a.allow) {                                                                                                                 \
         hipLaunchKernelGGL((zs_k_head_scan<DT, LG, true>), dim3(n * a.chunks), dim3(HS_NT), 0, stream, a, r0);                     \
-        hipLaunchKernelGGL((zs_k_head_pick<DT, true>), dim3(n), dim3(HP_NT), 0, stream, a, r0, lgs);                               \
+        HP_GO(DT, true)                                                                                                            \
     } else {                                                                                                                       \
         hipLaunchKernelGGL((zs_k_head_scan<DT, LG, false>), dim3(n * a.chunks), dim3(HS_NT), 0, stream, a, r0);                    \
-        hipLaunchKernelGGL((zs_k_head_pick<DT, false>), dim3(n), dim3(HP_NT), 0, stream, a, r0, lgs);                              \
+        HP_GO(DT, false)                                                                                                           \
     }
 #define HS_GS(DT, L4)                                                                                                              \
     if (gs == 4) { HS_GO(DT, L4) } else if (gs == 6) { HS_GO(DT, L4 * 4) } else { HS_GO(DT, L4 * 16) }

@@ -27,6 +27,7 @@ struct hd_args {
     uint32_t width;
     unsigned long long* list;   // [R][K]
     double* lse;                // [R]
+    uint32_t* count;            // [R / width] rows of the request that are done (cleared by the pass)
     // the pass: group maxima and, per wave, (maximum, sum exp((x - maximum) / T))
     uint32_t chunks;            // workgroups a row
     uint32_t gstride, recs;     // groups and records a row
@@ -37,7 +38,8 @@ struct hd_args {
     float* logp;
     float* lse_out;
 };
-int hd_head_launch(const hd_args& a, uint32_t dtype, hipStream_t stream);
+struct bm_args;
+int hd_head_launch(const hd_args& a, const bm_args* beam, uint32_t dtype, hipStream_t stream);   // beam: the step too
 
 // log2 of the values in a group: 64, or 16 where a row has few groups for the
 // list that is wanted (a threshold from group maxima is close only when there
@@ -66,6 +68,8 @@ inline uint64_t hd_work(hd_args& a, void* work, bool beam) {
         p += hd_pad(a.R * a.K * 8u);
         a.lse = (double*)p;
         p += hd_pad(a.R * 8u);
+        a.count = (uint32_t*)p;
+        p += hd_pad(a.R * 4u);
     }
     return (uint64_t)(p - (char*)work);
 }
