@@ -1192,8 +1192,8 @@ extern "C" int zs_beam_reorder(zs_ctx* ctx, uint32_t groups, uint32_t width, con
             o.total = o.cols * s.n_inner * s.n_outer;
             o.first = blocks;
             o.blocks = ro_blocks(o.total, groups);
-            ro_div(o.cols, o.mul_cols, o.sh_cols);
-            ro_div(o.n_inner, o.mul_inner, o.sh_inner);
+            o.by_cols = zs_div_of(o.cols);
+            o.by_inner = zs_div_of(o.n_inner);
             blocks += o.blocks;
         }
         if (a.n) rc = ro_launch(a, blocks, groups, (hipStream_t)stream);

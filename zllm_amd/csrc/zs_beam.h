@@ -1,7 +1,7 @@
 // zs_beam.h -- kernel arguments of the beam step and of the reordering.
 #pragma once
 #include <hip/hip_runtime.h>
-#include "zs_internal.h"
+#include "zs_head_args.h"
 
 struct bm_args {
     uint32_t width, K, n_eos, early;
@@ -23,7 +23,7 @@ struct bm_state {
     char* base;
     uint64_t row_stride, outer_stride, inner_stride, cols, total;
     uint32_t n_inner, unit, first, blocks;   // blocks [first, first + blocks) of the launch
-    uint32_t mul_cols, sh_cols, mul_inner, sh_inner;   // ro_div of cols and n_inner (total < 2^31)
+    zs_div by_cols, by_inner;                // (total < 2^31)
 };
 struct ro_args {
     const int32_t* parent;
@@ -31,16 +31,6 @@ struct ro_args {
     bm_state s[ZS_REORDER_BATCH];
 };
 int ro_launch(const ro_args& a, uint32_t blocks, uint32_t groups, hipStream_t stream);
-// n / d = mulhi(n, mul) >> (sh - 32) for n < 2^31, d >= 2: mul = ceil(2^sh / d)
-// with 2^sh the first power at or above 2^31 d; the excess e = mul d - 2^sh < d
-// then gives n e < 2^31 d <= 2^sh. sh 0: d is 1.
-inline void ro_div(uint64_t d, uint32_t& mul, uint32_t& sh) {
-    mul = sh = 0;
-    if (d <= 1 || d >= 1ull << 31) return;   // (rows of 2^31 columns divide in 64 bits)
-    sh = 31;
-    while (1ull << (sh - 31) < d) sh++;
-    mul = (uint32_t)(((1ull << sh) + d - 1) / d);
-}
 // Workgroups for `total` columns of a group's rows: a column per thread up to
 // about 32 workgroups a CU over all groups, loops past that.
 inline uint32_t ro_blocks(uint64_t total, uint32_t groups) {

@@ -11,15 +11,12 @@
 // ---------------------------------------------------------------------------
 #define RO_NT 256
 #define RO_GLOBAL __attribute__((address_space(1)))
-// n / d for n < 2^31, from ro_div's multiplier
-__device__ __forceinline__ uint32_t ro_quot(uint32_t n, uint32_t mul, uint32_t sh) { return sh >= 32u ? __umulhi(n, mul) >> (sh - 32u) : n; }
-
 template <class T, int W>
 __device__ __forceinline__ void ro_column(const bm_state& s, uint64_t col, uint64_t row0, const int (&parent)[W]) {
     uint64_t blk, o;
     if (s.total < 1ull << 31) {
-        blk = ro_quot((uint32_t)col, s.mul_cols, s.sh_cols);
-        o = ro_quot((uint32_t)blk, s.mul_inner, s.sh_inner);
+        blk = zs_quot((uint32_t)col, s.by_cols);
+        o = zs_quot((uint32_t)blk, s.by_inner);
     } else {
         blk = col / s.cols;
         o = blk / s.n_inner;
@@ -62,10 +59,10 @@ __global__ __launch_bounds__(RO_NT) void zs_k_beam_reorder(ro_args a_) {
     s.cols = a->s[i].cols;
     s.total = a->s[i].total;
     s.n_inner = a->s[i].n_inner;
-    s.mul_cols = a->s[i].mul_cols;
-    s.sh_cols = a->s[i].sh_cols;
-    s.mul_inner = a->s[i].mul_inner;
-    s.sh_inner = a->s[i].sh_inner;
+    s.by_cols.mul = a->s[i].by_cols.mul;
+    s.by_cols.sh = a->s[i].by_cols.sh;
+    s.by_inner.mul = a->s[i].by_inner.mul;
+    s.by_inner.sh = a->s[i].by_inner.sh;
     const uint32_t first = a->s[i].first, blocks = a->s[i].blocks, unit = a->s[i].unit;
     const uint64_t row0 = (uint64_t)g * width;
     for (uint64_t col = (uint64_t)(blockIdx.x - first) * RO_NT + threadIdx.x; col < s.total; col += (uint64_t)blocks * RO_NT) {

@@ -33,10 +33,12 @@ struct ds_args {
     uint64_t ld_grad;
     // scratch
     uint32_t chunks, recs;   // workgroups and records a row
+    zs_div by_chunks;
     float4* rec;             // [N][recs] per wave: maximum, sums at T and at 1, the first outside the list
     ds_coef* coef;           // [N]
     float* p;                // [N][K] probability of an entry's id (an id listed twice has both), -1 for absent entries
 };
+#define DS_WAVE 2048         // values of a row that a wave takes
 #define DS_LOSS 1
 #define DS_GRAD 2
 int ds_launch(const ds_args& a, uint32_t dtype, int what, hipStream_t stream);
@@ -45,7 +47,8 @@ int ds_launch(const ds_args& a, uint32_t dtype, int what, hipStream_t stream);
 inline uint64_t ds_work(ds_args& a, void* work) {
     char* p = (char*)work;
     a.chunks = (a.V + 7u + HD_CHUNK - 1u) / HD_CHUNK;
-    a.recs = a.chunks * (HD_CHUNK / HD_WAVE);
+    a.recs = a.chunks * (HD_CHUNK / DS_WAVE);
+    a.by_chunks = zs_div_of(a.chunks);
     a.rec = (float4*)p;
     p += hd_pad(a.N * a.recs * sizeof(float4));
     a.coef = (ds_coef*)p;

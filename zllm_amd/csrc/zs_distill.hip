@@ -27,23 +27,10 @@ __device__ __forceinline__ bool ds_skip(const ds_args& a, uint64_t r) { return a
 template <int DT, int U>
 __device__ __forceinline__ void ds_load(const hd_row<DT>& row, uint32_t first, float (&x)[U][hd_elem<DT>::E]) {
     constexpr int E = hd_elem<DT>::E;
-    const uint32_t j0 = first + threadIdx.x;
-    if (row.inside(first) && row.inside(first + U * DS_NT - 1u)) {
-        uint4 v[U];
+    hd_u4 v[U];
+    row.take(first + threadIdx.x, DS_NT, row.inside(first) && row.inside(first + U * DS_NT - 1u), v);
 #pragma unroll
-        for (int u = 0; u < U; u++) v[u] = row.once(j0 + (uint32_t)u * DS_NT);
-#pragma unroll
-        for (int u = 0; u < U; u++) hd_unpack<DT>(v[u], x[u]);
-    } else {
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const uint32_t j = j0 + (uint32_t)u * DS_NT;
-            if (j < row.nvec) row.get(j, x[u], -INFINITY);
-            else
-#pragma unroll
-                for (int q = 0; q < E; q++) x[u][q] = -INFINITY;
-        }
-    }
+    for (int u = 0; u < U; u++) hd_unpack<DT>(v[u], x[u]);
 }
 
 // ---------------------------------------------------------------------------
@@ -51,10 +38,10 @@ __device__ __forceinline__ void ds_load(const hd_row<DT>& row, uint32_t first, f
 // ---------------------------------------------------------------------------
 template <int DT, bool TAIL, bool TWO>
 __global__ __launch_bounds__(DS_NT) void zs_k_distill_scan(ds_args a, uint64_t r0) {
-    constexpr int E = hd_elem<DT>::E, U = HD_WAVE / 64 / E;
+    constexpr int E = hd_elem<DT>::E, U = DS_WAVE / 64 / E;
     __shared__ uint32_t mask[U * DS_NT / 4];   // a byte a vector: its ids in the list
-    const uint64_t r = r0 + blockIdx.x / a.chunks;
-    const uint32_t chunk = blockIdx.x % a.chunks, t = threadIdx.x;
+    const uint32_t n = zs_quot(blockIdx.x, a.by_chunks), chunk = blockIdx.x - n * a.chunks, t = threadIdx.x;
+    const uint64_t r = r0 + n;
     const hd_row<DT> row(a.logits, a.ld, r, a.V);
     const uint32_t first = chunk * (U * DS_NT);
     if (first >= row.nvec || ds_skip(a, r)) return;
@@ -112,7 +99,7 @@ __global__ __launch_bounds__(DS_NT) void zs_k_distill_scan(ds_args a, uint64_t r
     float none;
     sums(a.c, s, so, true);
     if (TWO) sums((float)HD_LOG2E, s1, none, false);
-    if (zs_lane() == 0) a.rec[r * a.recs + chunk * (HD_CHUNK / HD_WAVE) + (uint32_t)zs_wid()] = make_float4(m, s, s1, so);
+    if (zs_lane() == 0) a.rec[r * a.recs + chunk * (HD_CHUNK / DS_WAVE) + (uint32_t)zs_wid()] = make_float4(m, s, s1, so);
 }
 
 // ---------------------------------------------------------------------------
@@ -233,7 +220,7 @@ __global__ __launch_bounds__(DF_NT) void zs_k_distill_row(ds_args a, uint64_t r0
     if (WHAT & DS_LOSS) {
         const float xk = l.there ? row.at(l.id) : 0.0f, xl = a.labels && !bad_label ? row.at((uint32_t)label) : NAN;
         constexpr int E = hd_elem<DT>::E;
-        const uint32_t recs = (row.nvec * E + HD_CHUNK - 1u) / HD_CHUNK * (HD_CHUNK / HD_WAVE);
+        const uint32_t recs = (row.nvec * E + HD_CHUNK - 1u) / HD_CHUNK * (HD_CHUNK / DS_WAVE);
         const float4* rec = a.rec + r * a.recs;
         float mf = -INFINITY;
         for (uint32_t i = t; i < recs; i += DF_NT) mf = fmaxf(mf, rec[i].x);
@@ -290,10 +277,10 @@ template <int DT>
 __device__ __forceinline__ void ds_store(typename hd_elem<DT>::T* grad, uint32_t V, bool whole, int i0, const float (&y)[hd_elem<DT>::E]) {
     constexpr int E = hd_elem<DT>::E;
     if (whole) {
-        uint4 v;
-        if constexpr (DT == ZS_F32) v = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
-        else v = make_uint4(hd_pack2<DT>(y[0], y[1]), hd_pack2<DT>(y[2], y[3]), hd_pack2<DT>(y[E / 2], y[E / 2 + 1]), hd_pack2<DT>(y[E - 2], y[E - 1]));
-        *reinterpret_cast<uint4*>(grad + i0) = v;
+        hd_u4 v;
+        if constexpr (DT == ZS_F32) v = hd_u4{__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])};
+        else v = hd_u4{hd_pack2<DT>(y[0], y[1]), hd_pack2<DT>(y[2], y[3]), hd_pack2<DT>(y[E / 2], y[E / 2 + 1]), hd_pack2<DT>(y[E - 2], y[E - 1])};
+        *reinterpret_cast<hd_u4*>(grad + i0) = v;
     } else {
 #pragma unroll
         for (int q = 0; q < E; q++)
@@ -314,13 +301,13 @@ __device__ __forceinline__ float ds_at(const ds_coef& k, float x, bool listed, f
 // arrive in order: no test per vector, and nothing is waited for.
 template <int DT, bool TWO>
 __global__ __launch_bounds__(DS_NT) void zs_k_distill_grad(ds_args a, uint64_t r0) {
-    constexpr int E = hd_elem<DT>::E, U = HD_WAVE / 64 / E;
+    constexpr int E = hd_elem<DT>::E, U = DS_WAVE / 64 / E;
     typedef typename hd_elem<DT>::T T;
     __shared__ uint32_t hid[DS_K + 1];
     __shared__ float hy[DS_K + 1];
     __shared__ uint32_t hits;
-    const uint64_t r = r0 + blockIdx.x / a.chunks;
-    const uint32_t chunk = blockIdx.x % a.chunks, t = threadIdx.x;
+    const uint32_t n = zs_quot(blockIdx.x, a.by_chunks), chunk = blockIdx.x - n * a.chunks, t = threadIdx.x;
+    const uint64_t r = r0 + n;
     const hd_row<DT> row(a.logits, a.ld, r, a.V);
     const uint32_t first = chunk * (U * DS_NT);
     if (first >= row.nvec) return;
@@ -413,11 +400,11 @@ __global__ __launch_bounds__(FU_NT, 4) void zs_k_distill_fused(ds_args a, uint64
     const uint32_t lo = row.shift ? 1u : 0u, hi = (a.V + row.shift) / E - 1u;
     const uint32_t edge = t == 0 ? 0u : row.nvec - 1u;
     const bool has_edge = t < 2u && (t == 0 ? lo > 0u : hi + 1u < row.nvec);
-    auto fetch = [&](uint32_t b, uint4 (&v)[U]) {
+    auto fetch = [&](uint32_t b, hd_u4 (&v)[U]) {
 #pragma unroll
         for (int u = 0; u < U; u++) v[u] = row.load(min(max(b * BV + t + (uint32_t)u * FU_NT, lo), hi));
     };
-    auto unpack = [&](const uint4 (&v)[U], uint32_t b, float (&x)[U][E]) {
+    auto unpack = [&](const hd_u4 (&v)[U], uint32_t b, float (&x)[U][E]) {
 #pragma unroll
         for (int u = 0; u < U; u++) hd_unpack<DT>(v[u], x[u]);
         if (b * BV < lo || b * BV + BV - 1u > hi) {
@@ -429,7 +416,7 @@ __global__ __launch_bounds__(FU_NT, 4) void zs_k_distill_fused(ds_args a, uint64
             }
         }
     };
-    uint4 cur[U], nxt[U];
+    hd_u4 cur[U], nxt[U];
     fetch(0, cur);
     if (TAIL)
         for (uint32_t i = t; i < nb * (BV / 4); i += FU_NT) mask[i] = 0;

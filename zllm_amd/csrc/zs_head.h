@@ -12,6 +12,7 @@
 // row's first element, and the ids of vector j are j * E - shift + q. Only the
 // first and the last vector can hold ids outside the row; those two are read
 // element by element, so that nothing outside the row is touched.
+typedef uint32_t hd_u4 __attribute__((ext_vector_type(4)));
 template <int DT> struct hd_elem;
 template <> struct hd_elem<ZS_F32> { typedef float T; static constexpr int E = 4; };
 template <> struct hd_elem<ZS_F16> { typedef _Float16 T; static constexpr int E = 8; };
@@ -22,7 +23,7 @@ __device__ __forceinline__ float hd_float(_Float16 v) { return (float)v; }
 __device__ __forceinline__ float hd_float(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 
 template <int DT>
-__device__ __forceinline__ void hd_unpack(const uint4& v, float (&x)[hd_elem<DT>::E]) {
+__device__ __forceinline__ void hd_unpack(const hd_u4& v, float (&x)[hd_elem<DT>::E]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -67,15 +68,13 @@ struct hd_row {
     }
     __device__ __forceinline__ int id0(uint32_t j) const { return (int)(j * E) - (int)shift; }
     __device__ __forceinline__ bool inside(uint32_t j) const { const int i = id0(j); return i >= 0 && (uint32_t)i + E <= V; }
+    __device__ __forceinline__ hd_u4 load(uint32_t j) const { return zs_gload(reinterpret_cast<const hd_u4*>(row + id0(j))); }
     // one that is not read again (7.2 TB/s of a large read where plain loads reach 6.5)
-    __device__ __forceinline__ uint4 once(uint32_t j) const {
-        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-        const u4 v = __builtin_nontemporal_load((const __attribute__((address_space(1))) u4*)(row + id0(j)));
-        return make_uint4(v.x, v.y, v.z, v.w);
+    __device__ __forceinline__ hd_u4 once(uint32_t j) const {
+        return __builtin_nontemporal_load((const __attribute__((address_space(1))) hd_u4*)(row + id0(j)));
     }
-    __device__ __forceinline__ uint4 load(uint32_t j) const { return zs_gload(reinterpret_cast<const uint4*>(row + id0(j))); }
     // the vector as it stands, -inf where it has no id of the row
-    __device__ __forceinline__ uint4 raw(uint32_t j) const {
+    __device__ __forceinline__ hd_u4 raw(uint32_t j) const {
         if (inside(j)) return load(j);
         uint32_t w[4];
         const int i = id0(j);
@@ -91,9 +90,40 @@ struct hd_row {
                 w[k] = lo | hi << 16;
             }
         }
-        return make_uint4(w[0], w[1], w[2], w[3]);
+        const hd_u4 v = {w[0], w[1], w[2], w[3]};
+        return v;
     }
     __device__ __forceinline__ float at(uint32_t id) const { return hd_float(zs_gload(row + id)); }
+    // a vector of no ids
+    static __device__ __forceinline__ hd_u4 none() {
+        constexpr uint32_t w = DT == ZS_F32 ? 0xff800000u : DT == ZS_F16 ? 0xfc00fc00u : 0xff80ff80u;
+        const hd_u4 v = {w, w, w, w};
+        return v;
+    }
+    // vectors j, j + step, ... of a workgroup, -inf where they have no id of
+    // the row; the loads are in flight together
+    template <int U>
+    __device__ __forceinline__ void take(uint32_t j, uint32_t step, bool whole, hd_u4 (&v)[U]) const {
+        if (whole) {
+#pragma unroll
+            for (int u = 0; u < U; u++) v[u] = once(j + (uint32_t)u * step);
+            return;
+        }
+        // whole vectors lo .. hi, if any, and those before and behind them
+        const uint32_t lo = shift ? 1u : 0u, hi = (V + shift) / E;   // (hi: one behind)
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t i = j + (uint32_t)u * step;
+            v[u] = none();
+            if (i >= lo && i < hi) v[u] = once(i);
+        }
+        if (lo > 0u && j == 0u) v[0] = raw(0);
+        if (hi + 1u == nvec && hi >= lo && (nvec - 1u - j) % step == 0u && nvec - 1u >= j) {
+            const hd_u4 w = raw(nvec - 1u);
+#pragma unroll
+            for (int u = 0; u < U; u++) v[u] = j + (uint32_t)u * step == nvec - 1u ? w : v[u];
+        }
+    }
     // the vector's values; `none` where it has no id of the row
     __device__ __forceinline__ void get(uint32_t j, float (&x)[E], float none) const {
         if (inside(j)) {
@@ -147,7 +177,7 @@ __device__ __forceinline__ double hd_lse(float m, double inv_t, double sum) { re
 
 // Is row r's head wanted?
 __device__ __forceinline__ bool hd_live(const hd_args& a, uint64_t r) {
-    return !a.scores || (!a.done[r / a.width] && fabsf(a.scores[r]) <= __FLT_MAX__);
+    return !a.scores || (!a.done[zs_quot((uint32_t)r, a.by_width)] && fabsf(a.scores[r]) <= __FLT_MAX__);   // (beams' rows number below 2^31)
 }
 // Entry t of row r, e = ~key << 32 | id (~0: none); by threads t < K.
 __device__ __forceinline__ void hd_put(const hd_args& a, uint64_t r, uint32_t t, unsigned long long e, double lse) {

@@ -18,69 +18,80 @@
 // ---------------------------------------------------------------------------
 #define HS_NT 256
 
-// Maximum over lanes whose numbers differ in the bits FROM .. TO / 2.
-template <int FROM, int TO>
-__device__ __forceinline__ float hs_max(float v) {
-    if constexpr (FROM < TO) return hs_max<FROM * 2, TO>(fmaxf(v, zs_lane_xor<FROM>(v)));
-    else return v;
+// A value's key for maxima: 0 for what is not above -inf, after hs_cut.
+__device__ __forceinline__ uint32_t hs_key(float v) {
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return b ^ (uint32_t)((int)b >> 31 | (int)0x80000000);
+}
+__device__ __forceinline__ uint32_t hs_cut(uint32_t k) { return k > 0x007fffffu ? k : 0u; }   // (-inf's)
+// Maximum over LG neighbouring lanes (of integers: the move is part of the
+// maximum's instruction; of floats it takes two more).
+template <int CTRL>
+__device__ __forceinline__ uint32_t hs_dpp(uint32_t k) {
+    return max(k, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)k, CTRL, 0xf, 0xf, false));
+}
+template <int LG>
+__device__ __forceinline__ uint32_t hs_max(uint32_t k) {
+    if constexpr (LG >= 2) k = hs_dpp<0xB1>(k);     // quad_perm [1,0,3,2]
+    if constexpr (LG >= 4) k = hs_dpp<0x4E>(k);     // quad_perm [2,3,0,1]
+    if constexpr (LG >= 8) k = hs_dpp<0x141>(k);    // row_half_mirror
+    if constexpr (LG >= 16) k = hs_dpp<0x140>(k);   // row_mirror
+    if constexpr (LG >= 32) k = max(k, zs_lane_xor<16>(k));
+    if constexpr (LG >= 64) k = max(k, zs_lane_xor<32>(k));
+    return k;
 }
 
-// LG: lanes of a group
+// LG: lanes of a group. The exponentials and what goes with them bound the
+// pass over 16-bit values, not their bytes: a value takes one shift or mask,
+// half a maximum, one fma, one exponential (a quarter of the rate) and one
+// addition; sums are relative to each thread's own maximum.
 template <int DT, int LG, bool MASK>
 __global__ __launch_bounds__(HS_NT) void zs_k_head_scan(hd_args a, uint64_t r0) {
     constexpr int E = hd_elem<DT>::E, U = HD_WAVE / 64 / E;
-    const uint64_t r = r0 + blockIdx.x / a.chunks;
-    const uint32_t chunk = blockIdx.x % a.chunks;
-    if (a.count && chunk == 0 && threadIdx.x == 0 && r % a.width == 0) a.count[r / a.width] = 0;
+    const uint32_t n = zs_quot(blockIdx.x, a.by_chunks), chunk = blockIdx.x - n * a.chunks;
+    const uint64_t r = r0 + n;
+    if (a.count && chunk == 0 && threadIdx.x == 0) {
+        const uint32_t g = zs_quot((uint32_t)r, a.by_width);
+        if (g * a.width == (uint32_t)r) a.count[g] = 0;
+    }
     if (!hd_live(a, r)) return;
     const hd_row<DT> row(a.logits, a.ld, r, a.V);
     const uint32_t t = threadIdx.x, lane = (uint32_t)zs_lane();
     const uint32_t first = chunk * (U * HS_NT), j0 = first + t;
     if (first >= row.nvec) return;
-    float x[U][E];
-    if (row.inside(first) && row.inside(first + U * HS_NT - 1u)) {
-        uint4 v[U];
+    uint32_t g[U];
+    float m, s;
+    auto pass = [&](bool clean) {
+        float x[U][E];
+        {
+            hd_u4 v[U];
+            row.take(j0, HS_NT, row.inside(first) && row.inside(first + U * HS_NT - 1u), v);
+            uint32_t b[U];
+            if (MASK) {
+                const uint32_t* allow = a.allow + r * a.allow_words;
 #pragma unroll
-        for (int u = 0; u < U; u++) v[u] = row.once(j0 + (uint32_t)u * HS_NT);
+                for (int u = 0; u < U; u++) b[u] = hd_allow<E>(allow, a.allow_words, row.id0(j0 + (uint32_t)u * HS_NT));
+            }
 #pragma unroll
-        for (int u = 0; u < U; u++) hd_unpack<DT>(v[u], x[u]);
-    } else {
+            for (int u = 0; u < U; u++) {
+                hd_unpack<DT>(v[u], x[u]);
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const uint32_t j = j0 + (uint32_t)u * HS_NT;
-            if (j < row.nvec) row.get(j, x[u], -INFINITY);
-            else
-#pragma unroll
-                for (int q = 0; q < E; q++) x[u][q] = -INFINITY;
+                for (int q = 0; q < E; q++) {
+                    if (MASK) x[u][q] = b[u] >> q & 1u ? x[u][q] : -INFINITY;
+                    if (clean) x[u][q] = hd_clean(x[u][q]);
+                }
+            }
         }
-    }
-    if (MASK) {
-        const uint32_t* allow = a.allow + r * a.allow_words;
-        uint32_t b[U];
-#pragma unroll
-        for (int u = 0; u < U; u++) b[u] = hd_allow<E>(allow, a.allow_words, row.id0(j0 + (uint32_t)u * HS_NT));
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int q = 0; q < E; q++) x[u][q] = b[u] >> q & 1u ? x[u][q] : -INFINITY;
-    }
-    float g[U], m;
-    auto maxima = [&]() {
         m = -INFINITY;
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            float v = x[u][0];
+            float vm = x[u][0];
 #pragma unroll
-            for (int q = 1; q < E; q++) v = fmaxf(v, x[u][q]);
-            g[u] = hs_max<1, LG>(v);
-            m = fmaxf(m, g[u]);
+            for (int q = 1; q < E; q++) vm = fmaxf(vm, x[u][q]);
+            m = fmaxf(m, vm);
+            g[u] = hs_key(vm);
         }
-        m = hs_max<LG, 64>(m);
-    };
-    maxima();
-    // 2^(x c - mc): one fma a value; mc's rounding is a factor of all of them
-    float s;
-    auto sum = [&]() {
+        // 2^(x c - mc): one fma a value; mc's rounding is a factor of all of them
         const float mr = m > -INFINITY ? m : 0.0f, c = hd_factor(mr, a.c), mc = mr * c;
         s = 0.0f;
 #pragma unroll
@@ -90,29 +101,27 @@ __global__ __launch_bounds__(HS_NT) void zs_k_head_scan(hd_args a, uint64_t r0) 
             for (int q = 0; q < E; q++) e[q] = __builtin_amdgcn_exp2f(fmaf(x[u][q], c, -mc));
             s += hd_sum(e);
         }
-        s = zs_wave_reduce(s, [](float p, float q) { return p + q; }) * __builtin_amdgcn_exp2f(-fmaf(mr, c, -mc));
+        const float M = wave_max_f(m), Mr = M > -INFINITY ? M : 0.0f, cM = hd_factor(Mr, a.c), Mc = Mr * cM;
+        s *= m == M ? 1.0f : m > -INFINITY && c == cM ? __builtin_amdgcn_exp2f(mc - Mc) : 0.0f;
+        m = M;
+        s = zs_wave_reduce(s, [](float p, float q) { return p + q; }) * __builtin_amdgcn_exp2f(-fmaf(Mr, cM, -Mc));
     };
-    sum();
-    if (!(s < INFINITY)) {   // NaN or +inf among the values
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int q = 0; q < E; q++) x[u][q] = hd_clean(x[u][q]);
-        maxima();
-        sum();
-    }
-    if (lane == 0) a.rec[r * a.recs + chunk * (HS_NT / 64) + (uint32_t)zs_wid()] = make_float2(m, s);
+    pass(false);
+    if (!(s < INFINITY)) pass(true);   // NaN or +inf among the values
+    if (lane == 0) a.rec[r * a.recs + chunk * (HD_CHUNK / HD_WAVE) + (uint32_t)zs_wid()] = make_float2(m, s);
     // a group's lanes store their vectors' groups in turn
     uint32_t* gmax = a.gmax + r * a.gstride;
     constexpr int ST = LG < U ? LG : U;
     const uint32_t i = lane & (uint32_t)(LG - 1);
 #pragma unroll
-    for (int u = 0; u < U; u += ST) {
-        float v = g[u];
+    for (int u = 0; u < U; u++) g[u] = hs_max<LG>(g[u]);
 #pragma unroll
-        for (int k = 1; k < ST; k++) v = i == (uint32_t)k ? g[u + k] : v;
+    for (int u = 0; u < U; u += ST) {
+        uint32_t k = g[u];
+#pragma unroll
+        for (int w = 1; w < ST; w++) k = i == (uint32_t)w ? g[u + w] : k;
         const uint32_t j = j0 + ((uint32_t)u + i) * HS_NT;
-        if (i < (uint32_t)ST && j - i < row.nvec) gmax[j / LG] = hd_key(v);
+        if (i < (uint32_t)ST && j - i < row.nvec) gmax[j / LG] = hs_cut(k);
     }
 }
 
@@ -243,7 +252,7 @@ __device__ __forceinline__ void hp_pick(const hd_args& a, uint64_t r, uint32_t l
         constexpr int NU = 4;
         const bool wide = row.nvec >= 3u;
         for (uint32_t i0 = 0; i0 < nit; i0 += NU * HP_NT) {
-            uint4 v[NU];
+            hd_u4 v[NU];
             uint32_t jv[NU];
 #pragma unroll
             for (int w = 0; w < NU; w++) {
@@ -363,12 +372,12 @@ __device__ __forceinline__ void hp_pick(const hd_args& a, uint64_t r, uint32_t l
 
 // BEAM: the workgroup that is the last of its request's takes the step.
 template <int DT, bool MASK, bool BEAM>
-__global__ __launch_bounds__(HP_NT) void zs_k_head_pick(hd_args a, bm_args m, uint64_t r0, uint32_t lgs) {
+__global__ __launch_bounds__(HP_NT, BEAM ? 7 : 8) void zs_k_head_pick(hd_args a, bm_args m, uint64_t r0, uint32_t lgs) {
     const uint64_t r = r0 + blockIdx.x;
     if (hd_live(a, r)) hp_pick<DT, MASK>(a, r, lgs);
     if (!BEAM) return;
     __shared__ uint32_t last;
-    const uint32_t g = (uint32_t)(r / a.width);
+    const uint32_t g = zs_quot((uint32_t)r, a.by_width);
     // The list goes past the L2 (hd_put) and is waited for before the count; a
     // release of the whole L2 by every workgroup took 3 times the pick's time
     // (32 x 32 beams: 93 us instead of 32).

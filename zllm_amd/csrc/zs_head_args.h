@@ -5,14 +5,32 @@
 #include "zs_internal.h"
 
 #define HD_KMAX 128            // entries of a head at most
-#define HD_WAVE 2048           // values of a row that a wave of the pass takes
-#define HD_CHUNK (4 * HD_WAVE) // and a workgroup
+#define HD_WAVE 2048           // values of a row that a wave of the head's pass takes
+#define HD_CHUNK 8192          // values that a workgroup takes
 #define HD_GROUPS 5120         // groups of a row at most (the pick holds their maxima in registers)
 #define HD_BLOCKS (1u << 22)   // workgroups per launch at most
 
 // The heads of R rows. For a teacher (d_ids) the list goes out as ids and
 // log-probabilities; for the beam step into `list` (bits of x~ << 32 | id,
 // ~0 for none) and `lse`, of the rows whose beam lives.
+// n / d for n < 2^31 by a product: n / d = mulhi(n, mul) >> (sh - 32), d >= 2,
+// with mul = ceil(2^sh / d) and 2^sh the first power at or above 2^31 d (the
+// excess e = mul d - 2^sh < d gives n e < 2^31 d <= 2^sh). sh 0: d is 1.
+struct zs_div {
+    uint32_t mul, sh;
+};
+inline zs_div zs_div_of(uint64_t d) {
+    zs_div q = {0, 0};
+    if (d <= 1 || d >= 1ull << 31) return q;
+    q.sh = 31;
+    while (1ull << (q.sh - 31) < d) q.sh++;
+    q.mul = (uint32_t)(((1ull << q.sh) + d - 1) / d);
+    return q;
+}
+#if defined(__HIPCC__)
+__device__ __forceinline__ uint32_t zs_quot(uint32_t n, zs_div q) { return q.sh ? __umulhi(n, q.mul) >> (q.sh - 32u) : n; }
+#endif
+
 struct hd_args {
     const void* logits;
     uint64_t ld, R;
@@ -30,6 +48,7 @@ struct hd_args {
     uint32_t* count;            // [R / width] rows of the request that are done (cleared by the pass)
     // the pass: group maxima and, per wave, (maximum, sum exp((x - maximum) / T))
     uint32_t chunks;            // workgroups a row
+    zs_div by_chunks, by_width;
     uint32_t gstride, recs;     // groups and records a row
     uint32_t* gmax;             // [R][gstride] keys
     float2* rec;                // [R][recs]
@@ -58,6 +77,8 @@ inline uint64_t hd_work(hd_args& a, void* work, bool beam) {
     const uint32_t gs = hd_group_shift(a.V, a.K);
     a.chunks = (a.V + 7u + HD_CHUNK - 1u) / HD_CHUNK;
     a.recs = a.chunks * (HD_CHUNK / HD_WAVE);
+    a.by_chunks = zs_div_of(a.chunks);
+    a.by_width = zs_div_of(a.width);
     a.gstride = (a.V + 7u + (1u << gs) - 1u) >> gs;
     a.gmax = (uint32_t*)p;
     p += hd_pad(a.R * a.gstride * 4u);
