@@ -62,26 +62,32 @@ __device__ __forceinline__ void bm_merge(const bm_args& a, uint32_t g) {
     }
     __syncthreads();
     if (lane >= 64u) return;
-    // the beam's next candidate and the one behind it
+    // the key of the beam's next candidate (0: none) and the one behind it
     float s = -INFINITY, s2 = -INFINITY;
-    uint32_t id = 0, id2 = 0, next = 0;
+    uint32_t id = 0, id2 = 0, next = 0, key = 0;
     auto ahead = [&]() {
         const bool some = beam && next < K;
         s2 = some ? cs_[lane * K + next] : -INFINITY;
         id2 = some ? ci_[lane * K + next] : 0u;
         next++;
     };
+    auto step = [&]() {
+        s = s2;
+        id = id2;
+        key = s > -INFINITY ? zs_total_key(s + 0.0f) : 0u;
+        ahead();
+    };
     ahead();
-    s = s2;
-    id = id2;
-    ahead();
+    step();
     int o_parent = -1, o_token = -1;
     float o_score = -INFINITY;
     uint32_t n_live = 0, n_fin = 0;
     for (uint32_t rank = 0; n_live < W; rank++) {
-        const float cs = wave_max_f(s);
-        if (!(cs > -INFINITY)) break;
-        const uint32_t b = (uint32_t)__ffsll((long long)__ballot(s == cs)) - 1u;   // the lowest beam of equals
+        // (beams are in the first 32 lanes: the last lane of the second row has their maximum)
+        const uint32_t top = zs_readlane_u(zs_dpp_max<0x142, 0xa>(zs_group_max<16>(key)), 31);   // row_bcast:15
+        if (!top) break;
+        const uint32_t b = (uint32_t)__builtin_ctzll(__ballot(key == top));   // the lowest beam of equals
+        const float cs = zs_readlane_f(s, b);
         const uint32_t cid = zs_readlane_u(id, b);
         if (cid >> 31) {   // EOS
             if (rank < W) {
@@ -92,11 +98,7 @@ __device__ __forceinline__ void bm_merge(const bm_args& a, uint32_t g) {
             if (lane == n_live) { o_parent = (int)b; o_token = (int)cid; o_score = cs; }
             n_live++;
         }
-        if (lane == b) {
-            s = s2;
-            id = id2;
-            ahead();
-        }
+        if (lane == b) step();
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");   // (one wave from here on)
     // the pool and what finished, the pool first among equals: lane i's place

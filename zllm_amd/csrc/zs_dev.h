@@ -92,6 +92,20 @@ __device__ __forceinline__ uint32_t wave_sum_u(uint32_t v) { return zs_wave_redu
 __device__ __forceinline__ int wave_min_i(int v) { return zs_wave_reduce(v, [](int a, int b) { return min(a, b); }); }
 __device__ __forceinline__ int wave_max_i(int v) { return zs_wave_reduce(v, [](int a, int b) { return max(a, b); }); }
 __device__ __forceinline__ uint32_t wave_or_u(uint32_t v) { return zs_wave_reduce(v, [](uint32_t a, uint32_t b) { return a | b; }); }
+// Unsigned maximum with a lane move that is part of its instruction.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t zs_dpp_max(uint32_t k) {
+    return max(k, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)k, CTRL, ROWS, 0xf, false));
+}
+// Maximum over LG neighbouring lanes (LG a power of two up to 16).
+template <int LG>
+__device__ __forceinline__ uint32_t zs_group_max(uint32_t k) {
+    if constexpr (LG >= 2) k = zs_dpp_max<0xB1>(k);     // quad_perm [1,0,3,2]
+    if constexpr (LG >= 4) k = zs_dpp_max<0x4E>(k);     // quad_perm [2,3,0,1]
+    if constexpr (LG >= 8) k = zs_dpp_max<0x141>(k);    // row_half_mirror
+    if constexpr (LG >= 16) k = zs_dpp_max<0x140>(k);   // row_mirror
+    return k;
+}
 // Inclusive scan (plain add) over the wave.
 __device__ __forceinline__ uint32_t wave_incl_scan_u(uint32_t x) {
     int lane = zs_lane();

@@ -26,16 +26,9 @@ __device__ __forceinline__ uint32_t hs_key(float v) {
 __device__ __forceinline__ uint32_t hs_cut(uint32_t k) { return k > 0x007fffffu ? k : 0u; }   // (-inf's)
 // Maximum over LG neighbouring lanes (of integers: the move is part of the
 // maximum's instruction; of floats it takes two more).
-template <int CTRL>
-__device__ __forceinline__ uint32_t hs_dpp(uint32_t k) {
-    return max(k, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)k, CTRL, 0xf, 0xf, false));
-}
 template <int LG>
 __device__ __forceinline__ uint32_t hs_max(uint32_t k) {
-    if constexpr (LG >= 2) k = hs_dpp<0xB1>(k);     // quad_perm [1,0,3,2]
-    if constexpr (LG >= 4) k = hs_dpp<0x4E>(k);     // quad_perm [2,3,0,1]
-    if constexpr (LG >= 8) k = hs_dpp<0x141>(k);    // row_half_mirror
-    if constexpr (LG >= 16) k = hs_dpp<0x140>(k);   // row_mirror
+    k = zs_group_max<LG < 16 ? LG : 16>(k);
     if constexpr (LG >= 32) k = max(k, zs_lane_xor<16>(k));
     if constexpr (LG >= 64) k = max(k, zs_lane_xor<32>(k));
     return k;
@@ -206,7 +199,10 @@ __device__ __forceinline__ void hp_pick(const hd_args& a, uint64_t r, uint32_t l
         if (lane == 0) lse_s = hd_lse(m, a.inv_t, s);
     }
 #pragma unroll
-    for (int e = 0; e < HP_GPT; e++) tm = max(tm, k[e]);
+    for (int e = 0; e < HP_GPT; e++) {
+        if ((uint32_t)e * HP_NT >= ng) break;
+        tm = max(tm, k[e]);
+    }
     if (t < 4) u[t] = 0;
     // theta: in every wave the ceil(K / waves)-th largest thread maximum; the
     // smallest of them is reached by K groups (1: too few hold a candidate, all
@@ -221,16 +217,21 @@ __device__ __forceinline__ void hp_pick(const hd_args& a, uint64_t r, uint32_t l
     theta = max(theta, 1u);
     uint32_t ngt = 0;
 #pragma unroll
-    for (int e = 0; e < HP_GPT; e++) ngt += k[e] >= theta ? 1u : 0u;
+    for (int e = 0; e < HP_GPT; e++) {
+        if ((uint32_t)e * HP_NT >= ng) break;
+        ngt += k[e] >= theta ? 1u : 0u;
+    }
     uint32_t p = ngt ? atomicAdd(&u[0], ngt) : 0u;
 #pragma unroll
     for (int e = 0; e < HP_GPT; e++) {
+        if ((uint32_t)e * HP_NT >= ng) break;
         if (k[e] < theta) continue;
         if (p < HP_GL) gl[p] = NW * lane + wid + (uint32_t)e * HP_NT;
         p++;
     }
     __syncthreads();
     const uint32_t n_gl = u[0], lm = (1u << lgs) - 1u;
+    const float theta_f = theta > 1u ? zs_key_to_float(theta) : -__FLT_MAX__;
     auto keys_of = [&](const float (&x)[E], uint32_t j, uint32_t (&kq)[E]) {
         uint32_t b = ~0u;
         if (MASK) b = hd_allow<E>(allow, a.allow_words, row.id0(j));
@@ -262,23 +263,25 @@ __device__ __forceinline__ void hp_pick(const hd_args& a, uint64_t r, uint32_t l
             }
 #pragma unroll
             for (int w = 0; w < NU; w++) {
+                if (i0 + (uint32_t)w * HP_NT >= nit) break;
                 const uint32_t j = jv[w];
-                uint32_t kq[E], n = 0;
-                if (wide && row.inside(j)) {
-                    float x[E];
-                    hd_unpack<DT>(v[w], x);
-                    keys_of(x, j, kq);
-                } else if (j < row.nvec) {
-                    keys(j, kq);
-                } else {
+                float x[E];
+                if (wide && row.inside(j)) hd_unpack<DT>(v[w], x);
+                else if (j < row.nvec) row.get(j, x, -INFINITY);
+                else {
 #pragma unroll
-                    for (int q = 0; q < E; q++) kq[q] = 0u;
+                    for (int q = 0; q < E; q++) x[q] = -INFINITY;
                 }
-                // (one atomic a wave: one a lane is served lane by lane)
-                uint32_t p = 0;
+                if (MASK) {
+                    const uint32_t b = j < row.nvec ? hd_allow<E>(allow, a.allow_words, row.id0(j)) : 0u;
+#pragma unroll
+                    for (int q = 0; q < E; q++) x[q] = b >> q & 1u ? x[q] : -INFINITY;
+                }
+                // (one atomic a wave: one a lane is served lane by lane; NaN reaches nothing)
+                uint32_t p = 0, n = 0;
 #pragma unroll
                 for (int q = 0; q < E; q++) {
-                    const unsigned long long m = __ballot(kq[q] >= theta);
+                    const unsigned long long m = __ballot(x[q] >= theta_f);
                     p = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, p));
                     n += (uint32_t)__popcll(m);
                 }
@@ -288,8 +291,8 @@ __device__ __forceinline__ void hp_pick(const hd_args& a, uint64_t r, uint32_t l
                 p += (uint32_t)__builtin_amdgcn_readfirstlane((int)p0);
 #pragma unroll
                 for (int q = 0; q < E; q++) {
-                    if (kq[q] < theta) continue;
-                    if (p < HP_LIST) list[p] = entry(kq[q], j, q);
+                    if (!(x[q] >= theta_f)) continue;
+                    if (p < HP_LIST) list[p] = entry(hd_key(hd_clean(x[q])), j, q);
                     p++;
                 }
             }
@@ -372,7 +375,7 @@ __device__ __forceinline__ void hp_pick(const hd_args& a, uint64_t r, uint32_t l
 
 // BEAM: the workgroup that is the last of its request's takes the step.
 template <int DT, bool MASK, bool BEAM>
-__global__ __launch_bounds__(HP_NT, BEAM ? 7 : 8) void zs_k_head_pick(hd_args a, bm_args m, uint64_t r0, uint32_t lgs) {
+__global__ __launch_bounds__(HP_NT, 6) void zs_k_head_pick(hd_args a, bm_args m, uint64_t r0, uint32_t lgs) {
     const uint64_t r = r0 + blockIdx.x;
     if (hd_live(a, r)) hp_pick<DT, MASK>(a, r, lgs);
     if (!BEAM) return;
