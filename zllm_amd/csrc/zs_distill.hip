@@ -18,7 +18,7 @@
 #define DS_FUSED_ROWS 512
 #endif
 #define DS_FUSED_VOCAB 4096
-#define DS_FUSED_LDS 49152
+#define DS_FUSED_LDS (160 * 1024 - 6400)   // what the kernel's own shared memory leaves
 
 // A row that takes no part: its label is ignore_index.
 __device__ __forceinline__ bool ds_skip(const ds_args& a, uint64_t r) { return a.labels && zs_gload(a.labels + r) == a.ignore; }
@@ -177,6 +177,15 @@ __device__ __forceinline__ void ds_loss(const ds_args& a, uint64_t r, const ds_e
     a.loss[r] = (float)loss;
     if (a.stats) *reinterpret_cast<float4*>(a.stats + r * 4) = make_float4((float)m, (float)S, (float)S1, (float)So);
 }
+// 2^-d of the rounding d of a product
+__device__ __forceinline__ double df_undo(float m, float c) {
+    const double d = (double)fmaf(m, c, -(m * c));
+    if (fabs(d) < 0x1p-8) {   // (three terms: within 2^-36)
+        const double y = d * 0.6931471805599453;
+        return fma(y, fma(y, fma(y, -1.0 / 6.0, 0.5), -1.0), 1.0);
+    }
+    return exp2(-d);
+}
 // The gradient's factors.
 __device__ __forceinline__ ds_coef ds_factors(const ds_args& a, uint64_t r, const ds_entry& l, bool bad_label, double m, double S,
                                               double S1, double So) {
@@ -189,7 +198,7 @@ __device__ __forceinline__ ds_coef ds_factors(const ds_args& a, uint64_t r, cons
     k.mc = mf * k.c;
     k.c1 = hd_factor(mf, (float)HD_LOG2E);
     k.m1 = mf * k.c1;
-    const double f = exp2(-(double)fmaf(mf, k.c, -k.mc)), f1 = exp2(-(double)fmaf(mf, k.c1, -k.m1));
+    const double f = df_undo(mf, k.c), f1 = df_undo(mf, k.c1);
     const double one = a.labels ? ce / S1 : 0.0;
     const double in = kl * l.P / S + (a.two ? 0.0 : one);
     k.fi = (float)(in * f);
@@ -366,21 +375,36 @@ __global__ __launch_bounds__(DS_NT) void zs_k_distill_grad(ds_args a, uint64_t r
 // ---------------------------------------------------------------------------
 // loss and gradient by one workgroup a row
 // ---------------------------------------------------------------------------
-#define FU_NT 512
-// The row is read twice by the workgroup that holds it, the second time from
-// its end backwards. Loads run a batch ahead of their use; they are issued
-// without conditions (vectors at the row's ends are clamped to whole ones, the
-// ends themselves read apart), or the compiler waits for all of them at every
-// join of the branches.
-template <int DT, bool TAIL, bool TWO>
-__global__ __launch_bounds__(FU_NT, 4) void zs_k_distill_fused(ds_args a, uint64_t r0) {
+// The row is read once for its sums and passes again, from its end backwards,
+// for its gradient: the last two batches are still in registers, the first ones
+// in shared memory (with 1024 threads, one workgroup a compute unit: up to two
+// batches of 64 KB), what lies between is read again. Loads run a batch ahead of
+// their use; they are issued without conditions (vectors at the row's ends are
+// clamped to whole ones, the ends themselves read apart), or the compiler waits
+// for all of them at every join of the branches. Bound by memory: 4096 rows of
+// 151936 bf16, 2.49 GB, 517 us without the tail (4.8 TB/s) and 590 with it (what
+// is not hidden: the list's and the row's end); every batch read twice, 578 and
+// 621; by 512 threads, two workgroups a unit, 635; as passes of their own, 709.
+// What is kept of a row's list while the row passes.
+struct df_kept {
+    double p[DS_K], pt, P;
+    float x[DS_K + 1], pid[DS_K];   // logits of the entries (the label's last), probabilities of their ids
+};
+struct df_wave {
+    double s, s1, so;
+    float m;
+};
+template <int DT, bool TAIL, bool TWO, int FU_NT>
+__global__ __launch_bounds__(FU_NT, 4) void zs_k_distill_fused(ds_args a, uint64_t r0, uint32_t room) {
     constexpr int E = hd_elem<DT>::E, U = 4, BV = U * FU_NT;   // vectors of a batch
     typedef typename hd_elem<DT>::T T;
-    extern __shared__ uint32_t mask[];   // (TAIL) a byte a vector, whole batches: its ids in the list
+    extern __shared__ hd_u4 shared[];   // room batches of the row, then (TAIL) a byte a vector, whole batches: its ids in the list
     __shared__ uint32_t hid[DS_K + 1];
-    __shared__ float hy[DS_K + 1], shf[FU_NT / 64];
+    __shared__ float hy[DS_K + 1];
     __shared__ double shd[FU_NT / 64];
-    __shared__ ds_coef coef;
+    __shared__ df_wave wv[FU_NT / 64];
+    __shared__ df_kept kept;
+    __shared__ ds_ids ids;
     const uint64_t r = r0 + blockIdx.x;
     const uint32_t t = threadIdx.x;
     const hd_row<DT> row(a.logits, a.ld, r, a.V);
@@ -416,19 +440,36 @@ __global__ __launch_bounds__(FU_NT, 4) void zs_k_distill_fused(ds_args a, uint64
             }
         }
     };
-    hd_u4 cur[U], nxt[U];
+    // the last two batches stay in registers, the first ones in shared memory
+    const uint32_t keep = min(room, nb > 2u ? nb - 2u : 0u);
+    uint32_t* mask = reinterpret_cast<uint32_t*>(shared + room * BV);
+    hd_u4 cur[U], nxt[U], was[U];
     fetch(0, cur);
+#pragma unroll
+    for (int u = 0; u < U; u++) was[u] = cur[u];
     if (TAIL)
         for (uint32_t i = t; i < nb * (BV / 4); i += FU_NT) mask[i] = 0;
-    const ds_entry l = ds_list<FU_NT>(a, r, shd);   // (its barriers order the clearing)
-    const float xk = l.there ? row.at(l.id) : 0.0f, xl = a.labels && !bad_label ? row.at((uint32_t)label) : NAN;
-    if (TAIL && l.there) {
-        const uint32_t pos = l.id + row.shift, j = pos / E;
-        atomicOr(&mask[j / 4], 1u << (j % 4 * 8 + pos % E));
+    bool listed;
+    {
+        const ds_entry l = ds_list<FU_NT>(a, r, shd);   // (its barriers order the clearing)
+        if (TAIL && l.there) {
+            const uint32_t pos = l.id + row.shift, j = pos / E;
+            atomicOr(&mask[j / 4], 1u << (j % 4 * 8 + pos % E));
+        }
+        const float pid = ds_of_id<FU_NT>(l, a.K, ids);
+        if (t < DS_K) {
+            hid[t] = l.there ? l.id : 0xffffffffu;
+            kept.p[t] = l.p;
+            kept.pid[t] = pid;
+            kept.x[t] = l.there ? row.at(l.id) : 0.0f;
+        }
+        if (t == DS_K) {
+            kept.x[DS_K] = a.labels && !bad_label ? row.at((uint32_t)label) : NAN;
+            kept.pt = l.pt;
+            kept.P = l.P;
+        }
+        listed = __syncthreads_or(l.there && (int64_t)l.id == label);
     }
-    __shared__ ds_ids ids;
-    const float pid = ds_of_id<FU_NT>(l, a.K, ids);
-    if (t < DS_K) hid[t] = l.there ? l.id : 0xffffffffu;
     const uint8_t* in_list = reinterpret_cast<const uint8_t*>(mask);
     // first pass: a maximum and sums per thread, relative to 2^ref
     const float c1 = (float)HD_LOG2E;
@@ -470,8 +511,12 @@ __global__ __launch_bounds__(FU_NT, 4) void zs_k_distill_fused(ds_args a, uint64
         }
     };
     for (uint32_t b = 0; b < nb; b++) {
-        // (behind the last batch, the one that the second pass takes after it)
-        fetch(b + 1u < nb ? b + 1u : nb >= 2u ? nb - 2u : 0u, nxt);
+        // (behind the last batch, the one that the second pass takes third)
+        fetch(b + 1u < nb ? b + 1u : nb >= keep + 3u ? nb - 3u : b, nxt);
+        if (b < keep) {
+#pragma unroll
+            for (int u = 0; u < U; u++) shared[b * BV + t + (uint32_t)u * FU_NT] = cur[u];
+        }
         float x[U][E], bm = m;
         uint32_t in[U];
 #pragma unroll
@@ -486,7 +531,10 @@ __global__ __launch_bounds__(FU_NT, 4) void zs_k_distill_fused(ds_args a, uint64
         for (int u = 0; u < U; u++) add(x[u], in[u]);
         if (b + 1u < nb) {
 #pragma unroll
-            for (int u = 0; u < U; u++) cur[u] = nxt[u];
+            for (int u = 0; u < U; u++) {
+                was[u] = cur[u];
+                cur[u] = nxt[u];
+            }
         }
     }
     if (has_edge) {
@@ -497,33 +545,42 @@ __global__ __launch_bounds__(FU_NT, 4) void zs_k_distill_fused(ds_args a, uint64
         raise(bm);
         add(x, TAIL ? in_list[edge] : 0u);
     }
-    const float M = block_max_f<FU_NT>(m, shf);
-    double S, S1, So;
-    const float Mr = M > -INFINITY ? M : 0.0f;
-    auto total = [&](float v, float c0) {   // of sums relative to 2^(m c), to 2^(M c)
-        const float c = hd_factor(Mr, c0);
-        const float f = m == M ? 1.0f : m > -INFINITY && c == c0 ? __builtin_amdgcn_exp2f(m * c - Mr * c) : 0.0f;
-        return block_sum_d<FU_NT>((double)(v * f), shd) * exp2(-(double)fmaf(Mr, c, -(Mr * c)));
+    // the wave's relative to its maximum, then every wave by itself the row's
+    // from theirs: one barrier, and no value from one thread to the others
+    const auto join = [&](float v, float m, float M, float c0) {   // the factor from 2^(m c) to 2^(M c)
+        const float Mr = M > -INFINITY ? M : 0.0f, c = hd_factor(Mr, c0);
+        return m == M ? 1.0f : m > -INFINITY && hd_factor(m, c0) == c ? __builtin_amdgcn_exp2f(m * c - Mr * c) : 0.0f;
     };
-    S = total(s, a.c);
-    S1 = TWO ? total(s1, c1) : S;
-    So = TAIL ? total(so, a.c) : 0.0;
-    if (!(M > -INFINITY)) S = S1 = NAN;   // a row of nothing has no distribution
-    ds_loss<FU_NT>(a, r, l, xk, label, xl, (double)M, S, S1, So, shd);
-    const bool listed = __syncthreads_or(l.there && (int64_t)l.id == label);
-    if (t == 0) {
-        coef = ds_factors(a, r, l, bad_label, (double)M, S, S1, So);
-        coef.lone = label < 0 || bad_label || listed ? 0xffffffffu : (uint32_t)label;
+    const float mw = wave_max_f(m);
+    {
+        const float f = join(s, m, mw, a.c);
+        df_wave w;
+        w.m = mw;
+        w.s = wave_sum_d((double)(s * f));
+        w.so = TAIL ? wave_sum_d((double)(so * f)) : 0.0;
+        w.s1 = TWO ? wave_sum_d((double)(s1 * join(s1, m, mw, c1))) : 0.0;
+        if (zs_lane() == 0) wv[zs_wid()] = w;
     }
     __syncthreads();
+    df_wave w = {0.0, 0.0, 0.0, -INFINITY};
+    if (zs_lane() < FU_NT / 64) w = wv[zs_lane()];
+    const float M = wave_max_f(w.m), Mr = M > -INFINITY ? M : 0.0f;
+    const double f = (double)join(0.0f, w.m, M, a.c), u = df_undo(Mr, hd_factor(Mr, a.c));
+    double S = wave_sum_d(w.s * f) * u, So = TAIL ? wave_sum_d(w.so * f) * u : 0.0, S1 = S;
+    if (TWO) S1 = wave_sum_d(w.s1 * (double)join(0.0f, w.m, M, c1)) * df_undo(Mr, hd_factor(Mr, c1));
+    if (!(M > -INFINITY)) S = S1 = NAN;   // a row of nothing has no distribution
+    ds_entry l;
+    l.there = t < DS_K && hid[t] < a.V;
+    l.pt = kept.pt;
+    l.P = kept.P;
+    ds_coef k = ds_factors(a, r, l, bad_label, (double)M, S, S1, So);
     // second pass, from the batch at hand backwards: every id as one outside
     // the list; the others are written over it as in zs_k_distill_grad
-    const ds_coef k = coef;
     if (t < DS_K) {
-        if (l.there) hy[t] = ds_at<TWO>(k, xk, true, pid, (int64_t)l.id == label);
+        if (l.there) hy[t] = ds_at<TWO>(k, kept.x[t], true, kept.pid[t], (int64_t)hid[t] == label);
     } else if (t == DS_K) {
-        hid[DS_K] = k.lone;
-        hy[DS_K] = ds_at<TWO>(k, xl, false, 0.0f, true);
+        hid[DS_K] = label < 0 || bad_label || listed ? 0xffffffffu : (uint32_t)label;
+        hy[DS_K] = ds_at<TWO>(k, kept.x[DS_K], false, 0.0f, true);
     }
     __syncthreads();
     auto derive = [&](float (&x)[E]) {   // a vector's gradient in the place of its values
@@ -534,18 +591,40 @@ __global__ __launch_bounds__(FU_NT, 4) void zs_k_distill_fused(ds_args a, uint64
             x[q] = TWO ? e * k.fo + e1 : e * k.fo;
         }
     };
-    for (uint32_t b = nb; b-- > 0;) {
+    auto out = [&](uint32_t b, const hd_u4 (&v)[U]) {
         float x[U][E];
-        unpack(cur, b, x);
-#pragma unroll
-        for (int u = 0; u < U; u++) cur[u] = nxt[u];
-        fetch(b >= 2u ? b - 2u : 0u, nxt);
+        unpack(v, b, x);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const uint32_t j = b * BV + t + (uint32_t)u * FU_NT;
             derive(x[u]);
             if (j >= lo && j <= hi) ds_store<DT>(grad, a.V, aligned, row.id0(j), x[u]);
         }
+    };
+    auto next = [&]() {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            cur[u] = was[u];
+            was[u] = nxt[u];
+        }
+    };
+    uint32_t b = nb;
+    while (b > keep + 3u) {
+        b--;
+        out(b, cur);
+        next();
+        fetch(b - 3u, nxt);
+    }
+    while (b > keep) {
+        b--;
+        out(b, cur);
+        next();
+    }
+    while (b > 0u) {
+        b--;
+#pragma unroll
+        for (int u = 0; u < U; u++) cur[u] = shared[b * BV + t + (uint32_t)u * FU_NT];
+        out(b, cur);
     }
     if (has_edge) {
         float x[E];
@@ -559,17 +638,31 @@ __global__ __launch_bounds__(FU_NT, 4) void zs_k_distill_fused(ds_args a, uint64
         const uint32_t owner = j < lo || j > hi ? 0u : j % FU_NT >> 6;
         if (id < a.V && owner == (uint32_t)zs_wid()) ds_store1<DT>(grad + id, hy[h]);
     }
+    // the loss last: its logarithms pass while the stores do
+    l.p = l.there ? kept.p[t] : 0.0;
+    ds_loss<FU_NT>(a, r, l, t < DS_K ? kept.x[t] : 0.0f, label, kept.x[DS_K], (double)M, S, S1, So, shd);
 }
 
+template <int DT, int NT>
+static void ds_fused(const ds_args& a, uint64_t r0, uint32_t n, hipStream_t stream) {
+    const uint32_t batch = 4u * NT, nb = ((a.V + 7u) / hd_elem<DT>::E + 1u + batch - 1u) / batch;
+    const uint32_t mask = a.tail ? nb * batch : 0u;   // a byte a vector, whole batches
+    const uint32_t left = NT == 1024 ? (DS_FUSED_LDS - mask) / (batch * 16u) : 0u, room = left < nb ? left : nb, lds = room * batch * 16u + mask;
+    if (a.tail && a.two) hipLaunchKernelGGL((zs_k_distill_fused<DT, true, true, NT>), dim3(n), dim3(NT), lds, stream, a, r0, room);
+    else if (a.tail) hipLaunchKernelGGL((zs_k_distill_fused<DT, true, false, NT>), dim3(n), dim3(NT), lds, stream, a, r0, room);
+    else if (a.two) hipLaunchKernelGGL((zs_k_distill_fused<DT, false, true, NT>), dim3(n), dim3(NT), lds, stream, a, r0, room);
+    else hipLaunchKernelGGL((zs_k_distill_fused<DT, false, false, NT>), dim3(n), dim3(NT), lds, stream, a, r0, room);
+}
 template <int DT>
 static void ds_go(const ds_args& a, int what, uint64_t r0, uint32_t n, hipStream_t stream) {
     const dim3 grid(n * a.chunks), wg(DS_NT);
-    const uint32_t lds = a.tail ? ((a.V + 7u) / hd_elem<DT>::E / (4u * FU_NT) + 1u) * (4u * FU_NT) : 0u;   // a byte a vector, whole batches
-    if (what == (DS_LOSS | DS_GRAD) && a.N >= DS_FUSED_ROWS && a.V >= DS_FUSED_VOCAB && lds <= DS_FUSED_LDS) {
-        if (a.tail && a.two) hipLaunchKernelGGL((zs_k_distill_fused<DT, true, true>), dim3(n), dim3(FU_NT), lds, stream, a, r0);
-        else if (a.tail) hipLaunchKernelGGL((zs_k_distill_fused<DT, true, false>), dim3(n), dim3(FU_NT), lds, stream, a, r0);
-        else if (a.two) hipLaunchKernelGGL((zs_k_distill_fused<DT, false, true>), dim3(n), dim3(FU_NT), lds, stream, a, r0);
-        else hipLaunchKernelGGL((zs_k_distill_fused<DT, false, false>), dim3(n), dim3(FU_NT), lds, stream, a, r0);
+    const uint32_t vec = (a.V + 7u) / hd_elem<DT>::E + 1u;   // vectors of a row at most
+    if (what == (DS_LOSS | DS_GRAD) && a.N >= DS_FUSED_ROWS && a.V >= DS_FUSED_VOCAB && vec <= 49152u) {
+        // 16384 bf16 rows of 32000: 483 us by 256 threads, 544 by 512, 827 by
+        // 1024; 8192 of 65536: 540, 478, 571; 4096 of 151936 without the tail: 729, 635, 517
+        if (vec <= 4u * 1024u) ds_fused<DT, 256>(a, r0, n, stream);
+        else if (vec <= 4u * 2048u + 1u) ds_fused<DT, 512>(a, r0, n, stream);
+        else ds_fused<DT, 1024>(a, r0, n, stream);
         return;
     }
     if (what & DS_LOSS) {

@@ -62,8 +62,7 @@ int hd_head_launch(const hd_args& a, const bm_args* beam, uint32_t dtype, hipStr
 
 // log2 of the values in a group: 64, or 16 where a row has few groups for the
 // list that is wanted (a threshold from group maxima is close only when there
-// are several times K of them), or 256 where 64 would make too many. 2048 rows
-// of 151936 bf16, K = 64: see zs_head.hip.
+// are several times K of them), or 256 where 64 would make more than HD_GROUPS.
 inline uint32_t hd_group_shift(uint32_t V, uint32_t K) {
     if ((V >> 6) + 2u > HD_GROUPS) return 8;
     return (V >> 6) >= 8u * K || (V >> 4) + 2u > HD_GROUPS ? 6 : 4;
