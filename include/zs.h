@@ -399,7 +399,8 @@ int zs_lane_step(zs_ctx* ctx, const float* d_logits, uint32_t m, uint32_t V, uin
 /* ---- beam search -----------------------------------------------------------
  * One step for `groups` requests of `width` beams, row = group * width + beam.
  * Candidates are the pairs (beam, id):
- *     s(b, v) = scores[b] + x~[b][v] - ln sum_u exp(x~[b][u])     (f32, rounded once)
+ *     s(b, v) = scores[b] + x~[b][v] - ln sum_u exp(x~[b][u])     (f32, rounded once,
+ *                                              the logarithm relative to the row's maximum)
  * over the row's masked logits x~ (ids whose allow bit is 0 and NaN count as
  * -inf, +inf as the largest f32; no candidates at -inf, nor of a beam whose
  * score is not finite: its row is not read). They are taken in the order
@@ -481,7 +482,7 @@ typedef struct zs_teacher {
     uint32_t N, V, K, dtype;
     uint64_t ld;
     const void* d_logits;             /* [N][ld] */
-    float temperature;                /* > 0, finite */
+    float temperature;                /* > 0, finite, not denormal */
     uint32_t pad;
     uint32_t* d_ids;                  /* [N][K] */
     float* d_logp;                    /* [N][K] */
@@ -500,8 +501,9 @@ int zs_teacher_topk(zs_ctx* ctx, const zs_teacher* args, void* stream);
  *       KL = sum_k p_k (ln p_k - ln q_k)                 (0 for an empty list)
  *   with it the ids outside the list are one more outcome: p_t = max(0, 1 -
  *       sum_k p_k), q_t = sum of q outside the list, KL += p_t (ln p_t - ln q_t)
+ *       (a p_t below 2^-20, the rounding of logp, counts as none where q_t is 0)
  *   CE = -ln softmax(x)[label]                            (d_labels given)
- *   loss[r] = kl_weight * KL + ce_weight * CE
+ *   loss[r] = kl_weight * KL + ce_weight * CE   (a term of weight 0 is left out)
  * A row whose label is ignore_index has loss 0 and gradient 0, and is not
  * read; a label outside [0, V) otherwise gives NaN. NaN and infinities of x
  * are not looked for: they come out as the formulas have them.

@@ -62,12 +62,12 @@ def ref_select(x, scores, pool, W, eos, alpha, early, allow=None):
             m = row.max()
             if m == NINF:
                 continue
-            lse = m + np.log(np.exp(row - m).sum())
+            lns = np.log(np.exp(row - m).sum())
             order = np.lexsort((np.arange(V), -row))[:W + len(eos)]
             for v in order:
                 if row[v] == NINF:
                     continue
-                f = np.float32(float(s) + (row[v] - lse))
+                f = np.float32(float(s) + ((row[v] - m) - lns))
                 if f > NINF:
                     cand.append((-f, b, -row[v], v))
         cand.sort()
@@ -181,6 +181,27 @@ def test_values_that_are_no_numbers(dtype):
     o = check(rows_at(x, dtype, 1, 1), beams(rng, G, W), empty_pool(G, W), W, eos=(4,), what="no numbers")
     assert o.parents[2].tolist() == [-1] * 3 and o.pool.done.tolist() == [0, 0, 1]
     assert torch.isneginf(o.scores[2]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [300, 9001])
+def test_rows_of_huge_values(V, dtype):
+    """Rows that are all at a mask's finite value (any from -1e9 to the type's
+    lowest) are even ones; equal values at the top of huge ones share."""
+    rng = np.random.default_rng(V)
+    G, W = 3, 4
+    x = np.empty((G * W, V), np.float32)
+    for r, v in enumerate((-1e9, -1e10, -1e30, -3.3e38, 1e10, 1e30, 3.3e38, -5e9)):
+        x[r] = v
+    x[3] = torch.finfo(TYPES[dtype]).min
+    x[7, 40] = 2.0
+    x[8] = -1e30
+    x[8, 10:15] = rng.normal(0, 1, 5)
+    x[9] = 5e29
+    x[9, [3, 77, V - 1]] = 1e30
+    x[10] = 3e12 + 1e11 * rng.normal(0, 1, V)
+    x[11] = rng.normal(0, 1, V)
+    check(rows_at(x, dtype, 1, 2), beams(rng, G, W), empty_pool(G, W), W, (4,), what="huge")
 
 
 def test_beams_that_do_not_live():

@@ -56,7 +56,7 @@ def check_teacher(xt, K, T, what=""):
         L = m + np.log(np.exp(z - m).sum())
         tol = ltol(V) + 2.0 ** -23 * abs(L)
         assert abs(lse[r] - L) <= tol
-        want = z[order] - L
+        want = (z[order] - m) - np.log(np.exp(z - m).sum())
         assert (np.abs(logp[r, :n] - want) <= ltol(V) + 2.0 ** -23 * np.abs(want)).all()
 
 
@@ -94,6 +94,26 @@ def test_teacher_rows_of_ties_and_orders(V, dtype):
     xt = rows_at(x, dtype, 1, 2)
     for K in (1, 33, 64, 65, 128):
         check_teacher(xt, K, 1.0, "orders")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_teacher_rows_of_huge_values(dtype):
+    """Rows all at a mask's finite value are even ones, equal values at the top
+    of huge ones share; temperatures that make ordinary rows huge."""
+    rng = np.random.default_rng(1)
+    V = 9001
+    x = np.empty((8, V), np.float32)
+    for r, v in enumerate((-1e9, -1e10, -1e30, torch.finfo(TYPES[dtype]).min, 1e10, 3.3e38)):
+        x[r] = v
+    x[6] = 5e29
+    x[6, [3, 77, V - 1]] = 1e30
+    x[7] = -1e30
+    x[7, 10:15] = rng.normal(0, 1, 5)
+    for T in (1.0, 3.0, 1e20):
+        check_teacher(rows_at(x, dtype, 1, 2), 100, T, "huge")
+    y = np.concatenate([rng.normal(0, 1000, (2, V)), np.full((1, V), -7.0), np.zeros((1, V))])
+    for T in (1e-7, 1e-12, 1e-25, 1e-34):
+        check_teacher(rows_at(y, dtype, 1, 2), 100, T, "cold")
 
 
 def test_teacher_rows_far_apart():
@@ -257,6 +277,87 @@ def test_lists_that_go_wrong(tail, dtype):
         for T in (1.0, 2.0):
             check(rows_at(x, dtype, shift, 1), ids, logp, DistillConfig(temperature=T, tail=tail, ce_weight=0.5), labels,
                   None, f"lists shift={shift}")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 57])
+def test_students_of_huge_values(n, dtype):
+    """Rows all at a mask's finite value are even ones; huge values beside
+    ordinary ones; by passes and (513 rows) a workgroup a row."""
+    from zllm_amd.distill import DistillConfig
+    rng = np.random.default_rng(n)
+    V, K = 4500, 12
+    x = np.empty((9, V), np.float32)
+    for r, v in enumerate((-1e9, -1e10, -1e30, torch.finfo(TYPES[dtype]).min, 1e10, 3.3e38)):
+        x[r] = v
+    x[6] = -1e30
+    x[6, 10:400] = rng.normal(0, 1, 390)
+    x[7] = -2e10
+    x[7, 4000] = -1e10
+    x[8] = 1e12 + 1e11 * rng.normal(0, 1, V)
+    ids, logp = lists(rng, rng.normal(0, 2, (9, V)), K)
+    ids[6] = 10 + np.arange(K)
+    labels = ids[:, 2].copy()
+    x, ids, logp, labels = (np.concatenate([a] * n) for a in (x, ids, logp, labels))
+    for kw in (dict(), dict(tail=True), dict(tail=True, temperature=2.0, ce_weight=0.5), dict(temperature=1e-3)):
+        check(rows_at(x, dtype, 1, 2), ids, logp, DistillConfig(**kw), labels if "ce_weight" in kw else None, None, "huge")
+
+
+@pytest.mark.parametrize("n", [3, 520])
+def test_lists_of_all_there_is(n):
+    """Lists that have every id, or every id that is allowed: what rounding
+    leaves of 1 is no tail that the student would have to have."""
+    from zllm_amd.distill import DistillConfig, distill_loss, distill_loss_grad
+    rng = np.random.default_rng(n)
+    V, K = 4200 if n > 100 else 60, 60
+    t, x = rng.normal(0, 2, (n, K)), rng.normal(0, 2, (n, K))
+    logp = (t - np.log(np.exp(t).sum(1, keepdims=True))).astype(np.float32)
+    logp -= np.float32(2.0 ** -22)               # (what is left is positive in every row)
+    ids = np.stack([rng.choice(V, K, replace=False) for _ in range(n)])
+    full = np.full((n, V), -np.inf, np.float32)
+    np.put_along_axis(full, ids, x.astype(np.float32), 1)
+    p = np.exp(logp.astype(np.float64))
+    assert (p.sum(1) < 1).all() and (1 - p.sum(1) < 2.0 ** -20).all()
+    x = x.astype(np.float32).astype(np.float64)
+    lq = x - np.log(np.exp(x).sum(1, keepdims=True))
+    want = (p * (logp - lq)).sum(1)
+    xt, it, lt = torch.from_numpy(full).cuda(), torch.from_numpy(ids).to(torch.int32).cuda(), torch.from_numpy(logp).cuda()
+    cfg = DistillConfig(tail=True)
+    print(f"[case] distill lists of all n={n} V={V}", flush=True)
+    loss = distill_loss(_ctx(), xt, it, lt, cfg)[0]
+    l2, g = distill_loss_grad(_ctx(), xt, it, lt, cfg, torch.ones(n, device="cuda"))
+    for l in (loss, l2):
+        assert (np.abs(l.double().cpu().numpy() - want) <= 3 * ltol(V) + 2.0 ** -23 * np.abs(want)).all()
+    g = g.double().cpu().numpy()
+    at = np.take_along_axis(g, ids, 1)
+    assert (np.abs(at - (np.exp(lq) - p)) <= (np.exp(lq) + p) * (2 * ltol(V) + 2.0 ** -21) + TINY["f32"]).all()
+    np.put_along_axis(g, ids, 0.0, 1)
+    assert not g.any()
+
+
+@pytest.mark.parametrize("n", [5, 515])
+def test_terms_of_no_weight(n):
+    """A term of weight 0 has no part in the loss, were it infinite; labels
+    outside the vocabulary are still NaN."""
+    from zllm_amd.distill import DistillConfig, distill_loss, distill_loss_grad
+    V = 4100
+    x = torch.randn((n, V), device="cuda")
+    x[:, 9] = -float("inf")
+    labels = torch.full((n,), 9, device="cuda")
+    labels[1], labels[2] = V, -100
+    ids = torch.tensor([[3, 4, 5]], dtype=torch.int32, device="cuda").expand(n, 3).contiguous()
+    logp = torch.full((n, 3), -1.2, device="cuda")
+    far = torch.full((n, 3), 9, dtype=torch.int32, device="cuda")
+    w = torch.ones(n, device="cuda")
+    print(f"[case] distill weights of 0 n={n}", flush=True)
+    for cfg, i, lab in ((DistillConfig(ce_weight=0.0), ids, 9), (DistillConfig(kl_weight=0.0, ce_weight=1.0), far, 3)):
+        labels[labels == 9] = lab
+        loss = distill_loss(_ctx(), x, i, logp, cfg, labels)[0]
+        l2, g = distill_loss_grad(_ctx(), x, i, logp, cfg, w, labels)
+        for l in (loss, l2):
+            assert torch.isnan(l[1]) and l[2] == 0
+            assert torch.isfinite(l[0]) and torch.isfinite(l[3:]).all() and (l[3:] != 0).all()
+        assert torch.isnan(g[1]).all() and torch.isfinite(g[0]).all() and torch.isfinite(g[2:]).all()
 
 
 def test_student_that_has_learnt_the_list():

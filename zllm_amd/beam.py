@@ -195,7 +195,8 @@ def _blocks(t: torch.Tensor, row_dim: int) -> List[BeamStateDesc]:
     for stride, n in rest[2:]:
         starts = [s + i * stride for s in starts for i in range(n)]
     inner, outer = (rest + [(0, 1), (0, 1)])[:2]
-    return [BeamStateDesc(t.data_ptr() + s, t.stride(row_dim) * size, outer[0], inner[0], block, outer[1], inner[1])
+    row = t.stride(row_dim) * size if t.shape[row_dim] > 1 else block   # (a single row's is of no meaning)
+    return [BeamStateDesc(t.data_ptr() + s, row, outer[0], inner[0], block, outer[1], inner[1])
             for s in starts]
 
 

@@ -1141,7 +1141,7 @@ extern "C" int zs_beam_select(zs_ctx* ctx, const zs_beam* b, void* stream) {
     m.width = b->width; m.K = h.K; m.n_eos = b->n_eos; m.early = b->flags & ZS_BEAM_EARLY;
     for (uint32_t i = 0; i < b->n_eos; i++) m.eos[i] = b->eos[i];
     m.length_penalty = b->length_penalty;
-    m.scores = b->d_scores; m.list = h.list; m.lse = h.lse;
+    m.scores = b->d_scores; m.list = h.list; m.norm = h.norm;
     m.fin_score = b->d_fin_score; m.fin_length = b->d_fin_length; m.fin_parent = b->d_fin_parent; m.fin_token = b->d_fin_token;
     m.steps = b->d_steps; m.done = b->d_done;
     m.fin_score_o = b->d_fin_score_out; m.fin_length_o = b->d_fin_length_out; m.fin_parent_o = b->d_fin_parent_out;
@@ -1213,8 +1213,8 @@ extern "C" int zs_teacher_topk(zs_ctx* ctx, const zs_teacher* b, void* stream) {
     if (!ctx || !b) return zs_set_error(ctx, ZS_EINVAL, "%s: null argument", who);
     if (b->K == 0 || b->K > ZS_TEACHER_KMAX || b->K > b->V)
         return zs_set_error(ctx, ZS_ELIMIT, "%s: K=%u outside 1..min(V, %d)", who, b->K, ZS_TEACHER_KMAX);
-    if (!(b->temperature > 0.0f) || !(b->temperature <= 3.4e38f))
-        return zs_set_error(ctx, ZS_EINVAL, "%s: temperature must be positive and finite", who);
+    if (!(b->temperature >= 1.17549435e-38f) || !(b->temperature <= 3.4e38f))   // (1 / T is a float)
+        return zs_set_error(ctx, ZS_EINVAL, "%s: temperature must be positive, normal and finite", who);
     if (b->N == 0) return ZS_OK;
     int rc = rows_check(ctx, b->V, b->dtype, b->ld, b->d_logits, who);
     if (rc) return rc;
@@ -1247,8 +1247,8 @@ static int distill_call(zs_ctx* ctx, const zs_distill* b, int what, const char* 
     if (b->K == 0 || b->K > ZS_DISTILL_KMAX)
         return zs_set_error(ctx, ZS_ELIMIT, "%s: K=%u outside 1..%d", who, b->K, ZS_DISTILL_KMAX);
     if (b->flags & ~(uint32_t)ZS_DISTILL_TAIL) return zs_set_error(ctx, ZS_EINVAL, "%s: unknown flags %#x", who, b->flags);
-    if (!(b->temperature > 0.0f) || !(b->temperature <= 3.4e38f))
-        return zs_set_error(ctx, ZS_EINVAL, "%s: temperature must be positive and finite", who);
+    if (!(b->temperature >= 1.17549435e-38f) || !(b->temperature <= 3.4e38f))   // (1 / T is a float)
+        return zs_set_error(ctx, ZS_EINVAL, "%s: temperature must be positive, normal and finite", who);
     if (!(b->kl_weight - b->kl_weight == 0.0f) || !(b->ce_weight - b->ce_weight == 0.0f))
         return zs_set_error(ctx, ZS_EINVAL, "%s: weights must be finite", who);
     if (b->N == 0) return ZS_OK;

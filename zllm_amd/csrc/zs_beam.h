@@ -9,7 +9,7 @@ struct bm_args {
     float length_penalty;
     const float* scores;
     const unsigned long long* list;   // [groups*width][K]
-    const double* lse;                // [groups*width]
+    const double* norm;               // [groups*width][2] maximum, ln sum exp(x~ - maximum)
     const float* fin_score;
     const int32_t *fin_length, *fin_parent, *fin_token, *steps, *done;
     float* fin_score_o;

@@ -24,7 +24,7 @@ __device__ __forceinline__ void bm_merge(const bm_args& a, uint32_t g) {
     __shared__ float cs_[ZS_BEAM_MAX_WIDTH * (ZS_BEAM_MAX_WIDTH + ZS_BEAM_MAX_EOS)];      // the lists' scores and ids
     __shared__ uint32_t ci_[ZS_BEAM_MAX_WIDTH * (ZS_BEAM_MAX_WIDTH + ZS_BEAM_MAX_EOS)];
     __shared__ float bs_[ZS_BEAM_MAX_WIDTH];
-    __shared__ double bl_[ZS_BEAM_MAX_WIDTH];
+    __shared__ double bm_[ZS_BEAM_MAX_WIDTH], bl_[ZS_BEAM_MAX_WIDTH];
     __shared__ float fin_s[ZS_BEAM_MAX_WIDTH];
     __shared__ int fin_p[ZS_BEAM_MAX_WIDTH], fin_t[ZS_BEAM_MAX_WIDTH];
     const uint32_t lane = threadIdx.x, W = a.width, K = a.K;
@@ -33,7 +33,9 @@ __device__ __forceinline__ void bm_merge(const bm_args& a, uint32_t g) {
     // all loads at once: what is not needed is dropped afterwards
     const int was = a.done[g], steps = a.steps[g];
     const float score = beam ? a.scores[at + lane] : -INFINITY;
-    const double lse = beam ? __hip_atomic_load(a.lse + at + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+    const double* norm = a.norm + (at + (beam ? lane : 0u)) * 2u;
+    const double m = __hip_atomic_load(norm, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const double lns = __hip_atomic_load(norm + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     unsigned long long e[NL];
 #pragma unroll
     for (int k = 0; k < NL; k++) {
@@ -47,7 +49,8 @@ __device__ __forceinline__ void bm_merge(const bm_args& a, uint32_t g) {
     if (beam) {
         // (beams that do not live left no list)
         bs_[lane] = !was && fabsf(score) <= __FLT_MAX__ ? score : -INFINITY;
-        bl_[lane] = lse;
+        bm_[lane] = m;
+        bl_[lane] = lns;
     }
     __syncthreads();
 #pragma unroll
@@ -57,7 +60,7 @@ __device__ __forceinline__ void bm_merge(const bm_args& a, uint32_t g) {
         const uint32_t b = i / K;
         const float bs = bs_[b];
         const bool some = bs > -INFINITY && e[k] != ~0ull;
-        cs_[i] = some ? (float)((double)bs + ((double)zs_u2f((uint32_t)(e[k] >> 32)) - bl_[b])) : -INFINITY;
+        cs_[i] = some ? (float)((double)bs + (((double)zs_u2f((uint32_t)(e[k] >> 32)) - bm_[b]) - bl_[b])) : -INFINITY;
         ci_[i] = (uint32_t)e[k] | (bm_is_eos(a, (uint32_t)e[k]) ? 0x80000000u : 0u);
     }
     __syncthreads();
@@ -103,10 +106,11 @@ __device__ __forceinline__ void bm_merge(const bm_args& a, uint32_t g) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");   // (one wave from here on)
     // the pool and what finished, the pool first among equals: lane i's place
     // is the number of lanes in front of it
-    const float len = (float)(steps + 1), norm = a.length_penalty == 1.0f ? len : a.length_penalty == 0.0f ? 1.0f : powf(len, a.length_penalty);
+    const float len = (float)(steps + 1), div = a.length_penalty == 1.0f ? len : a.length_penalty == 0.0f ? 1.0f : powf(len, a.length_penalty);
     if (lane >= W && lane < W + n_fin && lane < 64u) {
         const uint32_t i = lane - W;
-        ps = fin_s[i] / norm;
+        ps = fin_s[i] / div;
+        if (!(ps == ps)) ps = -INFINITY;   // (0 / 0: a length penalty past the floats)
         pl = steps + 1;
         pp = fin_p[i];
         pt = fin_t[i];
@@ -121,7 +125,7 @@ __device__ __forceinline__ void bm_merge(const bm_args& a, uint32_t g) {
     const float worst = worst_m ? zs_readlane_f(ps, (uint32_t)__ffsll((long long)worst_m) - 1u) : -INFINITY;
     const float best = zs_readlane_f(o_score, 0);
     const bool full = worst > -INFINITY;
-    const bool done = n_live == 0 || (full && (a.early || worst >= best / norm));
+    const bool done = n_live == 0 || (full && (a.early || worst >= best / div));
     if (stays) {
         const bool some = ps > -INFINITY;
         a.fin_score_o[at + place] = ps;

@@ -171,9 +171,11 @@ __device__ __forceinline__ void ds_loss(const ds_args& a, uint64_t r, const ds_e
     if (l.there && l.p != 0.0) term = l.p * (log(l.p) - (((double)xk - m) * a.inv_t - log(S)));   // (NaN stays)
     term = block_sum_d<NT>(term, shd);
     if (threadIdx.x) return;
-    if (l.pt > 0.0) term += l.pt * (log(l.pt) - (log(So) - log(S)));
-    double loss = (double)a.kl * term;
-    if (a.labels) loss += (double)a.ce * (log(S1) - ((double)xl - m));
+    // (where the student has nothing outside, the rounding of the list's
+    // probabilities is no tail: 128 of them are within 2^-21 of their sum)
+    if (l.pt > 0.0 && !(So == 0.0 && l.pt < 0x1p-20)) term += l.pt * (log(l.pt) - (log(So) - log(S)));
+    double loss = a.kl != 0.0f ? (double)a.kl * term : 0.0;
+    if (a.labels) loss += a.ce != 0.0f ? (double)a.ce * (log(S1) - ((double)xl - m)) : xl == xl ? 0.0 : NAN;
     a.loss[r] = (float)loss;
     if (a.stats) *reinterpret_cast<float4*>(a.stats + r * 4) = make_float4((float)m, (float)S, (float)S1, (float)So);
 }

@@ -157,11 +157,15 @@ __device__ __forceinline__ float hd_sum(const float (&e)[E]) {
     else return ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
 }
 
-// The factor of the exponent for values of at most m: c, or, where m c is past
-// the floats, 2^-32. There the next float below m lies over 2^100 / c under it,
-// so that every value but m itself has no mass with either factor, and with a
-// power of two m's product is exact.
-__device__ __forceinline__ float hd_factor(float m, float c) { return fabsf(m * c) < INFINITY ? c : 0x1p-32f; }
+// The factor of the exponent for values of at most m: c, as long as the rounding
+// of m c stays below 64 and 2^ it a float. Past that the next float below m lies
+// at least 2^6 / c under it, so that every value but m itself has no mass, and
+// with a power of two that takes m to 2^125 (or as far as there is one) neither
+// has its next value, and m's own product is exact.
+__device__ __forceinline__ float hd_factor(float m, float c) {
+    const uint32_t e = __float_as_uint(m) >> 23 & 255u;
+    return fabsf(m * c) < 0x1p31f ? c : __uint_as_float(min(379u - e, 254u) << 23);
+}
 
 // A value as the heads of rows see it: NaN counts as -inf (nothing is known of
 // it), +inf as the largest number (an id that is certain; several share).
@@ -172,26 +176,30 @@ __device__ __forceinline__ uint32_t hd_key(float x) { return x > -INFINITY ? zs_
 
 #define HD_LOG2E 1.44269504088896340736
 
-// ln sum exp(x / T) from sum = sum exp((x - m) / T); -inf for no mass
-__device__ __forceinline__ double hd_lse(float m, double inv_t, double sum) { return sum > 0.0 ? (double)m * inv_t + log(sum) : -INFINITY; }
+// A row's normaliser: its maximum m and lns = ln sum exp((x - m) / T), -inf for
+// no mass. Kept apart: their sum would lose lns where m is large (a row that
+// is all at a mask's 1e30 has probabilities of 1 / V, not of 1).
+struct hd_norm {
+    double m, lns;
+};
 
 // Is row r's head wanted?
 __device__ __forceinline__ bool hd_live(const hd_args& a, uint64_t r) {
     return !a.scores || (!a.done[zs_quot((uint32_t)r, a.by_width)] && fabsf(a.scores[r]) <= __FLT_MAX__);   // (beams' rows number below 2^31)
 }
 // Entry t of row r, e = ~key << 32 | id (~0: none); by threads t < K.
-__device__ __forceinline__ void hd_put(const hd_args& a, uint64_t r, uint32_t t, unsigned long long e, double lse) {
+__device__ __forceinline__ void hd_put(const hd_args& a, uint64_t r, uint32_t t, unsigned long long e, hd_norm o) {
     if (t >= a.K) return;
     const bool some = e != ~0ull;
     const float x = zs_key_to_float(~(uint32_t)(e >> 32));
     if (a.ids) {
         a.ids[r * a.K + t] = some ? (uint32_t)e : 0xffffffffu;
-        a.logp[r * a.K + t] = some ? (float)((double)x * a.inv_t - lse) : -INFINITY;
-        if (t == 0) a.lse_out[r] = (float)lse;
+        a.logp[r * a.K + t] = some ? (float)(((double)x - o.m) * a.inv_t - o.lns) : -INFINITY;
+        if (t == 0) a.lse_out[r] = o.lns > -INFINITY ? (float)(o.m * a.inv_t + o.lns) : -INFINITY;
     } else {
         // (past the L2, which other parts of the GPU do not share)
         __hip_atomic_store(a.list + r * a.K + t, some ? ((unsigned long long)zs_f2u(x) << 32) | (uint32_t)e : ~0ull,
                            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (t == 0) __hip_atomic_store(a.lse + r, lse, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (t < 2) __hip_atomic_store(a.norm + r * 2u + t, t ? o.lns : o.m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
 }

@@ -162,7 +162,7 @@ __device__ __forceinline__ void hp_pick(const hd_args& a, uint64_t r, uint32_t l
     __shared__ unsigned long long list[HP_LIST];
     __shared__ uint32_t gl[HP_GL], pl[ZS_TEACHER_KMAX];
     __shared__ uint32_t hist[256], u[4], wthr[NW];
-    __shared__ double lse_s;
+    __shared__ hd_norm norm;
     const hd_row<DT> row(a.logits, a.ld, r, a.V);
     const uint32_t* allow = MASK ? a.allow + r * a.allow_words : nullptr;
     const uint32_t t = threadIdx.x, lane = (uint32_t)zs_lane(), wid = (uint32_t)zs_wid(), K = a.K;
@@ -177,7 +177,7 @@ __device__ __forceinline__ void hp_pick(const hd_args& a, uint64_t r, uint32_t l
         k[e] = (uint32_t)e * HP_NT < ng ? zs_gload(gm + min(g, ng - 1u)) : 0u;
         if (g >= ng) k[e] = 0u;
     }
-    if (wid == NW - 1u) {   // ln sum exp(x / T) of the row
+    if (wid == NW - 1u) {   // the row's normaliser
         const uint32_t recs = (row.nvec * E + HD_CHUNK - 1u) / HD_CHUNK * (HD_CHUNK / HD_WAVE);
         const float2* rec = a.rec + r * a.recs;
         // (two a lane at once: rows of 262144 ids; longer ones take turns)
@@ -196,7 +196,7 @@ __device__ __forceinline__ void hp_pick(const hd_args& a, uint64_t r, uint32_t l
         add(v[1]);
         for (uint32_t i = lane + 128u; i < recs; i += 64u) add(rec[i]);
         s = wave_sum_d(s);
-        if (lane == 0) lse_s = hd_lse(m, a.inv_t, s);
+        if (lane == 0) norm = {(double)m, log(s)};
     }
 #pragma unroll
     for (int e = 0; e < HP_GPT; e++) {
@@ -361,7 +361,7 @@ __device__ __forceinline__ void hp_pick(const hd_args& a, uint64_t r, uint32_t l
         // entries of no candidate (~0 all) lie behind the others as they stand
         if (e == ~0ull && t < n)
             for (i = 0; i < t; i++) place += list[i] == ~0ull ? 1u : 0u;
-        hd_put(a, r, t < n ? place : t, e, lse_s);
+        hd_put(a, r, t < n ? place : t, e, norm);
         return;
     }
     uint32_t np2 = 256;
@@ -370,7 +370,7 @@ __device__ __forceinline__ void hp_pick(const hd_args& a, uint64_t r, uint32_t l
     __syncthreads();
     if (np2 <= HP_NT) block_sort_reg_u64<HP_NT, 1>(list, np2);
     else block_sort_reg_u64<HP_NT, HP_LIST / HP_NT>(list, np2);
-    hd_put(a, r, t, t < n ? list[t] : ~0ull, lse_s);
+    hd_put(a, r, t, t < n ? list[t] : ~0ull, norm);
 }
 
 // BEAM: the workgroup that is the last of its request's takes the step.

@@ -12,7 +12,7 @@
 
 // The heads of R rows. For a teacher (d_ids) the list goes out as ids and
 // log-probabilities; for the beam step into `list` (bits of x~ << 32 | id,
-// ~0 for none) and `lse`, of the rows whose beam lives.
+// ~0 for none) and `norm`, of the rows whose beam lives.
 // n / d for n < 2^31 by a product: n / d = mulhi(n, mul) >> (sh - 32), d >= 2,
 // with mul = ceil(2^sh / d) and 2^sh the first power at or above 2^31 d (the
 // excess e = mul d - 2^sh < d gives n e < 2^31 d <= 2^sh). sh 0: d is 1.
@@ -44,7 +44,7 @@ struct hd_args {
     const int32_t* done;
     uint32_t width;
     unsigned long long* list;   // [R][K]
-    double* lse;                // [R]
+    double* norm;               // [R][2] maximum, ln sum exp(x~ - maximum)
     uint32_t* count;            // [R / width] rows of the request that are done (cleared by the pass)
     // the pass: group maxima and, per wave, (maximum, sum exp((x - maximum) / T))
     uint32_t chunks;            // workgroups a row
@@ -86,8 +86,8 @@ inline uint64_t hd_work(hd_args& a, void* work, bool beam) {
     if (beam) {
         a.list = (unsigned long long*)p;
         p += hd_pad(a.R * a.K * 8u);
-        a.lse = (double*)p;
-        p += hd_pad(a.R * 8u);
+        a.norm = (double*)p;
+        p += hd_pad(a.R * 16u);
         a.count = (uint32_t*)p;
         p += hd_pad(a.R * 4u);
     }
