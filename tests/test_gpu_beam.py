@@ -283,6 +283,32 @@ def test_masks(V, dtype):
               bits=torch.from_numpy(bits).cuda(), what=f"mask shift={shift}")
 
 
+def test_a_group_in_two_launches():
+    """A launch ends inside a request's rows (2^22 workgroups, five a row): the
+    requests on both sides come out as in a call of their own; the others are
+    done and not read (68 GB, most of it never written)."""
+    from zllm_amd.beam import BeamPool, beam_select
+    W, V = 32, 32800
+    G = (1 << 20) // W
+    mid = (1 << 22) // 5 // W
+    assert (1 << 22) // 5 % W
+    x = torch.empty((G * W, V), dtype=torch.bfloat16, device="cuda")
+    near = slice((mid - 1) * W, (mid + 2) * W)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x[near] = torch.randn((3 * W, V), device="cuda", generator=gen).to(torch.bfloat16)
+    scores = torch.randn((G, W), device="cuda", generator=gen).sub_(5.0)
+    pool = BeamPool.empty(G, W)
+    pool.done.fill_(1)
+    pool.done[mid - 1:mid + 2] = 0
+    print("[case] beam_select a group in two launches", flush=True)
+    o = beam_select(_ctx(), x, scores, pool, (3,))
+    a = beam_select(_ctx(), x[near], scores[mid - 1:mid + 2].contiguous(), BeamPool.empty(3, W), (3,))
+    for k in ("parents", "tokens", "scores"):
+        assert torch.equal(getattr(o, k)[mid - 1:mid + 2], getattr(a, k)), k
+    assert (a.parents >= 0).all() and (o.parents[:mid - 1] == -1).all() and (o.parents[mid + 2:] == -1).all()
+    assert o.pool.steps.sum() == 3
+
+
 def test_in_place_and_other_streams():
     """Outputs that are the inputs themselves; work queued on a stream of its own."""
     from zllm_amd.beam import BeamStep, beam_select

@@ -7,6 +7,8 @@ L = (V / 256 + 64) 2^-23. A loss is a few such logarithms weighted by at most
 kl_weight and ce_weight, rounded once: 3 (kl + ce) L + 2^-23 |loss|. A
 gradient is weight * (f q - p): q within 2 L of itself (and the factors' 2^-22),
 p within 2^-22, then rounded to the logits' type."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -358,6 +360,63 @@ def test_terms_of_no_weight(n):
             assert torch.isnan(l[1]) and l[2] == 0
             assert torch.isfinite(l[0]) and torch.isfinite(l[3:]).all() and (l[3:] != 0).all()
         assert torch.isnan(g[1]).all() and torch.isfinite(g[0]).all() and torch.isfinite(g[2:]).all()
+
+
+@pytest.mark.parametrize("V,dtype", [(4096, "bf16"), (4099, "f32"), (16385, "f32"), (32761, "bf16"), (50257, "f16"),
+                                     (65537, "bf16"), (100003, "f32"), (151936, "bf16"), (196597, "f32")])
+def test_many_rows(V, dtype):
+    """As many rows as a training step has (a workgroup a row there): 10 rows
+    that go wrong in their own ways, 52 times each. Copies that begin alike in
+    their 16 bytes (which orders the sums) come out bit for bit alike, all of
+    them by the formulas; into other places and in place alike."""
+    from zllm_amd.distill import DistillConfig, distill_loss_grad
+    rng = np.random.default_rng(V)
+    n, times, K = 10, 52, 40
+    x = rng.normal(0, 2, (n, V)).astype(np.float32)
+    ids, logp = lists(rng, x, K)
+    ids[0, ::4] = [V, V + 7, 2 ** 31 - 1, -1, -2, V, V, V, -1, V]
+    ids[1, 5:9] = ids[1, 4]
+    ids[2], logp[2] = -1, -np.inf
+    ids[3, :20], ids[3, 20:] = np.arange(20), V - 1 - np.arange(20)
+    x[4, ids[4]] += 30.0                        # learnt
+    x[5, rng.random(V) < 0.6] = -np.inf
+    ids[5] = rng.choice(np.flatnonzero(np.isfinite(x[5])), K, replace=False)
+    x[6, V // 2] = np.nan
+    x[7, V - 1], x[8, 0] = 25.0, 25.0           # the row's ends
+    ids[7, 0], ids[8, 0] = V - 1, 0
+    labels = ids[:, 1].copy()
+    labels[0], labels[1], labels[2], labels[7], labels[8], labels[9] = V - 1, 77, 0, V - 1, 0, -100
+    w = rng.normal(0, 1, n).astype(np.float32)
+    X, I, P, L, W = (torch.from_numpy(np.concatenate([a] * times)).cuda() for a in (x, ids.astype(np.int32), logp, labels, w))
+    for k, kw in enumerate((dict(tail=True, ce_weight=0.5, temperature=1.5), dict(tail=True, ce_weight=0.3), dict(),
+                            dict(ce_weight=0.2, temperature=2.0))):
+        cfg = DistillConfig(**kw)
+        lab = L if "ce_weight" in kw else None
+        base = torch.full((n * times, V + (0, 3, 8, 5)[k]), float("nan"), dtype=TYPES[dtype], device="cuda")
+        xt = base[:, (0, 1, 8, 2)[k]:][:, :V]
+        xt.copy_(X)
+        print(f"[case] distill many rows V={V} {dtype} {cfg} ld={xt.stride(0)}", flush=True)
+        loss, g = distill_loss_grad(_ctx(), xt, I, P, cfg, W, lab)
+        loss64, grad, size = ref(xt[:n].double().cpu().numpy(), ids, logp, None if lab is None else labels, cfg, w)
+        bits = lambda t: t.contiguous().view(torch.int32 if t.dtype == torch.float32 else torch.int16)
+        alike = 16 // math.gcd(16, n * xt.stride(0) * xt.element_size())      # copies from one to the next alike
+        for a in (bits(loss).view(times, n), bits(g).view(times, n, V)):
+            assert all(torch.equal(a[c], a[c % alike]) for c in range(times))
+        weight = 1.0 + kw.get("ce_weight", 0.0)
+        for c in range(alike):
+            l, d = (t[c * n:(c + 1) * n].double().cpu().numpy() for t in (loss, g))
+            ok = (l == loss64) | (np.isnan(l) & np.isnan(loss64))
+            assert (ok | (np.abs(l - loss64) <= 3 * weight * ltol(V) + 2.0 ** -23 * np.abs(loss64))).all(), (l, loss64)
+            tol = size * (2 * ltol(V) + 2.0 ** -21) + EPS[dtype] * np.abs(grad) + TINY[dtype]
+            assert ((np.isnan(d) & np.isnan(grad)) | (np.abs(d - grad) <= tol)).all(), np.nanmax(np.abs(d - grad) - tol)
+        out = torch.zeros((n * times, V + 9), dtype=TYPES[dtype], device="cuda")
+        distill_loss_grad(_ctx(), xt, I, P, cfg, W, lab, out=out[:, 3:V + 3])
+        assert torch.equal(bits(out[:, 3:V + 3]), bits(g)) and not out[:, :3].any() and not out[:, V + 3:].any()
+        del out
+        distill_loss_grad(_ctx(), xt, I, P, cfg, W, lab, out=xt)
+        assert torch.equal(bits(xt), bits(g))
+        lo = (0, 1, 8, 2)[k]
+        assert torch.isnan(base[:, :lo]).all() and torch.isnan(base[:, lo + V:]).all()
 
 
 def test_student_that_has_learnt_the_list():
