@@ -198,16 +198,17 @@ SIGNATURES = {
     "zs_logprobs_json": (C.c_int, [C.c_int, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p,
                                    C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_char_p, C.c_size_t,
                                    C.POINTER(C.c_size_t)]),
+    # (the argument structures may be given as their bytes)
     "zs_beam_select_work": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_uint64)]),
-    "zs_beam_select": (C.c_int, [C.c_void_p, C.POINTER(Beam), C.c_void_p]),
+    "zs_beam_select": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "zs_beam_reorder": (C.c_int, [C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p, C.POINTER(BeamStateDesc),
                                   C.c_uint32, C.c_void_p]),
     "zs_teacher_topk_work": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_uint64)]),
-    "zs_teacher_topk": (C.c_int, [C.c_void_p, C.POINTER(Teacher), C.c_void_p]),
+    "zs_teacher_topk": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "zs_distill_work": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_uint64)]),
-    "zs_distill_loss": (C.c_int, [C.c_void_p, C.POINTER(Distill), C.c_void_p]),
-    "zs_distill_grad": (C.c_int, [C.c_void_p, C.POINTER(Distill), C.c_void_p]),
-    "zs_distill_loss_grad": (C.c_int, [C.c_void_p, C.POINTER(Distill), C.c_void_p]),
+    "zs_distill_loss": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "zs_distill_grad": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "zs_distill_loss_grad": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "zs_tool_call_envelope_regex": (C.c_int, [C.POINTER(C.c_char_p), C.POINTER(C.c_char_p), C.c_uint32, C.c_char_p,
                                               C.c_size_t, C.POINTER(C.c_size_t), C.c_char_p, C.c_size_t]),
 }

@@ -47,7 +47,7 @@ def teacher_topk(ctx: Context, logits: torch.Tensor, K: int, temperature: float 
     work, at = _work(nbytes, dev)
     raw = _TEACHER.pack(N, V, K, DTYPES[logits.dtype], _ld(logits), logits.data_ptr(), temperature, 0, ids.data_ptr(),
                         logp.data_ptr(), lse.data_ptr(), at, nbytes)
-    rc = lib().zs_teacher_topk(ctx.h, C.byref(Teacher.from_buffer_copy(raw)), _stream(dev))
+    rc = lib().zs_teacher_topk(ctx.h, raw, _stream(dev))
     if rc:
         _check(ctx.h, rc, what)
     return ids, logp, lse
@@ -82,7 +82,7 @@ def _call(ctx, entry, what, logits, ids, logp, cfg, labels, loss=0, stats=0, row
                         lab, cfg.ignore_index, cfg.temperature, cfg.kl_weight, cfg.ce_weight,
                         ZS_DISTILL_TAIL if cfg.tail else 0, loss, stats, row_grad, row_grad_stride, grad, ld_grad, at,
                         nbytes)
-    rc = getattr(lib(), entry)(ctx.h, C.byref(Distill.from_buffer_copy(raw)), _stream(dev))
+    rc = getattr(lib(), entry)(ctx.h, raw, _stream(dev))
     if rc:
         _check(ctx.h, rc, what)
 
@@ -96,7 +96,7 @@ def _grad(what, logits, row_grad, out):
             (row_grad.dim() == 1 and row_grad.shape[0] != N):
         raise ValueError(f"{what}: row_grad is a float32 tensor [N] (or of no dimension: one value for all rows)")
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        out = torch.empty_like(logits)
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or \
             (out.shape[1] > 1 and out.stride(1) != 1) or (N > 1 and out.stride(0) < out.shape[1]):
         raise ValueError(f"{what}: out is like logits, the values of a row adjacent")
