@@ -21,8 +21,7 @@ __device__ __forceinline__ bool bm_is_eos(const bm_args& a, uint32_t id) {
 #define BM_NT 256
 __device__ __forceinline__ void bm_merge(const bm_args& a, uint32_t g) {
     constexpr int NL = ZS_BEAM_MAX_WIDTH * (ZS_BEAM_MAX_WIDTH + ZS_BEAM_MAX_EOS) / BM_NT;   // entries a thread at most
-    __shared__ float cs_[ZS_BEAM_MAX_WIDTH * (ZS_BEAM_MAX_WIDTH + ZS_BEAM_MAX_EOS)];      // the lists' scores and ids
-    __shared__ uint32_t ci_[ZS_BEAM_MAX_WIDTH * (ZS_BEAM_MAX_WIDTH + ZS_BEAM_MAX_EOS)];
+    __shared__ uint2 c_[ZS_BEAM_MAX_WIDTH * (ZS_BEAM_MAX_WIDTH + ZS_BEAM_MAX_EOS)];       // the lists' scores (keys; 0: none) and ids
     __shared__ float bs_[ZS_BEAM_MAX_WIDTH];
     __shared__ double bm_[ZS_BEAM_MAX_WIDTH], bl_[ZS_BEAM_MAX_WIDTH];
     __shared__ float fin_s[ZS_BEAM_MAX_WIDTH];
@@ -60,38 +59,32 @@ __device__ __forceinline__ void bm_merge(const bm_args& a, uint32_t g) {
         const uint32_t b = i / K;
         const float bs = bs_[b];
         const bool some = bs > -INFINITY && e[k] != ~0ull;
-        cs_[i] = some ? (float)((double)bs + (((double)zs_u2f((uint32_t)(e[k] >> 32)) - bm_[b]) - bl_[b])) : -INFINITY;
-        ci_[i] = (uint32_t)e[k] | (bm_is_eos(a, (uint32_t)e[k]) ? 0x80000000u : 0u);
+        const float s = some ? (float)((double)bs + (((double)zs_u2f((uint32_t)(e[k] >> 32)) - bm_[b]) - bl_[b])) : -INFINITY;
+        c_[i] = make_uint2(s > -INFINITY ? zs_total_key(s + 0.0f) : 0u, (uint32_t)e[k] | (bm_is_eos(a, (uint32_t)e[k]) ? 0x80000000u : 0u));
     }
     __syncthreads();
     if (lane >= 64u) return;
-    // the key of the beam's next candidate (0: none) and the one behind it
-    float s = -INFINITY, s2 = -INFINITY;
-    uint32_t id = 0, id2 = 0, next = 0, key = 0;
-    auto ahead = [&]() {
-        const bool some = beam && next < K;
-        s2 = some ? cs_[lane * K + next] : -INFINITY;
-        id2 = some ? ci_[lane * K + next] : 0u;
+    // the beam's next candidate (key 0: none) and the one behind it
+    uint2 c = make_uint2(0u, 0u), c2 = c;
+    uint32_t next = lane * K;
+    const uint32_t end = beam ? next + K : 0u;
+    auto step = [&]() {
+        c = c2;
+        c2 = next < end ? c_[next] : make_uint2(0u, 0u);
         next++;
     };
-    auto step = [&]() {
-        s = s2;
-        id = id2;
-        key = s > -INFINITY ? zs_total_key(s + 0.0f) : 0u;
-        ahead();
-    };
-    ahead();
+    step();
     step();
     int o_parent = -1, o_token = -1;
     float o_score = -INFINITY;
     uint32_t n_live = 0, n_fin = 0;
     for (uint32_t rank = 0; n_live < W; rank++) {
         // (beams are in the first 32 lanes: the last lane of the second row has their maximum)
-        const uint32_t top = zs_readlane_u(zs_dpp_max<0x142, 0xa>(zs_group_max<16>(key)), 31);   // row_bcast:15
+        const uint32_t top = zs_readlane_u(zs_dpp_max<0x142, 0xa>(zs_group_max<16>(c.x)), 31);   // row_bcast:15
         if (!top) break;
-        const uint32_t b = (uint32_t)__builtin_ctzll(__ballot(key == top));   // the lowest beam of equals
-        const float cs = zs_readlane_f(s, b);
-        const uint32_t cid = zs_readlane_u(id, b);
+        const uint32_t b = (uint32_t)__builtin_ctzll(__ballot(c.x == top));   // the lowest beam of equals
+        const float cs = zs_key_to_float(top);
+        const uint32_t cid = zs_readlane_u(c.y, b);
         if (cid >> 31) {   // EOS
             if (rank < W) {
                 if (lane == 0) { fin_s[n_fin] = cs; fin_p[n_fin] = (int)b; fin_t[n_fin] = (int)(cid & 0x7fffffffu); }

@@ -177,16 +177,19 @@ __device__ __forceinline__ void hp_pick(const hd_args& a, uint64_t r, uint32_t l
         k[e] = (uint32_t)e * HP_NT < ng ? zs_gload(gm + min(g, ng - 1u)) : 0u;
         if (g >= ng) k[e] = 0u;
     }
-    if (wid == NW - 1u) {   // the row's normaliser
-        const uint32_t recs = (row.nvec * E + HD_CHUNK - 1u) / HD_CHUNK * (HD_CHUNK / HD_WAVE);
-        const float2* rec = a.rec + r * a.recs;
-        // (two a lane at once: rows of 262144 ids; longer ones take turns)
-        float2 v[2];
+    // The row's normaliser, by the last wave: its records are read here (two a
+    // lane at once: rows of 262144 ids; longer ones take turns), and summed where
+    // that wave has nothing else to do (in front of the list the others waited for it).
+    const uint32_t recs = (row.nvec * E + HD_CHUNK - 1u) / HD_CHUNK * (HD_CHUNK / HD_WAVE);
+    const float2* rec = a.rec + r * a.recs;
+    float2 v[2];
 #pragma unroll
-        for (int w = 0; w < 2; w++) {
-            const uint32_t i = lane + 64u * (uint32_t)w;
-            v[w] = i < recs ? rec[i] : make_float2(-INFINITY, 0.0f);
-        }
+    for (int w = 0; w < 2; w++) {
+        const uint32_t i = lane + 64u * (uint32_t)w;
+        v[w] = wid == NW - 1u && i < recs ? rec[i] : make_float2(-INFINITY, 0.0f);
+    }
+    auto normalise = [&]() {
+        if (wid != NW - 1u) return;
         float m = fmaxf(v[0].x, v[1].x);
         for (uint32_t i = lane + 128u; i < recs; i += 64u) m = fmaxf(m, rec[i].x);
         m = wave_max_f(m);
@@ -197,7 +200,7 @@ __device__ __forceinline__ void hp_pick(const hd_args& a, uint64_t r, uint32_t l
         for (uint32_t i = lane + 128u; i < recs; i += 64u) add(rec[i]);
         s = wave_sum_d(s);
         if (lane == 0) norm = {(double)m, log(s)};
-    }
+    };
 #pragma unroll
     for (int e = 0; e < HP_GPT; e++) {
         if ((uint32_t)e * HP_NT >= ng) break;
@@ -215,19 +218,16 @@ __device__ __forceinline__ void hp_pick(const hd_args& a, uint64_t r, uint32_t l
 #pragma unroll
     for (uint32_t w = 1; w < NW; w++) theta = min(theta, wthr[w]);
     theta = max(theta, 1u);
-    uint32_t ngt = 0;
+    uint32_t reach = 0;
 #pragma unroll
     for (int e = 0; e < HP_GPT; e++) {
         if ((uint32_t)e * HP_NT >= ng) break;
-        ngt += k[e] >= theta ? 1u : 0u;
+        reach |= k[e] >= theta ? 1u << e : 0u;
     }
-    uint32_t p = ngt ? atomicAdd(&u[0], ngt) : 0u;
-#pragma unroll
-    for (int e = 0; e < HP_GPT; e++) {
-        if ((uint32_t)e * HP_NT >= ng) break;
-        if (k[e] < theta) continue;
-        if (p < HP_GL) gl[p] = NW * lane + wid + (uint32_t)e * HP_NT;
-        p++;
+    if (reach) {
+        uint32_t p = atomicAdd(&u[0], (uint32_t)__popc(reach));
+        for (; reach; reach &= reach - 1u, p++)
+            if (p < HP_GL) gl[p] = NW * lane + wid + ((uint32_t)__ffs((int)reach) - 1u) * HP_NT;
     }
     __syncthreads();
     const uint32_t n_gl = u[0], lm = (1u << lgs) - 1u;
@@ -350,20 +350,27 @@ __device__ __forceinline__ void hp_pick(const hd_args& a, uint64_t r, uint32_t l
     static_assert(ZS_TEACHER_KMAX * 8 <= HP_LIST && ZS_TEACHER_KMAX <= HP_GL, "the first K groups and their vectors' values fit");
     if (n <= 128u) {
         // an entry's place is the number of entries in front of it
-        if (t >= 128u) return;
-        const unsigned long long e = t < n ? list[t] : ~0ull;
-        uint32_t place = 0, i = 0;
-        for (; i + 4u <= n; i += 4u) {
+        unsigned long long e = ~0ull;
+        uint32_t place = t;
+        if (t < n) {
+            e = list[t];
+            place = 0;
+            uint32_t i = 0;
+            for (; i + 4u <= n; i += 4u) {
 #pragma unroll
-            for (int q = 0; q < 4; q++) place += list[i + (uint32_t)q] < e ? 1u : 0u;
+                for (int q = 0; q < 4; q++) place += list[i + (uint32_t)q] < e ? 1u : 0u;
+            }
+            for (; i < n; i++) place += list[i] < e ? 1u : 0u;
+            // entries of no candidate (~0 all) lie behind the others as they stand
+            if (e == ~0ull)
+                for (i = 0; i < t; i++) place += list[i] == ~0ull ? 1u : 0u;
         }
-        for (; i < n; i++) place += list[i] < e ? 1u : 0u;
-        // entries of no candidate (~0 all) lie behind the others as they stand
-        if (e == ~0ull && t < n)
-            for (i = 0; i < t; i++) place += list[i] == ~0ull ? 1u : 0u;
-        hd_put(a, r, t < n ? place : t, e, norm);
+        normalise();
+        __syncthreads();
+        if (t < 128u) hd_put(a, r, place, e, norm);
         return;
     }
+    normalise();
     uint32_t np2 = 256;
     while (np2 < n) np2 <<= 1;
     for (uint32_t i = n + t; i < np2; i += HP_NT) list[i] = ~0ull;
