@@ -163,6 +163,27 @@ def test_ties_between_beams_and_ids():
         assert o.parents[1].tolist() == [0, 0, 1, 1] and o.tokens[1].tolist() == [16, 17, 16, 17]
 
 
+@pytest.mark.parametrize("W,eos", [(11, ()), (13, (1,)), (32, ()), (32, tuple(range(8)))])
+def test_wide_beams_of_every_shape(W, eos):
+    """Many candidates at one score (more than are placed at once), a beam that
+    has all of the next ones, beams of a few candidates each, whole numbers,
+    EOS ids first in every beam."""
+    rng = np.random.default_rng(W + len(eos))
+    G, V = 7, 900
+    x = rng.normal(0, 2, (G, W, V)).astype(np.float32)
+    s = beams(rng, G, W)
+    x[0], s[0] = -1.0, 0.0
+    x[1], s[1] = np.round(rng.normal(0, 1, (1, V))), -2.0
+    s[2, 1:] -= 200.0
+    s[3, : W - 1] -= 200.0
+    x[4] = -np.inf
+    x[4, :, 5:8] = rng.normal(0, 1, (W, 3))
+    x[5, :, :8] += 9.0
+    x[6, ::2], s[6, 1::2] = -np.inf, -1.0
+    for dtype in ("f32", "bf16"):
+        check(rows_at(x.reshape(G * W, V), dtype, 1, 0), s, empty_pool(G, W), W, eos, what="wide")
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_values_that_are_no_numbers(dtype):
     """NaN and -inf are no candidates and have no mass, +inf is the largest

@@ -1138,6 +1138,7 @@ extern "C" int zs_beam_select(zs_ctx* ctx, const zs_beam* b, void* stream) {
     h.scores = b->d_scores; h.done = b->d_done; h.width = b->width;
     hd_work(h, b->d_work, true);
     bm_args m{};
+    m.by_kw = zs_div_of((h.K + 3u) / 4u);
     m.width = b->width; m.K = h.K; m.n_eos = b->n_eos; m.early = b->flags & ZS_BEAM_EARLY;
     for (uint32_t i = 0; i < b->n_eos; i++) m.eos[i] = b->eos[i];
     m.length_penalty = b->length_penalty;

@@ -16,6 +16,7 @@ struct bm_args {
     int32_t *fin_length_o, *fin_parent_o, *fin_token_o, *steps_o, *done_o;
     int32_t *parent, *token;
     float* score_o;
+    zs_div by_kw;   // ceil(K / 4)
 };
 
 // One state array: `total` columns of `unit` bytes per row in blocks of `cols`.
