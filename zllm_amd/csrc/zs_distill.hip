@@ -14,10 +14,9 @@
 
 #define DS_NT 256
 #define DS_K ZS_DISTILL_KMAX
-#ifndef DS_FUSED_ROWS
-#define DS_FUSED_ROWS 512
-#endif
-#define DS_FUSED_VOCAB 4096
+#define DS_FUSED_VOCAB 4096    // (rows have whole vectors, and a batch of them)
+#define DS_FUSED_SHORT 32768   // rows up to here by one workgroup each, were there one row,
+#define DS_FUSED_ROWS 96       // longer ones from this many on
 #define DS_FUSED_LDS (160 * 1024 - 6400)   // what the kernel's own shared memory leaves
 
 // A row that takes no part: its label is ignore_index.
@@ -659,7 +658,13 @@ template <int DT>
 static void ds_go(const ds_args& a, int what, uint64_t r0, uint32_t n, hipStream_t stream) {
     const dim3 grid(n * a.chunks), wg(DS_NT);
     const uint32_t vec = (a.V + 7u) / hd_elem<DT>::E + 1u;   // vectors of a row at most
-    if (what == (DS_LOSS | DS_GRAD) && a.N >= DS_FUSED_ROWS && a.V >= DS_FUSED_VOCAB && vec <= 49152u) {
+    if (what == (DS_LOSS | DS_GRAD) && (a.N >= DS_FUSED_ROWS || a.V <= DS_FUSED_SHORT) && a.V >= DS_FUSED_VOCAB && vec <= 49152u) {
+        // against passes of their own (us, one launch against three): bf16 rows
+        // of 4096 10 and 14 (16 rows), 30 and 27 (2048); of 32000 14 and 14 (16),
+        // 17 and 22 (256), 61 and 91 (2048); of 65536 16 and 13 (16), 18 and 18
+        // (96), 19 and 21 (128); of 151936 27 and 15 (16), 31 and 28 (96), 31 and
+        // 33 (128), 291 and 351 (2048); f32 rows of 32000 13 and 15 (16), of
+        // 151936 38 and 41 (96), 172 and 169 (512), 612 and 681 (2048)
         // 16384 bf16 rows of 32000: 483 us by 256 threads, 544 by 512, 827 by
         // 1024; 8192 of 65536: 540, 478, 571; 4096 of 151936 without the tail: 729, 635, 517
         if (vec <= 4u * 1024u) ds_fused<DT, 256>(a, r0, n, stream);

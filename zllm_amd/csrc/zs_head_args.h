@@ -63,6 +63,9 @@ int hd_head_launch(const hd_args& a, const bm_args* beam, uint32_t dtype, hipStr
 // log2 of the values in a group: 64, or 16 where a row has few groups for the
 // list that is wanted (a threshold from group maxima is close only when there
 // are several times K of them), or 256 where 64 would make more than HD_GROUPS.
+// By 16 and by 64, us: 256 f32 rows of 20000 13.8 and 16.6 for K = 64, 20.8 and
+// 25.5 for 128; of 32000 16.6 and 17.9, 23.5 and 28.4; 2048 of 50257 for 128 110
+// and 113; bf16 52 and 61 (2048 rows of 20000, K = 128).
 inline uint32_t hd_group_shift(uint32_t V, uint32_t K) {
     if ((V >> 6) + 2u > HD_GROUPS) return 8;
     return (V >> 6) >= 8u * K || (V >> 4) + 2u > HD_GROUPS ? 6 : 4;
