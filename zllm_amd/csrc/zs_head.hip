@@ -37,7 +37,8 @@ __device__ __forceinline__ uint32_t hs_max(uint32_t k) {
 // LG: lanes of a group. The exponentials and what goes with them bound the
 // pass over 16-bit values, not their bytes: a value takes one shift or mask,
 // half a maximum, one fma, one exponential (a quarter of the rate) and one
-// addition; sums are relative to each thread's own maximum.
+// addition; sums are relative to each thread's own maximum. 2048 x 151936 bf16:
+// 102 us, 6.1 TB/s; 1024 x 151936 f32 100 us, 6.2 (a large read reaches 7.2).
 template <int DT, int LG, bool MASK>
 __global__ __launch_bounds__(HS_NT) void zs_k_head_scan(hd_args a, uint64_t r0) {
     constexpr int E = hd_elem<DT>::E, U = HD_WAVE / 64 / E;
@@ -121,6 +122,11 @@ __global__ __launch_bounds__(HS_NT) void zs_k_head_scan(hd_args a, uint64_t r0) 
 // ---------------------------------------------------------------------------
 // the pick
 // ---------------------------------------------------------------------------
+// Bound by a chain of waits, not by what it moves: the groups' maxima (0.5 us),
+// their sort and threshold (0.5), the list of groups (0.6), their values from
+// memory (1.2), the places (1): 4 us for a row alone, 30 for 2048 rows, of which
+// a third is the wait for the groups' values; the normaliser's exponentials and
+// logarithm are taken beside it by the last wave.
 #define HP_NT 256
 #define HP_GPT (HD_GROUPS / HP_NT)   // groups per thread at most
 #define HP_GL 512                    // listed groups at most (rows in no order: K + 20 to K + 80, of K = 128 up to 270;
