@@ -187,19 +187,21 @@ struct hd_norm {
 __device__ __forceinline__ bool hd_live(const hd_args& a, uint64_t r) {
     return !a.scores || (!a.done[zs_quot((uint32_t)r, a.by_width)] && fabsf(a.scores[r]) <= __FLT_MAX__);   // (beams' rows number below 2^31)
 }
-// Entry t of row r, e = ~key << 32 | id (~0: none); by threads t < K.
+// Place t of row r, e = ~key << 32 | id (~0: none), for every t < K, and for 0
+// and 1 whatever K is: the normaliser's halves go out with them.
 __device__ __forceinline__ void hd_put(const hd_args& a, uint64_t r, uint32_t t, unsigned long long e, hd_norm o) {
-    if (t >= a.K) return;
     const bool some = e != ~0ull;
     const float x = zs_key_to_float(~(uint32_t)(e >> 32));
     if (a.ids) {
+        if (t >= a.K) return;
         a.ids[r * a.K + t] = some ? (uint32_t)e : 0xffffffffu;
         a.logp[r * a.K + t] = some ? (float)(((double)x - o.m) * a.inv_t - o.lns) : -INFINITY;
         if (t == 0) a.lse_out[r] = o.lns > -INFINITY ? (float)(o.m * a.inv_t + o.lns) : -INFINITY;
     } else {
         // (past the L2, which other parts of the GPU do not share)
-        __hip_atomic_store(a.list + r * a.K + t, some ? ((unsigned long long)zs_f2u(x) << 32) | (uint32_t)e : ~0ull,
-                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (t < a.K)
+            __hip_atomic_store(a.list + r * a.K + t, some ? ((unsigned long long)zs_f2u(x) << 32) | (uint32_t)e : ~0ull,
+                               __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if (t < 2) __hip_atomic_store(a.norm + r * 2u + t, t ? o.lns : o.m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
 }
