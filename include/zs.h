@@ -511,6 +511,8 @@ int zs_teacher_topk(zs_ctx* ctx, const zs_teacher* args, void* stream);
  *       sum exp((x - m) / T), sum exp(x - m) and sum outside the list of
  *       exp((x - m) / T); the third is the second's value where CE is not
  *       taken or T = 1, the fourth 0 without the tail, all 0 for ignored rows
+ *       (below the floats it is 0 as well: rows whose fourth is under 2^-64 are
+ *       read again for it, relative to the largest logit outside the list)
  *   zs_distill_grad       reads d_stats and writes d_grad = row_grad[r] *
  *       d loss[r] / d x, rounded once to the logits' type; d_grad may be
  *       d_logits itself (ld_grad = ld)

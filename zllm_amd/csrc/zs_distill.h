@@ -4,12 +4,13 @@
 #include <hip/hip_runtime.h>
 #include "zs_head_args.h"
 
-// What the gradient of a row goes by: y = e * (in the list ? fi : fo) + e1 * f1
-// - fp * p - fc * [the label], e = 2^(x c - mc), e1 = 2^(x c1 - m1).
+// What the gradient of a row goes by. At an id of the list y = e * fi + e1 * f1
+// - fp * p - fc * [the label] with e = 2^(x c - mc), outside it y = eo * fo +
+// e1 * f1 (- fc) with eo = 2^(x co - mco); e1 = 2^(x c1 - m1).
 struct ds_coef {
     float c, mc, c1, m1, fi, fo, f1, fp, fc;
     uint32_t lone;   // the label, where the list does not have it (~0 else)
-    float pad[2];
+    float co, mco;   // c and mc, or those of the outside ids' own maximum
 };
 
 struct ds_args {

@@ -8,7 +8,11 @@
 //   dKL / dx_j = (P e_j / S - p_j - [j outside the list] p_t e_j / S_out) / T
 //   dCE / dx_j = e1_j / S1 - [j = label]
 // S_out is summed over its own ids: S minus the list's share would lose all of
-// its digits where the student has learnt the list.
+// its digits where the student has learnt the list. Where it is less than 2^-64
+// of the row's largest term, its terms leave the floats (e below 2^-126 is 0, and
+// p_t / S_out times it 0 times infinity): such a row is read once more for the
+// sum relative to the outside ids' own maximum (ds_outside), and those ids'
+// gradient is formed with that maximum too.
 #include "zs_head.h"
 #include "zs_distill.h"
 
@@ -161,23 +165,6 @@ __device__ __forceinline__ float ds_of_id(const ds_entry& l, uint32_t K, ds_ids&
     }
     return p;
 }
-// The row's loss (and what the backward pass needs) from its maximum and
-// sums; xk: the entry's logit. Called by every thread.
-template <int NT>
-__device__ __forceinline__ void ds_loss(const ds_args& a, uint64_t r, const ds_entry& l, float xk, int64_t label, float xl,
-                                        double m, double S, double S1, double So, double* shd) {
-    double term = 0.0;
-    if (l.there && l.p != 0.0) term = l.p * (log(l.p) - (((double)xk - m) * a.inv_t - log(S)));   // (NaN stays)
-    term = block_sum_d<NT>(term, shd);
-    if (threadIdx.x) return;
-    // (where the student has nothing outside, the rounding of the list's
-    // probabilities is no tail: 128 of them are within 2^-21 of their sum)
-    if (l.pt > 0.0 && !(So == 0.0 && l.pt < 0x1p-20)) term += l.pt * (log(l.pt) - (log(So) - log(S)));
-    double loss = a.kl != 0.0f ? (double)a.kl * term : 0.0;
-    if (a.labels) loss += a.ce != 0.0f ? (double)a.ce * (log(S1) - ((double)xl - m)) : xl == xl ? 0.0 : NAN;
-    a.loss[r] = (float)loss;
-    if (a.stats) *reinterpret_cast<float4*>(a.stats + r * 4) = make_float4((float)m, (float)S, (float)S1, (float)So);
-}
 // 2^-d of the rounding d of a product
 __device__ __forceinline__ double df_undo(float m, float c) {
     const double d = (double)fmaf(m, c, -(m * c));
@@ -187,10 +174,90 @@ __device__ __forceinline__ double df_undo(float m, float c) {
     }
     return exp2(-d);
 }
-// The gradient's factors.
-__device__ __forceinline__ ds_coef ds_factors(const ds_args& a, uint64_t r, const ds_entry& l, bool bad_label, double m, double S,
+// The sum of exp((x - m) / T) over the ids outside the list, and its m: the
+// row's maximum, or that of those ids.
+struct ds_out {
+    double s, m;
+};
+// Is it wanted relative to their own? The terms that a sum relative to the row's
+// maximum has lost are less than 2^-106 in all, 2^-42 of it at 2^-64. (w: the
+// weight of the tail's term; the second test keeps w pt / s a float.) The same
+// on every thread of the workgroup.
+__device__ __forceinline__ bool ds_far(const ds_args& a, double pt, double s, float w) {
+    const float sf = (float)s, pf = (float)pt;
+    const bool far = a.kl != 0.0f && pf > 0.0f && (sf < 0x1p-64f || fabsf(w) * pf > sf * 0x1p100f);
+    return __builtin_amdgcn_readfirstlane(far);
+}
+// The factor from sums relative to 2^(m c) to those relative to 2^(M c), m <= M.
+__device__ __forceinline__ float ds_join(float m, float M, float c0) {
+    const float Mr = M > -INFINITY ? M : 0.0f, c = hd_factor(Mr, c0);
+    return m == M ? 1.0f : m > -INFINITY && hd_factor(m, c0) == c ? __builtin_amdgcn_exp2f(m * c - Mr * c) : 0.0f;
+}
+// begin(j0): called by every thread, vectors from j0 on are next; in(j): bits of
+// vector j's ids that are in the list. Called by every thread.
+template <int DT, int NT, int U, class Begin, class In>
+__device__ __forceinline__ ds_out ds_outside(const ds_args& a, const hd_row<DT>& row, double m_row, double* shd, Begin begin, In in) {
+    constexpr int E = hd_elem<DT>::E;
+    float m = -INFINITY, s = 0.0f;
+#pragma unroll 1
+    for (uint32_t j0 = 0; j0 < row.nvec; j0 += U * NT) {
+        hd_u4 v[U];
+        row.take(j0 + threadIdx.x, NT, row.inside(j0) && row.inside(j0 + U * NT - 1u), v);
+        begin(j0);
+        float x[U][E], M = m;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t b = in(j0 + threadIdx.x + (uint32_t)(u * NT));
+            hd_unpack<DT>(v[u], x[u]);
+#pragma unroll
+            for (int q = 0; q < E; q++) {
+                x[u][q] = b >> q & 1u ? -INFINITY : x[u][q];
+                M = fmaxf(M, x[u][q]);
+            }
+        }
+        const float Mr = M > -INFINITY ? M : 0.0f, c = hd_factor(Mr, a.c), Mc = Mr * c;
+        s *= ds_join(m, M, a.c);
+        m = M;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float e[E];
+#pragma unroll
+            for (int q = 0; q < E; q++) e[q] = __builtin_amdgcn_exp2f(fmaf(x[u][q], c, -Mc));
+            s += hd_sum(e);
+        }
+    }
+    const float M = block_max_f<NT>(m, reinterpret_cast<float*>(shd));
+    const double S = block_sum_d<NT>((double)(s * ds_join(m, M, a.c)), shd);
+    if (!(M > -INFINITY)) return {0.0, m_row};   // nothing is outside
+    return {S * df_undo(M, hd_factor(M, a.c)), (double)M};
+}
+// The row's loss (and what the backward pass needs) from its maximum and
+// sums; xk: the entry's logit. Called by every thread.
+template <int NT>
+__device__ __forceinline__ void ds_loss(const ds_args& a, uint64_t r, const ds_entry& l, float xk, int64_t label, float xl,
+                                        double m, double S, double S1, ds_out o, double* shd) {
+    double term = 0.0;
+    if (l.there && l.p != 0.0) term = l.p * (log(l.p) - (((double)xk - m) * a.inv_t - log(S)));   // (NaN stays)
+    term = block_sum_d<NT>(term, shd);
+    if (threadIdx.x) return;
+    // (where the student has nothing outside, the rounding of the list's
+    // probabilities is no tail: 128 of them are within 2^-21 of their sum)
+    if (l.pt > 0.0 && !(o.s == 0.0 && l.pt < 0x1p-20)) {
+        const double d = o.m == m ? 0.0 : (o.m - m) * a.inv_t;
+        term += l.pt * (log(l.pt) - (log(o.s) - log(S) + d));
+    }
+    double loss = a.kl != 0.0f ? (double)a.kl * term : 0.0;
+    if (a.labels) loss += a.ce != 0.0f ? (double)a.ce * (log(S1) - ((double)xl - m)) : xl == xl ? 0.0 : NAN;
+    a.loss[r] = (float)loss;
+    if (a.stats) {
+        const double So = o.m == m ? o.s : o.s * exp((o.m - m) * a.inv_t);
+        *reinterpret_cast<float4*>(a.stats + r * 4) = make_float4((float)m, (float)S, (float)S1, (float)So);
+    }
+}
+// The gradient's factors; w: the loss's own.
+__device__ __forceinline__ ds_coef ds_factors(const ds_args& a, float w, const ds_entry& l, bool bad_label, double m, double S,
                                               double S1, double So) {
-    const double g = bad_label ? (double)NAN : (double)a.row_grad[r * a.row_grad_stride];
+    const double g = bad_label ? (double)NAN : (double)w;
     const double kl = g * a.kl * a.inv_t, ce = a.labels ? g * a.ce : 0.0;
     ds_coef k;
     // e = 2^(x c - mc) has mc's rounding for a factor
@@ -204,10 +271,23 @@ __device__ __forceinline__ ds_coef ds_factors(const ds_args& a, uint64_t r, cons
     const double in = kl * l.P / S + (a.two ? 0.0 : one);
     k.fi = (float)(in * f);
     k.fo = (float)((in - (a.tail && So > 0.0 ? kl * l.pt / So : 0.0)) * f);
+    k.co = k.c;
+    k.mco = k.mc;
     k.f1 = (float)(one * f1);
     k.fp = (float)kl;
     k.fc = (float)ce;
     return k;
+}
+
+// Those of the ids outside the list, from a sum relative to their own maximum.
+__device__ __forceinline__ void ds_factors_out(const ds_args& a, float w, const ds_entry& l, bool bad_label, double m, double S, ds_out o,
+                                               ds_coef& k) {
+    if (o.m == m) return;   // (none of them has mass, or the row's maximum is theirs)
+    const double g = bad_label ? (double)NAN : (double)w, kl = g * a.kl * a.inv_t, in = kl * l.P / S + (a.labels && !a.two ? g * a.ce / S : 0.0);
+    const float mo = (float)o.m;
+    k.co = hd_factor(mo, a.c);
+    k.mco = mo * k.co;
+    k.fo = (float)((in * exp((o.m - m) * a.inv_t) - kl * l.pt / o.s) * df_undo(mo, k.co));
 }
 
 #define DF_NT 128   // a thread for every entry of the list
@@ -225,10 +305,13 @@ __global__ __launch_bounds__(DF_NT) void zs_k_distill_row(ds_args a, uint64_t r0
     }
     const hd_row<DT> row(a.logits, a.ld, r, a.V);
     const bool bad_label = a.labels && (label < 0 || label >= (int64_t)a.V);
+    const float w = WHAT & DS_GRAD ? a.row_grad[r * a.row_grad_stride] : 0.0f;
     const ds_entry l = ds_list<DF_NT>(a, r, shd);
     double m, S, S1, So;
+    float xk = 0.0f, xl = NAN;
     if (WHAT & DS_LOSS) {
-        const float xk = l.there ? row.at(l.id) : 0.0f, xl = a.labels && !bad_label ? row.at((uint32_t)label) : NAN;
+        if (l.there) xk = row.at(l.id);
+        if (a.labels && !bad_label) xl = row.at((uint32_t)label);
         constexpr int E = hd_elem<DT>::E;
         const uint32_t recs = (row.nvec * E + HD_CHUNK - 1u) / HD_CHUNK * (HD_CHUNK / DS_WAVE);
         const float4* rec = a.rec + r * a.recs;
@@ -247,7 +330,6 @@ __global__ __launch_bounds__(DF_NT) void zs_k_distill_row(ds_args a, uint64_t r0
         if (!(m > -INFINITY)) S = NAN;   // a row of nothing has no distribution
         S1 = a.two ? block_sum_d<DF_NT>(S1, shd) : S;
         So = a.tail ? block_sum_d<DF_NT>(So, shd) : 0.0;
-        ds_loss<DF_NT>(a, r, l, xk, label, xl, m, S, S1, So, shd);
     } else {
         const float4 st = *reinterpret_cast<const float4*>(a.stats + r * 4);
         m = st.x;
@@ -255,13 +337,39 @@ __global__ __launch_bounds__(DF_NT) void zs_k_distill_row(ds_args a, uint64_t r0
         S1 = st.z;
         So = st.w;
     }
+    __shared__ ds_ids ids;
+    float p = 0.0f;
+    if (WHAT & DS_GRAD) p = ds_of_id<DF_NT>(l, a.K, ids);
+    ds_out o = {So, m};
+    // (a workgroup a row: where all rows are such, the loss of 512 x 128256 f32
+    // takes 114 us for 49, of one bf16 row of 151936 40 for 14, the gradient of
+    // 2048 x 50257 bf16 119 for 78; where none is, what it took without this)
+    const bool far = __builtin_expect(ds_far(a, l.pt, So, WHAT & DS_GRAD ? w * a.kl * (float)a.inv_t : a.kl), 0);
+    if (far) {
+        constexpr int E = hd_elem<DT>::E, U = 4;
+        __shared__ uint32_t mask[U * DF_NT / 4];   // a byte a vector: its ids in the list
+        uint32_t at = 0;
+        o = ds_outside<DT, DF_NT, U>(
+            a, row, m, shd,
+            [&](uint32_t j0) {
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < U / 4; i++) mask[i * DF_NT + t] = 0;
+                __syncthreads();
+                const uint32_t pos = l.id + row.shift, j = pos / E - j0;
+                if (l.there && j < U * DF_NT) atomicOr(&mask[j / 4], 1u << (j % 4 * 8 + pos % E));
+                __syncthreads();
+                at = j0;
+            },
+            [&](uint32_t j) { return (uint32_t) reinterpret_cast<const uint8_t*>(mask)[j - at]; });
+    }
+    if (WHAT & DS_LOSS) ds_loss<DF_NT>(a, r, l, xk, label, xl, m, S, S1, o, shd);
     if (WHAT & DS_GRAD) {
-        __shared__ ds_ids ids;
-        const float p = ds_of_id<DF_NT>(l, a.K, ids);
         if (t < a.K) a.p[r * a.K + t] = l.there ? p : -1.0f;
         const bool listed = __syncthreads_or(l.there && (int64_t)l.id == label);
         if (t == 0) {
-            ds_coef k = ds_factors(a, r, l, bad_label, m, S, S1, So);
+            ds_coef k = ds_factors(a, w, l, bad_label, m, S, S1, So);
+            if (far) ds_factors_out(a, w, l, bad_label, m, S, o, k);
             k.lone = label < 0 || bad_label || listed ? 0xffffffffu : (uint32_t)label;
             a.coef[r] = k;
         }
@@ -276,10 +384,10 @@ __device__ __forceinline__ void ds_store1(void* p, float y) {
     if constexpr (DT == ZS_F32) *(float*)p = y;
     else *(uint16_t*)p = (uint16_t)hd_pack2<DT>(y, 0.0f);
 }
-// e and e1 (times its factor) of one value
+// e (in the list; outside it eo) and e1 (times its factor) of one value
 template <bool TWO>
-__device__ __forceinline__ void ds_exps(const ds_coef& k, float x, float& e, float& e1) {
-    e = __builtin_amdgcn_exp2f(fmaf(x, k.c, -k.mc));
+__device__ __forceinline__ void ds_exps(const ds_coef& k, float x, bool listed, float& e, float& e1) {
+    e = __builtin_amdgcn_exp2f(fmaf(x, listed ? k.c : k.co, -(listed ? k.mc : k.mco)));
     e1 = TWO ? __builtin_amdgcn_exp2f(fmaf(x, k.c1, -k.m1)) * k.f1 : 0.0f;
 }
 // A vector of the gradient to ids i0 .. i0 + E - 1 of the row.
@@ -302,7 +410,7 @@ __device__ __forceinline__ void ds_store(typename hd_elem<DT>::T* grad, uint32_t
 template <bool TWO>
 __device__ __forceinline__ float ds_at(const ds_coef& k, float x, bool listed, float p, bool label) {
     float e, e1;
-    ds_exps<TWO>(k, x, e, e1);
+    ds_exps<TWO>(k, x, listed, e, e1);
     return e * (listed ? k.fi : k.fo) + (e1 - ((listed ? k.fp * p : 0.0f) + (label ? k.fc : 0.0f)));
 }
 
@@ -353,7 +461,7 @@ __global__ __launch_bounds__(DS_NT) void zs_k_distill_grad(ds_args a, uint64_t r
 #pragma unroll
             for (int q = 0; q < E; q++) {
                 float e, e1;
-                ds_exps<TWO>(k, x[u][q], e, e1);
+                ds_exps<TWO>(k, x[u][q], false, e, e1);
                 x[u][q] = TWO ? e * k.fo + e1 : e * k.fo;
             }
     } else {
@@ -419,6 +527,7 @@ __global__ __launch_bounds__(FU_NT, 4) void zs_k_distill_fused(ds_args a, uint64
         return;
     }
     const bool bad_label = a.labels && (label < 0 || label >= (int64_t)a.V);
+    const float rg = a.row_grad[r * a.row_grad_stride];   // (long before its use)
     const uint32_t nb = (row.nvec + BV - 1u) / BV;
     // whole vectors lo .. hi (rows of DS_FUSED_VOCAB ids have some); threads 0
     // and 1 have the vectors before and behind them
@@ -548,33 +657,36 @@ __global__ __launch_bounds__(FU_NT, 4) void zs_k_distill_fused(ds_args a, uint64
     }
     // the wave's relative to its maximum, then every wave by itself the row's
     // from theirs: one barrier, and no value from one thread to the others
-    const auto join = [&](float v, float m, float M, float c0) {   // the factor from 2^(m c) to 2^(M c)
-        const float Mr = M > -INFINITY ? M : 0.0f, c = hd_factor(Mr, c0);
-        return m == M ? 1.0f : m > -INFINITY && hd_factor(m, c0) == c ? __builtin_amdgcn_exp2f(m * c - Mr * c) : 0.0f;
-    };
     const float mw = wave_max_f(m);
     {
-        const float f = join(s, m, mw, a.c);
+        const float f = ds_join(m, mw, a.c);
         df_wave w;
         w.m = mw;
         w.s = wave_sum_d((double)(s * f));
         w.so = TAIL ? wave_sum_d((double)(so * f)) : 0.0;
-        w.s1 = TWO ? wave_sum_d((double)(s1 * join(s1, m, mw, c1))) : 0.0;
+        w.s1 = TWO ? wave_sum_d((double)(s1 * ds_join(m, mw, c1))) : 0.0;
         if (zs_lane() == 0) wv[zs_wid()] = w;
     }
     __syncthreads();
     df_wave w = {0.0, 0.0, 0.0, -INFINITY};
     if (zs_lane() < FU_NT / 64) w = wv[zs_lane()];
     const float M = wave_max_f(w.m), Mr = M > -INFINITY ? M : 0.0f;
-    const double f = (double)join(0.0f, w.m, M, a.c), u = df_undo(Mr, hd_factor(Mr, a.c));
+    const double f = (double)ds_join(w.m, M, a.c), u = df_undo(Mr, hd_factor(Mr, a.c));
     double S = wave_sum_d(w.s * f) * u, So = TAIL ? wave_sum_d(w.so * f) * u : 0.0, S1 = S;
-    if (TWO) S1 = wave_sum_d(w.s1 * (double)join(0.0f, w.m, M, c1)) * df_undo(Mr, hd_factor(Mr, c1));
+    if (TWO) S1 = wave_sum_d(w.s1 * (double)ds_join(w.m, M, c1)) * df_undo(Mr, hd_factor(Mr, c1));
     if (!(M > -INFINITY)) S = S1 = NAN;   // a row of nothing has no distribution
     ds_entry l;
     l.there = t < DS_K && hid[t] < a.V;
     l.pt = kept.pt;
     l.P = kept.P;
-    ds_coef k = ds_factors(a, r, l, bad_label, (double)M, S, S1, So);
+    ds_coef k = ds_factors(a, rg, l, bad_label, (double)M, S, S1, So);
+    ds_out o = {So, (double)M};
+    // (not expected, or every row keeps ready what it needs: 534 us for 527 of
+    // 4096 x 151936 bf16; where all rows are such 818)
+    if (TAIL && __builtin_expect(ds_far(a, l.pt, So, rg * a.kl * (float)a.inv_t), 0)) {
+        o = ds_outside<DT, FU_NT, 1>(a, row, (double)M, shd, [](uint32_t) {}, [&](uint32_t j) { return (uint32_t)in_list[j]; });
+        ds_factors_out(a, rg, l, bad_label, (double)M, S, o, k);
+    }
     // second pass, from the batch at hand backwards: every id as one outside
     // the list; the others are written over it as in zs_k_distill_grad
     if (t < DS_K) {
@@ -588,7 +700,7 @@ __global__ __launch_bounds__(FU_NT, 4) void zs_k_distill_fused(ds_args a, uint64
 #pragma unroll
         for (int q = 0; q < E; q++) {
             float e, e1;
-            ds_exps<TWO>(k, x[q], e, e1);
+            ds_exps<TWO>(k, x[q], false, e, e1);
             x[q] = TWO ? e * k.fo + e1 : e * k.fo;
         }
     };
@@ -641,7 +753,7 @@ __global__ __launch_bounds__(FU_NT, 4) void zs_k_distill_fused(ds_args a, uint64
     }
     // the loss last: its logarithms pass while the stores do
     l.p = l.there ? kept.p[t] : 0.0;
-    ds_loss<FU_NT>(a, r, l, t < DS_K ? kept.x[t] : 0.0f, label, kept.x[DS_K], (double)M, S, S1, So, shd);
+    ds_loss<FU_NT>(a, r, l, t < DS_K ? kept.x[t] : 0.0f, label, kept.x[DS_K], (double)M, S, S1, o, shd);
 }
 
 template <int DT, int NT>
