@@ -104,14 +104,24 @@ class BeamPool:
         return cls(torch.full((groups, width), -float("inf"), device=device), i(0, groups, width), i(-1, groups, width),
                    i(-1, groups, width), i(0, groups), i(0, groups))
 
-    def _pointers(self, G: int, W: int, dev, what: str):
-        if getattr(self, "_checked", None) != (G, W, dev):   # (the fields do not change)
-            for name in _POOL:
-                _like(getattr(self, name), (G,) if name in ("steps", "done") else (G, W),
-                      torch.float32 if name == "score" else torch.int32, dev, what, "pool." + name)
-            object.__setattr__(self, "_checked", (G, W, dev))
+    def _at(self):
         return (self.score.data_ptr(), self.length.data_ptr(), self.parent.data_ptr(), self.token.data_ptr(),
                 self.steps.data_ptr(), self.done.data_ptr())
+
+    def _pointers(self, G: int, W: int, dev, what: str):
+        # In every call: a tensor may have been resized or put elsewhere since
+        # the last. (In one expression 1.5 us of a call's 23, with a _like each 4.)
+        s, l, p, t, n, d = self.score, self.length, self.parent, self.token, self.steps, self.done
+        gw, g, i32, at = (G, W), (G,), torch.int32, -1 if dev.index is None else dev.index
+        if not (s.shape == gw and l.shape == gw and p.shape == gw and t.shape == gw and n.shape == g and d.shape == g and
+                s.dtype is torch.float32 and l.dtype is i32 and p.dtype is i32 and t.dtype is i32 and n.dtype is i32 and
+                d.dtype is i32 and s.get_device() == at and l.get_device() == at and p.get_device() == at and
+                t.get_device() == at and n.get_device() == at and d.get_device() == at and s.is_contiguous() and l.is_contiguous() and p.is_contiguous() and
+                t.is_contiguous() and n.is_contiguous() and d.is_contiguous()):
+            for name in _POOL:
+                _like(getattr(self, name), g if name in ("steps", "done") else gw,
+                      torch.float32 if name == "score" else i32, dev, what, "pool." + name)
+        return self._at()
 
 
 @dataclass(frozen=True)
@@ -127,9 +137,8 @@ class BeamStep:
         a part of one that is taken apart 0.4.)"""
         i = torch.empty((7, groups, width), dtype=torch.int32, device=device).unbind(0)
         steps, done = torch.empty((2, groups), dtype=torch.int32, device=device).unbind(0)
-        pool = BeamPool(i[5].view(torch.float32), i[2], i[3], i[4], steps, done)
-        object.__setattr__(pool, "_checked", (groups, width, device))
-        return cls(i[0], i[1], i[6].view(torch.float32), pool)
+        return cls(i[0], i[1], i[6].view(torch.float32),
+                   BeamPool(i[5].view(torch.float32), i[2], i[3], i[4], steps, done))
 
 
 def beam_select(ctx: Context, logits: torch.Tensor, scores: torch.Tensor, pool: BeamPool, eos: Sequence[int] = (),
@@ -150,7 +159,10 @@ def beam_select(ctx: Context, logits: torch.Tensor, scores: torch.Tensor, pool: 
     if R != G * W:
         raise ValueError(f"{what}: {R} rows of logits for {G} groups of {W} beams")
     n_eos = len(eos)
-    if n_eos > MAX_EOS or any(not 0 <= e < 2 ** 32 for e in eos):
+    ends = n_eos <= MAX_EOS
+    for e in eos:
+        ends = ends and 0 <= e < 2 ** 32
+    if not ends:
         raise ValueError(f"{what}: at most {MAX_EOS} EOS ids, not negative")
     _like(scores, (G, W), torch.float32, dev, what, "scores")
     allow, words = 0, 0
@@ -162,7 +174,9 @@ def beam_select(ctx: Context, logits: torch.Tensor, scores: torch.Tensor, pool: 
     before = pool._pointers(G, W, dev, what)
     if out is None:
         out = BeamStep.alloc(G, W, dev)
+        after = out.pool._at()
     else:
+        after = before if out.pool is pool else out.pool._pointers(G, W, dev, what)
         _like(out.parents, (G, W), torch.int32, dev, what, "out.parents")
         _like(out.tokens, (G, W), torch.int32, dev, what, "out.tokens")
         _like(out.scores, (G, W), torch.float32, dev, what, "out.scores")
@@ -170,7 +184,7 @@ def beam_select(ctx: Context, logits: torch.Tensor, scores: torch.Tensor, pool: 
     work, at = _work(nbytes, dev)
     raw = _BEAM.pack(G, W, V, DTYPES[logits.dtype], _ld(logits), logits.data_ptr(), allow, words, n_eos, *eos,
                      *(0,) * (MAX_EOS - n_eos), length_penalty, ZS_BEAM_EARLY if early_stopping else 0, scores.data_ptr(),
-                     *before, *out.pool._pointers(G, W, dev, what), out.parents.data_ptr(),
+                     *before, *after, out.parents.data_ptr(),
                      out.tokens.data_ptr(), out.scores.data_ptr(), at, nbytes)
     rc = lib().zs_beam_select(ctx.h, raw, _stream(dev))
     if rc:
