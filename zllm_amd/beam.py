@@ -42,13 +42,14 @@ def _stream(dev: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
-def _rows(logits: torch.Tensor, what: str) -> None:
+def _rows(ctx: Context, logits: torch.Tensor, what: str) -> None:
     """Checks a [rows, V] tensor of logits: any of the three types, any row
-    stride, the values of a row adjacent."""
+    stride, the values of a row adjacent, on the context's GPU (whose kernels
+    are launched; the stream is the logits')."""
     if logits.dim() != 2 or logits.dtype not in DTYPES:
         raise ValueError(f"{what}: logits are [rows, V] of float32, float16 or bfloat16")
-    if not logits.is_cuda:
-        raise ValueError(f"{what}: logits are on {logits.device}, not on a GPU")
+    if logits.get_device() != ctx.device:
+        raise ValueError(f"{what}: logits are on {logits.device}, not on the context's GPU {ctx.device}")
     if logits.shape[1] > 1 and logits.stride(1) != 1:
         raise ValueError(f"{what}: the logits of a row are not adjacent")
 
@@ -150,7 +151,7 @@ def beam_select(ctx: Context, logits: torch.Tensor, scores: torch.Tensor, pool: 
     ByteDfa.mask writes them; the scores are of the masked distribution. `out`
     may hold `scores` and the tensors of `pool` themselves. No host sync."""
     what = "beam_select"
-    _rows(logits, what)
+    _rows(ctx, logits, what)
     dev = logits.device
     if scores.dim() != 2 or not 1 <= scores.shape[1] <= MAX_WIDTH:
         raise ValueError(f"{what}: scores are [groups, width], width 1 to {MAX_WIDTH}")
@@ -252,6 +253,8 @@ def beam_reorder(ctx: Context, states: BeamStates, parents: torch.Tensor) -> Non
     if not states.n:
         return
     dev = states.tensors[0].device
+    if dev.index != ctx.device:
+        raise ValueError(f"beam_reorder: states are on {dev}, not on the context's GPU {ctx.device}")
     _like(parents, (states.rows // states.width, states.width), torch.int32, dev, "beam_reorder", "parents")
     rc = lib().zs_beam_reorder(ctx.h, parents.shape[0], states.width, parents.data_ptr(), states.descs, states.n,
                                _stream(dev))

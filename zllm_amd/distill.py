@@ -35,7 +35,7 @@ def teacher_topk(ctx: Context, logits: torch.Tensor, K: int, temperature: float 
     ln sum exp(logits / temperature) float32 [N] (zs_teacher_topk). Rows of
     fewer than K values above -inf end with ids -1, logp -inf. No host sync."""
     what = "teacher_topk"
-    _rows(logits, what)
+    _rows(ctx, logits, what)
     N, V = logits.shape
     if not 1 <= K <= min(V, MAX_TOP):
         raise ValueError(f"{what}: K is 1 to min(V, {MAX_TOP})")
@@ -67,7 +67,7 @@ class DistillConfig:
 
 def _call(ctx, entry, what, logits, ids, logp, cfg, labels, loss=0, stats=0, row_grad=0, row_grad_stride=0, grad=0,
           ld_grad=0):
-    _rows(logits, what)
+    _rows(ctx, logits, what)
     N, V = logits.shape
     dev = logits.device
     if ids.dim() != 2 or ids.shape[0] != N or not 1 <= ids.shape[1] <= MAX_TOP:
@@ -87,9 +87,9 @@ def _call(ctx, entry, what, logits, ids, logp, cfg, labels, loss=0, stats=0, row
         _check(ctx.h, rc, what)
 
 
-def _grad(what, logits, row_grad, out):
+def _grad(ctx, what, logits, row_grad, out):
     """The gradient's arguments and its tensor."""
-    _rows(logits, what)
+    _rows(ctx, logits, what)
     N = logits.shape[0]
     dev = logits.device
     if row_grad.dtype != torch.float32 or row_grad.device != dev or row_grad.dim() > 1 or \
@@ -123,7 +123,7 @@ def distill_grad(ctx: Context, logits: torch.Tensor, ids: torch.Tensor, logp: to
     """Gradient of sum_r row_grad[r] * loss[r] by the logits, in their type;
     stats from distill_loss. out may be the logits themselves."""
     what = "distill_grad"
-    kw, out = _grad(what, logits, row_grad, out)
+    kw, out = _grad(ctx, what, logits, row_grad, out)
     st = _like(stats, (logits.shape[0], 4), torch.float32, logits.device, what, "stats").data_ptr()
     _call(ctx, "zs_distill_grad", what, logits, ids, logp, cfg, labels, stats=st, **kw)
     return out
@@ -135,7 +135,7 @@ def distill_loss_grad(ctx: Context, logits: torch.Tensor, ids: torch.Tensor, log
     """distill_loss and distill_grad in one call, where the rows' weights are
     known before the loss (a mean over the rows: row_grad = 1 / N)."""
     what = "distill_loss_grad"
-    kw, out = _grad(what, logits, row_grad, out)
+    kw, out = _grad(ctx, what, logits, row_grad, out)
     loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
     _call(ctx, "zs_distill_loss_grad", what, logits, ids, logp, cfg, labels, loss.data_ptr(), **kw)
     return loss, out
