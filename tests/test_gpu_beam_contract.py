@@ -1,5 +1,5 @@
 """What beam search and distillation owe their callers beside their numbers:
-tensors of another device than the context's."""
+writes that autograd sees, tensors of another device than the context's."""
 import types
 
 import pytest
@@ -13,6 +13,53 @@ pytestmark = pytest.mark.gpu
 def lists(N, V, K=4):
     ids = torch.arange(K, dtype=torch.int32, device="cuda").expand(N, K).contiguous()
     return ids, torch.full((N, K), -1.6, device="cuda")
+
+
+def test_gradients_written_over_saved_logits_are_seen():
+    """A backward pass over logits that were overwritten since raises, as it
+    does after any in-place operation."""
+    from zllm_amd.distill import DistillConfig, DistillLoss, distill_grad, distill_loss, distill_loss_grad
+    N, V = 3, 40
+    ids, logp = lists(N, V)
+    cfg, w = DistillConfig(), torch.ones(N, device="cuda")
+    for write in ("grad", "both"):
+        leaf = torch.randn((N, V), device="cuda", requires_grad=True)
+        logits = leaf * 1.0
+        loss = DistillLoss(_ctx(), cfg)(logits, ids, logp).sum()
+        over = logits.detach()
+        if write == "grad":
+            stats = distill_loss(_ctx(), over, ids, logp, cfg)[1]
+            distill_grad(_ctx(), over, ids, logp, cfg, stats, w, out=over)
+        else:
+            distill_loss_grad(_ctx(), over, ids, logp, cfg, w, out=over)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
+def test_states_and_steps_written_in_place_are_seen():
+    from zllm_amd.beam import BeamPool, BeamStates, BeamStep, beam_reorder, beam_select
+    state = torch.randn((4, 2, 5), device="cuda")
+    view = state[:, :, 1:]
+    parents = torch.tensor([[1, 0], [0, 0]], dtype=torch.int32, device="cuda")
+    before = state._version
+    beam_reorder(_ctx(), BeamStates([(view, 0)], 2), parents)
+    assert state._version > before
+    logits, scores, pool = torch.randn((4, 9), device="cuda"), torch.zeros((2, 2), device="cuda"), BeamPool.empty(2, 2)
+    out = BeamStep(torch.empty_like(parents), torch.empty_like(parents), scores, pool)
+    written = [out.parents, out.tokens, scores] + [getattr(pool, k) for k in ("score", "length", "parent", "token", "steps",
+                                                                              "done")]
+    before = [t._version for t in written]
+    beam_select(_ctx(), logits, scores, pool, out=out)
+    assert all(t._version > b for t, b in zip(written, before))
+
+
+def test_inference_tensors_are_taken():
+    """(they have no version)"""
+    from zllm_amd.beam import BeamStates, beam_reorder
+    with torch.inference_mode():
+        state = torch.arange(4, dtype=torch.int32, device="cuda")
+        beam_reorder(_ctx(), BeamStates([(state, 0)], 2), torch.tensor([[1, 0], [0, 0]], dtype=torch.int32, device="cuda"))
+    assert state.tolist() == [1, 0, 2, 2]
 
 
 def test_tensors_of_another_device_than_the_contexts_are_refused():

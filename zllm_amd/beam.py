@@ -20,6 +20,7 @@ from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
+from torch.autograd.graph import increment_version
 
 from ._lib import Beam, BeamStateDesc, ZsError, lib
 from .engine import Context, _check
@@ -173,7 +174,8 @@ def beam_select(ctx: Context, logits: torch.Tensor, scores: torch.Tensor, pool: 
         allow, words = _like(allow_bits, allow_bits.shape, torch.int32, dev, what, "allow_bits").data_ptr(), \
             allow_bits.shape[1]
     before = pool._pointers(G, W, dev, what)
-    if out is None:
+    given = out is not None
+    if not given:
         out = BeamStep.alloc(G, W, dev)
         after = out.pool._at()
     else:
@@ -190,6 +192,9 @@ def beam_select(ctx: Context, logits: torch.Tensor, scores: torch.Tensor, pool: 
     rc = lib().zs_beam_select(ctx.h, raw, _stream(dev))
     if rc:
         _check(ctx.h, rc, what)
+    if given:   # (autograd is told of writes in place)
+        p = out.pool
+        increment_version((out.parents, out.tokens, out.scores, p.score, p.length, p.parent, p.token, p.steps, p.done))
     return out
 
 
@@ -243,6 +248,8 @@ class BeamStates:
         if self.rows is not None and self.rows % width:
             raise ValueError("BeamStates: the rows are not whole groups")
         self.n = len(descs)
+        self.device = self.tensors[0].device if self.tensors else None
+        self.parents_shape = (self.rows // width, width) if self.tensors else None
         self.descs = (BeamStateDesc * max(self.n, 1))(*descs)
 
 
@@ -252,14 +259,15 @@ def beam_reorder(ctx: Context, states: BeamStates, parents: torch.Tensor) -> Non
     negative ones stay. No host sync."""
     if not states.n:
         return
-    dev = states.tensors[0].device
+    dev, shape = states.device, states.parents_shape
     if dev.index != ctx.device:
         raise ValueError(f"beam_reorder: states are on {dev}, not on the context's GPU {ctx.device}")
-    _like(parents, (states.rows // states.width, states.width), torch.int32, dev, "beam_reorder", "parents")
-    rc = lib().zs_beam_reorder(ctx.h, parents.shape[0], states.width, parents.data_ptr(), states.descs, states.n,
+    _like(parents, shape, torch.int32, dev, "beam_reorder", "parents")
+    rc = lib().zs_beam_reorder(ctx.h, shape[0], shape[1], parents.data_ptr(), states.descs, states.n,
                                _stream(dev))
     if rc:
         _check(ctx.h, rc, "beam_reorder")
+    increment_version(states.tensors)   # (autograd is told of writes in place)
 
 
 @dataclass

@@ -15,6 +15,7 @@ from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from ._lib import Distill, Teacher, lib
 from .beam import DTYPES, MAX_VOCAB, _ld, _like, _rows, _stream, _work, _work_bytes
@@ -123,9 +124,12 @@ def distill_grad(ctx: Context, logits: torch.Tensor, ids: torch.Tensor, logp: to
     """Gradient of sum_r row_grad[r] * loss[r] by the logits, in their type;
     stats from distill_loss. out may be the logits themselves."""
     what = "distill_grad"
+    given = out is not None
     kw, out = _grad(ctx, what, logits, row_grad, out)
     st = _like(stats, (logits.shape[0], 4), torch.float32, logits.device, what, "stats").data_ptr()
     _call(ctx, "zs_distill_grad", what, logits, ids, logp, cfg, labels, stats=st, **kw)
+    if given:
+        increment_version(out)   # (autograd is told of writes in place)
     return out
 
 
@@ -135,9 +139,12 @@ def distill_loss_grad(ctx: Context, logits: torch.Tensor, ids: torch.Tensor, log
     """distill_loss and distill_grad in one call, where the rows' weights are
     known before the loss (a mean over the rows: row_grad = 1 / N)."""
     what = "distill_loss_grad"
+    given = out is not None
     kw, out = _grad(ctx, what, logits, row_grad, out)
     loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
     _call(ctx, "zs_distill_loss_grad", what, logits, ids, logp, cfg, labels, loss.data_ptr(), **kw)
+    if given:
+        increment_version(out)
     return loss, out
 
 
