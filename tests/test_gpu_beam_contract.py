@@ -1,5 +1,7 @@
-"""What beam search and distillation owe their callers beside their numbers:
-writes that autograd sees, tensors of another device than the context's."""
+"""What beam search and distillation owe their callers beside their numbers: the
+loop that the module documents, writes that autograd sees, tensors of another
+device than the context's."""
+import textwrap
 import types
 
 import pytest
@@ -8,6 +10,42 @@ import torch
 from tests.test_gpu_beam import _ctx
 
 pytestmark = pytest.mark.gpu
+
+
+def documented_loop():
+    """The indented lines of zllm_amd.beam's docstring."""
+    from zllm_amd import beam
+    lines = beam.__doc__.splitlines()
+    return textwrap.dedent("\n".join(l for l in lines if l.startswith("    ")))
+
+
+def test_the_documented_loop_runs():
+    """Under a model that takes ids of its vocabulary alone, with beams that are
+    absent after the first step (fewer ids allowed than beams)."""
+    from zllm_amd import beam
+    V, groups, width = 50, 2, 3
+    table = torch.randn((V, V), generator=torch.Generator().manual_seed(1))
+    table[7:9, 3:] = -float("inf")
+    table[7:9, 2] = -float("inf")           # two ids at the first step: the third beam is absent
+
+    def model(tokens, *_):
+        assert tokens.shape == (groups * width,)
+        return torch.nn.functional.embedding(tokens.cpu(), table).cuda()     # (an id outside raises here)
+    names = dict(vars(beam), ctx=_ctx(), groups=groups, width=width, max_steps=5, g=1, model=model,
+                 first=torch.tensor([7, 8], device="cuda").repeat_interleave(width),
+                 kv_cache=torch.zeros((2, 2, groups * width, 2, 5, 8), device="cuda"),
+                 grammar_state=torch.zeros(groups * width, dtype=torch.int32, device="cuda"))
+    print("[case] the documented loop", flush=True)
+    exec(documented_loop(), names)
+    assert names["best"] and all(0 <= t < V for t in names["best"])
+
+
+def test_before_the_first_step_every_beam_is_absent():
+    from zllm_amd.beam import BeamSearch
+    for steps in (0, 1, 4):
+        s = BeamSearch(_ctx(), 2, 3, steps)
+        assert (s.parents == -1).all() and (s.tokens == -1).all() and s.tokens.shape == (2, 3)
+        assert s.sequences() == [[], []] and s.finished() == (steps == 0)
 
 
 def lists(N, V, K=4):

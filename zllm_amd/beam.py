@@ -3,12 +3,15 @@ logits, and the reordering of the states that follow them.
 
     search = BeamSearch(ctx, groups, width, max_steps, eos=(2,))
     states = BeamStates([(kv_cache, 2), (grammar_state, 0)], width)
+    tokens = first                                  # the beams' first inputs, [groups * width]
     while not search.finished():
-        logits = model(search.tokens, ...)          # [groups * width, V]
-        search.step(logits)
+        search.step(model(tokens))                  # logits [groups * width, V]
         beam_reorder(ctx, states, search.parents)
+        tokens = search.tokens.view(-1).clamp_min(0)
     best = search.sequences()[g][0].tokens
 
+Absent beams have the token -1, which no model takes: their rows of logits are
+not read, so any id stands for it.
 The reference decodes one hypothesis per request; there is no counterpart.
 torch holds the device memory and the stream; the computation is libzs's.
 """
@@ -289,17 +292,19 @@ class BeamSearch:
         self.scores = torch.full((groups, width), -float("inf"), device=device)
         self.scores[:, 0] = 0.0
         self.pool = BeamPool.empty(groups, width, device)
-        self._trace = torch.full((max_steps, 2, groups, width), -1, dtype=torch.int32, device=device)
+        self._trace = torch.full((max_steps or 1, 2, groups, width), -1, dtype=torch.int32, device=device)
         self.t = 0
 
     @property
     def parents(self) -> torch.Tensor:
-        """Parents of the last step's beams (int32 [groups, width])."""
+        """Parents of the last step's beams (int32 [groups, width]; -1 for
+        absent ones, and in front of the first step for all)."""
         return self._trace[self.t - 1, 0]
 
     @property
     def tokens(self) -> torch.Tensor:
-        """Tokens of the last step's beams (int32 [groups, width])."""
+        """Tokens of the last step's beams (int32 [groups, width]; -1 as for
+        parents)."""
         return self._trace[self.t - 1, 1]
 
     def step(self, logits: torch.Tensor, allow_bits: Optional[torch.Tensor] = None) -> None:
