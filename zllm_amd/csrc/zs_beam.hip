@@ -10,8 +10,8 @@
 // array needs no second copy. The loads are issued without conditions, those of
 // rows that stay from a parent that is loaded anyway: behind a branch each the
 // compiler waits for every one by itself (5 beams, 294 MB: 193 us, so 67; 4
-// beams, 4058 MB: 660 to 790, so 640 to 740; waiting for all before the first
-// store: 675 to 780).
+// beams, 4058 MB: 660 to 790, so 640 to 740, and in other runs up to 815, by where
+// the caches lie; waiting for all before the first store: 675 to 780).
 // ---------------------------------------------------------------------------
 #define RO_NT 256
 #define RO_GLOBAL __attribute__((address_space(1)))

@@ -491,9 +491,10 @@ __global__ __launch_bounds__(DS_NT) void zs_k_distill_grad(ds_args a, uint64_t r
 // their use; they are issued without conditions (vectors at the row's ends are
 // clamped to whole ones, the ends themselves read apart), or the compiler waits
 // for all of them at every join of the branches. Bound by memory: 4096 rows of
-// 151936 bf16, 2.49 GB, 517 us without the tail (4.8 TB/s) and 590 with it (what
-// is not hidden: the list's and the row's end); every batch read twice, 578 and
-// 621; by 512 threads, two workgroups a unit, 635; as passes of their own, 709.
+// 151936 bf16, 2.49 GB, 506 us without the tail (4.9 TB/s) and 527 with it (what
+// is not hidden: the list's and the row's end). As it was first, 517 and 590,
+// against every batch read twice, 578 and 621, 512 threads, two workgroups a
+// unit, 635, and passes of their own, 709.
 // What is kept of a row's list while the row passes.
 struct df_kept {
     double p[DS_K], pt, P;
@@ -779,6 +780,7 @@ static void ds_go(const ds_args& a, int what, uint64_t r0, uint32_t n, hipStream
         // 151936 38 and 41 (96), 172 and 169 (512), 612 and 681 (2048)
         // 16384 bf16 rows of 32000: 483 us by 256 threads, 544 by 512, 827 by
         // 1024; 8192 of 65536: 540, 478, 571; 4096 of 151936 without the tail: 729, 635, 517
+        // (506 now)
         if (vec <= 4u * 1024u) ds_fused<DT, 256>(a, r0, n, stream);
         else if (vec <= 4u * 2048u + 1u) ds_fused<DT, 512>(a, r0, n, stream);
         else ds_fused<DT, 1024>(a, r0, n, stream);

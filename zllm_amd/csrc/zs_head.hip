@@ -38,7 +38,9 @@ __device__ __forceinline__ uint32_t hs_max(uint32_t k) {
 // pass over 16-bit values, not their bytes: a value takes one shift or mask,
 // half a maximum, one fma, one exponential (a quarter of the rate) and one
 // addition; sums are relative to each thread's own maximum. 2048 x 151936 bf16:
-// 102 us, 6.1 TB/s; 1024 x 151936 f32 100 us, 6.2 (a large read reaches 7.2).
+// 102 us, 6.1 TB/s, the vector units busy for 85 % of them; over f32 they are for
+// half, and memory bounds the pass: 1024 x 151936 100 us, 6.2 TB/s (a large read
+// reaches 7.2).
 template <int DT, int LG, bool MASK>
 __global__ __launch_bounds__(HS_NT) void zs_k_head_scan(hd_args a, uint64_t r0) {
     constexpr int E = hd_elem<DT>::E, U = HD_WAVE / 64 / E;
@@ -124,7 +126,8 @@ __global__ __launch_bounds__(HS_NT) void zs_k_head_scan(hd_args a, uint64_t r0) 
 // ---------------------------------------------------------------------------
 // Bound by a chain of waits, not by what it moves: the groups' maxima (0.5 us),
 // their sort and threshold (0.5), the list of groups (0.6), their values from
-// memory (1.2), the places (1): 4 us for a row alone, 30 for 2048 rows, of which
+// memory (1.2), the places (1): 4 us of a row; the kernel of a row alone takes 5
+// to 6 (K = 16 of 50257 f32; K = 64 of 151936 bf16 11), of 2048 rows 29, of which
 // a third is the wait for the groups' values; the normaliser's exponentials and
 // logarithm are taken beside it by the last wave.
 #define HP_NT 256

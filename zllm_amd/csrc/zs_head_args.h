@@ -10,9 +10,6 @@
 #define HD_GROUPS 5120         // groups of a row at most (the pick holds their maxima in registers)
 #define HD_BLOCKS (1u << 22)   // workgroups per launch at most
 
-// The heads of R rows. For a teacher (d_ids) the list goes out as ids and
-// log-probabilities; for the beam step into `list` (bits of x~ << 32 | id,
-// ~0 for none) and `norm`, of the rows whose beam lives.
 // n / d for n < 2^31 by a product: n / d = mulhi(n, mul) >> (sh - 32), d >= 2,
 // with mul = ceil(2^sh / d) and 2^sh the first power at or above 2^31 d (the
 // excess e = mul d - 2^sh < d gives n e < 2^31 d <= 2^sh). sh 0: d is 1.
@@ -31,6 +28,9 @@ inline zs_div zs_div_of(uint64_t d) {
 __device__ __forceinline__ uint32_t zs_quot(uint32_t n, zs_div q) { return q.sh ? __umulhi(n, q.mul) >> (q.sh - 32u) : n; }
 #endif
 
+// The heads of R rows. For a teacher (d_ids) the list goes out as ids and
+// log-probabilities; for the beam step into `list` (bits of x~ << 32 | id,
+// ~0 for none) and `norm`, of the rows whose beam lives.
 struct hd_args {
     const void* logits;
     uint64_t ld, R;
