@@ -461,8 +461,8 @@ int zs_beam_select(zs_ctx* ctx, const zs_beam* args, void* stream);
  * all arrays in as few launches as they need (ZS_REORDER_BATCH arrays each);
  * rows whose parent is their own beam, negative or >= width stay. A row of an
  * array is n_outer * n_inner blocks of `bytes` bytes, block (o, i) of row r
- * at base + o * outer_stride + r * row_stride + i * inner_stride (bytes);
- * blocks of different rows, or of different arrays, must not overlap. */
+ * at base + o * outer_stride + r * row_stride + i * inner_stride (bytes); no
+ * two blocks, of one row, of different ones or of different arrays, may overlap. */
 #define ZS_REORDER_BATCH 40
 typedef struct zs_beam_state {
     void* d_base;

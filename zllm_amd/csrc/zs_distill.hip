@@ -343,9 +343,11 @@ __global__ __launch_bounds__(DF_NT) void zs_k_distill_row(ds_args a, uint64_t r0
     ds_out o = {So, m};
     // (a workgroup a row: where all rows are such, the loss of 512 x 128256 f32
     // takes 114 us for 49, of one bf16 row of 151936 40 for 14, the gradient of
-    // 2048 x 50257 bf16 119 for 78; where none is, what it took without this)
-    const bool far = __builtin_expect(ds_far(a, l.pt, So, WHAT & DS_GRAD ? w * a.kl * (float)a.inv_t : a.kl), 0);
-    if (far) {
+    // 2048 x 50257 bf16 119 for 78. Where none is, 49, 14 and 78 as without it; of
+    // 65536 rows of 1000, which are mostly ends, 258 for 247 and the gradient 242
+    // for 230)
+    const bool far = ds_far(a, l.pt, So, WHAT & DS_GRAD ? w * a.kl * (float)a.inv_t : a.kl);
+    if (__builtin_expect(far, 0)) {
         constexpr int E = hd_elem<DT>::E, U = 4;
         __shared__ uint32_t mask[U * DF_NT / 4];   // a byte a vector: its ids in the list
         uint32_t at = 0;
@@ -369,7 +371,7 @@ __global__ __launch_bounds__(DF_NT) void zs_k_distill_row(ds_args a, uint64_t r0
         const bool listed = __syncthreads_or(l.there && (int64_t)l.id == label);
         if (t == 0) {
             ds_coef k = ds_factors(a, w, l, bad_label, m, S, S1, So);
-            if (far) ds_factors_out(a, w, l, bad_label, m, S, o, k);
+            if (__builtin_expect(far, 0)) ds_factors_out(a, w, l, bad_label, m, S, o, k);
             k.lone = label < 0 || bad_label || listed ? 0xffffffffu : (uint32_t)label;
             a.coef[r] = k;
         }
