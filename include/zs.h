@@ -61,6 +61,7 @@ int zs_abi_version(void);
 #define ZS_LAYOUT_BEAM_STATE 6
 #define ZS_LAYOUT_TEACHER 7
 #define ZS_LAYOUT_DISTILL 8
+#define ZS_LAYOUT_CE 9
 int zs_struct_layout(int which, size_t* size, size_t* offsets, size_t cap);
 
 /* Context on HIP device `device`, with scratch sized for batches of up to
@@ -543,6 +544,55 @@ int zs_distill_work(uint32_t N, uint32_t V, uint32_t K, uint64_t* bytes);
 int zs_distill_loss(zs_ctx* ctx, const zs_distill* args, void* stream);
 int zs_distill_grad(zs_ctx* ctx, const zs_distill* args, void* stream);
 int zs_distill_loss_grad(zs_ctx* ctx, const zs_distill* args, void* stream);
+
+/* ---- cross entropy of the vocabulary head ------------------------------------
+ * Row r has a hidden state h (D values) and a label; the head is a weight W of
+ * V rows. With z_v = h . W_v, never kept as a whole, and L = ln sum_v exp(z_v),
+ *     loss[r] = L - z[label] + z_weight * L^2,   lse[r] = L
+ *     d_v = row_grad[r] * ((1 + 2 z_weight L) exp(z_v - L) - [v is the label])
+ *     dhidden[r] = sum_v d_v W_v,   dweight_v = sum_r d_v h_r
+ * hidden, weight and the gradients are of one type, sums in f32, z in f32 (of
+ * f32 operands to 2^-26 of the sum of |h W_v|'s terms per product); d is
+ * rounded to the type on its way into the gradients' products (f16: scaled so
+ * that its largest factor is near 2^15; f32: kept whole), the gradients once.
+ * A row whose label is ignore_index has loss, lse and gradient 0, and its
+ * hidden state, whatever it holds, is in no sum; a label outside [0, V)
+ * otherwise gives NaN. What is not finite comes out as not finite.
+ * Results do not depend on the order in which the GPU works.
+ *   zs_ce_loss       writes d_loss and d_lse
+ *   zs_ce_loss_grad  also d_dhidden and d_dweight (either may be NULL: not
+ *                    wanted), which overlap none of the other arrays
+ * row_grad_stride 0 reads one value for all rows. `want` of zs_ce_work says
+ * which gradients a call will have and whether rows of the weight do not all
+ * begin at 16 bytes or are longer than ZS_CE_LD values (they are then copied;
+ * as are f32 weights always). */
+#define ZS_CE_MAX_HIDDEN 65536u
+#define ZS_CE_LD 4194304u
+#define ZS_CE_DHIDDEN 1u
+#define ZS_CE_DWEIGHT 2u
+#define ZS_CE_COPY 4u
+typedef struct zs_ce {
+    uint32_t N, V, D, dtype;
+    uint64_t ld_hidden, ld_weight;
+    const void* d_hidden;             /* [N][ld_hidden] */
+    const void* d_weight;             /* [V][ld_weight] */
+    const int64_t* d_labels;          /* [N] */
+    int64_t ignore_index;
+    float z_weight;                   /* finite */
+    uint32_t pad;
+    float* d_loss;                    /* [N] */
+    float* d_lse;                     /* [N] */
+    const float* d_row_grad;          /* [N] at row_grad_stride */
+    uint64_t row_grad_stride;
+    void* d_dhidden;                  /* [N][ld_dhidden] or NULL */
+    void* d_dweight;                  /* [V][ld_dweight] or NULL */
+    uint64_t ld_dhidden, ld_dweight;
+    void* d_work;
+    uint64_t work_bytes;
+} zs_ce;
+int zs_ce_work(uint32_t N, uint32_t V, uint32_t D, uint32_t dtype, uint32_t want, uint64_t* bytes);
+int zs_ce_loss(zs_ctx* ctx, const zs_ce* args, void* stream);
+int zs_ce_loss_grad(zs_ctx* ctx, const zs_ce* args, void* stream);
 
 /* ---- profiling ----------------------------------------------------------
  * When enabled, zs_sample and zs_spec_verify record a HIP event around their

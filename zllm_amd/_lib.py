@@ -137,6 +137,17 @@ class Distill(C.Structure):
     ]
 
 
+class Ce(C.Structure):
+    _fields_ = [
+        ("N", C.c_uint32), ("V", C.c_uint32), ("D", C.c_uint32), ("dtype", C.c_uint32), ("ld_hidden", C.c_uint64),
+        ("ld_weight", C.c_uint64), ("d_hidden", C.c_void_p), ("d_weight", C.c_void_p), ("d_labels", C.c_void_p),
+        ("ignore_index", C.c_int64), ("z_weight", C.c_float), ("pad", C.c_uint32), ("d_loss", C.c_void_p),
+        ("d_lse", C.c_void_p), ("d_row_grad", C.c_void_p), ("row_grad_stride", C.c_uint64), ("d_dhidden", C.c_void_p),
+        ("d_dweight", C.c_void_p), ("ld_dhidden", C.c_uint64), ("ld_dweight", C.c_uint64), ("d_work", C.c_void_p),
+        ("work_bytes", C.c_uint64),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/zs.h declares
 SIGNATURES = {
     "zs_abi_version": (C.c_int, []),
@@ -209,6 +220,9 @@ SIGNATURES = {
     "zs_distill_loss": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "zs_distill_grad": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "zs_distill_loss_grad": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "zs_ce_work": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_uint64)]),
+    "zs_ce_loss": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "zs_ce_loss_grad": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "zs_tool_call_envelope_regex": (C.c_int, [C.POINTER(C.c_char_p), C.POINTER(C.c_char_p), C.c_uint32, C.c_char_p,
                                               C.c_size_t, C.POINTER(C.c_size_t), C.c_char_p, C.c_size_t]),
 }
@@ -218,7 +232,7 @@ ABI_VERSION = 2
 
 # zs_struct_layout ids (ZS_LAYOUT_*) of the Structures above
 LAYOUTS = {0: Batch, 1: RowParams, 2: SpecBatch, 3: LaneStream, 4: HallucReport, 5: Beam, 6: BeamStateDesc,
-           7: Teacher, 8: Distill}
+           7: Teacher, 8: Distill, 9: Ce}
 
 
 def layout_mismatches(lib_):

@@ -14,6 +14,7 @@
 #include "zs_head_args.h"
 #include "zs_beam.h"
 #include "zs_distill.h"
+#include "zs_ce.h"
 
 // launchers (zs_sample.hip, zs_dfa.hip)
 extern "C" int zs_sample_launch(zs_ctx* ctx, const zs_batch* bt, hipStream_t stream);
@@ -123,6 +124,13 @@ extern "C" int zs_struct_layout(int which, size_t* size, size_t* offsets, size_t
         ZS_OFF(zs_distill, d_loss), ZS_OFF(zs_distill, d_stats), ZS_OFF(zs_distill, d_row_grad),
         ZS_OFF(zs_distill, row_grad_stride), ZS_OFF(zs_distill, d_grad), ZS_OFF(zs_distill, ld_grad),
         ZS_OFF(zs_distill, d_work), ZS_OFF(zs_distill, work_bytes)};
+    static const size_t ce[] = {
+        ZS_OFF(zs_ce, N), ZS_OFF(zs_ce, V), ZS_OFF(zs_ce, D), ZS_OFF(zs_ce, dtype), ZS_OFF(zs_ce, ld_hidden),
+        ZS_OFF(zs_ce, ld_weight), ZS_OFF(zs_ce, d_hidden), ZS_OFF(zs_ce, d_weight), ZS_OFF(zs_ce, d_labels),
+        ZS_OFF(zs_ce, ignore_index), ZS_OFF(zs_ce, z_weight), ZS_OFF(zs_ce, pad), ZS_OFF(zs_ce, d_loss),
+        ZS_OFF(zs_ce, d_lse), ZS_OFF(zs_ce, d_row_grad), ZS_OFF(zs_ce, row_grad_stride), ZS_OFF(zs_ce, d_dhidden),
+        ZS_OFF(zs_ce, d_dweight), ZS_OFF(zs_ce, ld_dhidden), ZS_OFF(zs_ce, ld_dweight), ZS_OFF(zs_ce, d_work),
+        ZS_OFF(zs_ce, work_bytes)};
     const size_t* f;
     size_t n, sz;
     switch (which) {
@@ -135,6 +143,7 @@ extern "C" int zs_struct_layout(int which, size_t* size, size_t* offsets, size_t
         case ZS_LAYOUT_BEAM_STATE: f = bstate; n = sizeof(bstate) / sizeof(size_t); sz = sizeof(zs_beam_state); break;
         case ZS_LAYOUT_TEACHER: f = teach; n = sizeof(teach) / sizeof(size_t); sz = sizeof(zs_teacher); break;
         case ZS_LAYOUT_DISTILL: f = dist; n = sizeof(dist) / sizeof(size_t); sz = sizeof(zs_distill); break;
+        case ZS_LAYOUT_CE: f = ce; n = sizeof(ce) / sizeof(size_t); sz = sizeof(zs_ce); break;
         default: return ZS_EINVAL;
     }
     if (size) *size = sz;
@@ -1290,4 +1299,65 @@ extern "C" int zs_distill_grad(zs_ctx* ctx, const zs_distill* args, void* stream
 }
 extern "C" int zs_distill_loss_grad(zs_ctx* ctx, const zs_distill* args, void* stream) {
     return distill_call(ctx, args, DS_LOSS | DS_GRAD, "zs_distill_loss_grad", stream);
+}
+
+// ---- cross entropy of the vocabulary head
+extern "C" int zs_ce_work(uint32_t N, uint32_t V, uint32_t D, uint32_t dtype, uint32_t want, uint64_t* bytes) {
+    if (!bytes || dtype > ZS_BF16 || V == 0 || V > ZS_HEAD_MAX_VOCAB || D == 0 || D > ZS_CE_MAX_HIDDEN || want > 7u) return ZS_EINVAL;
+    *bytes = 0;
+    if (N == 0) return ZS_OK;
+    ce_args a{};
+    a.N = N; a.V = V; a.D = D; a.want = want;
+    *bytes = ce_work(a, dtype, (void*)256);
+    return ZS_OK;
+}
+static int ce_matrix(zs_ctx* ctx, const void* p, uint64_t ld, uint32_t D, uint32_t dtype, const char* name, const char* who) {
+    if (!p || ((uintptr_t)p & (dtype == ZS_F32 ? 3u : 1u)))
+        return zs_set_error(ctx, ZS_EINVAL, "%s: %s null or not aligned to its type", who, name);
+    if (ld < D) return zs_set_error(ctx, ZS_EINVAL, "%s: ld of %s < D", who, name);
+    return ZS_OK;
+}
+static int ce_call(zs_ctx* ctx, const zs_ce* b, bool grad, const char* who, void* stream) {
+    if (!ctx || !b) return zs_set_error(ctx, ZS_EINVAL, "%s: null argument", who);
+    if (b->dtype > ZS_BF16) return zs_set_error(ctx, ZS_EINVAL, "%s: unknown dtype %u", who, b->dtype);
+    if (b->V == 0 || b->V > ZS_HEAD_MAX_VOCAB)
+        return zs_set_error(ctx, ZS_ELIMIT, "%s: V=%u outside 1..%u", who, b->V, ZS_HEAD_MAX_VOCAB);
+    if (b->D == 0 || b->D > ZS_CE_MAX_HIDDEN)
+        return zs_set_error(ctx, ZS_ELIMIT, "%s: D=%u outside 1..%u", who, b->D, ZS_CE_MAX_HIDDEN);
+    if (!(b->z_weight - b->z_weight == 0.0f)) return zs_set_error(ctx, ZS_EINVAL, "%s: z_weight must be finite", who);
+    const uint32_t size = b->dtype == ZS_F32 ? 4u : 2u;
+    int rc;
+    if (grad && !b->d_dhidden && !b->d_dweight) return zs_set_error(ctx, ZS_EINVAL, "%s: no gradient wanted", who);
+    if (grad && b->d_dweight && (rc = ce_matrix(ctx, b->d_dweight, b->ld_dweight, b->D, b->dtype, "d_dweight", who))) return rc;
+    if (b->N == 0 && (!grad || !b->d_dweight)) return ZS_OK;
+    if ((rc = ce_matrix(ctx, b->d_weight, b->ld_weight, b->D, b->dtype, "d_weight", who))) return rc;
+    if (b->N && (rc = ce_matrix(ctx, b->d_hidden, b->ld_hidden, b->D, b->dtype, "d_hidden", who))) return rc;
+    if (b->N && grad && b->d_dhidden && (rc = ce_matrix(ctx, b->d_dhidden, b->ld_dhidden, b->D, b->dtype, "d_dhidden", who)))
+        return rc;
+    if (b->N && (!b->d_labels || !b->d_loss || !b->d_lse || (grad && !b->d_row_grad)))
+        return zs_set_error(ctx, ZS_EINVAL, "%s: null required pointer", who);
+    ce_args a{};
+    a.hidden = b->d_hidden; a.weight = b->d_weight; a.ld_h = b->ld_hidden; a.ld_w = b->ld_weight;
+    a.labels = b->d_labels; a.ignore = b->ignore_index; a.N = b->N; a.V = b->V; a.D = b->D;
+    a.zw = b->z_weight; a.loss = b->d_loss; a.lse = b->d_lse;
+    a.row_grad = b->d_row_grad; a.row_grad_stride = b->row_grad_stride;
+    if (grad) {
+        a.dh = b->N ? b->d_dhidden : nullptr; a.dw = b->d_dweight; a.ld_dh = b->ld_dhidden; a.ld_dw = b->ld_dweight;
+        a.want = (a.dh ? CE_DH : 0u) | (a.dw ? CE_DW : 0u);
+    }
+    if (((uintptr_t)b->d_weight & 15u) || b->D % 8u || (b->V > 1u && b->ld_weight % 8u) || b->ld_weight > ZS_CE_LD || size == 4u)
+        a.want |= CE_COPY;
+    const int prev = zs_device_guard_begin(ctx);
+    if (b->N == 0) {
+        rc = ce_clear(b->d_dweight, b->V, b->D, b->ld_dweight, b->dtype, (hipStream_t)stream);
+    } else {
+        if (!(rc = work_check(ctx, b->d_work, b->work_bytes, ce_work(a, b->dtype, b->d_work), who)))
+            rc = ce_launch(a, b->dtype, (hipStream_t)stream) ? zs_set_error(ctx, ZS_EHIP, "%s: launch failed", who) : ZS_OK;
+    }
+    zs_device_guard_end(ctx, prev);
+    return rc;
+}
+extern "C" int zs_ce_loss(zs_ctx* ctx, const zs_ce* args, void* stream) { return ce_call(ctx, args, false, "zs_ce_loss", stream); }
+extern "C" int zs_ce_loss_grad(zs_ctx* ctx, const zs_ce* args, void* stream) {
+    return ce_call(ctx, args, true, "zs_ce_loss_grad", stream);
 }

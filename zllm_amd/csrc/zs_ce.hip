@@ -1,0 +1,464 @@
+// zs_ce.hip -- cross entropy of the vocabulary head from hidden states, and its
+// gradient, without the logits.
+#include <hip/hip_runtime.h>
+#include "zs_ce.h"
+#include "zs_head.h"
+
+#define CE_NT 256
+
+__device__ __forceinline__ uint16_t ce_bf16(float x) {
+    const __bf16 b = (__bf16)x;
+    return __builtin_bit_cast(uint16_t, b);
+}
+__device__ __forceinline__ float ce_of_bf16(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+// x as a sum of three bf16, each the nearest to what is left (24 bits in all);
+// where the first would be infinite for a finite x, the one below it.
+__device__ __forceinline__ void ce_split(float x, uint16_t (&p)[3]) {
+    p[0] = ce_bf16(x);
+    if ((p[0] & 0x7fffu) == 0x7f80u) p[0] = (uint16_t)(__float_as_uint(x) >> 16);
+    float r = x - ce_of_bf16(p[0]);
+    if ((p[0] & 0x7f80u) == 0x7f80u) r = 0.0f;
+    p[1] = ce_bf16(r);
+    p[2] = ce_bf16(r - ce_of_bf16(p[1]));
+}
+__device__ __forceinline__ float ce_exp(float x) {   // e^x
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_amdgcn_exp2f(x * 1.44269504f);
+#else
+    return x;
+#endif
+}
+// The power of two that brings the piece's gradients of logits to at most 2^15:
+// f16 has few exponents (row weights of 1 / N alone would leave most of a row
+// below its normal numbers). The other types need none.
+template <int DT>
+__device__ __forceinline__ int ce_shift(const ce_args& a) {
+    if constexpr (DT != ZS_F16) return 0;
+    const uint32_t m = a.st->amax;
+    if (m == 0u) return 0;
+    const int s = 15 - ((int)(m >> 23) - 126);
+    return s > 100 ? 100 : s;
+}
+__device__ __forceinline__ uint32_t ce_rows(const ce_args& a) {   // of the piece that have a label
+    const uint32_t n = a.st->rows;
+    return n <= a.lo ? 0u : n - a.lo < a.R ? n - a.lo : a.R;
+}
+template <int DT>
+__device__ __forceinline__ float ce_load(const void* p, uint64_t i) {
+    return hd_float(reinterpret_cast<const typename hd_elem<DT>::T*>(p)[i]);
+}
+// four values to out + at, those before `end`
+template <int DT>
+__device__ __forceinline__ void ce_store4(void* out, uint64_t at, const float (&v)[4], uint32_t n, bool vec) {
+    if constexpr (DT == ZS_F32) {
+        float* o = (float*)out + at;
+        if (vec) *(float4*)o = make_float4(v[0], v[1], v[2], v[3]);
+        else
+            for (uint32_t i = 0; i < 4u; i++)
+                if (i < n) o[i] = v[i];
+    } else {
+        uint16_t* o = (uint16_t*)out + at;
+        const uint2 u = make_uint2(hd_pack2<DT>(v[0], v[1]), hd_pack2<DT>(v[2], v[3]));
+        if (vec) *(uint2*)o = u;
+        else {
+            const uint16_t s[4] = {(uint16_t)u.x, (uint16_t)(u.x >> 16), (uint16_t)u.y, (uint16_t)(u.y >> 16)};
+            for (uint32_t i = 0; i < 4u; i++)
+                if (i < n) o[i] = s[i];
+        }
+    }
+}
+template <int DT>
+__device__ __forceinline__ void ce_zero(void* row, uint32_t n) {
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
+        if constexpr (DT == ZS_F32) ((float*)row)[i] = 0.0f;
+        else ((uint16_t*)row)[i] = 0;
+    }
+}
+
+// The rows with a label in order, behind them the others from the end on.
+__global__ __launch_bounds__(1024) void zs_k_ce_rows(ce_args a) {
+    __shared__ uint32_t sh[16];
+    const uint32_t t = threadIdx.x, w = t >> 6, l = t & 63u;
+    uint32_t done = 0;
+    for (uint64_t r0 = 0; r0 < a.N; r0 += 1024u) {
+        const uint64_t r = r0 + t;
+        const bool in = r < a.N, has = in && a.labels[r] != a.ignore;
+        const uint64_t m = __ballot(has);
+        if (l == 0u) sh[w] = (uint32_t)__popcll(m);
+        __syncthreads();
+        uint32_t before = done + (uint32_t)__popcll(m & ((1ull << l) - 1u)), all = 0;
+        for (uint32_t i = 0; i < 16u; i++) {
+            before += i < w ? sh[i] : 0u;
+            all += sh[i];
+        }
+        if (has) a.idx[before] = (uint32_t)r;
+        else if (in) a.idx[a.N - 1u - (uint32_t)(r - before)] = (uint32_t)r;
+        done += all;
+        __syncthreads();
+    }
+    if (t == 0u) a.st->rows = done;
+}
+
+// Row lo + i: its hidden state to the operand (zeros behind the last row), the
+// logit of its label; rows without one get their zeros.
+template <int DT>
+__global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
+    __shared__ double sh[CE_NT / 64];
+    const uint32_t i = blockIdx.x, n = ce_rows(a), t = threadIdx.x;
+    const uint64_t plane = (uint64_t)a.R * a.Dp;
+    uint16_t* o = a.h + (uint64_t)i * a.Dp;
+    if (i == 0u && t == 0u) a.st->amax = 0u;
+    if (i >= n) {
+        if (i < (n + CE_TILE - 1u) / CE_TILE * CE_TILE)
+            for (int p = 0; p < (DT == ZS_F32 ? 3 : 1); p++) ce_zero<ZS_F16>(o + p * plane, a.Dp);
+        if (a.lo + (uint64_t)i < a.N) {
+            const uint64_t r = a.idx[a.lo + i];
+            if (t == 0u) a.loss[r] = a.lse[r] = 0.0f;
+            if (a.dh) ce_zero<DT>((char*)a.dh + r * a.ld_dh * (DT == ZS_F32 ? 4u : 2u), a.D);
+        }
+        return;
+    }
+    const uint64_t r = a.idx[a.lo + i];
+    const int64_t label = a.labels[r];
+    const bool bad = label < 0 || label >= (int64_t)a.V;
+    const uint64_t hr = r * a.ld_h, wr = (bad ? 0u : (uint64_t)label) * a.ld_w;
+    double dot = 0.0;
+    for (uint32_t d = t; d < a.Dp; d += CE_NT) {
+        const float x = d < a.D ? ce_load<DT>(a.hidden, hr + d) : 0.0f;
+        if constexpr (DT == ZS_F32) {
+            uint16_t p[3];
+            ce_split(x, p);
+            for (int k = 0; k < 3; k++) o[k * plane + d] = p[k];
+        } else {
+            o[d] = d < a.D ? ((const uint16_t*)a.hidden)[hr + d] : (uint16_t)0;
+        }
+        if (d < a.D) dot += (double)x * (double)ce_load<DT>(a.weight, wr + d);
+    }
+    dot = block_sum_d<CE_NT>(dot, sh);
+    if (t == 0u) {
+        a.at[i] = bad ? NAN : (float)dot;
+        a.row[i].label = bad ? ~0u : (uint32_t)label;
+    }
+}
+
+// The weight in rows of Dp, its planes apart, where its own rows do not serve.
+template <int DT>
+__global__ __launch_bounds__(CE_NT) void zs_k_ce_weight(ce_args a) {
+    const uint64_t plane = (uint64_t)a.V * a.Dp;
+    for (uint64_t v = blockIdx.x; v < a.V; v += gridDim.x)
+        for (uint32_t d = threadIdx.x; d < a.Dp; d += CE_NT) {
+            uint16_t* o = a.w + v * a.Dp + d;
+            if constexpr (DT == ZS_F32) {
+                uint16_t p[3];
+                ce_split(d < a.D ? ce_load<DT>(a.weight, v * a.ld_w + d) : 0.0f, p);
+                for (int k = 0; k < 3; k++) o[k * plane] = p[k];
+            } else {
+                *o = d < a.D ? ((const uint16_t*)a.weight)[v * a.ld_w + d] : (uint16_t)0;
+            }
+        }
+}
+
+template <int DT>
+__device__ __forceinline__ tp_mat ce_mat_w(const ce_args& a, bool slow) {
+    const bool own = a.w != nullptr;
+    const uint16_t* p = own ? a.w : (const uint16_t*)a.weight;
+    const uint64_t plane = (uint64_t)a.V * a.Dp;
+    const uint32_t d = own ? a.Dp : a.D;
+    tp_mat m = {{p, p + plane, p + 2 * plane}, own ? a.Dp : a.ld_w, slow ? d : a.V, slow ? a.V : d};
+    return m;
+}
+__device__ __forceinline__ tp_mat ce_mat_h(const ce_args& a, bool slow) {
+    const uint64_t plane = (uint64_t)a.R * a.Dp;
+    tp_mat m = {{a.h, a.h + plane, a.h + 2 * plane}, a.Dp, slow ? a.Dp : a.R, slow ? a.R : a.Dp};
+    return m;
+}
+__device__ __forceinline__ tp_mat ce_mat_dl(const ce_args& a, bool slow) {
+    const uint64_t plane = (uint64_t)a.R * a.Vp;
+    tp_mat m = {{a.dl, a.dl + plane, a.dl + 2 * plane}, a.Vp, slow ? a.Vp : a.R, slow ? a.R : a.Vp};
+    return m;
+}
+
+// Logits of 256 ids (m) and 256 rows (n), of which only what a softmax over the
+// vocabulary needs leaves the registers: per row and 128 ids their maximum and
+// the sum of exponentials relative to it, and for the gradient the exponentials.
+template <int DT, bool GRAD>
+__global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_logits(ce_args a) {
+    typedef tp_tile<DT, 4, 4, 2, false, false> T;
+    const uint32_t n = ce_rows(a);
+    const uint2 at = tp_place(blockIdx.x, a.Vp / CE_TILE, (n + CE_TILE - 1u) / CE_TILE);
+    if (at.x == ~0u) return;
+    const tp_mat mw = ce_mat_w<DT>(a, false), mh = ce_mat_h(a, false);
+    T tile(mw, mh, at.x, at.y);
+    tp_acc c[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int q = 0; q < 16; q++) c[i][j][q] = 0.0f;
+    tile.run(0, a.Dp / TP_KSTEP, c);
+    const uint32_t sub = at.x * 2u + T::wm();
+    if (tile.m0 + CE_TILE > a.V) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int q = 0; q < 16; q++)
+                if (tile.m_of(i, q / 4) + (uint32_t)(q & 3) >= a.V)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) c[i][j][q] = -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t r = tile.n_of(j);
+        float m = -INFINITY, s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int q = 0; q < 16; q++) m = fmaxf(m, c[i][j][q]);
+        m = fmaxf(m, zs_lane_xor<32>(m));
+        const float m0 = m > -INFINITY ? m : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                float e[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    e[k] = ce_exp(c[i][j][4 * q + k] - m0);
+                    s += e[k];
+                }
+                if constexpr (GRAD) {
+                    const uint64_t o = (uint64_t)r * a.Vp + tile.m_of(i, q);
+                    if constexpr (DT == ZS_F32) {
+                        ce_store4<ZS_F32>(a.e, o, e, 4, true);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) e[k] *= CE_E_SCALE;
+                        ce_store4<ZS_F16>(a.e, o, e, 4, true);
+                    }
+                }
+            }
+        s += zs_lane_xor<32>(s);
+        if (zs_lane() < 32) a.stat[(uint64_t)r * a.subs + sub] = make_float2(m, s);
+    }
+}
+
+// A row's normaliser and loss from its parts, and what its gradient goes by.
+template <int DT, bool GRAD>
+__global__ __launch_bounds__(CE_NT) void zs_k_ce_loss(ce_args a) {
+    __shared__ float shf[CE_NT / 64];
+    __shared__ double shd[CE_NT / 64];
+    const uint32_t i = blockIdx.x, t = threadIdx.x;
+    if (i >= ce_rows(a)) return;
+    const float2* st = a.stat + (uint64_t)i * a.subs;
+    float m = -INFINITY;
+    for (uint32_t k = t; k < a.subs; k += CE_NT) m = fmaxf(m, st[k].x);
+    m = block_max_f<CE_NT>(m, shf);
+    const float m0 = m > -INFINITY ? m : 0.0f;
+    double s = 0.0;
+    for (uint32_t k = t; k < a.subs; k += CE_NT) {
+        const float2 v = st[k];
+        s += (double)(v.y * ce_exp(v.x - m0));
+    }
+    s = block_sum_d<CE_NT>(s, shd);
+    const double lse = (double)m0 + log(s), at = (double)a.at[i];
+    const uint32_t r = a.idx[a.lo + i];
+    if (t == 0u) {
+        a.lse[r] = (float)lse;
+        a.loss[r] = (float)((lse - at) + (double)a.zw * lse * lse);
+    }
+    if constexpr (GRAD) {
+        const float g = a.row_grad[r * a.row_grad_stride], k1 = (float)(1.0 + 2.0 * (double)a.zw * lse);
+        const float bad = a.row[i].label == ~0u ? NAN : g;
+        const float f = bad * k1 * (float)exp((double)m0 - lse);
+        for (uint32_t k = t; k < a.subs; k += CE_NT) a.fac[(uint64_t)i * a.subs + k] = f * ce_exp(st[k].x - m0);
+        if (t == 0u) {
+            a.row[i].fix = (float)((double)bad * ((double)k1 * exp(at - lse) - 1.0));
+            const float top = fabsf(g) * fmaxf(1.0f, fabsf(k1));
+            if (DT == ZS_F16 && top < INFINITY) atomicMax(&a.st->amax, __float_as_uint(top));
+        }
+    }
+}
+
+// Exponentials to the gradient of the logits, in their place (f32: to three
+// planes); zeros in the rows up to where the products over the rows end.
+template <int DT>
+__global__ __launch_bounds__(CE_NT) void zs_k_ce_grad(ce_args a) {
+    const uint32_t i = blockIdx.y, n = ce_rows(a), v0 = (blockIdx.x * CE_NT + threadIdx.x) * 8u;
+    if (i >= (n + TP_KROUND - 1u) / TP_KROUND * TP_KROUND || v0 >= a.Vp) return;
+    const uint64_t at = (uint64_t)i * a.Vp + v0;
+    float x[8];
+    if (i < n) {
+        const int sh = ce_shift<DT>(a);
+        const float f = ldexpf(a.fac[(uint64_t)i * a.subs + v0 / CE_SUB], sh) * (DT == ZS_F32 ? 1.0f : 1.0f / CE_E_SCALE);
+        const ce_row row = a.row[i];
+        if constexpr (DT == ZS_F32) {
+            const float4 u = *(const float4*)((const float*)a.e + at), w = *(const float4*)((const float*)a.e + at + 4);
+            const float y[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+            for (int k = 0; k < 8; k++) x[k] = y[k] * f;
+        } else {
+            const hd_u4 u = *(const hd_u4*)((const uint16_t*)a.e + at);
+            hd_unpack<ZS_F16>(u, x);
+            for (int k = 0; k < 8; k++) x[k] *= f;
+        }
+        if (row.label - v0 < 8u) {
+            const float y = ldexpf(row.fix, sh);
+            for (uint32_t k = 0; k < 8u; k++)
+                if (row.label == v0 + k) x[k] = y;
+        }
+    } else {
+        for (int k = 0; k < 8; k++) x[k] = 0.0f;
+    }
+    if constexpr (DT == ZS_F32) {
+        const uint64_t plane = (uint64_t)a.R * a.Vp;
+        uint16_t p[8][3];
+        for (int k = 0; k < 8; k++) ce_split(x[k], p[k]);
+        for (int q = 0; q < 3; q++) {
+            hd_u4 o;
+            for (int k = 0; k < 4; k++) o[k] = (uint32_t)p[2 * k][q] | (uint32_t)p[2 * k + 1][q] << 16;
+            *(hd_u4*)(a.dl + q * plane + at) = o;
+        }
+    } else {
+        hd_u4 o;
+        for (int k = 0; k < 4; k++) o[k] = hd_pack2<DT>(x[2 * k], x[2 * k + 1]);
+        *(hd_u4*)(a.dl + at) = o;
+    }
+}
+
+// Gradient of the hidden states, 256 columns (m) of 256 rows (n), over the
+// vocabulary or a part of it.
+template <int DT>
+__global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_dhidden(ce_args a) {
+    typedef tp_tile<DT, 4, 4, 2, true, false> T;
+    const uint32_t n = ce_rows(a), steps = a.Vp / TP_KSTEP, k0 = blockIdx.y * a.split_steps;
+    const uint2 at = tp_place(blockIdx.x, (a.D + CE_TILE - 1u) / CE_TILE, (n + CE_TILE - 1u) / CE_TILE);
+    if (at.x == ~0u) return;
+    const tp_mat mw = ce_mat_w<DT>(a, true), md = ce_mat_dl(a, false);
+    T tile(mw, md, at.x, at.y);
+    tp_acc c[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int q = 0; q < 16; q++) c[i][j][q] = 0.0f;
+    tile.run(k0, steps - k0 < a.split_steps ? steps - k0 : a.split_steps, c);
+    const float un = ldexpf(1.0f, -ce_shift<DT>(a));
+    const bool vec = a.D % 4u == 0u && a.ld_dh % 4u == 0u && ((uintptr_t)a.dh & 15u) == 0u;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t r = tile.n_of(j);
+        if (r >= n) continue;
+        const uint64_t row = a.splits > 1u ? 0u : a.idx[a.lo + r];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const uint32_t d = tile.m_of(i, q);
+                if (d >= a.D) continue;
+                const float v[4] = {c[i][j][4 * q] * un, c[i][j][4 * q + 1] * un, c[i][j][4 * q + 2] * un, c[i][j][4 * q + 3] * un};
+                if (a.splits > 1u) ce_store4<ZS_F32>(a.part, ((uint64_t)blockIdx.y * a.R + r) * a.Dm + d, v, 4, true);
+                else ce_store4<DT>(a.dh, row * a.ld_dh + d, v, a.D - d, vec);
+            }
+    }
+}
+template <int DT>
+__global__ __launch_bounds__(CE_NT) void zs_k_ce_join(ce_args a) {
+    const uint32_t i = blockIdx.x;
+    if (i >= ce_rows(a)) return;
+    const uint64_t r = a.idx[a.lo + i], step = (uint64_t)a.R * a.Dm;
+    const bool vec = a.D % 4u == 0u && a.ld_dh % 4u == 0u && ((uintptr_t)a.dh & 15u) == 0u;
+    for (uint32_t d = threadIdx.x * 4u; d < a.D; d += CE_NT * 4u) {
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t s = 0; s < a.splits; s++) {
+            const float4 p = *(const float4*)(a.part + s * step + (uint64_t)i * a.Dm + d);
+            v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+        }
+        ce_store4<DT>(a.dh, r * a.ld_dh + d, v, a.D - d, vec);
+    }
+}
+
+// Gradient of the weight, 256 columns (m) of 256 ids (n), over the piece's rows.
+template <int DT>
+__global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_dweight(ce_args a) {
+    typedef tp_tile<DT, 4, 4, 2, true, true> T;
+    const uint32_t n = ce_rows(a);
+    const uint2 at = tp_place(blockIdx.x, (a.D + CE_TILE - 1u) / CE_TILE, a.Vp / CE_TILE);
+    if (at.x == ~0u) return;
+    const tp_mat mh = ce_mat_h(a, true), md = ce_mat_dl(a, true);
+    T tile(mh, md, at.x, at.y);
+    tp_acc c[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int q = 0; q < 16; q++) c[i][j][q] = 0.0f;
+    tile.run(0, (n + TP_KROUND - 1u) / TP_KROUND * (TP_KROUND / TP_KSTEP), c);
+    const float un = ldexpf(1.0f, -ce_shift<DT>(a));
+    const bool vec = a.D % 4u == 0u && a.ld_dw % 4u == 0u && ((uintptr_t)a.dw & 15u) == 0u;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t id = tile.n_of(j);
+        if (id >= a.V) continue;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const uint32_t d = tile.m_of(i, q);
+                if (d >= a.D) continue;
+                float v[4] = {c[i][j][4 * q] * un, c[i][j][4 * q + 1] * un, c[i][j][4 * q + 2] * un, c[i][j][4 * q + 3] * un};
+                float* acc = a.acc + (uint64_t)id * a.Dm + d;
+                if (!a.first) {
+                    const float4 p = *(const float4*)acc;
+                    v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+                }
+                if (!a.last) ce_store4<ZS_F32>(acc, 0, v, 4, true);
+                else ce_store4<DT>(a.dw, (uint64_t)id * a.ld_dw + d, v, a.D - d, vec);
+            }
+    }
+}
+
+template <int DT>
+static void ce_go(ce_args a, hipStream_t stream) {
+    const dim3 wg(CE_NT);
+    const uint32_t vt = a.Vp / CE_TILE, dt = (a.D + CE_TILE - 1u) / CE_TILE, rt = a.R / CE_TILE;
+    hipLaunchKernelGGL(zs_k_ce_rows, dim3(1), dim3(1024), 0, stream, a);
+    if (a.w) hipLaunchKernelGGL(zs_k_ce_weight<DT>, dim3(a.V < 16384u ? a.V : 16384u), wg, 0, stream, a);
+    for (uint32_t p = 0; p < a.pieces; p++) {
+        a.lo = p * a.R;
+        a.first = p == 0u;
+        a.last = p + 1u == a.pieces;
+        hipLaunchKernelGGL(zs_k_ce_pack<DT>, dim3(a.R), wg, 0, stream, a);
+        if (!(a.want & (CE_DH | CE_DW))) {
+            hipLaunchKernelGGL((zs_k_ce_logits<DT, false>), dim3(tp_places(vt, rt)), wg, 0, stream, a);
+            hipLaunchKernelGGL((zs_k_ce_loss<DT, false>), dim3(a.R), wg, 0, stream, a);
+            continue;
+        }
+        hipLaunchKernelGGL((zs_k_ce_logits<DT, true>), dim3(tp_places(vt, rt)), wg, 0, stream, a);
+        hipLaunchKernelGGL((zs_k_ce_loss<DT, true>), dim3(a.R), wg, 0, stream, a);
+        hipLaunchKernelGGL(zs_k_ce_grad<DT>, dim3((a.Vp / 8u + CE_NT - 1u) / CE_NT, a.R), wg, 0, stream, a);
+        if (a.want & CE_DH) {
+            hipLaunchKernelGGL(zs_k_ce_dhidden<DT>, dim3(tp_places(dt, rt), a.splits), wg, 0, stream, a);
+            if (a.splits > 1u) hipLaunchKernelGGL(zs_k_ce_join<DT>, dim3(a.R), wg, 0, stream, a);
+        }
+        if (a.want & CE_DW) hipLaunchKernelGGL(zs_k_ce_dweight<DT>, dim3(tp_places(dt, vt)), wg, 0, stream, a);
+    }
+}
+int ce_launch(const ce_args& a, uint32_t dtype, hipStream_t stream) {
+    if (dtype == ZS_F32) ce_go<ZS_F32>(a, stream);
+    else if (dtype == ZS_F16) ce_go<ZS_F16>(a, stream);
+    else ce_go<ZS_BF16>(a, stream);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+template <int DT>
+__global__ __launch_bounds__(CE_NT) void zs_k_ce_clear(char* p, uint32_t rows, uint32_t cols, uint64_t ld) {
+    for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) ce_zero<DT>(p + r * ld * (DT == ZS_F32 ? 4u : 2u), cols);
+}
+int ce_clear(void* p, uint32_t rows, uint32_t cols, uint64_t ld, uint32_t dtype, hipStream_t stream) {
+    const dim3 grid(rows < 16384u ? rows : 16384u), wg(CE_NT);
+    if (dtype == ZS_F32) hipLaunchKernelGGL(zs_k_ce_clear<ZS_F32>, grid, wg, 0, stream, (char*)p, rows, cols, ld);
+    else hipLaunchKernelGGL(zs_k_ce_clear<ZS_F16>, grid, wg, 0, stream, (char*)p, rows, cols, ld);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}

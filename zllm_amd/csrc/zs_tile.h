@@ -1,0 +1,280 @@
+// zs_tile.h -- products of 16-bit matrices by the matrix cores, one tile of the
+// result per workgroup: D[m][n] = sum_k A[m][k] B[n][k] in f32.
+#pragma once
+#include <hip/hip_runtime.h>
+#include "zs_internal.h"
+#include "zs_dev.h"
+
+// An operand lies k-fast (rows of A or B, k along a row) or k-slow (rows of k,
+// m or n along a row). It may have planes: bf16 matrices whose sum it is.
+struct tp_mat {
+    const uint16_t* p[3];
+    uint64_t ld;          // elements from row to row, a multiple of 8, at most TP_LD
+    uint32_t rows;        // m or n there are: what a tile reads past them is the last's
+    uint32_t k;           // k there are: what is read past them is the last eight's (k-fast) or the last's (k-slow), for
+                          // the other operand's zeros there
+};
+#define TP_LD (1u << 22)
+#define TP_KSTEP 32       // k of a step
+#define TP_KROUND 128     // k are a multiple of
+
+typedef __attribute__((address_space(3))) char tp_lds;
+typedef __attribute__((address_space(1))) const char tp_glb;
+typedef float tp_acc __attribute__((ext_vector_type(16)));
+typedef short tp_s4 __attribute__((ext_vector_type(4)));
+typedef short tp_s8 __attribute__((ext_vector_type(8)));
+
+template <int DT>
+__device__ __forceinline__ tp_acc tp_mfma(tp_s8 a, tp_s8 b, tp_acc c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    if constexpr (DT == ZS_F16) {
+        typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    } else {
+        typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    }
+#else
+    return c;
+#endif
+}
+
+// One operand of a tile of X rows (m or n): what a lane loads to shared memory
+// and what it reads from there. A step's X x 32 values lie in shared memory as
+// the loads write them, 16 bytes a lane one behind the other; which 16 bytes a
+// lane fetches is permuted so that the reads spread over the banks.
+//   k-fast: row r's four 16-byte pieces at r * 64 B, piece c in place c ^ s(r)
+//   k-slow: row k's X / 8 pieces at k * 2 X B, piece c in place c ^ ((k & 3) << 2)
+template <int X, bool SLOW>
+struct tp_side {
+    static constexpr int LOADS = X * 4 / 256;    // of a lane a step
+    const char* base;
+    uint32_t off[SLOW ? 1 : LOADS];
+    uint32_t kb, kmax, ld2, left;
+    uint32_t rd[SLOW ? 4 : 2];
+
+    __device__ __forceinline__ void start(const tp_mat& m, uint32_t x0, uint32_t wx) {
+        const uint32_t l = (uint32_t)zs_lane(), w = (uint32_t)__builtin_amdgcn_readfirstlane(zs_wid());
+        ld2 = (uint32_t)m.ld * 2u;
+        if constexpr (!SLOW) {
+            const uint32_t r = l >> 2;
+            kb = ((l & 3u) ^ swz(r)) * 16u;
+            kmax = m.k * 2u - 16u;
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+                uint32_t row = x0 + (uint32_t)(i * 4) * 16u + w * 16u + r;
+                row = row < m.rows ? row : m.rows - 1u;
+                off[i] = (row - x0) * ld2;
+            }
+            const uint32_t rr = l & 31u;
+#pragma unroll
+            for (int s = 0; s < 2; s++) rd[s] = (wx + rr) * 64u + ((((uint32_t)s * 2u + (l >> 5)) ^ swz(rr)) * 16u);
+        } else {
+            constexpr uint32_t C = X / 8;        // pieces a row: 16 or 32
+            constexpr uint32_t P = 64u / C;      // rows of a wave's load
+            const uint32_t r = w * P + l / C;
+            uint32_t c = (l % C) ^ ((r & 3u) << 2);
+            const uint32_t last = (m.rows >> 3) - 1u - (x0 >> 3);
+            c = c < last ? c : last;
+            kb = r;
+            off[0] = c * 16u;
+            left = m.k;
+            const uint32_t q = (l & 15u) >> 2, k = (l >> 5) * 8u + q;
+            const uint32_t c0 = wx / 8u + ((l >> 4) & 1u) * 2u + ((l & 3u) >> 1);
+#pragma unroll
+            for (int t = 0; t < 4; t++) rd[t] = k * (2u * X) + ((c0 + (uint32_t)t * 4u) ^ (q << 2)) * 16u + (l & 1u) * 8u;
+        }
+    }
+    static __device__ __forceinline__ uint32_t swz(uint32_t r) { return ((r >> 1) & 3u) ^ ((r >> 3) & 1u); }
+    __device__ __forceinline__ void plane(const tp_mat& m, int p, uint32_t x0) {
+        base = (const char*)m.p[p] + (SLOW ? (uint64_t)x0 * 2u : (uint64_t)x0 * m.ld * 2u);
+    }
+    // step kt's values to shared memory at s
+    __device__ __forceinline__ void load(uint32_t kt, tp_lds* s) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+        const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane(zs_wid());
+        if constexpr (!SLOW) {
+            uint32_t k = kt * 64u + kb;
+            k = k < kmax ? k : kmax;
+#pragma unroll
+            for (int i = 0; i < LOADS; i++)
+                __builtin_amdgcn_global_load_lds((tp_glb*)(base + (off[i] + k)), s + (i * 4096 + w * 1024u), 16, 0, 0);
+        } else {
+            constexpr uint32_t R = 4u * (64u / (X / 8));   // rows of the workgroup's load
+            const uint32_t k0 = kt * 32u < left ? kt * 32u : left - 1u, end = left - 1u - k0;
+            const char* b = base + (uint64_t)k0 * ld2;
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+                uint32_t k = kb + (uint32_t)i * R;
+                k = k < end ? k : end;
+                __builtin_amdgcn_global_load_lds((tp_glb*)(b + (__umul24(k, ld2) + off[0])), s + (i * 4096 + w * 1024u), 16, 0, 0);
+            }
+        }
+#endif
+    }
+    // the values of 32 rows t and 16 k s for the matrix cores: lane l has row l % 32, k (l / 32) * 8 .. + 7
+    __device__ __forceinline__ tp_s8 frag(const tp_lds* s, int t, int ks) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+        if constexpr (!SLOW) {
+            return *(const __attribute__((address_space(3))) tp_s8*)(s + rd[ks] + t * 2048);
+        } else {
+            typedef __attribute__((address_space(3))) tp_s4 ls4;
+            const tp_lds* p = s + rd[t] + ks * (32 * X);
+            const tp_s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4*)p);
+            const tp_s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4*)(p + 8 * X));
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+#else
+        return tp_s8{};
+#endif
+    }
+};
+
+// Which planes' products make an f32 product, the smallest first: with x = x0 + x1
+// + x2, each the bf16 nearest to what those before it leave, x1 y2, x2 y1 and
+// x2 y2 are left out (at most 2^-26 of |x y| together).
+#define TP_PAIRS 6
+__device__ __forceinline__ int tp_plane_a(int s) { return (int)(0x001102u >> (4 * s)) & 15; }
+__device__ __forceinline__ int tp_plane_b(int s) { return (int)(0x010120u >> (4 * s)) & 15; }
+
+// A tile of BM x BN = (32 MT WM) x (32 NT WN) by four waves, WM along m.
+template <int DT, int MT, int NT, int WM, bool AS, bool BS>
+struct tp_tile {
+    static constexpr int WN = 4 / WM, BM = 32 * MT * WM, BN = 32 * NT * WN;
+    static constexpr int SA = BM * 64, STAGE = (BM + BN) * 64;
+    static constexpr int PAIRS = DT == ZS_F32 ? TP_PAIRS : 1;
+    typedef tp_side<BM, AS> A;
+    typedef tp_side<BN, BS> B;
+    static constexpr int LOADS = A::LOADS + B::LOADS;
+    const tp_mat &ma, &mb;
+    A a;
+    B b;
+    uint32_t m0, n0, kt, ka, kz;    // the step that is loaded next, of ka .. kz - 1
+    int pair;
+
+    __device__ __forceinline__ static uint32_t wm() { return (uint32_t)__builtin_amdgcn_readfirstlane(zs_wid()) % WM; }
+    __device__ __forceinline__ static uint32_t wn() { return (uint32_t)__builtin_amdgcn_readfirstlane(zs_wid()) / WM; }
+    // m and n of a lane's values: n by j, m by i and q, four of them from c[i][j][4 q]
+    __device__ __forceinline__ uint32_t n_of(int j) const { return n0 + wn() * (32 * NT) + (uint32_t)j * 32u + ((uint32_t)zs_lane() & 31u); }
+    __device__ __forceinline__ uint32_t m_of(int i, int q) const {
+        return m0 + wm() * (32 * MT) + (uint32_t)i * 32u + (uint32_t)q * 8u + ((uint32_t)zs_lane() >> 5) * 4u;
+    }
+
+    __device__ __forceinline__ tp_tile(const tp_mat& ma_, const tp_mat& mb_, uint32_t m, uint32_t n) : ma(ma_), mb(mb_), m0(m * BM), n0(n * BN) {
+        a.start(ma, m0, wm() * (32 * MT));
+        b.start(mb, n0, wn() * (32 * NT));
+    }
+    struct regs {
+        tp_s8 a[MT][2], b[NT][2];
+    };
+    __device__ __forceinline__ void get(const tp_lds* s, regs& r) const {
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+#pragma unroll
+            for (int i = 0; i < MT; i++) r.a[i][ks] = a.frag(s, i, ks);
+#pragma unroll
+            for (int i = 0; i < NT; i++) r.b[i][ks] = b.frag(s + SA, i, ks);
+        }
+    }
+    __device__ __forceinline__ static void mul(const regs& r, tp_acc (&c)[MT][NT]) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int j = 0; j < NT; j++) c[i][j] = tp_mfma<DT>(r.a[i][ks], r.b[j][ks], c[i][j]);
+    }
+    // all but the last N of a lane's loads are there, in every wave
+    template <int N>
+    __device__ __forceinline__ static void arrived() {
+#if defined(__HIP_DEVICE_COMPILE__)
+        // (the wait's fields: vector memory N, its two upper bits apart; the other counters are not waited for)
+        __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0f70);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#endif
+    }
+    // the next step's values; past the last the last again, which nobody reads
+    __device__ __forceinline__ void put(tp_lds* s) {
+        a.load(kt, s);
+        b.load(kt, s + SA);
+        if (++kt == kz) {
+            kt = kz - 1u;
+            if (PAIRS > 1 && pair + 1 < PAIRS) {
+                pair++;
+                kt = ka;
+                planes();
+            }
+        }
+    }
+    __device__ __forceinline__ void planes() {
+        a.plane(ma, PAIRS > 1 ? tp_plane_a(pair) : 0, m0);
+        b.plane(mb, PAIRS > 1 ? tp_plane_b(pair) : 0, n0);
+    }
+    // c += A B over steps k0 .. k0 + n - 1, n a multiple of four
+    __device__ __forceinline__ void run(uint32_t k0, uint32_t n, tp_acc (&c)[MT][NT]) {
+        // four steps' values in shared memory: one that the waves have read, one
+        // that they read, two on their way. (Arrays of their own: the compiler
+        // tells from them that a read does not wait for the later steps' loads.)
+        __shared__ char s0_[STAGE], s1_[STAGE], s2_[STAGE], s3_[STAGE];
+        tp_lds *s0 = (tp_lds*)s0_, *s1 = (tp_lds*)s1_, *s2 = (tp_lds*)s2_, *s3 = (tp_lds*)s3_;
+        if (n == 0u) return;
+        regs r0, r1;
+        kt = ka = k0;
+        kz = k0 + n;
+        pair = 0;
+        planes();
+        put(s0);
+        put(s1);
+        put(s2);
+        arrived<2 * LOADS>();
+        get(s0, r0);
+        for (uint32_t k = 0; k < n * PAIRS; k += 4u) {
+            arrived<LOADS>();
+            put(s3);
+            get(s1, r1);
+            mul(r0, c);
+            sched();
+            arrived<LOADS>();
+            put(s0);
+            get(s2, r0);
+            mul(r1, c);
+            sched();
+            arrived<LOADS>();
+            put(s1);
+            get(s3, r1);
+            mul(r0, c);
+            sched();
+            arrived<LOADS>();
+            put(s2);
+            get(s0, r0);
+            mul(r1, c);
+            sched();
+        }
+        arrived<0>();
+    }
+    // the order of a step's instructions: reads and loads evenly between the products
+    template <int I = 0>
+    __device__ __forceinline__ static void sched() {
+#if defined(__HIP_DEVICE_COMPILE__)
+        constexpr int M = MT * NT * 2, D = MT * 2 * (AS ? 2 : 1) + NT * 2 * (BS ? 2 : 1);
+        constexpr int d = (I + 1) * D / M - I * D / M, v = (I + 1) * LOADS / M - I * LOADS / M;
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if constexpr (d > 0) __builtin_amdgcn_sched_group_barrier(0x100, d, 0);
+        if constexpr (v > 0) __builtin_amdgcn_sched_group_barrier(0x020, v, 0);
+        if constexpr (I + 1 < M) sched<I + 1>();
+#endif
+    }
+};
+
+// Workgroup id's tile of mt x nt (~0: none). Workgroups id, id + 8, ... run on
+// one XCD: each XCD has a run of tiles of its own, in groups of four along m,
+// n by n, so that the tiles in its CUs share their operands in its L2.
+__device__ __forceinline__ uint2 tp_place(uint32_t id, uint32_t mt, uint32_t nt) {
+    const uint32_t all = mt * nt, per = (all + 7u) >> 3, t = (id & 7u) * per + (id >> 3);
+    if ((id >> 3) >= per || t >= all) return make_uint2(~0u, 0u);
+    const uint32_t g = t / (4u * nt), gm = mt - g * 4u < 4u ? mt - g * 4u : 4u, r = t - g * 4u * nt;
+    return make_uint2(g * 4u + r % gm, r / gm);
+}
+inline uint32_t tp_places(uint32_t mt, uint32_t nt) { return (mt * nt + 7u) / 8u * 8u; }
