@@ -62,6 +62,7 @@ int zs_abi_version(void);
 #define ZS_LAYOUT_TEACHER 7
 #define ZS_LAYOUT_DISTILL 8
 #define ZS_LAYOUT_CE 9
+#define ZS_LAYOUT_Q4 10
 int zs_struct_layout(int which, size_t* size, size_t* offsets, size_t cap);
 
 /* Context on HIP device `device`, with scratch sized for batches of up to
@@ -593,6 +594,46 @@ typedef struct zs_ce {
 int zs_ce_work(uint32_t N, uint32_t V, uint32_t D, uint32_t dtype, uint32_t want, uint64_t* bytes);
 int zs_ce_loss(zs_ctx* ctx, const zs_ce* args, void* stream);
 int zs_ce_loss_grad(zs_ctx* ctx, const zs_ce* args, void* stream);
+
+/* ---- a vocabulary head held in 4 bits ----------------------------------------
+ * W of V rows and D columns in groups of `group` (32, 64 or 128) columns of a
+ * row: codes 0 to 15, two to a byte (the even column's in the low half), and a
+ * scale per group, f16:
+ *     w = scale * (code - 8),   with minima (f16)   w = scale * code + min
+ * D is a multiple of group. The codes are laid out once for the kernels
+ * (zs_q4_pack, into d_head of zs_q4_bytes bytes); logits are
+ *     logits[r][v] = sum_d hidden[r][d] W_vd
+ * in f32: codes and hidden states (f32: as three bf16, to 2^-26) multiplied
+ * exactly, summed in f32 over a group, scaled, and summed in f32. They are what
+ * zs_sample, zs_lane_step, zs_beam_select and the others read (those that ask
+ * for it with ld % 4 == 0).
+ *   zs_q4_quantize    codes and scales of a weight of any of the three types:
+ *                     scale = f16(max |w| / 7), code = round(w / scale) + 8; with
+ *                     d_mins scale = f16((max - min) / 15), min = f16(min), code =
+ *                     round((w - min) / scale); limited to 0 .. 15, halves to even,
+ *                     a scale of 0 has w = 0 (min)
+ *   zs_q4_logits      B rows; scratch for f32 rows and for those that do not all
+ *                     begin at 16 bytes (`copy`) */
+#define ZS_Q4_MINS 1u
+#define ZS_Q4_MAX_ROWS 1048560u
+typedef struct zs_q4 {
+    uint32_t V, D, group, flags;      /* flags: 0 or ZS_Q4_MINS */
+    const void* d_head;               /* from zs_q4_pack, 256-byte aligned */
+    uint32_t B, dtype;
+    const void* d_hidden;             /* [B][ld_hidden] */
+    uint64_t ld_hidden;
+    float* d_logits;                  /* [B][ld] */
+    uint64_t ld;
+    void* d_work;
+    uint64_t work_bytes;
+} zs_q4;
+int zs_q4_bytes(uint32_t V, uint32_t D, uint32_t group, uint32_t flags, uint64_t* bytes);
+int zs_q4_quantize(zs_ctx* ctx, const void* d_weight, uint64_t ld_weight, uint32_t dtype, uint32_t V, uint32_t D,
+                   uint32_t group, uint8_t* d_codes, void* d_scales, void* d_mins, void* stream);
+int zs_q4_pack(zs_ctx* ctx, const uint8_t* d_codes, const void* d_scales, const void* d_mins, uint32_t V, uint32_t D,
+               uint32_t group, void* d_head, void* stream);
+int zs_q4_logits_work(uint32_t B, uint32_t D, uint32_t dtype, uint32_t copy, uint64_t* bytes);
+int zs_q4_logits(zs_ctx* ctx, const zs_q4* args, void* stream);
 
 /* ---- profiling ----------------------------------------------------------
  * When enabled, zs_sample and zs_spec_verify record a HIP event around their

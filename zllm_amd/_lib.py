@@ -148,6 +148,14 @@ class Ce(C.Structure):
     ]
 
 
+class Q4(C.Structure):
+    _fields_ = [
+        ("V", C.c_uint32), ("D", C.c_uint32), ("group", C.c_uint32), ("flags", C.c_uint32), ("d_head", C.c_void_p),
+        ("B", C.c_uint32), ("dtype", C.c_uint32), ("d_hidden", C.c_void_p), ("ld_hidden", C.c_uint64),
+        ("d_logits", C.c_void_p), ("ld", C.c_uint64), ("d_work", C.c_void_p), ("work_bytes", C.c_uint64),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/zs.h declares
 SIGNATURES = {
     "zs_abi_version": (C.c_int, []),
@@ -223,6 +231,13 @@ SIGNATURES = {
     "zs_ce_work": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_uint64)]),
     "zs_ce_loss": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "zs_ce_loss_grad": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "zs_q4_bytes": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_uint64)]),
+    "zs_q4_quantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32,
+                                 C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "zs_q4_pack": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32,
+                             C.c_void_p, C.c_void_p]),
+    "zs_q4_logits_work": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_uint64)]),
+    "zs_q4_logits": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "zs_tool_call_envelope_regex": (C.c_int, [C.POINTER(C.c_char_p), C.POINTER(C.c_char_p), C.c_uint32, C.c_char_p,
                                               C.c_size_t, C.POINTER(C.c_size_t), C.c_char_p, C.c_size_t]),
 }
@@ -232,7 +247,7 @@ ABI_VERSION = 2
 
 # zs_struct_layout ids (ZS_LAYOUT_*) of the Structures above
 LAYOUTS = {0: Batch, 1: RowParams, 2: SpecBatch, 3: LaneStream, 4: HallucReport, 5: Beam, 6: BeamStateDesc,
-           7: Teacher, 8: Distill, 9: Ce}
+           7: Teacher, 8: Distill, 9: Ce, 10: Q4}
 
 
 def layout_mismatches(lib_):

@@ -15,6 +15,7 @@
 #include "zs_beam.h"
 #include "zs_distill.h"
 #include "zs_ce.h"
+#include "zs_q4.h"
 
 // launchers (zs_sample.hip, zs_dfa.hip)
 extern "C" int zs_sample_launch(zs_ctx* ctx, const zs_batch* bt, hipStream_t stream);
@@ -131,6 +132,10 @@ extern "C" int zs_struct_layout(int which, size_t* size, size_t* offsets, size_t
         ZS_OFF(zs_ce, d_lse), ZS_OFF(zs_ce, d_row_grad), ZS_OFF(zs_ce, row_grad_stride), ZS_OFF(zs_ce, d_dhidden),
         ZS_OFF(zs_ce, d_dweight), ZS_OFF(zs_ce, ld_dhidden), ZS_OFF(zs_ce, ld_dweight), ZS_OFF(zs_ce, d_work),
         ZS_OFF(zs_ce, work_bytes)};
+    static const size_t q4[] = {
+        ZS_OFF(zs_q4, V), ZS_OFF(zs_q4, D), ZS_OFF(zs_q4, group), ZS_OFF(zs_q4, flags), ZS_OFF(zs_q4, d_head), ZS_OFF(zs_q4, B),
+        ZS_OFF(zs_q4, dtype), ZS_OFF(zs_q4, d_hidden), ZS_OFF(zs_q4, ld_hidden), ZS_OFF(zs_q4, d_logits), ZS_OFF(zs_q4, ld),
+        ZS_OFF(zs_q4, d_work), ZS_OFF(zs_q4, work_bytes)};
     const size_t* f;
     size_t n, sz;
     switch (which) {
@@ -144,6 +149,7 @@ extern "C" int zs_struct_layout(int which, size_t* size, size_t* offsets, size_t
         case ZS_LAYOUT_TEACHER: f = teach; n = sizeof(teach) / sizeof(size_t); sz = sizeof(zs_teacher); break;
         case ZS_LAYOUT_DISTILL: f = dist; n = sizeof(dist) / sizeof(size_t); sz = sizeof(zs_distill); break;
         case ZS_LAYOUT_CE: f = ce; n = sizeof(ce) / sizeof(size_t); sz = sizeof(zs_ce); break;
+        case ZS_LAYOUT_Q4: f = q4; n = sizeof(q4) / sizeof(size_t); sz = sizeof(zs_q4); break;
         default: return ZS_EINVAL;
     }
     if (size) *size = sz;
@@ -1360,4 +1366,82 @@ static int ce_call(zs_ctx* ctx, const zs_ce* b, bool grad, const char* who, void
 extern "C" int zs_ce_loss(zs_ctx* ctx, const zs_ce* args, void* stream) { return ce_call(ctx, args, false, "zs_ce_loss", stream); }
 extern "C" int zs_ce_loss_grad(zs_ctx* ctx, const zs_ce* args, void* stream) {
     return ce_call(ctx, args, true, "zs_ce_loss_grad", stream);
+}
+
+// ---- a head held in 4 bits
+static bool q4_sizes(uint32_t V, uint32_t D, uint32_t group, uint32_t flags) {
+    return V != 0 && V <= ZS_HEAD_MAX_VOCAB && (group == 32u || group == 64u || group == 128u) && D != 0 &&
+           D <= ZS_CE_MAX_HIDDEN && D % group == 0 && !(flags & ~(uint32_t)ZS_Q4_MINS);
+}
+extern "C" int zs_q4_bytes(uint32_t V, uint32_t D, uint32_t group, uint32_t flags, uint64_t* bytes) {
+    if (!bytes || !q4_sizes(V, D, group, flags)) return ZS_EINVAL;
+    *bytes = q4_of(V, D, group, flags & ZS_Q4_MINS).end;
+    return ZS_OK;
+}
+extern "C" int zs_q4_quantize(zs_ctx* ctx, const void* d_weight, uint64_t ld_weight, uint32_t dtype, uint32_t V, uint32_t D,
+                              uint32_t group, uint8_t* d_codes, void* d_scales, void* d_mins, void* stream) {
+    const char* who = "zs_q4_quantize";
+    if (!ctx) return ZS_EINVAL;
+    if (!q4_sizes(V, D, group, 0) || dtype > ZS_BF16) return zs_set_error(ctx, ZS_EINVAL, "%s: sizes, group or dtype outside their ranges", who);
+    int rc = ce_matrix(ctx, d_weight, ld_weight, D, dtype, "d_weight", who);
+    if (rc) return rc;
+    if (!d_codes || !d_scales || ((uintptr_t)d_scales & 1u) || ((uintptr_t)d_mins & 1u))
+        return zs_set_error(ctx, ZS_EINVAL, "%s: null or misaligned output", who);
+    q4_pack_args a{};
+    a.V = V; a.D = D; a.group = group; a.codes = d_codes; a.scales = (uint16_t*)d_scales; a.mins = (uint16_t*)d_mins;
+    a.weight = d_weight; a.ld_w = ld_weight;
+    const int prev = zs_device_guard_begin(ctx);
+    rc = q4_quantize(a, dtype, (hipStream_t)stream);
+    zs_device_guard_end(ctx, prev);
+    return rc ? zs_set_error(ctx, ZS_EHIP, "%s: launch failed", who) : ZS_OK;
+}
+extern "C" int zs_q4_pack(zs_ctx* ctx, const uint8_t* d_codes, const void* d_scales, const void* d_mins, uint32_t V, uint32_t D,
+                          uint32_t group, void* d_head, void* stream) {
+    const char* who = "zs_q4_pack";
+    if (!ctx) return ZS_EINVAL;
+    if (!q4_sizes(V, D, group, 0)) return zs_set_error(ctx, ZS_EINVAL, "%s: sizes or group outside their ranges", who);
+    if (!d_codes || !d_scales || !d_head || ((uintptr_t)d_scales & 1u) || ((uintptr_t)d_mins & 1u) || ((uintptr_t)d_head & 255u))
+        return zs_set_error(ctx, ZS_EINVAL, "%s: null pointer, or d_head not 256-byte aligned", who);
+    q4_pack_args a{};
+    a.at = q4_of(V, D, group, d_mins != nullptr);
+    a.V = V; a.D = D; a.group = group; a.codes = (uint8_t*)d_codes; a.scales = (uint16_t*)d_scales; a.mins = (uint16_t*)d_mins;
+    a.head = (char*)d_head;
+    const int prev = zs_device_guard_begin(ctx);
+    const int rc = q4_pack(a, (hipStream_t)stream);
+    zs_device_guard_end(ctx, prev);
+    return rc ? zs_set_error(ctx, ZS_EHIP, "%s: launch failed", who) : ZS_OK;
+}
+extern "C" int zs_q4_logits_work(uint32_t B, uint32_t D, uint32_t dtype, uint32_t copy, uint64_t* bytes) {
+    if (!bytes || dtype > ZS_BF16 || D == 0 || D > ZS_CE_MAX_HIDDEN || B > ZS_Q4_MAX_ROWS) return ZS_EINVAL;
+    *bytes = copy || dtype == ZS_F32 ? hd_pad((uint64_t)B * D * (dtype == ZS_F32 ? 6u : 2u)) : 0;
+    return ZS_OK;
+}
+extern "C" int zs_q4_logits(zs_ctx* ctx, const zs_q4* b, void* stream) {
+    const char* who = "zs_q4_logits";
+    if (!ctx || !b) return zs_set_error(ctx, ZS_EINVAL, "%s: null argument", who);
+    if (!q4_sizes(b->V, b->D, b->group, b->flags)) return zs_set_error(ctx, ZS_EINVAL, "%s: sizes, group or flags outside their ranges", who);
+    if (b->dtype > ZS_BF16) return zs_set_error(ctx, ZS_EINVAL, "%s: unknown dtype %u", who, b->dtype);
+    if (b->B > ZS_Q4_MAX_ROWS) return zs_set_error(ctx, ZS_ELIMIT, "%s: B=%u above %u", who, b->B, ZS_Q4_MAX_ROWS);
+    if (b->B == 0) return ZS_OK;
+    int rc = ce_matrix(ctx, b->d_hidden, b->ld_hidden, b->D, b->dtype, "d_hidden", who);
+    if (rc) return rc;
+    if (!b->d_head || ((uintptr_t)b->d_head & 255u) || !b->d_logits || ((uintptr_t)b->d_logits & 3u) || b->ld < b->V)
+        return zs_set_error(ctx, ZS_EINVAL, "%s: null or misaligned pointer, or ld < V", who);
+    const bool copy = b->dtype == ZS_F32 || ((uintptr_t)b->d_hidden & 15u) || (b->B > 1u && b->ld_hidden % 8u);
+    uint64_t need = 0;
+    (void)zs_q4_logits_work(b->B, b->D, b->dtype, copy, &need);
+    if ((rc = work_check(ctx, b->d_work, b->work_bytes, need, who))) return rc;
+    q4_args a{};
+    a.head = (const char*)b->d_head;
+    a.at = q4_of(b->V, b->D, b->group, b->flags & ZS_Q4_MINS);
+    a.V = b->V; a.D = b->D; a.B = b->B;
+    a.hidden = copy ? b->d_work : b->d_hidden;
+    a.ld_h = copy ? b->D : b->ld_hidden;
+    a.plane = (uint64_t)b->B * b->D;
+    a.logits = b->d_logits; a.ld = b->ld;
+    q4_x_args x = {b->d_hidden, b->ld_hidden, b->B, b->D, (uint16_t*)b->d_work};
+    const int prev = zs_device_guard_begin(ctx);
+    rc = q4_logits(a, copy ? &x : nullptr, b->dtype, b->group, b->flags & ZS_Q4_MINS, (hipStream_t)stream);
+    zs_device_guard_end(ctx, prev);
+    return rc ? zs_set_error(ctx, ZS_EHIP, "%s: launch failed", who) : ZS_OK;
 }

@@ -6,21 +6,6 @@
 
 #define CE_NT 256
 
-__device__ __forceinline__ uint16_t ce_bf16(float x) {
-    const __bf16 b = (__bf16)x;
-    return __builtin_bit_cast(uint16_t, b);
-}
-__device__ __forceinline__ float ce_of_bf16(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
-// x as a sum of three bf16, each the nearest to what is left (24 bits in all);
-// where the first would be infinite for a finite x, the one below it.
-__device__ __forceinline__ void ce_split(float x, uint16_t (&p)[3]) {
-    p[0] = ce_bf16(x);
-    if ((p[0] & 0x7fffu) == 0x7f80u) p[0] = (uint16_t)(__float_as_uint(x) >> 16);
-    float r = x - ce_of_bf16(p[0]);
-    if ((p[0] & 0x7f80u) == 0x7f80u) r = 0.0f;
-    p[1] = ce_bf16(r);
-    p[2] = ce_bf16(r - ce_of_bf16(p[1]));
-}
 __device__ __forceinline__ float ce_exp(float x) {   // e^x
 #if defined(__HIP_DEVICE_COMPILE__)
     return __builtin_amdgcn_exp2f(x * 1.44269504f);
@@ -127,7 +112,7 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
         const float x = d < a.D ? ce_load<DT>(a.hidden, hr + d) : 0.0f;
         if constexpr (DT == ZS_F32) {
             uint16_t p[3];
-            ce_split(x, p);
+            zs_split3(x, p);
             for (int k = 0; k < 3; k++) o[k * plane + d] = p[k];
         } else {
             o[d] = d < a.D ? ((const uint16_t*)a.hidden)[hr + d] : (uint16_t)0;
@@ -150,7 +135,7 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_weight(ce_args a) {
             uint16_t* o = a.w + v * a.Dp + d;
             if constexpr (DT == ZS_F32) {
                 uint16_t p[3];
-                ce_split(d < a.D ? ce_load<DT>(a.weight, v * a.ld_w + d) : 0.0f, p);
+                zs_split3(d < a.D ? ce_load<DT>(a.weight, v * a.ld_w + d) : 0.0f, p);
                 for (int k = 0; k < 3; k++) o[k * plane] = p[k];
             } else {
                 *o = d < a.D ? ((const uint16_t*)a.weight)[v * a.ld_w + d] : (uint16_t)0;
@@ -312,7 +297,7 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_grad(ce_args a) {
     if constexpr (DT == ZS_F32) {
         const uint64_t plane = (uint64_t)a.R * a.Vp;
         uint16_t p[8][3];
-        for (int k = 0; k < 8; k++) ce_split(x[k], p[k]);
+        for (int k = 0; k < 8; k++) zs_split3(x[k], p[k]);
         for (int q = 0; q < 3; q++) {
             hd_u4 o;
             for (int k = 0; k < 4; k++) o[k] = (uint32_t)p[2 * k][q] | (uint32_t)p[2 * k + 1][q] << 16;

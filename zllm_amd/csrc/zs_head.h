@@ -54,6 +54,21 @@ __device__ __forceinline__ uint32_t hd_pack2(float a, float b) {
     }
 }
 
+__device__ __forceinline__ uint16_t zs_bf16(float x) {
+    const __bf16 b = (__bf16)x;
+    return __builtin_bit_cast(uint16_t, b);
+}
+// x as a sum of three bf16, each the nearest to what is left (24 bits in all);
+// where the first would be infinite for a finite x, the one below it.
+__device__ __forceinline__ void zs_split3(float x, uint16_t (&p)[3]) {
+    p[0] = zs_bf16(x);
+    if ((p[0] & 0x7fffu) == 0x7f80u) p[0] = (uint16_t)(__float_as_uint(x) >> 16);
+    float r = x - hd_float(p[0]);
+    if ((p[0] & 0x7f80u) == 0x7f80u) r = 0.0f;
+    p[1] = zs_bf16(r);
+    p[2] = zs_bf16(r - hd_float(p[1]));
+}
+
 template <int DT>
 struct hd_row {
     typedef typename hd_elem<DT>::T T;

@@ -1,0 +1,53 @@
+// zs_q4.h -- a vocabulary head held in 4 bits: its layout, and kernel arguments.
+#pragma once
+#include <hip/hip_runtime.h>
+#include "zs_head_args.h"
+
+// The head lies in tiles of 16 rows (ids) by 128 columns, one behind the other
+// along the columns, 1 KB each: lane l of a wave has row l % 16 and, of each of
+// four blocks of 32 columns, the eight from (l / 16) * 8 on, as one 32-bit word.
+// A word holds column 2 j in the four bits from 4 j on and column 2 j + 1 in
+// those from 16 + 4 j on, where one shift and one mask make operands of them.
+// Behind the tiles the scales (f16, 128 / group of a row and tile side by side,
+// rows next to each other), behind those the minima likewise.
+struct q4_layout {
+    uint32_t tiles, blocks;      // of rows, of columns
+    uint64_t scales, mins, end;  // bytes
+};
+inline q4_layout q4_of(uint32_t V, uint32_t D, uint32_t group, bool mins) {
+    q4_layout q;
+    q.tiles = (V + 15u) / 16u;
+    q.blocks = (D + 127u) / 128u;
+    const uint64_t n = (uint64_t)q.tiles * q.blocks, s = hd_pad(n * 16u * (128u / group) * 2u);
+    q.scales = n * 1024u;
+    q.mins = q.scales + s;
+    q.end = q.mins + (mins ? s : 0u);
+    return q;
+}
+struct q4_args {
+    const char* head;
+    q4_layout at;
+    uint32_t V, D, B;
+    const void* hidden;          // rows of 16-bit values at 16 bytes each (planes one behind the other)
+    uint64_t ld_h, plane;        // elements
+    float* logits;
+    uint64_t ld;
+};
+struct q4_pack_args {
+    q4_layout at;
+    uint32_t V, D, group;
+    uint8_t* codes;              // [V][D / 2]
+    uint16_t *scales, *mins;     // [V][D / group] f16
+    char* head;
+    const void* weight;          // to be quantised
+    uint64_t ld_w;
+};
+struct q4_x_args {               // hidden states to rows the kernel takes
+    const void* hidden;
+    uint64_t ld_h;
+    uint32_t B, D;
+    uint16_t* out;               // [planes][B][D]
+};
+int q4_pack(const q4_pack_args& a, hipStream_t stream);
+int q4_quantize(const q4_pack_args& a, uint32_t dtype, hipStream_t stream);
+int q4_logits(const q4_args& a, const q4_x_args* x, uint32_t dtype, uint32_t group, bool mins, hipStream_t stream);

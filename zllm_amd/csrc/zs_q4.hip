@@ -1,0 +1,252 @@
+// zs_q4.hip -- logits of a vocabulary head held in 4 bits with scales per group
+// of columns.
+#include <hip/hip_runtime.h>
+#include "zs_q4.h"
+#include "zs_head.h"
+
+#define Q4_NT 256
+
+typedef float q4_f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t q4_u4 __attribute__((ext_vector_type(4)));
+
+// ------------------------------------------------------------------ quantising, laying out
+// A group's scale and minimum from its extremes, then its codes, two to a byte.
+// Without minima w ~ scale * (code - 8) with scale = max |w| / 7; with them
+// w ~ scale * code + min with scale = (max - min) / 15. Both are rounded to f16
+// first and the codes taken by the rounded ones; a scale of 0 has codes of 0 (8).
+template <int DT>
+__global__ __launch_bounds__(Q4_NT) void zs_k_q4_quantize(q4_pack_args a) {
+    const uint32_t per = a.D / a.group, w = zs_wid(), l = zs_lane();
+    const uint64_t groups = (uint64_t)a.V * per;
+    typedef typename hd_elem<DT>::T T;
+    for (uint64_t g = (uint64_t)blockIdx.x * (Q4_NT / 64) + w; g < groups; g += (uint64_t)gridDim.x * (Q4_NT / 64)) {
+        const uint64_t v = g / per;
+        const uint32_t c0 = (uint32_t)(g - v * per) * a.group;
+        const T* x = reinterpret_cast<const T*>(a.weight) + v * a.ld_w + c0;
+        float y[2] = {0.0f, 0.0f};
+        const bool in = 2u * l < a.group;
+        float lo = INFINITY, hi = -INFINITY;
+        if (in)
+            for (int i = 0; i < 2; i++) {
+                y[i] = hd_float(x[2u * l + i]);
+                lo = fminf(lo, y[i]), hi = fmaxf(hi, y[i]);
+            }
+        hi = wave_max_f(hi);
+        lo = -wave_max_f(-lo);
+        _Float16 s, m = (_Float16)0.0f;
+        if (a.mins) {
+            s = (_Float16)((hi - lo) / 15.0f);
+            m = (_Float16)lo;
+        } else {
+            s = (_Float16)(fmaxf(fabsf(lo), fabsf(hi)) / 7.0f);
+        }
+        const float sf = (float)s, mf = (float)m;
+        uint32_t code = 0;
+        for (int i = 0; i < 2; i++) {
+            float q = sf != 0.0f ? rintf(a.mins ? (y[i] - mf) / sf : y[i] / sf) : 0.0f;
+            q = fminf(fmaxf(a.mins ? q : q + 8.0f, 0.0f), 15.0f);
+            code |= (uint32_t)q << (4 * i);
+        }
+        if (in) a.codes[(v * a.D + c0) / 2u + l] = (uint8_t)code;
+        if (l == 0u) {
+            a.scales[g] = __builtin_bit_cast(uint16_t, s);
+            if (a.mins) a.mins[g] = __builtin_bit_cast(uint16_t, m);
+        }
+    }
+}
+// One workgroup a tile of 16 rows and 128 columns: its words, scales and minima
+// (zeros past the last row or column).
+__global__ __launch_bounds__(64) void zs_k_q4_pack(q4_pack_args a) {
+    const uint32_t l = threadIdx.x, per = 128u / a.group;
+    const uint64_t n = (uint64_t)a.at.tiles * a.at.blocks;
+    for (uint64_t t = blockIdx.x; t < n; t += gridDim.x) {
+        const uint64_t v0 = t / a.at.blocks * 16u, v = v0 + (l & 15u);
+        const uint32_t c0 = (uint32_t)(t % a.at.blocks) * 128u;
+        q4_u4 o;
+        for (uint32_t b = 0; b < 4u; b++) {
+            const uint32_t c = c0 + b * 32u + (l >> 4) * 8u;
+            uint32_t word = 0;
+            if (v < a.V && c < a.D)
+                for (uint32_t j = 0; j < 4u; j++) {
+                    const uint32_t two = a.codes[(v * a.D + c) / 2u + j];
+                    word |= (two & 15u) << (4u * j) | (two >> 4) << (16u + 4u * j);
+                }
+            o[b] = word;
+        }
+        *(q4_u4*)(a.head + t * 1024u + l * 16u) = o;
+        for (uint32_t i = l; i < 16u * per; i += 64u) {
+            const uint64_t r = v0 + i / per, g = c0 / a.group + i % per;
+            const bool in = r < a.V && g < a.D / a.group;
+            const uint64_t to = t * 16u * per + i, from = r * (a.D / a.group) + g;
+            ((uint16_t*)(a.head + a.at.scales))[to] = in ? a.scales[from] : (uint16_t)0;
+            if (a.mins) ((uint16_t*)(a.head + a.at.mins))[to] = in ? a.mins[from] : (uint16_t)0;
+        }
+    }
+}
+
+// ------------------------------------------------------------------ hidden states
+// Rows at 16 bytes each; f32 as three bf16 whose sum is the value to 2^-26 of it.
+template <int DT>
+__global__ __launch_bounds__(Q4_NT) void zs_k_q4_rows(q4_x_args a) {
+    const uint64_t n = (uint64_t)a.B * a.D;
+    for (uint64_t i = (uint64_t)blockIdx.x * Q4_NT + threadIdx.x; i < n; i += (uint64_t)gridDim.x * Q4_NT) {
+        const uint64_t r = i / a.D, from = r * a.ld_h + (i - r * a.D);
+        if constexpr (DT == ZS_F32) {
+            uint16_t p[3];
+            zs_split3(((const float*)a.hidden)[from], p);
+            for (int k = 0; k < 3; k++) a.out[k * n + i] = p[k];
+        } else {
+            a.out[i] = ((const uint16_t*)a.hidden)[from];
+        }
+    }
+}
+
+// ------------------------------------------------------------------ logits
+// A code q becomes the 16-bit float 16 + q by one shift and one and-or: the
+// leading mantissa bits of a number between 16 and 32 count ones. What that adds
+// comes off by the matrix cores too: c0 = sum x * -24 (-16 with minima) is the
+// sum the products start from. Operand register j holds columns 2 j, 2 j + 1.
+template <int DT>
+struct q4_num {
+    static constexpr uint32_t ONE = DT == ZS_F16 ? 6 : 3;                                   // log2 of a unit's bits
+    static constexpr uint32_t BASE = DT == ZS_F16 ? 0x4c004c00u : 0x41804180u, MASK = 0x000f000fu << ONE;
+    static constexpr uint32_t M16 = DT == ZS_F16 ? 0xcc00cc00u : 0xc180c180u, M24 = DT == ZS_F16 ? 0xce00ce00u : 0xc1c0c1c0u;
+    static __device__ __forceinline__ q4_u4 operand(uint32_t w) {
+        q4_u4 o;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int s = 4 * j - (int)ONE;
+            o[j] = ((s >= 0 ? w >> s : w << -s) & MASK) | BASE;
+        }
+        return o;
+    }
+    static __device__ __forceinline__ q4_f4 mul(q4_u4 a, q4_u4 b, q4_f4 c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        if constexpr (DT == ZS_F16) {
+            typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+            return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+        } else {
+            typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+            return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+        }
+#else
+        return c;
+#endif
+    }
+};
+
+// T tiles of 16 ids by 16 rows of hidden states: each wave takes a part of the
+// columns, their sums are joined through shared memory.
+template <int DT, int G, bool MINS, int T>
+__global__ __launch_bounds__(Q4_NT) void zs_k_q4_logits(q4_args a) {
+    constexpr int P = DT == ZS_F32 ? 3 : 1, PER = 128 / G, KS = Q4_NT / 64;
+    typedef q4_num<DT> num;
+    __shared__ q4_f4 sh[KS][T][64];
+    const uint32_t l = (uint32_t)zs_lane(), w = (uint32_t)__builtin_amdgcn_readfirstlane(zs_wid());
+    const uint32_t t0 = blockIdx.x * T, r0 = blockIdx.y * 16u;
+    const uint32_t b0 = a.at.blocks * w / KS, b1 = a.at.blocks * (w + 1u) / KS;
+    const uint32_t r = r0 + (l & 15u) < a.B ? r0 + (l & 15u) : a.B - 1u;
+    const uint16_t* x = (const uint16_t*)a.hidden + r * a.ld_h + (l >> 4) * 8u;
+    q4_f4 acc[T];
+#pragma unroll
+    for (int t = 0; t < T; t++) acc[t] = q4_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    const q4_u4 off = {MINS ? num::M16 : num::M24, MINS ? num::M16 : num::M24, MINS ? num::M16 : num::M24, MINS ? num::M16 : num::M24};
+    for (uint32_t b = b0; b < b1; b++) {
+        q4_u4 wv[T], xv[P][4];
+        _Float16 s[T][PER], m[T][PER];
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            const uint32_t tile = t0 + t < a.at.tiles ? t0 + t : a.at.tiles - 1u;
+            const uint64_t at = (uint64_t)tile * a.at.blocks + b;
+            wv[t] = __builtin_nontemporal_load((const __attribute__((address_space(1))) q4_u4*)(a.head + at * 1024u + l * 16u));
+            const _Float16* sp = (const _Float16*)(a.head + a.at.scales) + (at * 16u + (l & 15u)) * PER;
+            const _Float16* mp = (const _Float16*)(a.head + a.at.mins) + (at * 16u + (l & 15u)) * PER;
+#pragma unroll
+            for (int k = 0; k < PER; k++) {
+                s[t][k] = sp[k];
+                if (MINS) m[t][k] = mp[k];
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                xv[p][k] = q4_u4{0u, 0u, 0u, 0u};
+                if (b * 128u + k * 32u < a.D) xv[p][k] = *(const q4_u4*)(x + p * a.plane + b * 128u + k * 32u);
+            }
+#pragma unroll
+        for (int g = 0; g < PER; g++) {
+            q4_f4 c0 = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = g * (G / 32); k < (g + 1) * (G / 32); k++)
+#pragma unroll
+                for (int p = P - 1; p >= 0; p--) c0 = num::mul(xv[p][k], off, c0);
+#pragma unroll
+            for (int t = 0; t < T; t++) {
+                q4_f4 d = c0;
+#pragma unroll
+                for (int k = g * (G / 32); k < (g + 1) * (G / 32); k++) {
+                    const q4_u4 op = num::operand(wv[t][k]);
+#pragma unroll
+                    for (int p = P - 1; p >= 0; p--) d = num::mul(xv[p][k], op, d);
+                }
+                const float sf = (float)s[t][g], mf = MINS ? (float)m[t][g] * -0.0625f : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    acc[t][i] = __builtin_fmaf(sf, d[i], acc[t][i]);
+                    if (MINS) acc[t][i] = __builtin_fmaf(mf, c0[i], acc[t][i]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < T; t++) sh[w][t][l] = acc[t];
+    __syncthreads();
+    for (uint32_t t = w; t < T; t += KS) {
+        q4_f4 v = sh[0][t][l];
+        for (int k = 1; k < KS; k++) v += sh[k][t][l];
+        const uint32_t id = (t0 + t) * 16u + (l & 15u);
+        if (id >= a.V) continue;
+        for (uint32_t i = 0; i < 4u; i++) {
+            const uint32_t row = r0 + (l >> 4) * 4u + i;
+            if (row < a.B) a.logits[row * a.ld + id] = v[i];
+        }
+    }
+}
+
+int q4_pack(const q4_pack_args& a, hipStream_t stream) {
+    const uint64_t n = (uint64_t)a.at.tiles * a.at.blocks;
+    hipLaunchKernelGGL(zs_k_q4_pack, dim3(n < 65536u ? (uint32_t)n : 65536u), dim3(64), 0, stream, a);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+int q4_quantize(const q4_pack_args& a, uint32_t dtype, hipStream_t stream) {
+    const uint64_t n = ((uint64_t)a.V * (a.D / a.group) + Q4_NT / 64 - 1u) / (Q4_NT / 64);
+    const dim3 grid(n < 65536u ? (uint32_t)n : 65536u), wg(Q4_NT);
+    if (dtype == ZS_F32) hipLaunchKernelGGL(zs_k_q4_quantize<ZS_F32>, grid, wg, 0, stream, a);
+    else if (dtype == ZS_F16) hipLaunchKernelGGL(zs_k_q4_quantize<ZS_F16>, grid, wg, 0, stream, a);
+    else hipLaunchKernelGGL(zs_k_q4_quantize<ZS_BF16>, grid, wg, 0, stream, a);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+template <int DT, int G, bool MINS>
+static void q4_go(const q4_args& a, hipStream_t stream) {
+    constexpr int T = 4;
+    hipLaunchKernelGGL((zs_k_q4_logits<DT, G, MINS, T>), dim3((a.at.tiles + T - 1u) / T, (a.B + 15u) / 16u), dim3(Q4_NT), 0, stream, a);
+}
+template <int DT>
+static void q4_group(const q4_args& a, uint32_t group, bool mins, hipStream_t stream) {
+    if (group == 32u) mins ? q4_go<DT, 32, true>(a, stream) : q4_go<DT, 32, false>(a, stream);
+    else if (group == 64u) mins ? q4_go<DT, 64, true>(a, stream) : q4_go<DT, 64, false>(a, stream);
+    else mins ? q4_go<DT, 128, true>(a, stream) : q4_go<DT, 128, false>(a, stream);
+}
+int q4_logits(const q4_args& a, const q4_x_args* x, uint32_t dtype, uint32_t group, bool mins, hipStream_t stream) {
+    if (x) {
+        const uint64_t n = ((uint64_t)x->B * x->D + Q4_NT - 1u) / Q4_NT;
+        const dim3 grid(n < 4096u ? (uint32_t)n : 4096u), wg(Q4_NT);
+        if (dtype == ZS_F32) hipLaunchKernelGGL(zs_k_q4_rows<ZS_F32>, grid, wg, 0, stream, *x);
+        else hipLaunchKernelGGL(zs_k_q4_rows<ZS_F16>, grid, wg, 0, stream, *x);
+    }
+    if (dtype == ZS_F32) q4_group<ZS_F32>(a, group, mins, stream);
+    else if (dtype == ZS_F16) q4_group<ZS_F16>(a, group, mins, stream);
+    else q4_group<ZS_BF16>(a, group, mins, stream);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}

@@ -593,10 +593,13 @@ class LaneBatcher:
     `active` order) and hands the logits [m, V] to step(), which picks every
     stream's next token on the GPU with one zs_lane_step call (top-64 pool +
     nucleus / Gumbel sampling / argmax, seeds step_seed(base, gen_index)),
-    reads back m ids and retires finished streams as the reference does."""
+    reads back m ids and retires finished streams as the reference does.
+    With a head (zllm_amd.head.Q4Head) step() and select() take the streams'
+    hidden states [m, D] in the logits' place."""
 
-    def __init__(self, ctx: Context):
+    def __init__(self, ctx: Context, head=None):
         self.ctx = ctx
+        self.head = head
         self.active: List[LaneSeq] = []
         self.last_path = None
 
@@ -622,6 +625,8 @@ class LaneBatcher:
 
     def select(self, logits: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Device ids for the active streams (no host sync)."""
+        if self.head is not None:
+            logits = self.head.logits(logits)
         m, V = logits.shape
         assert m == len(self.active) and logits.dtype == torch.float32 and logits.stride(1) == 1
         if out is None:

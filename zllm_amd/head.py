@@ -1,12 +1,19 @@
 """The vocabulary head over libzs: its cross entropy from hidden states, without
-logits, with the gradients.
+logits, with the gradients; and a head held in 4 bits, whose logits the sampler,
+the lanes and beam search read.
 
     loss_of = HeadLoss(ctx)
     loss_of(hidden, head_weight, labels).mean().backward()
 
 or, without autograd, head_loss (evaluation, the scores of given tokens: their
-log-probabilities are -loss) and head_loss_grad. The formulas are in
-include/zs.h. The reference trains nothing; there is no counterpart.
+log-probabilities are -loss) and head_loss_grad;
+
+    head = Q4Head.quantize(ctx, head_weight, group=64)      # once
+    lanes = LaneBatcher(ctx, head=head)
+    lanes.step(hidden)                                      # the active streams' next tokens
+
+or head.logits(hidden). The formulas are in include/zs.h. The reference trains
+nothing; the loss has no counterpart.
 torch holds the device memory and the stream; the computation is libzs's.
 """
 import ctypes as C
@@ -15,8 +22,9 @@ from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.graph import increment_version
 
-from ._lib import Ce, lib
+from ._lib import Ce, Q4, lib
 from .beam import DTYPES, MAX_VOCAB, _ld, _like, _stream, _work, _work_bytes
 from .engine import Context, _check
 
@@ -25,7 +33,9 @@ MAX_LD = 4194304
 _DHIDDEN, _DWEIGHT, _COPY = 1, 2, 4
 # the arguments are packed to bytes, as zllm_amd.beam's
 _CE = struct.Struct("=4I2Q3QqfI10Q")
-assert _CE.size == C.sizeof(Ce)
+_Q4 = struct.Struct("=4IQ2I6Q")
+assert _CE.size == C.sizeof(Ce) and _Q4.size == C.sizeof(Q4)
+GROUPS = (32, 64, 128)
 
 
 @dataclass(frozen=True)
@@ -129,3 +139,90 @@ class HeadLoss(torch.nn.Module):
 
     def forward(self, hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
         return _HeadLossFunction.apply(hidden, weight, labels, self.ctx, self.cfg)
+
+
+def _group_of(V: int, D: int, groups: int, what: str) -> int:
+    group = D // groups if groups else 0
+    if group not in GROUPS or group * groups != D or not 1 <= V <= MAX_VOCAB or not D <= MAX_HIDDEN:
+        raise ValueError(f"{what}: groups are of 32, 64 or 128 columns, V 1 to {MAX_VOCAB}, D up to {MAX_HIDDEN}")
+    return group
+
+
+def q4_quantize(ctx: Context, weight: torch.Tensor, group: int = 32, mins: bool = False
+                ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+    """Codes (uint8 [V, D / 2]), scales and, asked for, minima (float16 [V, D /
+    group]) of a weight [V, D] of any of the three types (zs_q4_quantize)."""
+    what = "q4_quantize"
+    _matrix(ctx, weight, what, "weight")
+    V, D = weight.shape
+    if group not in GROUPS:
+        raise ValueError(f"{what}: groups are of 32, 64 or 128 columns")
+    _group_of(V, D, D // group, what)
+    dev = weight.device
+    codes = torch.empty((V, D // 2), dtype=torch.uint8, device=dev)
+    scales = torch.empty((V, D // group), dtype=torch.float16, device=dev)
+    lows = torch.empty_like(scales) if mins else None
+    rc = lib().zs_q4_quantize(ctx.h, weight.data_ptr(), _ld(weight), DTYPES[weight.dtype], V, D, group, codes.data_ptr(),
+                              scales.data_ptr(), lows.data_ptr() if mins else None, _stream(dev))
+    if rc:
+        _check(ctx.h, rc, what)
+    return codes, scales, lows
+
+
+class Q4Head:
+    """A head held in 4 bits: codes uint8 [V, D / 2] (0 to 15, the even
+    column's in the low half of a byte), scales float16 [V, D / group] and
+    perhaps minima likewise; w = scale * (code - 8), or scale * code + min. The
+    codes are laid out once, when it is made; what it is made from is not kept."""
+
+    def __init__(self, ctx: Context, codes: torch.Tensor, scales: torch.Tensor, mins: Optional[torch.Tensor] = None):
+        what = "Q4Head"
+        if codes.dim() != 2 or scales.dim() != 2:
+            raise ValueError(f"{what}: codes are [V, D / 2], scales [V, D / group]")
+        if codes.get_device() != ctx.device:
+            raise ValueError(f"{what}: codes are on {codes.device}, not on the context's GPU {ctx.device}")
+        dev, (V, half), groups = codes.device, codes.shape, scales.shape[1]
+        self.ctx, self.V, self.D, self.group, self.mins = ctx, V, 2 * half, _group_of(V, 2 * half, groups, what), mins is not None
+        _like(codes, (V, half), torch.uint8, dev, what, "codes")
+        _like(scales, (V, groups), torch.float16, dev, what, "scales")
+        if mins is not None:
+            _like(mins, (V, groups), torch.float16, dev, what, "mins")
+        self._data = torch.empty(_work_bytes("zs_q4_bytes", V, self.D, self.group, int(self.mins)), dtype=torch.uint8, device=dev)
+        rc = lib().zs_q4_pack(ctx.h, codes.data_ptr(), scales.data_ptr(), mins.data_ptr() if self.mins else None, V, self.D,
+                              self.group, self._data.data_ptr(), _stream(dev))
+        if rc:
+            _check(ctx.h, rc, what)
+
+    @classmethod
+    def quantize(cls, ctx: Context, weight: torch.Tensor, group: int = 32, mins: bool = False) -> "Q4Head":
+        return cls(ctx, *q4_quantize(ctx, weight, group, mins))
+
+    def logits(self, hidden: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """float32 [B, V] for hidden [B, D] of any of the three types and any
+        row stride. Without out the rows lie 4 values' multiples apart, as
+        zs_sample and zs_lane_step take them. No host sync."""
+        what = "Q4Head.logits"
+        _matrix(self.ctx, hidden, what, "hidden")
+        B, dev = hidden.shape[0], hidden.device
+        if hidden.shape[1] != self.D:
+            raise ValueError(f"{what}: hidden is [B, {self.D}]")
+        if dev != self._data.device:
+            raise ValueError(f"{what}: hidden is on {dev}, the head on {self._data.device}")
+        given = out is not None
+        if not given:
+            out = torch.empty((B, (self.V + 3) // 4 * 4), dtype=torch.float32, device=dev)[:, : self.V]
+        elif out.shape != (B, self.V) or out.dtype != torch.float32 or out.device != dev or \
+                (self.V > 1 and out.stride(1) != 1) or (B > 1 and out.stride(0) < self.V):
+            raise ValueError(f"{what}: out is float32 [{B}, {self.V}], the values of a row adjacent")
+        at, ld = hidden.data_ptr(), _ld(hidden)
+        copy = hidden.dtype == torch.float32 or at % 16 != 0 or (B > 1 and ld % 8 != 0)
+        nbytes = _work_bytes("zs_q4_logits_work", B, self.D, DTYPES[hidden.dtype], 1) if copy and B else 0
+        work, work_at = _work(nbytes, dev)
+        raw = _Q4.pack(self.V, self.D, self.group, int(self.mins), self._data.data_ptr(), B, DTYPES[hidden.dtype], at, ld,
+                       out.data_ptr(), _ld(out), work_at, nbytes)
+        rc = lib().zs_q4_logits(self.ctx.h, raw, _stream(dev))
+        if rc:
+            _check(self.ctx.h, rc, what)
+        if given:
+            increment_version(out)   # (autograd is told of writes in place)
+        return out
