@@ -612,8 +612,8 @@ int zs_ce_loss_grad(zs_ctx* ctx, const zs_ce* args, void* stream);
  *                     d_mins scale = f16((max - min) / 15), min = f16(min), code =
  *                     round((w - min) / scale); limited to 0 .. 15, halves to even,
  *                     a scale of 0 has w = 0 (min)
- *   zs_q4_logits      B rows; scratch for f32 rows and for those that do not all
- *                     begin at 16 bytes (`copy`) */
+ *   zs_q4_logits      B rows; scratch for f32 rows, for those that do not all
+ *                     begin at 16 bytes (`copy`) and for more than 16 */
 #define ZS_Q4_MINS 1u
 #define ZS_Q4_MAX_ROWS 1048560u
 typedef struct zs_q4 {

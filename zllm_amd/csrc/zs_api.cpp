@@ -1413,7 +1413,9 @@ extern "C" int zs_q4_pack(zs_ctx* ctx, const uint8_t* d_codes, const void* d_sca
 }
 extern "C" int zs_q4_logits_work(uint32_t B, uint32_t D, uint32_t dtype, uint32_t copy, uint64_t* bytes) {
     if (!bytes || dtype > ZS_BF16 || D == 0 || D > ZS_CE_MAX_HIDDEN || B > ZS_Q4_MAX_ROWS) return ZS_EINVAL;
-    *bytes = copy || dtype == ZS_F32 ? hd_pad((uint64_t)B * D * (dtype == ZS_F32 ? 6u : 2u)) : 0;
+    q4_x_args x{};
+    x.B = B; x.D = D; x.Bp = q4_bp(B);
+    *bytes = B ? q4_work(x, dtype, copy, (void*)256) : 0;
     return ZS_OK;
 }
 extern "C" int zs_q4_logits(zs_ctx* ctx, const zs_q4* b, void* stream) {
@@ -1428,20 +1430,21 @@ extern "C" int zs_q4_logits(zs_ctx* ctx, const zs_q4* b, void* stream) {
     if (!b->d_head || ((uintptr_t)b->d_head & 255u) || !b->d_logits || ((uintptr_t)b->d_logits & 3u) || b->ld < b->V)
         return zs_set_error(ctx, ZS_EINVAL, "%s: null or misaligned pointer, or ld < V", who);
     const bool copy = b->dtype == ZS_F32 || ((uintptr_t)b->d_hidden & 15u) || (b->B > 1u && b->ld_hidden % 8u);
-    uint64_t need = 0;
-    (void)zs_q4_logits_work(b->B, b->D, b->dtype, copy, &need);
-    if ((rc = work_check(ctx, b->d_work, b->work_bytes, need, who))) return rc;
+    q4_x_args x{};
+    x.hidden = b->d_hidden; x.ld_h = b->ld_hidden; x.B = b->B; x.D = b->D; x.group = b->group; x.Bp = q4_bp(b->B);
+    x.off = b->flags & ZS_Q4_MINS ? -16.0f : -24.0f;
+    if ((rc = work_check(ctx, b->d_work, b->work_bytes, q4_work(x, b->dtype, copy, b->d_work), who))) return rc;
     q4_args a{};
     a.head = (const char*)b->d_head;
     a.at = q4_of(b->V, b->D, b->group, b->flags & ZS_Q4_MINS);
     a.V = b->V; a.D = b->D; a.B = b->B;
-    a.hidden = copy ? b->d_work : b->d_hidden;
+    a.hidden = copy ? x.out : b->d_hidden;
     a.ld_h = copy ? b->D : b->ld_hidden;
     a.plane = (uint64_t)b->B * b->D;
+    a.sums = x.sums; a.Bp = x.Bp;
     a.logits = b->d_logits; a.ld = b->ld;
-    q4_x_args x = {b->d_hidden, b->ld_hidden, b->B, b->D, (uint16_t*)b->d_work};
     const int prev = zs_device_guard_begin(ctx);
-    rc = q4_logits(a, copy ? &x : nullptr, b->dtype, b->group, b->flags & ZS_Q4_MINS, (hipStream_t)stream);
+    rc = q4_logits(a, x.out || x.sums ? &x : nullptr, b->dtype, b->group, b->flags & ZS_Q4_MINS, (hipStream_t)stream);
     zs_device_guard_end(ctx, prev);
     return rc ? zs_set_error(ctx, ZS_EHIP, "%s: launch failed", who) : ZS_OK;
 }

@@ -30,9 +30,12 @@ struct q4_args {
     uint32_t V, D, B;
     const void* hidden;          // rows of 16-bit values at 16 bytes each (planes one behind the other)
     uint64_t ld_h, plane;        // elements
+    const float* sums;           // of groups of more than Q4_FEW rows (q4_x_args)
+    uint32_t Bp;
     float* logits;
     uint64_t ld;
 };
+#define Q4_FEW 16u               // rows up to which each wave makes its operands and sums by itself
 struct q4_pack_args {
     q4_layout at;
     uint32_t V, D, group;
@@ -42,12 +45,28 @@ struct q4_pack_args {
     const void* weight;          // to be quantised
     uint64_t ld_w;
 };
-struct q4_x_args {               // hidden states to rows the kernel takes
+struct q4_x_args {               // hidden states to rows the kernels take
     const void* hidden;
     uint64_t ld_h;
-    uint32_t B, D;
-    uint16_t* out;               // [planes][B][D]
+    uint32_t B, D, group, Bp;
+    float off;                   // what codes are moved by as operands: -24, with minima -16
+    uint16_t* out;               // [planes][B][D], or NULL: they serve as they are
+    float* sums;                 // [D / group][Bp], or NULL
 };
+inline uint32_t q4_bp(uint32_t B) { return (B + 15u) / 16u * 16u + 64u; }   // (a part's last tile of rows may be past B)
+inline uint64_t q4_work(q4_x_args& x, uint32_t dtype, bool copy, void* work) {
+    char* p = (char*)work;
+    const bool wide = dtype == ZS_F32;
+    if (copy || wide) {
+        x.out = (uint16_t*)p;
+        p += hd_pad((uint64_t)x.B * x.D * (wide ? 6u : 2u));
+    }
+    if (x.B > Q4_FEW) {
+        x.sums = (float*)p;
+        p += hd_pad((uint64_t)(x.D / 32u + 4u) * x.Bp * 4u);
+    }
+    return (uint64_t)(p - (char*)work);
+}
 int q4_pack(const q4_pack_args& a, hipStream_t stream);
 int q4_quantize(const q4_pack_args& a, uint32_t dtype, hipStream_t stream);
 int q4_logits(const q4_args& a, const q4_x_args* x, uint32_t dtype, uint32_t group, bool mins, hipStream_t stream);

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 #include "zs_q4.h"
 #include "zs_head.h"
+#include "zs_tile.h"
 
 #define Q4_NT 256
 
@@ -85,19 +86,42 @@ __global__ __launch_bounds__(64) void zs_k_q4_pack(q4_pack_args a) {
 }
 
 // ------------------------------------------------------------------ hidden states
-// Rows at 16 bytes each; f32 as three bf16 whose sum is the value to 2^-26 of it.
-template <int DT>
+// Rows at 16 bytes each where they are not (COPY; f32 as three bf16 whose sum is
+// the value to 2^-26 of it), and their sums over the groups, times what
+// zs_k_q4_batch starts from. One wave a row's 128 columns.
+template <int DT, bool COPY>
 __global__ __launch_bounds__(Q4_NT) void zs_k_q4_rows(q4_x_args a) {
-    const uint64_t n = (uint64_t)a.B * a.D;
-    for (uint64_t i = (uint64_t)blockIdx.x * Q4_NT + threadIdx.x; i < n; i += (uint64_t)gridDim.x * Q4_NT) {
-        const uint64_t r = i / a.D, from = r * a.ld_h + (i - r * a.D);
-        if constexpr (DT == ZS_F32) {
-            uint16_t p[3];
-            zs_split3(((const float*)a.hidden)[from], p);
-            for (int k = 0; k < 3; k++) a.out[k * n + i] = p[k];
-        } else {
-            a.out[i] = ((const uint16_t*)a.hidden)[from];
-        }
+    const uint32_t l = zs_lane(), blocks = (a.D + 127u) / 128u, per = 128u / a.group;
+    const uint64_t n = (uint64_t)a.B * a.D, all = (uint64_t)a.B * blocks;
+    for (uint64_t i = (uint64_t)blockIdx.x * (Q4_NT / 64) + zs_wid(); i < all; i += (uint64_t)gridDim.x * (Q4_NT / 64)) {
+        const uint64_t r = i / blocks;
+        const uint32_t b = (uint32_t)(i - r * blocks), d = b * 128u + l * 2u;
+        const typename hd_elem<DT>::T* x = (const typename hd_elem<DT>::T*)a.hidden + r * a.ld_h + d;
+        float v[2] = {0.0f, 0.0f};
+        if (d < a.D)
+            for (int k = 0; k < 2; k++) {
+                v[k] = hd_float(x[k]);
+                if constexpr (COPY) {
+                    const uint64_t to = r * a.D + d + k;
+                    if constexpr (DT == ZS_F32) {
+                        uint16_t p[3];
+                        zs_split3(v[k], p);
+                        for (int q = 0; q < 3; q++) a.out[q * n + to] = p[q];
+                    } else {
+                        a.out[to] = __builtin_bit_cast(uint16_t, x[k]);
+                    }
+                }
+            }
+        if (!a.sums) continue;
+        double t = (double)v[0] + (double)v[1];
+        t += zs_lane_xor<1>(t);
+        t += zs_lane_xor<2>(t);
+        t += zs_lane_xor<4>(t);
+        t += zs_lane_xor<8>(t);
+        if (a.group > 32u) t += zs_lane_xor<16>(t);
+        if (a.group > 64u) t += zs_lane_xor<32>(t);
+        const uint32_t g = l / (a.group / 2u);
+        if (l % (a.group / 2u) == 0u) a.sums[((uint64_t)b * per + g) * a.Bp + r] = (float)(t * (double)a.off);
     }
 }
 
@@ -111,12 +135,19 @@ struct q4_num {
     static constexpr uint32_t ONE = DT == ZS_F16 ? 6 : 3;                                   // log2 of a unit's bits
     static constexpr uint32_t BASE = DT == ZS_F16 ? 0x4c004c00u : 0x41804180u, MASK = 0x000f000fu << ONE;
     static constexpr uint32_t M16 = DT == ZS_F16 ? 0xcc00cc00u : 0xc180c180u, M24 = DT == ZS_F16 ? 0xce00ce00u : 0xc1c0c1c0u;
-    static __device__ __forceinline__ q4_u4 operand(uint32_t w) {
+    uint32_t mask, base;
+    __device__ __forceinline__ q4_num() {
+        // in a scalar and a vector register, which one and-or takes: of two
+        // literals it takes none, and the compiler makes two instructions of it
+        mask = MASK, base = BASE;
+        asm volatile("" : "+s"(mask), "+v"(base));
+    }
+    __device__ __forceinline__ q4_u4 operand(uint32_t w) const {
         q4_u4 o;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int s = 4 * j - (int)ONE;
-            o[j] = ((s >= 0 ? w >> s : w << -s) & MASK) | BASE;
+            o[j] = ((s >= 0 ? w >> s : w << -s) & mask) | base;
         }
         return o;
     }
@@ -141,6 +172,7 @@ template <int DT, int G, bool MINS, int T>
 __global__ __launch_bounds__(Q4_NT) void zs_k_q4_logits(q4_args a) {
     constexpr int P = DT == ZS_F32 ? 3 : 1, PER = 128 / G, KS = Q4_NT / 64;
     typedef q4_num<DT> num;
+    const num nm;
     __shared__ q4_f4 sh[KS][T][64];
     const uint32_t l = (uint32_t)zs_lane(), w = (uint32_t)__builtin_amdgcn_readfirstlane(zs_wid());
     const uint32_t t0 = blockIdx.x * T, r0 = blockIdx.y * 16u;
@@ -186,7 +218,7 @@ __global__ __launch_bounds__(Q4_NT) void zs_k_q4_logits(q4_args a) {
                 q4_f4 d = c0;
 #pragma unroll
                 for (int k = g * (G / 32); k < (g + 1) * (G / 32); k++) {
-                    const q4_u4 op = num::operand(wv[t][k]);
+                    const q4_u4 op = nm.operand(wv[t][k]);
 #pragma unroll
                     for (int p = P - 1; p >= 0; p--) d = num::mul(xv[p][k], op, d);
                 }
@@ -214,6 +246,161 @@ __global__ __launch_bounds__(Q4_NT) void zs_k_q4_logits(q4_args a) {
     }
 }
 
+// The same for more rows: 16 RT rows by 64 T ids a workgroup, its waves side by
+// side along the ids. The hidden states of 128 columns at a time come to shared
+// memory as operands (lane l's 16 bytes at 16 l), two steps ahead of their use,
+// and the waves' codes and scales to registers likewise.
+template <int DT, int G, bool MINS, int T, int RT>
+struct q4_batch {
+    static constexpr int P = DT == ZS_F32 ? 3 : 1, PER = 128 / G, PIECES = P * RT * 4;
+    static constexpr int LOADS = T * (MINS ? 3 : 2) + P * RT + 1, STAGE = PIECES * 1024 + 1024;
+    typedef q4_num<DT> num;
+    typedef _Float16 hv __attribute__((ext_vector_type(PER)));
+    struct regs {
+        q4_u4 w[T];
+        hv s[T], m[MINS ? T : 1];
+    };
+    const q4_args& a;
+    uint32_t tile[T];
+    const uint16_t* x[RT];
+    const float* sums;
+    uint32_t l, w, kcol;
+    num nm;
+    q4_f4 acc[T][RT];
+
+    __device__ __forceinline__ q4_batch(const q4_args& a_, uint32_t t0, uint32_t r0) : a(a_) {
+        l = (uint32_t)zs_lane();
+        w = (uint32_t)__builtin_amdgcn_readfirstlane(zs_wid());
+        kcol = w * 32u;
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            const uint32_t n = t0 + w * T + t;
+            tile[t] = n < a.at.tiles ? n : a.at.tiles - 1u;
+#pragma unroll
+            for (int r = 0; r < RT; r++) acc[t][r] = q4_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            const uint32_t row = r0 + r * 16u + (l & 15u);
+            x[r] = (const uint16_t*)a.hidden + (row < a.B ? row : a.B - 1u) * a.ld_h + (l >> 4) * 8u;
+        }
+        sums = a.sums + (w % PER) * a.Bp + r0 + (l < 16u * RT ? l : 16u * RT - 1u);
+    }
+    // columns 128 b on, to registers and to shared memory at sh (past the last
+    // column the last 32 again: the scales there are 0)
+    __device__ __forceinline__ void put(uint32_t b, regs& g, tp_lds* sh) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+        b = b < a.at.blocks ? b : a.at.blocks - 1u;
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            const uint64_t at = (uint64_t)tile[t] * a.at.blocks + b;
+            g.w[t] = zs_gload((const q4_u4*)(a.head + at * 1024u + l * 16u));
+            g.s[t] = zs_gload((const hv*)(a.head + a.at.scales + (at * 16u + (l & 15u)) * (PER * 2)));
+            if constexpr (MINS) g.m[t] = zs_gload((const hv*)(a.head + a.at.mins + (at * 16u + (l & 15u)) * (PER * 2)));
+        }
+        uint32_t k = b * 128u + kcol;
+        k = k < a.D ? k : a.D - 32u;
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+                __builtin_amdgcn_global_load_lds((tp_glb*)(x[r] + p * a.plane + k), sh + ((p * RT + r) * 4 + (int)w) * 1024, 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((tp_glb*)(sums + (uint64_t)b * PER * a.Bp), sh + PIECES * 1024 + w * 256u, 4, 0, 0);
+#endif
+    }
+    __device__ __forceinline__ q4_u4 frag(const tp_lds* sh, int p, int r, int k) const {
+        return *(const __attribute__((address_space(3))) q4_u4*)(sh + ((p * RT + r) * 4 + k) * 1024 + l * 16u);
+    }
+    // (the products of a tile are scaled when the next one's are on their way)
+    __device__ __forceinline__ void mul(const regs& g, const tp_lds* sh) {
+#pragma unroll
+        for (int q = 0; q < PER; q++) {
+            q4_f4 c0[RT], d[T][RT];
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+                c0[r] = *(const __attribute__((address_space(3))) q4_f4*)(sh + PIECES * 1024 + q * 256 + r * 64 + (l >> 4) * 16u);
+            auto scaled = [&](int t) {
+                float sf = (float)g.s[t][q];
+                asm volatile("" : "+v"(sf));   // (converted once, not in every product)
+                const float mf = MINS ? (float)g.m[MINS ? t : 0][q] * -0.0625f : 0.0f;
+#pragma unroll
+                for (int r = 0; r < RT; r++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        acc[t][r][i] = __builtin_fmaf(sf, d[t][r][i], acc[t][r][i]);
+                        if (MINS) acc[t][r][i] = __builtin_fmaf(mf, c0[r][i], acc[t][r][i]);
+                    }
+            };
+#pragma unroll
+            for (int k = q * (G / 32); k < (q + 1) * (G / 32); k++) {
+                const bool first = k == q * (G / 32), last = k == (q + 1) * (G / 32) - 1;
+                q4_u4 f[P][RT];
+#pragma unroll
+                for (int p = 0; p < P; p++)
+#pragma unroll
+                    for (int r = 0; r < RT; r++) f[p][r] = frag(sh, p, r, k);
+#pragma unroll
+                for (int t = 0; t < T; t++) {
+                    const q4_u4 op = nm.operand(g.w[t][k]);
+#pragma unroll
+                    for (int p = P - 1; p >= 0; p--)
+#pragma unroll
+                        for (int r = 0; r < RT; r++) d[t][r] = num::mul(f[p][r], op, first && p == P - 1 ? c0[r] : d[t][r]);
+                    if (last && t > 0) scaled(t - 1);
+                }
+                if (last) scaled(T - 1);
+#if defined(__HIP_DEVICE_COMPILE__)
+                if (G > 32) __builtin_amdgcn_sched_barrier(0);   // (the operands of all columns at once do not fit the registers)
+#endif
+            }
+        }
+    }
+    __device__ __forceinline__ void run() {
+        __shared__ char s0_[STAGE], s1_[STAGE], s2_[STAGE];
+        tp_lds *s0 = (tp_lds*)s0_, *s1 = (tp_lds*)s1_, *s2 = (tp_lds*)s2_;
+        regs g0, g1, g2;
+        const uint32_t n = a.at.blocks, whole = n / 3u * 3u;
+        put(0, g0, s0);
+        tp_in_order();
+        put(1, g1, s1);
+        tp_in_order();
+        for (uint32_t b = 0; b < whole; b += 3u) {
+            tp_arrived<LOADS>();
+            put(b + 2u, g2, s2);
+            mul(g0, s0);
+            tp_arrived<LOADS>();
+            put(b + 3u, g0, s0);
+            mul(g1, s1);
+            tp_arrived<LOADS>();
+            put(b + 4u, g1, s1);
+            mul(g2, s2);
+        }
+        tp_arrived<0>();
+        if (n - whole > 0u) mul(g0, s0);
+        if (n - whole > 1u) mul(g1, s1);
+    }
+};
+template <int DT, int G, bool MINS, int T, int RT>
+__global__ __launch_bounds__(Q4_NT, 2) void zs_k_q4_batch(q4_args a, uint32_t parts) {
+    // the parts of the rows next to each other on one XCD, so that a part finds the codes in its L2
+    const uint32_t j = blockIdx.x >> 3, t0 = ((j / parts) * 8u + (blockIdx.x & 7u)) * (4 * T), r0 = j % parts * (16 * RT);
+    if (t0 >= a.at.tiles) return;
+    q4_batch<DT, G, MINS, T, RT> q(a, t0, r0);
+    q.run();
+#pragma unroll
+    for (int t = 0; t < T; t++) {
+        const uint32_t id = (t0 + q.w * T + t) * 16u + (q.l & 15u);
+        if (id >= a.V) continue;
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t row = r0 + r * 16u + (q.l >> 4) * 4u + i;
+                if (row < a.B) a.logits[row * a.ld + id] = q.acc[t][r][i];
+            }
+    }
+}
+
 int q4_pack(const q4_pack_args& a, hipStream_t stream) {
     const uint64_t n = (uint64_t)a.at.tiles * a.at.blocks;
     hipLaunchKernelGGL(zs_k_q4_pack, dim3(n < 65536u ? (uint32_t)n : 65536u), dim3(64), 0, stream, a);
@@ -227,8 +414,25 @@ int q4_quantize(const q4_pack_args& a, uint32_t dtype, hipStream_t stream) {
     else hipLaunchKernelGGL(zs_k_q4_quantize<ZS_BF16>, grid, wg, 0, stream, a);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
+template <int DT, int G, bool MINS, int T, int RT>
+static void q4_batch_go(const q4_args& a, hipStream_t stream) {
+    const uint32_t parts = (a.B + 16u * RT - 1u) / (16u * RT), groups = (a.at.tiles + 4u * T - 1u) / (4u * T);
+    hipLaunchKernelGGL((zs_k_q4_batch<DT, G, MINS, T, RT>), dim3((groups + 7u) / 8u * 8u * parts), dim3(Q4_NT), 0, stream, a, parts);
+}
 template <int DT, int G, bool MINS>
 static void q4_go(const q4_args& a, hipStream_t stream) {
+    if (a.B > 16u) {
+        // tiles a wave such that all workgroups find room at once, two a CU
+        const uint32_t t = (a.at.tiles + 2047u) / 2048u;
+        if constexpr (DT == ZS_F32) q4_batch_go<DT, G, MINS, 2, 2>(a, stream);
+        else if (a.B <= 32u) t <= 2u ? q4_batch_go<DT, G, MINS, 2, 2>(a, stream) : q4_batch_go<DT, G, MINS, 4, 2>(a, stream);
+        else if (a.B > 64u || t == 4u || t > (G == 32 && !MINS ? 5u : 4u)) q4_batch_go<DT, G, MINS, 4, 4>(a, stream);
+        else if (t == 1u) q4_batch_go<DT, G, MINS, 1, 4>(a, stream);
+        else if (t == 2u) q4_batch_go<DT, G, MINS, 2, 4>(a, stream);
+        else if (t == 3u) q4_batch_go<DT, G, MINS, 3, 4>(a, stream);
+        else if constexpr (G == 32 && !MINS) q4_batch_go<DT, G, MINS, 5, 4>(a, stream);
+        return;
+    }
     constexpr int T = 4;
     hipLaunchKernelGGL((zs_k_q4_logits<DT, G, MINS, T>), dim3((a.at.tiles + T - 1u) / T, (a.B + 15u) / 16u), dim3(Q4_NT), 0, stream, a);
 }
@@ -240,10 +444,13 @@ static void q4_group(const q4_args& a, uint32_t group, bool mins, hipStream_t st
 }
 int q4_logits(const q4_args& a, const q4_x_args* x, uint32_t dtype, uint32_t group, bool mins, hipStream_t stream) {
     if (x) {
-        const uint64_t n = ((uint64_t)x->B * x->D + Q4_NT - 1u) / Q4_NT;
+        const uint64_t n = ((uint64_t)x->B * ((x->D + 127u) / 128u) + Q4_NT / 64 - 1u) / (Q4_NT / 64);
         const dim3 grid(n < 4096u ? (uint32_t)n : 4096u), wg(Q4_NT);
-        if (dtype == ZS_F32) hipLaunchKernelGGL(zs_k_q4_rows<ZS_F32>, grid, wg, 0, stream, *x);
-        else hipLaunchKernelGGL(zs_k_q4_rows<ZS_F16>, grid, wg, 0, stream, *x);
+        if (dtype == ZS_F32) hipLaunchKernelGGL((zs_k_q4_rows<ZS_F32, true>), grid, wg, 0, stream, *x);
+        else if (dtype == ZS_F16 && x->out) hipLaunchKernelGGL((zs_k_q4_rows<ZS_F16, true>), grid, wg, 0, stream, *x);
+        else if (dtype == ZS_F16) hipLaunchKernelGGL((zs_k_q4_rows<ZS_F16, false>), grid, wg, 0, stream, *x);
+        else if (x->out) hipLaunchKernelGGL((zs_k_q4_rows<ZS_BF16, true>), grid, wg, 0, stream, *x);
+        else hipLaunchKernelGGL((zs_k_q4_rows<ZS_BF16, false>), grid, wg, 0, stream, *x);
     }
     if (dtype == ZS_F32) q4_group<ZS_F32>(a, group, mins, stream);
     else if (dtype == ZS_F16) q4_group<ZS_F16>(a, group, mins, stream);

@@ -39,6 +39,24 @@ __device__ __forceinline__ tp_acc tp_mfma(tp_s8 a, tp_s8 b, tp_acc c) {
 #endif
 }
 
+// All but the last N of a lane's loads are there, in every wave. (The wait's
+// fields: vector memory N, its two upper bits apart; the others are not waited for.)
+template <int N>
+__device__ __forceinline__ void tp_arrived() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0f70);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#endif
+}
+// Loads are counted: those in front of it are issued before those behind it.
+__device__ __forceinline__ void tp_in_order() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_sched_barrier(0);
+#endif
+}
+
 // One operand of a tile of X rows (m or n): what a lane loads to shared memory
 // and what it reads from there. A step's X x 32 values lie in shared memory as
 // the loads write them, 16 bytes a lane one behind the other; which 16 bytes a
@@ -184,17 +202,6 @@ struct tp_tile {
 #pragma unroll
                 for (int j = 0; j < NT; j++) c[i][j] = tp_mfma<DT>(r.a[i][ks], r.b[j][ks], c[i][j]);
     }
-    // all but the last N of a lane's loads are there, in every wave
-    template <int N>
-    __device__ __forceinline__ static void arrived() {
-#if defined(__HIP_DEVICE_COMPILE__)
-        // (the wait's fields: vector memory N, its two upper bits apart; the other counters are not waited for)
-        __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0f70);
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#endif
-    }
     // the next step's values; past the last the last again, which nobody reads
     __device__ __forceinline__ void put(tp_lds* s) {
         a.load(kt, s);
@@ -226,33 +233,36 @@ struct tp_tile {
         pair = 0;
         planes();
         put(s0);
+        tp_in_order();
         put(s1);
+        tp_in_order();
         put(s2);
-        arrived<2 * LOADS>();
+        tp_in_order();
+        tp_arrived<2 * LOADS>();
         get(s0, r0);
         for (uint32_t k = 0; k < n * PAIRS; k += 4u) {
-            arrived<LOADS>();
+            tp_arrived<LOADS>();
             put(s3);
             get(s1, r1);
             mul(r0, c);
             sched();
-            arrived<LOADS>();
+            tp_arrived<LOADS>();
             put(s0);
             get(s2, r0);
             mul(r1, c);
             sched();
-            arrived<LOADS>();
+            tp_arrived<LOADS>();
             put(s1);
             get(s3, r1);
             mul(r0, c);
             sched();
-            arrived<LOADS>();
+            tp_arrived<LOADS>();
             put(s2);
             get(s0, r0);
             mul(r1, c);
             sched();
         }
-        arrived<0>();
+        tp_arrived<0>();
     }
     // the order of a step's instructions: reads and loads evenly between the products
     template <int I = 0>

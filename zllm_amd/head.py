@@ -36,6 +36,7 @@ _CE = struct.Struct("=4I2Q3QqfI10Q")
 _Q4 = struct.Struct("=4IQ2I6Q")
 assert _CE.size == C.sizeof(Ce) and _Q4.size == C.sizeof(Q4)
 GROUPS = (32, 64, 128)
+_FEW = 16   # rows up to which Q4Head.logits may need no scratch
 
 
 @dataclass(frozen=True)
@@ -216,7 +217,7 @@ class Q4Head:
             raise ValueError(f"{what}: out is float32 [{B}, {self.V}], the values of a row adjacent")
         at, ld = hidden.data_ptr(), _ld(hidden)
         copy = hidden.dtype == torch.float32 or at % 16 != 0 or (B > 1 and ld % 8 != 0)
-        nbytes = _work_bytes("zs_q4_logits_work", B, self.D, DTYPES[hidden.dtype], 1) if copy and B else 0
+        nbytes = _work_bytes("zs_q4_logits_work", B, self.D, DTYPES[hidden.dtype], int(copy)) if copy or B > _FEW else 0
         work, work_at = _work(nbytes, dev)
         raw = _Q4.pack(self.V, self.D, self.group, int(self.mins), self._data.data_ptr(), B, DTYPES[hidden.dtype], at, ld,
                        out.data_ptr(), _ld(out), work_at, nbytes)
