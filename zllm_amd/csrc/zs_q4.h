@@ -6,8 +6,10 @@
 // The head lies in tiles of 16 rows (ids) by 128 columns, one behind the other
 // along the columns, 1 KB each: lane l of a wave has row l % 16 and, of each of
 // four blocks of 32 columns, the eight from (l / 16) * 8 on, as one 32-bit word.
-// A word holds column 2 j in the four bits from 4 j on and column 2 j + 1 in
-// those from 16 + 4 j on, where one shift and one mask make operands of them.
+// Its columns 2 j lie in the four bits from 3 + 4 j on, j < 3, its columns 2 j + 1
+// in those from 19 + 4 j on; column 6 has the bits 15 to 18, column 7 the bits 31
+// and 0 to 2. (Right by 4 j, at the end around, the pair j then stands at bits 3
+// and 19, where a mask makes bf16 operands of it: j = 0 without a shift.)
 // Behind the tiles the scales (f16, 128 / group of a row and tile side by side,
 // rows next to each other), behind those the minima likewise.
 struct q4_layout {

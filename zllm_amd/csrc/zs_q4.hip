@@ -70,7 +70,8 @@ __global__ __launch_bounds__(64) void zs_k_q4_pack(q4_pack_args a) {
             if (v < a.V && c < a.D)
                 for (uint32_t j = 0; j < 4u; j++) {
                     const uint32_t two = a.codes[(v * a.D + c) / 2u + j];
-                    word |= (two & 15u) << (4u * j) | (two >> 4) << (16u + 4u * j);
+                    const uint32_t pair = (two & 15u) << 3 | (two >> 4) << 19;
+                    word |= j ? pair << (4u * j) | pair >> (32u - 4u * j) : pair;
                 }
             o[b] = word;
         }
@@ -126,7 +127,7 @@ __global__ __launch_bounds__(Q4_NT) void zs_k_q4_rows(q4_x_args a) {
 }
 
 // ------------------------------------------------------------------ logits
-// A code q becomes the 16-bit float 16 + q by one shift and one and-or: the
+// A code q becomes the 16-bit float 16 + q by a shift and one and-or: the
 // leading mantissa bits of a number between 16 and 32 count ones. What that adds
 // comes off by the matrix cores too: c0 = sum x * -24 (-16 with minima) is the
 // sum the products start from. Operand register j holds columns 2 j, 2 j + 1.
@@ -146,8 +147,8 @@ struct q4_num {
         q4_u4 o;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const int s = 4 * j - (int)ONE;
-            o[j] = ((s >= 0 ? w >> s : w << -s) & mask) | base;
+            const int r = 4 * j + 3 - (int)ONE;   // to the right, around (only the last pair lies across the ends)
+            o[j] = ((r == 0 ? w : j == 3 ? w >> r | w << (32 - r) : r > 0 ? w >> r : w << -r) & mask) | base;
         }
         return o;
     }
@@ -166,81 +167,126 @@ struct q4_num {
     }
 };
 
-// T tiles of 16 ids by 16 rows of hidden states: each wave takes a part of the
-// columns, their sums are joined through shared memory.
-template <int DT, int G, bool MINS, int T>
-__global__ __launch_bounds__(Q4_NT) void zs_k_q4_logits(q4_args a) {
-    constexpr int P = DT == ZS_F32 ? 3 : 1, PER = 128 / G, KS = Q4_NT / 64;
+// T tiles of 16 ids by up to 16 rows of hidden states: each wave takes a part of
+// the columns, their sums are joined through shared memory. Codes, scales and
+// hidden states of the next 128 columns are on their way while these are used.
+// NI is how many of a lane's four rows there are: row b of the hidden states has
+// place 4 (b % 4) + b / 4 among the operand's, so that up to 4 rows are the first
+// of their lane, up to 8 the first two.
+template <int DT, int G, bool MINS, int T, int NI>
+struct q4_few {
+    static constexpr int P = DT == ZS_F32 ? 3 : 1, PER = 128 / G;
     typedef q4_num<DT> num;
+    typedef _Float16 hv __attribute__((ext_vector_type(PER)));
+    struct regs {
+        q4_u4 w[T], x[P][4];
+        hv s[T], m[MINS ? T : 1];
+    };
+    const q4_args& a;
     const num nm;
-    __shared__ q4_f4 sh[KS][T][64];
-    const uint32_t l = (uint32_t)zs_lane(), w = (uint32_t)__builtin_amdgcn_readfirstlane(zs_wid());
-    const uint32_t t0 = blockIdx.x * T, r0 = blockIdx.y * 16u;
-    const uint32_t b0 = a.at.blocks * w / KS, b1 = a.at.blocks * (w + 1u) / KS;
-    const uint32_t r = r0 + (l & 15u) < a.B ? r0 + (l & 15u) : a.B - 1u;
-    const uint16_t* x = (const uint16_t*)a.hidden + r * a.ld_h + (l >> 4) * 8u;
+    uint64_t tile[T];
+    const uint16_t* x;
+    uint32_t l;
     q4_f4 acc[T];
-#pragma unroll
-    for (int t = 0; t < T; t++) acc[t] = q4_f4{0.0f, 0.0f, 0.0f, 0.0f};
-    const q4_u4 off = {MINS ? num::M16 : num::M24, MINS ? num::M16 : num::M24, MINS ? num::M16 : num::M24, MINS ? num::M16 : num::M24};
-    for (uint32_t b = b0; b < b1; b++) {
-        q4_u4 wv[T], xv[P][4];
-        _Float16 s[T][PER], m[T][PER];
+
+    __device__ __forceinline__ q4_few(const q4_args& a_, uint32_t t0) : a(a_) {
+        l = (uint32_t)zs_lane();
+        const uint32_t r = (l & 3u) * 4u + ((l & 15u) >> 2);
+        x = (const uint16_t*)a.hidden + (r < a.B ? r : a.B - 1u) * a.ld_h + (l >> 4) * 8u;
 #pragma unroll
         for (int t = 0; t < T; t++) {
-            const uint32_t tile = t0 + t < a.at.tiles ? t0 + t : a.at.tiles - 1u;
-            const uint64_t at = (uint64_t)tile * a.at.blocks + b;
-            wv[t] = __builtin_nontemporal_load((const __attribute__((address_space(1))) q4_u4*)(a.head + at * 1024u + l * 16u));
-            const _Float16* sp = (const _Float16*)(a.head + a.at.scales) + (at * 16u + (l & 15u)) * PER;
-            const _Float16* mp = (const _Float16*)(a.head + a.at.mins) + (at * 16u + (l & 15u)) * PER;
-#pragma unroll
-            for (int k = 0; k < PER; k++) {
-                s[t][k] = sp[k];
-                if (MINS) m[t][k] = mp[k];
-            }
-        }
-#pragma unroll
-        for (int p = 0; p < P; p++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                xv[p][k] = q4_u4{0u, 0u, 0u, 0u};
-                if (b * 128u + k * 32u < a.D) xv[p][k] = *(const q4_u4*)(x + p * a.plane + b * 128u + k * 32u);
-            }
-#pragma unroll
-        for (int g = 0; g < PER; g++) {
-            q4_f4 c0 = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int k = g * (G / 32); k < (g + 1) * (G / 32); k++)
-#pragma unroll
-                for (int p = P - 1; p >= 0; p--) c0 = num::mul(xv[p][k], off, c0);
-#pragma unroll
-            for (int t = 0; t < T; t++) {
-                q4_f4 d = c0;
-#pragma unroll
-                for (int k = g * (G / 32); k < (g + 1) * (G / 32); k++) {
-                    const q4_u4 op = nm.operand(wv[t][k]);
-#pragma unroll
-                    for (int p = P - 1; p >= 0; p--) d = num::mul(xv[p][k], op, d);
-                }
-                const float sf = (float)s[t][g], mf = MINS ? (float)m[t][g] * -0.0625f : 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    acc[t][i] = __builtin_fmaf(sf, d[i], acc[t][i]);
-                    if (MINS) acc[t][i] = __builtin_fmaf(mf, c0[i], acc[t][i]);
-                }
-            }
+            tile[t] = (uint64_t)(t0 + t < a.at.tiles ? t0 + t : a.at.tiles - 1u) * a.at.blocks;
+            acc[t] = q4_f4{0.0f, 0.0f, 0.0f, 0.0f};
         }
     }
+    __device__ __forceinline__ void get(uint32_t b, regs& g) const {
 #pragma unroll
-    for (int t = 0; t < T; t++) sh[w][t][l] = acc[t];
+        for (int t = 0; t < T; t++) {
+            const uint64_t at = tile[t] + b;
+            // (not read again)
+            g.w[t] = __builtin_nontemporal_load((const __attribute__((address_space(1))) q4_u4*)(a.head + at * 1024u + l * 16u));
+            g.s[t] = zs_gload((const hv*)(a.head + a.at.scales + (at * 16u + (l & 15u)) * (PER * 2)));
+            if constexpr (MINS) g.m[t] = zs_gload((const hv*)(a.head + a.at.mins + (at * 16u + (l & 15u)) * (PER * 2)));
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            // (past the last column the last 32 again: the scales there are 0)
+            const uint32_t d = b * 128u + k * 32u, at = d < a.D ? d : a.D - 32u;
+#pragma unroll
+            for (int p = 0; p < P; p++) g.x[p][k] = zs_gload((const q4_u4*)(x + p * a.plane + at));
+        }
+    }
+    // (a group's products are scaled when the next group's are on their way)
+    __device__ __forceinline__ void mul(const regs& g) {
+        const uint32_t o = MINS ? num::M16 : num::M24;
+        const q4_u4 off = {o, o, o, o};
+        q4_f4 c0[PER], d[PER][T];
+        auto scaled = [&](int q) {
+#pragma unroll
+            for (int t = 0; t < T; t++) {
+                const float sf = (float)g.s[t][q], mf = MINS ? (float)g.m[MINS ? t : 0][q] * -0.0625f : 0.0f;
+#pragma unroll
+                for (int i = 0; i < NI; i++) {
+                    acc[t][i] = __builtin_fmaf(sf, d[q][t][i], acc[t][i]);
+                    if (MINS) acc[t][i] = __builtin_fmaf(mf, c0[q][i], acc[t][i]);
+                }
+            }
+        };
+#pragma unroll
+        for (int q = 0; q < PER; q++) {
+            c0[q] = q4_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = q * (G / 32); k < (q + 1) * (G / 32); k++)
+#pragma unroll
+                for (int p = P - 1; p >= 0; p--) c0[q] = num::mul(g.x[p][k], off, c0[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < PER; q++) {
+#pragma unroll
+            for (int k = q * (G / 32); k < (q + 1) * (G / 32); k++)
+#pragma unroll
+                for (int t = 0; t < T; t++) {
+                    const q4_u4 op = nm.operand(g.w[t][k]);
+#pragma unroll
+                    for (int p = P - 1; p >= 0; p--) d[q][t] = num::mul(g.x[p][k], op, k == q * (G / 32) && p == P - 1 ? c0[q] : d[q][t]);
+                }
+            if (q > 0) scaled(q - 1);
+        }
+        scaled(PER - 1);
+    }
+    __device__ __forceinline__ void run(uint32_t b0, uint32_t b1) {
+        if (b0 >= b1) return;
+        regs g0, g1;
+        get(b0, g0);
+        tp_in_order();
+        for (; b0 + 1u < b1; b0 += 2u) {
+            get(b0 + 1u, g1);
+            tp_in_order();
+            mul(g0);
+            get(b0 + 2u < b1 ? b0 + 2u : b0 + 1u, g0);
+            tp_in_order();
+            mul(g1);
+        }
+        if (b0 < b1) mul(g0);
+    }
+};
+template <int DT, int G, bool MINS, int T, int KS, int NI>
+__global__ __launch_bounds__(KS * 64) void zs_k_q4_logits(q4_args a) {
+    __shared__ q4_f4 sh[KS][T][64];
+    const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane(zs_wid()), t0 = blockIdx.x * T;
+    q4_few<DT, G, MINS, T, NI> q(a, t0);
+    q.run(a.at.blocks * w / KS, a.at.blocks * (w + 1u) / KS);
+#pragma unroll
+    for (int t = 0; t < T; t++) sh[w][t][q.l] = q.acc[t];
     __syncthreads();
     for (uint32_t t = w; t < T; t += KS) {
-        q4_f4 v = sh[0][t][l];
-        for (int k = 1; k < KS; k++) v += sh[k][t][l];
-        const uint32_t id = (t0 + t) * 16u + (l & 15u);
+        q4_f4 v = sh[0][t][q.l];
+        for (int k = 1; k < KS; k++) v += sh[k][t][q.l];
+        const uint32_t id = (t0 + t) * 16u + (q.l & 15u);
         if (id >= a.V) continue;
-        for (uint32_t i = 0; i < 4u; i++) {
-            const uint32_t row = r0 + (l >> 4) * 4u + i;
+#pragma unroll
+        for (uint32_t i = 0; i < NI; i++) {
+            const uint32_t row = i * 4u + (q.l >> 4);
             if (row < a.B) a.logits[row * a.ld + id] = v[i];
         }
     }
@@ -419,6 +465,14 @@ static void q4_batch_go(const q4_args& a, hipStream_t stream) {
     const uint32_t parts = (a.B + 16u * RT - 1u) / (16u * RT), groups = (a.at.tiles + 4u * T - 1u) / (4u * T);
     hipLaunchKernelGGL((zs_k_q4_batch<DT, G, MINS, T, RT>), dim3((groups + 7u) / 8u * 8u * parts), dim3(Q4_NT), 0, stream, a, parts);
 }
+template <int DT, int G, bool MINS, int KS>
+static void q4_few_go(const q4_args& a, hipStream_t stream) {
+    constexpr int T = 4;
+    const dim3 grid((a.at.tiles + T - 1u) / T), wg(KS * 64);
+    if (a.B <= 4u) hipLaunchKernelGGL((zs_k_q4_logits<DT, G, MINS, T, KS, 1>), grid, wg, 0, stream, a);
+    else if (a.B <= 8u) hipLaunchKernelGGL((zs_k_q4_logits<DT, G, MINS, T, KS, 2>), grid, wg, 0, stream, a);
+    else hipLaunchKernelGGL((zs_k_q4_logits<DT, G, MINS, T, KS, 4>), grid, wg, 0, stream, a);
+}
 template <int DT, int G, bool MINS>
 static void q4_go(const q4_args& a, hipStream_t stream) {
     if (a.B > 16u) {
@@ -433,8 +487,11 @@ static void q4_go(const q4_args& a, hipStream_t stream) {
         else if constexpr (G == 32 && !MINS) q4_batch_go<DT, G, MINS, 5, 4>(a, stream);
         return;
     }
-    constexpr int T = 4;
-    hipLaunchKernelGGL((zs_k_q4_logits<DT, G, MINS, T>), dim3((a.at.tiles + T - 1u) / T, (a.B + 15u) / 16u), dim3(Q4_NT), 0, stream, a);
+    // Waves along the columns where there are few ids: 4 against 1, us, 16 bf16
+    // rows of 4096, groups of 32: 32000 ids 19 and 24 (one row 15 and 19), 65536
+    // ids 38 and 32 (29 and 26), 151936 ids 83 and 84 (65 and 66)
+    if (a.at.tiles < 4096u) q4_few_go<DT, G, MINS, 4>(a, stream);
+    else q4_few_go<DT, G, MINS, 1>(a, stream);
 }
 template <int DT>
 static void q4_group(const q4_args& a, uint32_t group, bool mins, hipStream_t stream) {
