@@ -5,8 +5,9 @@
 #include "zs_head_args.h"
 #include "zs_tile.h"
 
-#define CE_SUB 128          // ids of a row whose exponentials are taken relative to one maximum
-#define CE_TILE 256         // ids, rows or columns of a product's tile
+#define CE_TILE 256         // ids, rows or columns of a product's tile; of few rows:
+#define CE_THIN_M 128       // ids or columns
+#define CE_THIN 64          // rows
 #define CE_ROOM (4ull << 30)   // bytes of exponentials kept at once (a piece of the rows)
 
 #define CE_DH 1u            // the gradient of the hidden states is wanted
@@ -35,20 +36,20 @@ struct ce_args {
     void *dh, *dw;
     uint64_t ld_dh, ld_dw;
     // the plan
-    uint32_t Dp, Vp, R, pieces, subs, splits, split_steps, Dm;
+    uint32_t Dp, Vp, R, pieces, sub, subs, thin, units, Dm;
     uint32_t lo, first, last;    // the piece at hand: its first row; whether it is the first, the last
     // scratch
     ce_state* st;
     uint32_t* idx;               // [N] the rows with a label in order, behind them the others
     float* at;                   // [R] logit of the label
     ce_row* row;                 // [R]
-    float2* stat;                // [R][subs] maximum and sum of exponentials
+    float2* stat;                // [R][subs] of `sub` ids each: maximum and sum of exponentials
     float* fac;                  // [R][subs] of an exponential in the gradient
     uint16_t* h;                 // [planes][R][Dp] rows with a label, zeros behind them
     uint16_t* w;                 // [planes][V][Dp], where the weight itself does not serve
     void* e;                     // [R][Vp] f16 (f32: f32) exponentials
     uint16_t* dl;                // [planes][R][Vp] gradient of the logits (16-bit types: e itself)
-    float* part;                 // [splits][R][Dm]
+    float* part;                 // the hidden states' gradient over parts of the vocabulary (ce_parts)
     float* acc;                  // [V][Dm] the weight's gradient so far (more than one piece)
 };
 int ce_launch(const ce_args& a, uint32_t dtype, hipStream_t stream);
@@ -62,18 +63,18 @@ inline uint64_t ce_work(ce_args& a, uint32_t dtype, void* work) {
     a.Dp = (uint32_t)ce_up(a.D, TP_KROUND);
     a.Vp = (uint32_t)ce_up(a.V, CE_TILE);
     a.Dm = (uint32_t)ce_up(a.D, 4);
-    a.subs = a.Vp / CE_SUB;
+    // A tile of 256 rows is 192 of them for nothing where there are 64: us of the
+    // logits TODO
+    a.thin = a.N <= CE_THIN;
+    a.sub = a.thin ? 32u : 128u;
+    a.subs = a.Vp / a.sub;
     uint64_t R = CE_ROOM / ((uint64_t)a.Vp * (wide ? 10u : 2u)) / CE_TILE * CE_TILE;
     const uint64_t most = grad ? 65280u : 16384u;   // (a launch's y; 1187 parts of 8 bytes a row at 151936 ids)
     if (!grad || R > most) R = most;
     if (R < CE_TILE) R = CE_TILE;
     a.R = (uint32_t)(R < a.N ? R : ce_up(a.N, CE_TILE));
     a.pieces = (uint32_t)((a.N + (uint64_t)a.R - 1u) / a.R);
-    const uint32_t steps = a.Vp / TP_KSTEP, tiles = (uint32_t)(ce_up(a.D, CE_TILE) / CE_TILE * (a.R / CE_TILE));
-    a.splits = tiles >= 256u ? 1u : 256u / tiles;
-    if (a.splits > steps / 16u) a.splits = steps / 16u ? steps / 16u : 1u;
-    a.split_steps = (uint32_t)ce_up((steps + a.splits - 1u) / a.splits, 4);
-    a.splits = (steps + a.split_steps - 1u) / a.split_steps;
+    a.units = a.thin ? 512u : 256u;   // workgroups that fill the card
     char* p = (char*)work;
     auto take = [&](uint64_t bytes) { char* at = p; p += hd_pad(bytes); return (void*)at; };
     a.st = (ce_state*)take(sizeof(ce_state));
@@ -87,7 +88,7 @@ inline uint64_t ce_work(ce_args& a, uint32_t dtype, void* work) {
         a.fac = (float*)take((uint64_t)a.R * a.subs * 4u);
         a.e = take((uint64_t)a.R * a.Vp * (wide ? 4u : 2u));
         a.dl = wide ? (uint16_t*)take(planes * a.R * a.Vp * 2u) : (uint16_t*)a.e;
-        if ((a.want & CE_DH) && a.splits > 1u) a.part = (float*)take((uint64_t)a.splits * a.R * a.Dm * 4u);
+        if (a.want & CE_DH) a.part = (float*)take((uint64_t)a.units * (a.thin ? CE_THIN_M * CE_THIN : CE_TILE * CE_TILE) * 4u);
         if ((a.want & CE_DW) && a.pieces > 1u) a.acc = (float*)take((uint64_t)a.V * a.Dm * 4u);
     }
     return (uint64_t)(p - (char*)work);

@@ -6,9 +6,17 @@
 
 #define CE_NT 256
 
-__device__ __forceinline__ float ce_exp(float x) {   // e^x
+// e^x for x <= 0. The rounding of x log2(e) alone is 2^-24 x of the result, 1e-6 at
+// the -15 of an ordinary tail: nothing beside 16-bit gradients, but of an f32
+// gradient's error the most, which so takes what the product leaves too.
+template <int DT>
+__device__ __forceinline__ float ce_exp(float x) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    return __builtin_amdgcn_exp2f(x * 1.44269504f);
+    constexpr float L = 1.44269504f, L1 = 1.92596299e-8f;   // log2(e) and what f32 leaves of it
+    const float y = x * L, e = __builtin_amdgcn_exp2f(y);
+    if constexpr (DT != ZS_F32) return e;
+    const float r = __builtin_fmaf(x, L1, __builtin_fmaf(x, L, -y));
+    return x > -100.0f ? __builtin_fmaf(e, r * 0.69314718f, e) : e;   // (r is no number at -inf)
 #else
     return x;
 #endif
@@ -127,20 +135,47 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
 }
 
 // The weight in rows of Dp, its planes apart, where its own rows do not serve.
+// A row may begin at any element: 16-bit rows are read as the aligned 16 bytes
+// that hold them, eight values of a row put together from two of those.
 template <int DT>
 __global__ __launch_bounds__(CE_NT) void zs_k_ce_weight(ce_args a) {
     const uint64_t plane = (uint64_t)a.V * a.Dp;
-    for (uint64_t v = blockIdx.x; v < a.V; v += gridDim.x)
-        for (uint32_t d = threadIdx.x; d < a.Dp; d += CE_NT) {
-            uint16_t* o = a.w + v * a.Dp + d;
+    const uint32_t per = a.Dp / 8u;
+    for (uint64_t v = blockIdx.x; v < a.V; v += gridDim.x) {
+        const hd_row<DT> row(a.weight, a.ld_w, v, a.D);
+        for (uint32_t j = threadIdx.x; j < per; j += CE_NT) {
+            uint16_t* o = a.w + v * a.Dp + j * 8u;
+            const uint32_t d0 = j * 8u;
             if constexpr (DT == ZS_F32) {
-                uint16_t p[3];
-                zs_split3(d < a.D ? ce_load<DT>(a.weight, v * a.ld_w + d) : 0.0f, p);
-                for (int k = 0; k < 3; k++) o[k * plane] = p[k];
+                uint16_t p[8][3];
+#pragma unroll
+                for (uint32_t k = 0; k < 8u; k++) zs_split3(d0 + k < a.D ? row.at(d0 + k) : 0.0f, p[k]);
+#pragma unroll
+                for (int q = 0; q < 3; q++) {
+                    hd_u4 u;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) u[k] = (uint32_t)p[2 * k][q] | (uint32_t)p[2 * k + 1][q] << 16;
+                    *(hd_u4*)(o + q * plane) = u;
+                }
             } else {
-                *o = d < a.D ? ((const uint16_t*)a.weight)[v * a.ld_w + d] : (uint16_t)0;
+                const hd_u4 lo = j < row.nvec ? row.raw(j) : hd_row<DT>::none(), hi = j + 1u < row.nvec ? row.raw(j + 1u) : hd_row<DT>::none();
+                const uint32_t w[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                uint32_t u[5];
+                // from word shift / 2 on (the row's own shift: the same for all lanes)
+#pragma unroll
+                for (int k = 0; k < 5; k++) u[k] = row.shift < 2u ? w[k] : row.shift < 4u ? w[k + 1] : row.shift < 6u ? w[k + 2] : w[(k + 3) & 7];
+                hd_u4 x;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    x[k] = row.shift & 1u ? u[k] >> 16 | u[k + 1] << 16 : u[k];
+                    // values past the row are none of it
+                    const uint32_t d = d0 + 2u * k;
+                    x[k] = d + 1u < a.D ? x[k] : d < a.D ? x[k] & 0xffffu : 0u;
+                }
+                *(hd_u4*)o = x;
             }
         }
+    }
 }
 
 template <int DT>
@@ -163,68 +198,83 @@ __device__ __forceinline__ tp_mat ce_mat_dl(const ce_args& a, bool slow) {
     return m;
 }
 
-// Logits of 256 ids (m) and 256 rows (n), of which only what a softmax over the
-// vocabulary needs leaves the registers: per row and 128 ids their maximum and
-// the sum of exponentials relative to it, and for the gradient the exponentials.
-template <int DT, bool GRAD>
-__global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_logits(ce_args a) {
-    typedef tp_tile<DT, 4, 4, 2, false, false> T;
-    const uint32_t n = ce_rows(a);
-    const uint2 at = tp_place(blockIdx.x, a.Vp / CE_TILE, (n + CE_TILE - 1u) / CE_TILE);
-    if (at.x == ~0u) return;
-    const tp_mat mw = ce_mat_w<DT>(a, false), mh = ce_mat_h(a, false);
-    T tile(mw, mh, at.x, at.y);
-    tp_acc c[4][4];
+// The tiles of the products: 256 x 256, or 128 x 64 where there are few rows.
+template <int DT, bool THIN, bool AS, bool BS>
+using ce_tile = tp_tile<DT, THIN ? 1 : 4, THIN ? 2 : 4, THIN ? 4 : 2, AS, BS>;
+template <int MT, int NT>
+__device__ __forceinline__ void ce_none(tp_acc (&c)[MT][NT]) {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+    for (int i = 0; i < MT; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++)
+        for (int j = 0; j < NT; j++)
 #pragma unroll
             for (int q = 0; q < 16; q++) c[i][j][q] = 0.0f;
+}
+__device__ __forceinline__ uint32_t ce_over(uint32_t n, uint32_t d) { return (n + d - 1u) / d; }
+
+// Logits of a tile of ids (m) and rows (n), of which only what a softmax over the
+// vocabulary needs leaves the registers: per row and wave (128 ids, or 32) their
+// maximum and the sum of exponentials relative to it, and for the gradient the
+// exponentials.
+template <int DT, bool GRAD, bool THIN>
+__global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_logits(ce_args a) {
+    typedef ce_tile<DT, THIN, false, false> T;
+    constexpr int MT = T::M, NT = T::N;
+    const uint32_t n = ce_rows(a), mt = a.Vp / T::BM, nt = ce_over(n, T::BN), t = tp_place(blockIdx.x, mt * nt);
+    if (t == ~0u) return;
+    const uint2 at = tp_order(t, mt, nt);
+    const tp_mat mw = ce_mat_w<DT>(a, false), mh = ce_mat_h(a, false);
+    T tile(mw, mh, at.x, at.y);
+    tp_acc c[MT][NT];
+    ce_none(c);
     tile.run(0, a.Dp / TP_KSTEP, c);
-    const uint32_t sub = at.x * 2u + T::wm();
-    if (tile.m0 + CE_TILE > a.V) {
+    const uint32_t sub = at.x * (T::BM / (32 * MT)) + T::wm();
+    if (tile.m0 + T::BM > a.V) {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < MT; i++)
 #pragma unroll
             for (int q = 0; q < 16; q++)
                 if (tile.m_of(i, q / 4) + (uint32_t)(q & 3) >= a.V)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) c[i][j][q] = -INFINITY;
+                    for (int j = 0; j < NT; j++) c[i][j][q] = -INFINITY;
     }
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < NT; j++) {
         const uint32_t r = tile.n_of(j);
         float m = -INFINITY, s = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < MT; i++)
 #pragma unroll
             for (int q = 0; q < 16; q++) m = fmaxf(m, c[i][j][q]);
         m = fmaxf(m, zs_lane_xor<32>(m));
         const float m0 = m > -INFINITY ? m : 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < MT; i++)
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                float e[4];
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    e[k] = ce_exp(c[i][j][4 * q + k] - m0);
-                    s += e[k];
-                }
-                if constexpr (GRAD) {
-                    const uint64_t o = (uint64_t)r * a.Vp + tile.m_of(i, q);
-                    if constexpr (DT == ZS_F32) {
-                        ce_store4<ZS_F32>(a.e, o, e, 4, true);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 4; k++) e[k] *= CE_E_SCALE;
-                        ce_store4<ZS_F16>(a.e, o, e, 4, true);
-                    }
-                }
+            for (int q = 0; q < 16; q++) {
+                c[i][j][q] = ce_exp<DT>(c[i][j][q] - m0);
+                s += c[i][j][q];
             }
+        if constexpr (GRAD && DT == ZS_F32) {
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const float e[4] = {c[i][j][4 * q], c[i][j][4 * q + 1], c[i][j][4 * q + 2], c[i][j][4 * q + 3]};
+                    ce_store4<ZS_F32>(a.e, (uint64_t)r * a.Vp + tile.m_of(i, q), e, 4, true);
+                }
+        }
         s += zs_lane_xor<32>(s);
         if (zs_lane() < 32) a.stat[(uint64_t)r * a.subs + sub] = make_float2(m, s);
+    }
+    if constexpr (GRAD && DT != ZS_F32) {
+        uint16_t* e = (uint16_t*)a.e + (uint64_t)(tile.n0 + T::wn() * (32 * NT)) * a.Vp + tile.m0 + T::wm() * (32 * MT);
+        tile.template rows<false>(
+            [&](int i, int j, int q) {
+                return make_uint2(hd_pack2<ZS_F16>(c[i][j][4 * q] * CE_E_SCALE, c[i][j][4 * q + 1] * CE_E_SCALE),
+                                  hd_pack2<ZS_F16>(c[i][j][4 * q + 2] * CE_E_SCALE, c[i][j][4 * q + 3] * CE_E_SCALE));
+            },
+            [&](uint32_t r, uint32_t m, hd_u4 v) { *(hd_u4*)(e + (uint64_t)r * a.Vp + m) = v; });
     }
 }
 
@@ -243,7 +293,7 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_loss(ce_args a) {
     double s = 0.0;
     for (uint32_t k = t; k < a.subs; k += CE_NT) {
         const float2 v = st[k];
-        s += (double)(v.y * ce_exp(v.x - m0));
+        s += (double)(v.y * ce_exp<DT>(v.x - m0));
     }
     s = block_sum_d<CE_NT>(s, shd);
     const double lse = (double)m0 + log(s), at = (double)a.at[i];
@@ -256,11 +306,13 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_loss(ce_args a) {
         const float g = a.row_grad[r * a.row_grad_stride], k1 = (float)(1.0 + 2.0 * (double)a.zw * lse);
         const float bad = a.row[i].label == ~0u ? NAN : g;
         const float f = bad * k1 * (float)exp((double)m0 - lse);
-        for (uint32_t k = t; k < a.subs; k += CE_NT) a.fac[(uint64_t)i * a.subs + k] = f * ce_exp(st[k].x - m0);
+        for (uint32_t k = t; k < a.subs; k += CE_NT) a.fac[(uint64_t)i * a.subs + k] = f * ce_exp<DT>(st[k].x - m0);
         if (t == 0u) {
             a.row[i].fix = (float)((double)bad * ((double)k1 * exp(at - lse) - 1.0));
             const float top = fabsf(g) * fmaxf(1.0f, fabsf(k1));
-            if (DT == ZS_F16 && top < INFINITY) atomicMax(&a.st->amax, __float_as_uint(top));
+            // (read first: few rows raise the maximum, and the others' atomics on one address would take 17 us of 1350 rows')
+            const uint32_t bits = __float_as_uint(top);
+            if (DT == ZS_F16 && top < INFINITY && bits > __hip_atomic_load(&a.st->amax, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(&a.st->amax, bits);
         }
     }
 }
@@ -275,7 +327,7 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_grad(ce_args a) {
     float x[8];
     if (i < n) {
         const int sh = ce_shift<DT>(a);
-        const float f = ldexpf(a.fac[(uint64_t)i * a.subs + v0 / CE_SUB], sh) * (DT == ZS_F32 ? 1.0f : 1.0f / CE_E_SCALE);
+        const float f = ldexpf(a.fac[(uint64_t)i * a.subs + v0 / a.sub], sh) * (DT == ZS_F32 ? 1.0f : 1.0f / CE_E_SCALE);
         const ce_row row = a.row[i];
         if constexpr (DT == ZS_F32) {
             const float4 u = *(const float4*)((const float*)a.e + at), w = *(const float4*)((const float*)a.e + at + 4);
@@ -310,104 +362,199 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_grad(ce_args a) {
     }
 }
 
-// Gradient of the hidden states, 256 columns (m) of 256 rows (n), over the
-// vocabulary or a part of it.
-template <int DT>
-__global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_dhidden(ce_args a) {
-    typedef tp_tile<DT, 4, 4, 2, true, false> T;
-    const uint32_t n = ce_rows(a), steps = a.Vp / TP_KSTEP, k0 = blockIdx.y * a.split_steps;
-    const uint2 at = tp_place(blockIdx.x, (a.D + CE_TILE - 1u) / CE_TILE, (n + CE_TILE - 1u) / CE_TILE);
-    if (at.x == ~0u) return;
-    const tp_mat mw = ce_mat_w<DT>(a, true), md = ce_mat_dl(a, false);
-    T tile(mw, md, at.x, at.y);
-    tp_acc c[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-            for (int q = 0; q < 16; q++) c[i][j][q] = 0.0f;
-    tile.run(k0, steps - k0 < a.split_steps ? steps - k0 : a.split_steps, c);
-    const float un = ldexpf(1.0f, -ce_shift<DT>(a));
-    const bool vec = a.D % 4u == 0u && a.ld_dh % 4u == 0u && ((uintptr_t)a.dh & 15u) == 0u;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const uint32_t r = tile.n_of(j);
-        if (r >= n) continue;
-        const uint64_t row = a.splits > 1u ? 0u : a.idx[a.lo + r];
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const uint32_t d = tile.m_of(i, q);
-                if (d >= a.D) continue;
-                const float v[4] = {c[i][j][4 * q] * un, c[i][j][4 * q + 1] * un, c[i][j][4 * q + 2] * un, c[i][j][4 * q + 3] * un};
-                if (a.splits > 1u) ce_store4<ZS_F32>(a.part, ((uint64_t)blockIdx.y * a.R + r) * a.Dm + d, v, 4, true);
-                else ce_store4<DT>(a.dh, row * a.ld_dh + d, v, a.D - d, vec);
-            }
+// A gradient's tile of 16-bit values, whole rows at a time: out[row(r)] for the
+// wave's rows r, from column d0 on, columns before D.
+template <int DT, class T, class P, class I>
+__device__ __forceinline__ void ce_out(const T& tile, void* out, uint64_t ld, uint32_t D, uint32_t d0, const P& put, const I& row) {
+    uint16_t* o = (uint16_t*)out;
+    if (D % 8u == 0u && ld % 8u == 0u && ((uintptr_t)out & 15u) == 0u) {
+        tile.template rows<false>(put, [&](uint32_t r, uint32_t m, hd_u4 v) {
+            const uint64_t to = row(r);
+            if (to != ~0ull && d0 + m < D) *(hd_u4*)(o + to * ld + d0 + m) = v;
+        });
+    } else {
+        tile.template rows<true>(put, [&](uint32_t r, uint32_t m, uint16_t v) {
+            const uint64_t to = row(r);
+            if (to != ~0ull && d0 + m < D) o[to * ld + d0 + m] = v;
+        });
     }
 }
-template <int DT>
-__global__ __launch_bounds__(CE_NT) void zs_k_ce_join(ce_args a) {
-    const uint32_t i = blockIdx.x;
-    if (i >= ce_rows(a)) return;
-    const uint64_t r = a.idx[a.lo + i], step = (uint64_t)a.R * a.Dm;
-    const bool vec = a.D % 4u == 0u && a.ld_dh % 4u == 0u && ((uintptr_t)a.dh & 15u) == 0u;
-    for (uint32_t d = threadIdx.x * 4u; d < a.D; d += CE_NT * 4u) {
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t s = 0; s < a.splits; s++) {
-            const float4 p = *(const float4*)(a.part + s * step + (uint64_t)i * a.Dm + d);
-            v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+
+// Into how many parts of the vocabulary the products over it go, so that all CUs
+// have work: with the rows that there are, which the host does not know.
+struct ce_cut {
+    uint32_t mt, nt, parts, steps;   // tiles; parts, of so many steps
+};
+template <class T>
+__device__ __forceinline__ ce_cut ce_parts(const ce_args& a) {
+    ce_cut p;
+    const uint32_t all = a.Vp / TP_KSTEP;
+    p.mt = ce_over(a.D, T::BM);
+    p.nt = ce_over(ce_rows(a), T::BN);
+    const uint32_t tiles = p.mt * p.nt;
+    uint32_t s = tiles ? a.units / tiles : 1u;
+    s = s < all / 16u ? s : all / 16u;
+    s = s ? s : 1u;
+    p.steps = (ce_over(all, s) + 3u) & ~3u;
+    p.parts = ce_over(all, p.steps);
+    return p;
+}
+
+// Gradient of the hidden states, a tile of columns (m) and rows (n), over the
+// vocabulary or a part of it.
+template <int DT, bool THIN>
+__global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_dhidden(ce_args a) {
+    typedef ce_tile<DT, THIN, true, false> T;
+    constexpr int MT = T::M, NT = T::N;
+    const ce_cut p = ce_parts<T>(a);
+    const uint32_t n = ce_rows(a), tiles = p.mt * p.nt, u = tp_place(blockIdx.x, tiles * p.parts);
+    if (u == ~0u) return;
+    const uint32_t part = u / tiles, k0 = part * p.steps, all = a.Vp / TP_KSTEP;
+    const uint2 at = tp_order(u - part * tiles, p.mt, p.nt);
+    const tp_mat mw = ce_mat_w<DT>(a, true), md = ce_mat_dl(a, false);
+    T tile(mw, md, at.x, at.y);
+    tp_acc c[MT][NT];
+    ce_none(c);
+    tile.run(k0, all - k0 < p.steps ? all - k0 : p.steps, c);
+    const float un = ldexpf(1.0f, -ce_shift<DT>(a));
+    if (DT == ZS_F32 || p.parts > 1u) {
+        const bool vec = a.D % 4u == 0u && a.ld_dh % 4u == 0u && ((uintptr_t)a.dh & 15u) == 0u;
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const uint32_t r = tile.n_of(j);
+            if (r >= n) continue;
+            const uint64_t row = p.parts > 1u ? 0u : a.idx[a.lo + r];
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const uint32_t d = tile.m_of(i, q);
+                    if (d >= a.D) continue;
+                    const float v[4] = {c[i][j][4 * q] * un, c[i][j][4 * q + 1] * un, c[i][j][4 * q + 2] * un, c[i][j][4 * q + 3] * un};
+                    if (p.parts > 1u) ce_store4<ZS_F32>(a.part, ((uint64_t)part * (p.nt * T::BN) + r) * a.Dm + d, v, 4, true);
+                    else ce_store4<DT>(a.dh, row * a.ld_dh + d, v, a.D - d, vec);
+                }
         }
-        ce_store4<DT>(a.dh, r * a.ld_dh + d, v, a.D - d, vec);
+        return;
     }
+    if constexpr (DT != ZS_F32) {
+        const uint32_t r0 = tile.n0 + T::wn() * (32 * NT);
+        ce_out<DT>(tile, a.dh, a.ld_dh, a.D, tile.m0 + T::wm() * (32 * MT),
+                   [&](int i, int j, int q) {
+                       return make_uint2(hd_pack2<DT>(c[i][j][4 * q] * un, c[i][j][4 * q + 1] * un),
+                                         hd_pack2<DT>(c[i][j][4 * q + 2] * un, c[i][j][4 * q + 3] * un));
+                   },
+                   [&](uint32_t r) { return r0 + r < n ? (uint64_t)a.idx[a.lo + r0 + r] : ~0ull; });
+    }
+}
+// The parts' sums, a row's 256 columns by 64 threads with four columns each, four
+// times over the parts.
+template <int DT, bool THIN>
+__global__ __launch_bounds__(CE_NT) void zs_k_ce_join(ce_args a) {
+    typedef ce_tile<DT, THIN, true, false> T;
+    __shared__ float4 sh[3][64];
+    const uint32_t i = blockIdx.x, l = threadIdx.x & 63u, w = threadIdx.x >> 6, d = (blockIdx.y * 64u + l) * 4u;
+    const ce_cut p = ce_parts<T>(a);
+    if (i >= ce_rows(a) || p.parts < 2u) return;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (d < a.D) {
+        const float* x = a.part + (uint64_t)i * a.Dm + d;
+        const uint64_t step = (uint64_t)p.nt * T::BN * a.Dm;
+#pragma unroll 4
+        for (uint32_t s = w; s < p.parts; s += 4u) {
+            const float4 y = *(const float4*)(x + s * step);
+            v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+        }
+    }
+    if (w > 0u) sh[w - 1u][l] = v;
+    __syncthreads();
+    if (w > 0u || d >= a.D) return;
+    for (int k = 0; k < 3; k++) {
+        const float4 y = sh[k][l];
+        v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+    }
+    const float o[4] = {v.x, v.y, v.z, v.w};
+    ce_store4<DT>(a.dh, (uint64_t)a.idx[a.lo + i] * a.ld_dh + d, o, a.D - d, a.D % 4u == 0u && a.ld_dh % 4u == 0u && ((uintptr_t)a.dh & 15u) == 0u);
 }
 
 // Gradient of the weight, 256 columns (m) of 256 ids (n), over the piece's rows.
 template <int DT>
 __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_dweight(ce_args a) {
-    typedef tp_tile<DT, 4, 4, 2, true, true> T;
-    const uint32_t n = ce_rows(a);
-    const uint2 at = tp_place(blockIdx.x, (a.D + CE_TILE - 1u) / CE_TILE, a.Vp / CE_TILE);
-    if (at.x == ~0u) return;
+    typedef ce_tile<DT, false, true, true> T;
+    const uint32_t n = ce_rows(a), mt = ce_over(a.D, T::BM), nt = a.Vp / T::BN, t = tp_place(blockIdx.x, mt * nt);
+    if (t == ~0u) return;
+    const uint2 at = tp_order(t, mt, nt);
     const tp_mat mh = ce_mat_h(a, true), md = ce_mat_dl(a, true);
     T tile(mh, md, at.x, at.y);
     tp_acc c[4][4];
+    ce_none(c);
+    tile.run(0, ce_over(n, TP_KROUND) * (TP_KROUND / TP_KSTEP), c);
+    const float un = ldexpf(1.0f, -ce_shift<DT>(a));
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int q = 0; q < 16; q++) c[i][j][q] = 0.0f;
-    tile.run(0, (n + TP_KROUND - 1u) / TP_KROUND * (TP_KROUND / TP_KSTEP), c);
-    const float un = ldexpf(1.0f, -ce_shift<DT>(a));
-    const bool vec = a.D % 4u == 0u && a.ld_dw % 4u == 0u && ((uintptr_t)a.dw & 15u) == 0u;
+            for (int q = 0; q < 16; q++) c[i][j][q] *= un;
+    if (!a.first || !a.last || DT == ZS_F32) {
+        const bool vec = a.D % 4u == 0u && a.ld_dw % 4u == 0u && ((uintptr_t)a.dw & 15u) == 0u;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const uint32_t id = tile.n_of(j);
-        if (id >= a.V) continue;
+        for (int j = 0; j < 4; j++) {
+            const uint32_t id = tile.n_of(j);
+            if (id >= a.V) continue;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const uint32_t d = tile.m_of(i, q);
-                if (d >= a.D) continue;
-                float v[4] = {c[i][j][4 * q] * un, c[i][j][4 * q + 1] * un, c[i][j][4 * q + 2] * un, c[i][j][4 * q + 3] * un};
-                float* acc = a.acc + (uint64_t)id * a.Dm + d;
-                if (!a.first) {
-                    const float4 p = *(const float4*)acc;
-                    v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+                for (int q = 0; q < 4; q++) {
+                    const uint32_t d = tile.m_of(i, q);
+                    if (d >= a.D) continue;
+                    float v[4] = {c[i][j][4 * q], c[i][j][4 * q + 1], c[i][j][4 * q + 2], c[i][j][4 * q + 3]};
+                    float* acc = a.acc + (uint64_t)id * a.Dm + d;
+                    if (!a.first) {
+                        const float4 p = *(const float4*)acc;
+                        v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+                    }
+                    if (!a.last) ce_store4<ZS_F32>(acc, 0, v, 4, true);
+                    else ce_store4<DT>(a.dw, (uint64_t)id * a.ld_dw + d, v, a.D - d, vec);
                 }
-                if (!a.last) ce_store4<ZS_F32>(acc, 0, v, 4, true);
-                else ce_store4<DT>(a.dw, (uint64_t)id * a.ld_dw + d, v, a.D - d, vec);
-            }
+        }
+        return;
+    }
+    if constexpr (DT != ZS_F32) {
+        const uint32_t id0 = tile.n0 + T::wn() * 128u;
+        ce_out<DT>(tile, a.dw, a.ld_dw, a.D, tile.m0 + T::wm() * 128u,
+                   [&](int i, int j, int q) {
+                       return make_uint2(hd_pack2<DT>(c[i][j][4 * q], c[i][j][4 * q + 1]), hd_pack2<DT>(c[i][j][4 * q + 2], c[i][j][4 * q + 3]));
+                   },
+                   [&](uint32_t r) { return id0 + r < a.V ? (uint64_t)(id0 + r) : ~0ull; });
     }
 }
 
+template <int DT, bool THIN>
+static void ce_products(const ce_args& a, hipStream_t stream) {
+    const dim3 wg(CE_NT);
+    const uint32_t bm = THIN ? CE_THIN_M : CE_TILE, rt = THIN ? 1u : a.R / CE_TILE, vt = a.Vp / bm, dt = (a.D + bm - 1u) / bm;
+    const dim3 grid(tp_places(vt * rt));
+    if (!(a.want & (CE_DH | CE_DW))) {
+        hipLaunchKernelGGL((zs_k_ce_logits<DT, false, THIN>), grid, wg, 0, stream, a);
+        hipLaunchKernelGGL((zs_k_ce_loss<DT, false>), dim3(a.R), wg, 0, stream, a);
+        return;
+    }
+    hipLaunchKernelGGL((zs_k_ce_logits<DT, true, THIN>), grid, wg, 0, stream, a);
+    hipLaunchKernelGGL((zs_k_ce_loss<DT, true>), dim3(a.R), wg, 0, stream, a);
+    hipLaunchKernelGGL(zs_k_ce_grad<DT>, dim3((a.Vp / 8u + CE_NT - 1u) / CE_NT, a.R), wg, 0, stream, a);
+    if (a.want & CE_DH) {
+        hipLaunchKernelGGL((zs_k_ce_dhidden<DT, THIN>), dim3(tp_places(dt * rt > a.units ? dt * rt : a.units)), wg, 0, stream, a);
+        hipLaunchKernelGGL((zs_k_ce_join<DT, THIN>), dim3(a.R, (a.D + 255u) / 256u), wg, 0, stream, a);
+    }
+    if (a.want & CE_DW) {
+        const uint32_t tiles = (a.D + CE_TILE - 1u) / CE_TILE * (a.Vp / CE_TILE);
+        hipLaunchKernelGGL(zs_k_ce_dweight<DT>, dim3(tp_places(tiles)), wg, 0, stream, a);
+    }
+}
 template <int DT>
 static void ce_go(ce_args a, hipStream_t stream) {
     const dim3 wg(CE_NT);
-    const uint32_t vt = a.Vp / CE_TILE, dt = (a.D + CE_TILE - 1u) / CE_TILE, rt = a.R / CE_TILE;
     hipLaunchKernelGGL(zs_k_ce_rows, dim3(1), dim3(1024), 0, stream, a);
     if (a.w) hipLaunchKernelGGL(zs_k_ce_weight<DT>, dim3(a.V < 16384u ? a.V : 16384u), wg, 0, stream, a);
     for (uint32_t p = 0; p < a.pieces; p++) {
@@ -415,19 +562,8 @@ static void ce_go(ce_args a, hipStream_t stream) {
         a.first = p == 0u;
         a.last = p + 1u == a.pieces;
         hipLaunchKernelGGL(zs_k_ce_pack<DT>, dim3(a.R), wg, 0, stream, a);
-        if (!(a.want & (CE_DH | CE_DW))) {
-            hipLaunchKernelGGL((zs_k_ce_logits<DT, false>), dim3(tp_places(vt, rt)), wg, 0, stream, a);
-            hipLaunchKernelGGL((zs_k_ce_loss<DT, false>), dim3(a.R), wg, 0, stream, a);
-            continue;
-        }
-        hipLaunchKernelGGL((zs_k_ce_logits<DT, true>), dim3(tp_places(vt, rt)), wg, 0, stream, a);
-        hipLaunchKernelGGL((zs_k_ce_loss<DT, true>), dim3(a.R), wg, 0, stream, a);
-        hipLaunchKernelGGL(zs_k_ce_grad<DT>, dim3((a.Vp / 8u + CE_NT - 1u) / CE_NT, a.R), wg, 0, stream, a);
-        if (a.want & CE_DH) {
-            hipLaunchKernelGGL(zs_k_ce_dhidden<DT>, dim3(tp_places(dt, rt), a.splits), wg, 0, stream, a);
-            if (a.splits > 1u) hipLaunchKernelGGL(zs_k_ce_join<DT>, dim3(a.R), wg, 0, stream, a);
-        }
-        if (a.want & CE_DW) hipLaunchKernelGGL(zs_k_ce_dweight<DT>, dim3(tp_places(dt, vt)), wg, 0, stream, a);
+        if (a.thin) ce_products<DT, true>(a, stream);
+        else ce_products<DT, false>(a, stream);
     }
 }
 int ce_launch(const ce_args& a, uint32_t dtype, hipStream_t stream) {

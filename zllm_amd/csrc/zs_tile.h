@@ -69,10 +69,11 @@ struct tp_side {
     const char* base;
     uint32_t off[SLOW ? 1 : LOADS];
     uint32_t kb, kmax, ld2, left;
-    uint32_t rd[SLOW ? 4 : 2];
+    uint32_t rd[SLOW ? 4 : 2];   // (of rows 32 t on, t < 4; of k 16 s on)
 
     __device__ __forceinline__ void start(const tp_mat& m, uint32_t x0, uint32_t wx) {
         const uint32_t l = (uint32_t)zs_lane(), w = (uint32_t)__builtin_amdgcn_readfirstlane(zs_wid());
+        const uint32_t x1 = first(m, x0);
         ld2 = (uint32_t)m.ld * 2u;
         if constexpr (!SLOW) {
             const uint32_t r = l >> 2;
@@ -82,7 +83,7 @@ struct tp_side {
             for (int i = 0; i < LOADS; i++) {
                 uint32_t row = x0 + (uint32_t)(i * 4) * 16u + w * 16u + r;
                 row = row < m.rows ? row : m.rows - 1u;
-                off[i] = (row - x0) * ld2;
+                off[i] = (row - x1) * ld2;
             }
             const uint32_t rr = l & 31u;
 #pragma unroll
@@ -92,7 +93,7 @@ struct tp_side {
             constexpr uint32_t P = 64u / C;      // rows of a wave's load
             const uint32_t r = w * P + l / C;
             uint32_t c = (l % C) ^ ((r & 3u) << 2);
-            const uint32_t last = (m.rows >> 3) - 1u - (x0 >> 3);
+            const uint32_t last = (m.rows >> 3) - 1u - (x1 >> 3);
             c = c < last ? c : last;
             kb = r;
             off[0] = c * 16u;
@@ -104,8 +105,14 @@ struct tp_side {
         }
     }
     static __device__ __forceinline__ uint32_t swz(uint32_t r) { return ((r >> 1) & 3u) ^ ((r >> 3) & 1u); }
+    // the tile's first row (m or n), or the last there is where it begins behind that
+    static __device__ __forceinline__ uint32_t first(const tp_mat& m, uint32_t x0) {
+        const uint32_t end = SLOW ? m.rows - 8u : m.rows - 1u;
+        return x0 < end ? x0 : end;
+    }
     __device__ __forceinline__ void plane(const tp_mat& m, int p, uint32_t x0) {
-        base = (const char*)m.p[p] + (SLOW ? (uint64_t)x0 * 2u : (uint64_t)x0 * m.ld * 2u);
+        const uint32_t x1 = first(m, x0);
+        base = (const char*)m.p[p] + (SLOW ? (uint64_t)x1 * 2u : (uint64_t)x1 * m.ld * 2u);
     }
     // step kt's values to shared memory at s
     __device__ __forceinline__ void load(uint32_t kt, tp_lds* s) const {
@@ -158,7 +165,7 @@ __device__ __forceinline__ int tp_plane_b(int s) { return (int)(0x010120u >> (4 
 // A tile of BM x BN = (32 MT WM) x (32 NT WN) by four waves, WM along m.
 template <int DT, int MT, int NT, int WM, bool AS, bool BS>
 struct tp_tile {
-    static constexpr int WN = 4 / WM, BM = 32 * MT * WM, BN = 32 * NT * WN;
+    static constexpr int M = MT, N = NT, WN = 4 / WM, BM = 32 * MT * WM, BN = 32 * NT * WN;
     static constexpr int SA = BM * 64, STAGE = (BM + BN) * 64;
     static constexpr int PAIRS = DT == ZS_F32 ? TP_PAIRS : 1;
     typedef tp_side<BM, AS> A;
@@ -181,6 +188,13 @@ struct tp_tile {
     __device__ __forceinline__ tp_tile(const tp_mat& ma_, const tp_mat& mb_, uint32_t m, uint32_t n) : ma(ma_), mb(mb_), m0(m * BM), n0(n * BN) {
         a.start(ma, m0, wm() * (32 * MT));
         b.start(mb, n0, wn() * (32 * NT));
+    }
+    // Four steps' values in shared memory: one that the waves have read, one that
+    // they read, two on their way. (Arrays of their own: the compiler tells from
+    // them that a read does not wait for the later steps' loads.)
+    __device__ __forceinline__ static tp_lds* stage(uint32_t i) {
+        __shared__ char s0_[STAGE], s1_[STAGE], s2_[STAGE], s3_[STAGE];
+        return i == 0u ? (tp_lds*)s0_ : i == 1u ? (tp_lds*)s1_ : i == 2u ? (tp_lds*)s2_ : (tp_lds*)s3_;
     }
     struct regs {
         tp_s8 a[MT][2], b[NT][2];
@@ -221,11 +235,7 @@ struct tp_tile {
     }
     // c += A B over steps k0 .. k0 + n - 1, n a multiple of four
     __device__ __forceinline__ void run(uint32_t k0, uint32_t n, tp_acc (&c)[MT][NT]) {
-        // four steps' values in shared memory: one that the waves have read, one
-        // that they read, two on their way. (Arrays of their own: the compiler
-        // tells from them that a read does not wait for the later steps' loads.)
-        __shared__ char s0_[STAGE], s1_[STAGE], s2_[STAGE], s3_[STAGE];
-        tp_lds *s0 = (tp_lds*)s0_, *s1 = (tp_lds*)s1_, *s2 = (tp_lds*)s2_, *s3 = (tp_lds*)s3_;
+        tp_lds *s0 = stage(0), *s1 = stage(1), *s2 = stage(2), *s3 = stage(3);
         if (n == 0u) return;
         regs r0, r1;
         kt = ka = k0;
@@ -264,6 +274,47 @@ struct tp_tile {
         }
         tp_arrived<0>();
     }
+    // A wave's values as 16-bit numbers, whole rows n at a time. A lane has four
+    // values of 32 rows next to each other's rows, so written from there a row's
+    // 256 bytes would go out in 16-byte pieces (2048 x 1024 x 50257: the logits'
+    // kernel 208 us so, TODO from here). put gives the two words of (i, j, q);
+    // row(r, m, v) takes eight values of the wave's row r from its column m on
+    // or, where EACH, a single one, a row's next to each other.
+    template <bool EACH, class P, class R>
+    __device__ __forceinline__ void rows(const P& put, const R& row) const {
+        constexpr uint32_t C = 4 * MT, B = 64 * MT;   // 16-byte pieces and bytes of a row
+        typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) u2 l2;
+        typedef __attribute__((address_space(3))) u4 l4;
+        typedef __attribute__((address_space(3))) uint16_t l1;
+        static_assert(32 * NT * B <= STAGE, "a wave's values fit a step's memory");
+        tp_lds* s = stage((uint32_t)__builtin_amdgcn_readfirstlane(zs_wid()));
+        const uint32_t l = (uint32_t)zs_lane(), n = l & 31u;
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const uint2 v = put(i, j, q);
+                    tp_lds* at = s + (j * 32u + n) * B + ((i * 4u + q) ^ (n & (C - 1u))) * 16u + (l >> 5) * 8u;
+                    *(l2*)at = u2{v.x, v.y};
+                }
+            if constexpr (EACH) {
+#pragma unroll 4
+                for (uint32_t r = 0; r < 32u; r++)
+                    for (uint32_t m = l; m < 32u * MT; m += 64u)
+                        row(j * 32u + r, m, *(const l1*)(s + (j * 32u + r) * B + ((m >> 3) ^ (r & (C - 1u))) * 16u + (m & 7u) * 2u));
+            } else {
+#pragma unroll
+                for (uint32_t t = 0; t < 32u; t += 64u / C) {
+                    const uint32_t r = t + l / C, c = l % C;
+                    row(j * 32u + r, c * 8u, *(const l4*)(s + (j * 32u + r) * B + (c ^ (r & (C - 1u))) * 16u));
+                }
+            }
+        }
+    }
     // the order of a step's instructions: reads and loads evenly between the products
     template <int I = 0>
     __device__ __forceinline__ static void sched() {
@@ -278,13 +329,16 @@ struct tp_tile {
     }
 };
 
-// Workgroup id's tile of mt x nt (~0: none). Workgroups id, id + 8, ... run on
-// one XCD: each XCD has a run of tiles of its own, in groups of four along m,
-// n by n, so that the tiles in its CUs share their operands in its L2.
-__device__ __forceinline__ uint2 tp_place(uint32_t id, uint32_t mt, uint32_t nt) {
-    const uint32_t all = mt * nt, per = (all + 7u) >> 3, t = (id & 7u) * per + (id >> 3);
-    if ((id >> 3) >= per || t >= all) return make_uint2(~0u, 0u);
+// Workgroup id's place among n pieces of work (~0: none). Workgroups id, id + 8,
+// ... run on one XCD: each XCD has a run of pieces of its own.
+__device__ __forceinline__ uint32_t tp_place(uint32_t id, uint32_t n) {
+    const uint32_t per = (n + 7u) >> 3, t = (id & 7u) * per + (id >> 3);
+    return (id >> 3) >= per || t >= n ? ~0u : t;
+}
+inline uint32_t tp_places(uint32_t n) { return (n + 7u) / 8u * 8u; }
+// Tile t of mt x nt, in groups of four along m, n by n, so that the tiles in an
+// XCD's CUs share their operands in its L2.
+__device__ __forceinline__ uint2 tp_order(uint32_t t, uint32_t mt, uint32_t nt) {
     const uint32_t g = t / (4u * nt), gm = mt - g * 4u < 4u ? mt - g * 4u : 4u, r = t - g * 4u * nt;
     return make_uint2(g * 4u + r % gm, r / gm);
 }
-inline uint32_t tp_places(uint32_t mt, uint32_t nt) { return (mt * nt + 7u) / 8u * 8u; }
