@@ -39,12 +39,13 @@ __device__ __forceinline__ tp_acc tp_mfma(tp_s8 a, tp_s8 b, tp_acc c) {
 #endif
 }
 
-// All but the last N of a lane's loads are there, in every wave. (The wait's
-// fields: vector memory N, its two upper bits apart; the others are not waited for.)
-template <int N>
+// All but the last N of a lane's loads are there, in every wave, and (READ) what
+// the waves have read of shared memory is in their registers. (The wait's fields:
+// vector memory N, its two upper bits apart; LDS; the others are not waited for.)
+template <int N, bool READ = false>
 __device__ __forceinline__ void tp_arrived() {
 #if defined(__HIP_DEVICE_COMPILE__)
-    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0f70);
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | (READ ? 0x0070 : 0x0f70));
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -189,32 +190,27 @@ struct tp_tile {
         a.start(ma, m0, wm() * (32 * MT));
         b.start(mb, n0, wn() * (32 * NT));
     }
-    // Four steps' values in shared memory: one that the waves have read, one that
-    // they read, two on their way. (Arrays of their own: the compiler tells from
-    // them that a read does not wait for the later steps' loads.)
+    // Three steps' values in shared memory: one that the waves read, two on their
+    // way. (Arrays of their own: the compiler tells from them that a read does not
+    // wait for the later steps' loads.)
     __device__ __forceinline__ static tp_lds* stage(uint32_t i) {
-        __shared__ char s0_[STAGE], s1_[STAGE], s2_[STAGE], s3_[STAGE];
-        return i == 0u ? (tp_lds*)s0_ : i == 1u ? (tp_lds*)s1_ : i == 2u ? (tp_lds*)s2_ : (tp_lds*)s3_;
+        __shared__ char s0_[STAGE], s1_[STAGE], s2_[STAGE];
+        return i == 0u ? (tp_lds*)s0_ : i == 1u ? (tp_lds*)s1_ : (tp_lds*)s2_;
     }
-    struct regs {
-        tp_s8 a[MT][2], b[NT][2];
+    struct regs {   // operands of half a step, 16 k
+        tp_s8 a[MT], b[NT];
     };
-    __device__ __forceinline__ void get(const tp_lds* s, regs& r) const {
+    __device__ __forceinline__ void get(const tp_lds* s, int ks, regs& r) const {
 #pragma unroll
-        for (int ks = 0; ks < 2; ks++) {
+        for (int i = 0; i < MT; i++) r.a[i] = a.frag(s, i, ks);
 #pragma unroll
-            for (int i = 0; i < MT; i++) r.a[i][ks] = a.frag(s, i, ks);
-#pragma unroll
-            for (int i = 0; i < NT; i++) r.b[i][ks] = b.frag(s + SA, i, ks);
-        }
+        for (int i = 0; i < NT; i++) r.b[i] = b.frag(s + SA, i, ks);
     }
     __device__ __forceinline__ static void mul(const regs& r, tp_acc (&c)[MT][NT]) {
 #pragma unroll
-        for (int ks = 0; ks < 2; ks++)
+        for (int i = 0; i < MT; i++)
 #pragma unroll
-            for (int i = 0; i < MT; i++)
-#pragma unroll
-                for (int j = 0; j < NT; j++) c[i][j] = tp_mfma<DT>(r.a[i][ks], r.b[j][ks], c[i][j]);
+            for (int j = 0; j < NT; j++) c[i][j] = tp_mfma<DT>(r.a[i], r.b[j], c[i][j]);
     }
     // the next step's values; past the last the last again, which nobody reads
     __device__ __forceinline__ void put(tp_lds* s) {
@@ -233,46 +229,44 @@ struct tp_tile {
         a.plane(ma, PAIRS > 1 ? tp_plane_a(pair) : 0, m0);
         b.plane(mb, PAIRS > 1 ? tp_plane_b(pair) : 0, n0);
     }
-    // c += A B over steps k0 .. k0 + n - 1, n a multiple of four
+    // c += A B over steps k0 .. k0 + n - 1
     __device__ __forceinline__ void run(uint32_t k0, uint32_t n, tp_acc (&c)[MT][NT]) {
-        tp_lds *s0 = stage(0), *s1 = stage(1), *s2 = stage(2), *s3 = stage(3);
+        tp_lds* const s[3] = {stage(0), stage(1), stage(2)};
         if (n == 0u) return;
         regs r0, r1;
         kt = ka = k0;
         kz = k0 + n;
         pair = 0;
         planes();
-        put(s0);
+        put(s[0]);
         tp_in_order();
-        put(s1);
+        put(s[1]);
         tp_in_order();
-        put(s2);
+        put(s[2]);
         tp_in_order();
         tp_arrived<2 * LOADS>();
-        get(s0, r0);
-        for (uint32_t k = 0; k < n * PAIRS; k += 4u) {
-            tp_arrived<LOADS>();
-            put(s3);
-            get(s1, r1);
+        get(s[0], 0, r0);
+        // A step: its first half's products while the second's operands are read;
+        // then the next step's values have arrived and this one's memory is free.
+        auto step = [&](tp_lds* now, tp_lds* next) {
+            get(now, 1, r1);
             mul(r0, c);
-            sched();
-            tp_arrived<LOADS>();
-            put(s0);
-            get(s2, r0);
+            sched<0>();
+            tp_arrived<LOADS, true>();
+            put(now);
+            get(next, 0, r0);
             mul(r1, c);
-            sched();
-            tp_arrived<LOADS>();
-            put(s1);
-            get(s3, r1);
-            mul(r0, c);
-            sched();
-            tp_arrived<LOADS>();
-            put(s2);
-            get(s0, r0);
-            mul(r1, c);
-            sched();
+            sched<LOADS>();
+        };
+        const uint32_t all = n * PAIRS, whole = all / 3u * 3u;
+        for (uint32_t k = 0; k < whole; k += 3u) {
+            step(s[0], s[1]);
+            step(s[1], s[2]);
+            step(s[2], s[0]);
         }
-        tp_arrived<0>();
+        if (all - whole > 0u) step(s[0], s[1]);
+        if (all - whole > 1u) step(s[1], s[2]);
+        tp_arrived<0, true>();
     }
     // A wave's values as 16-bit numbers, whole rows n at a time. A lane has four
     // values of 32 rows next to each other's rows, so written from there a row's
@@ -288,8 +282,9 @@ struct tp_tile {
         typedef __attribute__((address_space(3))) u2 l2;
         typedef __attribute__((address_space(3))) u4 l4;
         typedef __attribute__((address_space(3))) uint16_t l1;
-        static_assert(32 * NT * B <= STAGE, "a wave's values fit a step's memory");
-        tp_lds* s = stage((uint32_t)__builtin_amdgcn_readfirstlane(zs_wid()));
+        static_assert(32 * B <= STAGE / 2, "a wave's values fit its share of the memory");
+        const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane(zs_wid());
+        tp_lds* s = stage(w >> 1) + (w & 1u) * (STAGE / 2);   // (32 rows of the wave's at a time)
         const uint32_t l = (uint32_t)zs_lane(), n = l & 31u;
 #pragma unroll
         for (int j = 0; j < NT; j++) {
@@ -298,33 +293,33 @@ struct tp_tile {
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
                     const uint2 v = put(i, j, q);
-                    tp_lds* at = s + (j * 32u + n) * B + ((i * 4u + q) ^ (n & (C - 1u))) * 16u + (l >> 5) * 8u;
+                    tp_lds* at = s + n * B + ((i * 4u + q) ^ (n & (C - 1u))) * 16u + (l >> 5) * 8u;
                     *(l2*)at = u2{v.x, v.y};
                 }
             if constexpr (EACH) {
 #pragma unroll 4
                 for (uint32_t r = 0; r < 32u; r++)
                     for (uint32_t m = l; m < 32u * MT; m += 64u)
-                        row(j * 32u + r, m, *(const l1*)(s + (j * 32u + r) * B + ((m >> 3) ^ (r & (C - 1u))) * 16u + (m & 7u) * 2u));
+                        row(j * 32u + r, m, *(const l1*)(s + r * B + ((m >> 3) ^ (r & (C - 1u))) * 16u + (m & 7u) * 2u));
             } else {
 #pragma unroll
                 for (uint32_t t = 0; t < 32u; t += 64u / C) {
                     const uint32_t r = t + l / C, c = l % C;
-                    row(j * 32u + r, c * 8u, *(const l4*)(s + (j * 32u + r) * B + (c ^ (r & (C - 1u))) * 16u));
+                    row(j * 32u + r, c * 8u, *(const l4*)(s + r * B + (c ^ (r & (C - 1u))) * 16u));
                 }
             }
         }
     }
-    // the order of a step's instructions: reads and loads evenly between the products
-    template <int I = 0>
+    // the order of half a step's instructions: reads and V loads evenly between the products
+    template <int V, int I = 0>
     __device__ __forceinline__ static void sched() {
 #if defined(__HIP_DEVICE_COMPILE__)
-        constexpr int M = MT * NT * 2, D = MT * 2 * (AS ? 2 : 1) + NT * 2 * (BS ? 2 : 1);
-        constexpr int d = (I + 1) * D / M - I * D / M, v = (I + 1) * LOADS / M - I * LOADS / M;
+        constexpr int M = MT * NT, D = MT * (AS ? 2 : 1) + NT * (BS ? 2 : 1);
+        constexpr int d = (I + 1) * D / M - I * D / M, v = (I + 1) * V / M - I * V / M;
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         if constexpr (d > 0) __builtin_amdgcn_sched_group_barrier(0x100, d, 0);
         if constexpr (v > 0) __builtin_amdgcn_sched_group_barrier(0x020, v, 0);
-        if constexpr (I + 1 < M) sched<I + 1>();
+        if constexpr (I + 1 < M) sched<V, I + 1>();
 #endif
     }
 };
