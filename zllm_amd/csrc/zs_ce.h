@@ -13,11 +13,13 @@
 #define CE_DH 1u            // the gradient of the hidden states is wanted
 #define CE_DW 2u            // the weight's
 #define CE_COPY 4u          // the weight's rows do not begin at 16 bytes each: they are copied
+#define CE_E_SHIFT 15.0f
 #define CE_E_SCALE 32768.0f // exponentials are kept as f16 of e * 2^15: 11 bits down to 2^-29 of their maximum
 
 struct ce_state {           // what the device finds out
     uint32_t rows;          // that have a label
-    uint32_t amax;          // bits of the piece's largest factor of a row's gradient (f16)
+    uint32_t amax[64];      // bits of the piece's largest factors of a row's gradient, of every 64th row (f16; 1350
+                            // rows' atomics on one address took 17 us)
 };
 struct ce_row {             // of a piece
     float fix;              // the gradient at the label

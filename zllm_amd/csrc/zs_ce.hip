@@ -9,17 +9,20 @@
 // e^x for x <= 0. The rounding of x log2(e) alone is 2^-24 x of the result, 1e-6 at
 // the -15 of an ordinary tail: nothing beside 16-bit gradients, but of an f32
 // gradient's error the most, which so takes what the product leaves too.
-template <int DT>
-__device__ __forceinline__ float ce_exp(float x) {
+__device__ __forceinline__ float ce_exp2(float x) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr float L = 1.44269504f, L1 = 1.92596299e-8f;   // log2(e) and what f32 leaves of it
-    const float y = x * L, e = __builtin_amdgcn_exp2f(y);
-    if constexpr (DT != ZS_F32) return e;
-    const float r = __builtin_fmaf(x, L1, __builtin_fmaf(x, L, -y));
-    return x > -100.0f ? __builtin_fmaf(e, r * 0.69314718f, e) : e;   // (r is no number at -inf)
+    return __builtin_amdgcn_exp2f(x);
 #else
     return x;
 #endif
+}
+template <int DT>
+__device__ __forceinline__ float ce_exp(float x) {
+    constexpr float L = 1.44269504f, L1 = 1.92596299e-8f;   // log2(e) and what f32 leaves of it
+    const float y = x * L, e = ce_exp2(y);
+    if constexpr (DT != ZS_F32) return e;
+    const float r = __builtin_fmaf(x, L1, __builtin_fmaf(x, L, -y));
+    return x > -100.0f ? __builtin_fmaf(e, r * 0.69314718f, e) : e;   // (r is no number at -inf)
 }
 // The power of two that brings the piece's gradients of logits to at most 2^15:
 // f16 has few exponents (row weights of 1 / N alone would leave most of a row
@@ -27,7 +30,7 @@ __device__ __forceinline__ float ce_exp(float x) {
 template <int DT>
 __device__ __forceinline__ int ce_shift(const ce_args& a) {
     if constexpr (DT != ZS_F16) return 0;
-    const uint32_t m = a.st->amax;
+    const uint32_t m = zs_wave_reduce(a.st->amax[zs_lane()], [](uint32_t x, uint32_t y) { return max(x, y); });
     if (m == 0u) return 0;
     const int s = 15 - ((int)(m >> 23) - 126);
     return s > 100 ? 100 : s;
@@ -100,7 +103,7 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
     const uint32_t i = blockIdx.x, n = ce_rows(a), t = threadIdx.x;
     const uint64_t plane = (uint64_t)a.R * a.Dp;
     uint16_t* o = a.h + (uint64_t)i * a.Dp;
-    if (i == 0u && t == 0u) a.st->amax = 0u;
+    if (i == 0u && t < 64u) a.st->amax[t] = 0u;
     if (i >= n) {
         if (i < (n + CE_TILE - 1u) / CE_TILE * CE_TILE)
             for (int p = 0; p < (DT == ZS_F32 ? 3 : 1); p++) ce_zero<ZS_F16>(o + p * plane, a.Dp);
@@ -238,43 +241,54 @@ __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_logits(ce_args a) {
 #pragma unroll
                     for (int j = 0; j < NT; j++) c[i][j][q] = -INFINITY;
     }
-#pragma unroll
-    for (int j = 0; j < NT; j++) {
-        const uint32_t r = tile.n_of(j);
-        float m = -INFINITY, s = 0.0f;
+    float m, s;
+    auto largest = [&](int j) {
+        m = -INFINITY;
+        s = 0.0f;
 #pragma unroll
         for (int i = 0; i < MT; i++)
 #pragma unroll
             for (int q = 0; q < 16; q++) m = fmaxf(m, c[i][j][q]);
         m = fmaxf(m, zs_lane_xor<32>(m));
-        const float m0 = m > -INFINITY ? m : 0.0f;
+    };
+    auto part = [&](int j, float unit) {
+        s += zs_lane_xor<32>(s);
+        if (zs_lane() < 32) a.stat[(uint64_t)tile.n_of(j) * a.subs + sub] = make_float2(m, s * unit);
+    };
+    if constexpr (GRAD && DT != ZS_F32) {
+        uint16_t* e = (uint16_t*)a.e + (uint64_t)(tile.n0 + T::wn() * (32 * NT)) * a.Vp + tile.m0 + T::wm() * (32 * MT);
+        tile.template rows<false>(
+            largest,
+            [&](int i, int j, int q) {
+                const float m0 = m > -INFINITY ? m : 0.0f;
+                float x[4];
 #pragma unroll
-        for (int i = 0; i < MT; i++)
+                for (int k = 0; k < 4; k++) {
+                    x[k] = ce_exp2(__builtin_fmaf(c[i][j][4 * q + k] - m0, 1.44269504f, CE_E_SHIFT));
+                    s += x[k];
+                }
+                return make_uint2(hd_pack2<ZS_F16>(x[0], x[1]), hd_pack2<ZS_F16>(x[2], x[3]));
+            },
+            [&](int j) { part(j, 1.0f / CE_E_SCALE); }, [&](uint32_t r, uint32_t v, hd_u4 x) { *(hd_u4*)(e + (uint64_t)r * a.Vp + v) = x; });
+    } else {
 #pragma unroll
-            for (int q = 0; q < 16; q++) {
-                c[i][j][q] = ce_exp<DT>(c[i][j][q] - m0);
-                s += c[i][j][q];
-            }
-        if constexpr (GRAD && DT == ZS_F32) {
+        for (int j = 0; j < NT; j++) {
+            largest(j);
+            const float m0 = m > -INFINITY ? m : 0.0f;
 #pragma unroll
             for (int i = 0; i < MT; i++)
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
-                    const float e[4] = {c[i][j][4 * q], c[i][j][4 * q + 1], c[i][j][4 * q + 2], c[i][j][4 * q + 3]};
-                    ce_store4<ZS_F32>(a.e, (uint64_t)r * a.Vp + tile.m_of(i, q), e, 4, true);
+                    float x[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        x[k] = ce_exp<DT>(c[i][j][4 * q + k] - m0);
+                        s += x[k];
+                    }
+                    if constexpr (GRAD) ce_store4<ZS_F32>(a.e, (uint64_t)tile.n_of(j) * a.Vp + tile.m_of(i, q), x, 4, true);
                 }
+            part(j, 1.0f);
         }
-        s += zs_lane_xor<32>(s);
-        if (zs_lane() < 32) a.stat[(uint64_t)r * a.subs + sub] = make_float2(m, s);
-    }
-    if constexpr (GRAD && DT != ZS_F32) {
-        uint16_t* e = (uint16_t*)a.e + (uint64_t)(tile.n0 + T::wn() * (32 * NT)) * a.Vp + tile.m0 + T::wm() * (32 * MT);
-        tile.template rows<false>(
-            [&](int i, int j, int q) {
-                return make_uint2(hd_pack2<ZS_F16>(c[i][j][4 * q] * CE_E_SCALE, c[i][j][4 * q + 1] * CE_E_SCALE),
-                                  hd_pack2<ZS_F16>(c[i][j][4 * q + 2] * CE_E_SCALE, c[i][j][4 * q + 3] * CE_E_SCALE));
-            },
-            [&](uint32_t r, uint32_t m, hd_u4 v) { *(hd_u4*)(e + (uint64_t)r * a.Vp + m) = v; });
     }
 }
 
@@ -305,14 +319,12 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_loss(ce_args a) {
     if constexpr (GRAD) {
         const float g = a.row_grad[r * a.row_grad_stride], k1 = (float)(1.0 + 2.0 * (double)a.zw * lse);
         const float bad = a.row[i].label == ~0u ? NAN : g;
-        const float f = bad * k1 * (float)exp((double)m0 - lse);
+        const float f = (float)((double)bad * (double)k1 / s);
         for (uint32_t k = t; k < a.subs; k += CE_NT) a.fac[(uint64_t)i * a.subs + k] = f * ce_exp<DT>(st[k].x - m0);
         if (t == 0u) {
             a.row[i].fix = (float)((double)bad * ((double)k1 * exp(at - lse) - 1.0));
             const float top = fabsf(g) * fmaxf(1.0f, fabsf(k1));
-            // (read first: few rows raise the maximum, and the others' atomics on one address would take 17 us of 1350 rows')
-            const uint32_t bits = __float_as_uint(top);
-            if (DT == ZS_F16 && top < INFINITY && bits > __hip_atomic_load(&a.st->amax, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(&a.st->amax, bits);
+            if (DT == ZS_F16 && top < INFINITY) atomicMax(&a.st->amax[i & 63u], __float_as_uint(top));
         }
     }
 }
@@ -322,11 +334,11 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_loss(ce_args a) {
 template <int DT>
 __global__ __launch_bounds__(CE_NT) void zs_k_ce_grad(ce_args a) {
     const uint32_t i = blockIdx.y, n = ce_rows(a), v0 = (blockIdx.x * CE_NT + threadIdx.x) * 8u;
+    const int sh = ce_shift<DT>(a);   // (by whole waves)
     if (i >= (n + TP_KROUND - 1u) / TP_KROUND * TP_KROUND || v0 >= a.Vp) return;
     const uint64_t at = (uint64_t)i * a.Vp + v0;
     float x[8];
     if (i < n) {
-        const int sh = ce_shift<DT>(a);
         const float f = ldexpf(a.fac[(uint64_t)i * a.subs + v0 / a.sub], sh) * (DT == ZS_F32 ? 1.0f : 1.0f / CE_E_SCALE);
         const ce_row row = a.row[i];
         if constexpr (DT == ZS_F32) {
@@ -367,13 +379,14 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_grad(ce_args a) {
 template <int DT, class T, class P, class I>
 __device__ __forceinline__ void ce_out(const T& tile, void* out, uint64_t ld, uint32_t D, uint32_t d0, const P& put, const I& row) {
     uint16_t* o = (uint16_t*)out;
+    const auto none = [](int) {};
     if (D % 8u == 0u && ld % 8u == 0u && ((uintptr_t)out & 15u) == 0u) {
-        tile.template rows<false>(put, [&](uint32_t r, uint32_t m, hd_u4 v) {
+        tile.template rows<false>(none, put, none, [&](uint32_t r, uint32_t m, hd_u4 v) {
             const uint64_t to = row(r);
             if (to != ~0ull && d0 + m < D) *(hd_u4*)(o + to * ld + d0 + m) = v;
         });
     } else {
-        tile.template rows<true>(put, [&](uint32_t r, uint32_t m, uint16_t v) {
+        tile.template rows<true>(none, put, none, [&](uint32_t r, uint32_t m, uint16_t v) {
             const uint64_t to = row(r);
             if (to != ~0ull && d0 + m < D) o[to * ld + d0 + m] = v;
         });
@@ -490,12 +503,14 @@ __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_dweight(ce_args a) {
     ce_none(c);
     tile.run(0, ce_over(n, TP_KROUND) * (TP_KROUND / TP_KSTEP), c);
     const float un = ldexpf(1.0f, -ce_shift<DT>(a));
+    if constexpr (DT == ZS_F16) {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++)
+            for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int q = 0; q < 16; q++) c[i][j][q] *= un;
+                for (int q = 0; q < 16; q++) c[i][j][q] *= un;
+    }
     if (!a.first || !a.last || DT == ZS_F32) {
         const bool vec = a.D % 4u == 0u && a.ld_dw % 4u == 0u && ((uintptr_t)a.dw & 15u) == 0u;
 #pragma unroll

@@ -274,8 +274,9 @@ struct tp_tile {
     // kernel 208 us so, TODO from here). put gives the two words of (i, j, q);
     // row(r, m, v) takes eight values of the wave's row r from its column m on
     // or, where EACH, a single one, a row's next to each other.
-    template <bool EACH, class P, class R>
-    __device__ __forceinline__ void rows(const P& put, const R& row) const {
+    // begin(j) and end(j) come before and behind the values of 32 rows.
+    template <bool EACH, class J, class P, class E, class R>
+    __device__ __forceinline__ void rows(const J& begin, const P& put, const E& end, const R& row) const {
         constexpr uint32_t C = 4 * MT, B = 64 * MT;   // 16-byte pieces and bytes of a row
         typedef uint32_t u2 __attribute__((ext_vector_type(2)));
         typedef uint32_t u4 __attribute__((ext_vector_type(4)));
@@ -288,6 +289,7 @@ struct tp_tile {
         const uint32_t l = (uint32_t)zs_lane(), n = l & 31u;
 #pragma unroll
         for (int j = 0; j < NT; j++) {
+            begin(j);
 #pragma unroll
             for (int i = 0; i < MT; i++)
 #pragma unroll
@@ -296,6 +298,7 @@ struct tp_tile {
                     tp_lds* at = s + n * B + ((i * 4u + q) ^ (n & (C - 1u))) * 16u + (l >> 5) * 8u;
                     *(l2*)at = u2{v.x, v.y};
                 }
+            end(j);
             if constexpr (EACH) {
 #pragma unroll 4
                 for (uint32_t r = 0; r < 32u; r++)
