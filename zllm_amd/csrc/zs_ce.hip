@@ -5,6 +5,7 @@
 #include "zs_head.h"
 
 #define CE_NT 256
+#define CE_SELF 256u   // rows up to which a workgroup goes through all labels by itself
 
 // e^x for x <= 0. The rounding of x log2(e) alone is 2^-24 x of the result, 1e-6 at
 // the -15 of an ordinary tail: nothing beside 16-bit gradients, but of an f32
@@ -100,21 +101,46 @@ __global__ __launch_bounds__(1024) void zs_k_ce_rows(ce_args a) {
 template <int DT>
 __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
     __shared__ double sh[CE_NT / 64];
-    const uint32_t i = blockIdx.x, n = ce_rows(a), t = threadIdx.x;
+    const uint32_t i = blockIdx.x, t = threadIdx.x;
     const uint64_t plane = (uint64_t)a.R * a.Dp;
     uint16_t* o = a.h + (uint64_t)i * a.Dp;
     if (i == 0u && t < 64u) a.st->amax[t] = 0u;
+    uint32_t n, mine = 0;
+    if (a.N <= CE_SELF) {
+        // few rows: each workgroup finds out for itself which row is its own (a launch less)
+        __shared__ uint32_t all, own;
+        if (t < 64u) {
+            uint32_t with = 0;
+            for (uint32_t r0 = 0; r0 < a.N; r0 += 64u) {
+                const uint32_t r = r0 + t;
+                const bool has = r < a.N && a.labels[r] != a.ignore;
+                const uint64_t m = __ballot(has);
+                const uint32_t before = with + (uint32_t)__popcll(m & ((1ull << t) - 1u));
+                if (r < a.N && (has ? before : a.N - 1u - (r - before)) == i) own = r;
+                with += (uint32_t)__popcll(m);
+            }
+            if (t == 0u) all = with;
+        }
+        __syncthreads();
+        n = all;
+        mine = own;
+        if (t == 0u && i < a.N) a.idx[i] = mine;
+        if (t == 0u && i == 0u) a.st->rows = n;
+    } else {
+        n = ce_rows(a);
+        if (a.lo + (uint64_t)i < a.N) mine = a.idx[a.lo + i];
+    }
     if (i >= n) {
         if (i < (n + CE_TILE - 1u) / CE_TILE * CE_TILE)
             for (int p = 0; p < (DT == ZS_F32 ? 3 : 1); p++) ce_zero<ZS_F16>(o + p * plane, a.Dp);
         if (a.lo + (uint64_t)i < a.N) {
-            const uint64_t r = a.idx[a.lo + i];
+            const uint64_t r = mine;
             if (t == 0u) a.loss[r] = a.lse[r] = 0.0f;
             if (a.dh) ce_zero<DT>((char*)a.dh + r * a.ld_dh * (DT == ZS_F32 ? 4u : 2u), a.D);
         }
         return;
     }
-    const uint64_t r = a.idx[a.lo + i];
+    const uint64_t r = mine;
     const int64_t label = a.labels[r];
     const bool bad = label < 0 || label >= (int64_t)a.V;
     const uint64_t hr = r * a.ld_h, wr = (bad ? 0u : (uint64_t)label) * a.ld_w;
@@ -143,16 +169,26 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
 template <int DT>
 __global__ __launch_bounds__(CE_NT) void zs_k_ce_weight(ce_args a) {
     const uint64_t plane = (uint64_t)a.V * a.Dp;
-    const uint32_t per = a.Dp / 8u;
-    for (uint64_t v = blockIdx.x; v < a.V; v += gridDim.x) {
-        const hd_row<DT> row(a.weight, a.ld_w, v, a.D);
-        for (uint32_t j = threadIdx.x; j < per; j += CE_NT) {
+    const uint32_t per = a.Dp / 8u;   // (at most 2^33 of them in all: the ids go over y where they are many)
+    for (uint64_t v0 = (uint64_t)blockIdx.y * 65536u; v0 < a.V; v0 += (uint64_t)gridDim.y * 65536u) {
+        const uint32_t ids = (uint32_t)(a.V - v0 < 65536u ? a.V - v0 : 65536u);
+        for (uint32_t i = blockIdx.x * CE_NT + threadIdx.x; i < ids * per; i += gridDim.x * CE_NT) {
+            const uint64_t v = v0 + i / per;
+            const uint32_t j = i % per;
+            const hd_row<DT> row(a.weight, a.ld_w, v, a.D);
             uint16_t* o = a.w + v * a.Dp + j * 8u;
             const uint32_t d0 = j * 8u;
             if constexpr (DT == ZS_F32) {
                 uint16_t p[8][3];
+                if (d0 + 8u <= a.D) {
+                    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));   // (a row's float4 may lie anywhere)
+                    const f4 x = zs_gload((const f4*)(row.row + d0)), y = zs_gload((const f4*)(row.row + d0 + 4u));
 #pragma unroll
-                for (uint32_t k = 0; k < 8u; k++) zs_split3(d0 + k < a.D ? row.at(d0 + k) : 0.0f, p[k]);
+                    for (int k = 0; k < 4; k++) zs_split3(x[k], p[k]), zs_split3(y[k], p[k + 4]);
+                } else {
+#pragma unroll
+                    for (uint32_t k = 0; k < 8u; k++) zs_split3(d0 + k < a.D ? row.at(d0 + k) : 0.0f, p[k]);
+                }
 #pragma unroll
                 for (int q = 0; q < 3; q++) {
                     hd_u4 u;
@@ -257,7 +293,7 @@ __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_logits(ce_args a) {
     };
     if constexpr (GRAD && DT != ZS_F32) {
         uint16_t* e = (uint16_t*)a.e + (uint64_t)(tile.n0 + T::wn() * (32 * NT)) * a.Vp + tile.m0 + T::wm() * (32 * MT);
-        tile.template rows<false>(
+        tile.rows(
             largest,
             [&](int i, int j, int q) {
                 const float m0 = m > -INFINITY ? m : 0.0f;
@@ -379,17 +415,21 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_grad(ce_args a) {
 template <int DT, class T, class P, class I>
 __device__ __forceinline__ void ce_out(const T& tile, void* out, uint64_t ld, uint32_t D, uint32_t d0, const P& put, const I& row) {
     uint16_t* o = (uint16_t*)out;
-    const auto none = [](int) {};
+    if (d0 >= D) return;
     if (D % 8u == 0u && ld % 8u == 0u && ((uintptr_t)out & 15u) == 0u) {
-        tile.template rows<false>(none, put, none, [&](uint32_t r, uint32_t m, hd_u4 v) {
+        const auto none = [](int) {};
+        tile.rows(none, put, none, [&](uint32_t r, uint32_t m, hd_u4 v) {
             const uint64_t to = row(r);
             if (to != ~0ull && d0 + m < D) *(hd_u4*)(o + to * ld + d0 + m) = v;
         });
     } else {
-        tile.template rows<true>(none, put, none, [&](uint32_t r, uint32_t m, uint16_t v) {
-            const uint64_t to = row(r);
-            if (to != ~0ull && d0 + m < D) o[to * ld + d0 + m] = v;
-        });
+        tile.rows_any(
+            put,
+            [&](uint32_t r) {
+                const uint64_t to = row(r);
+                return to == ~0ull ? (uint16_t*)nullptr : o + to * ld + d0;
+            },
+            D - d0 < 32u * T::M ? D - d0 : 32u * T::M);
     }
 }
 
@@ -490,35 +530,37 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_join(ce_args a) {
     ce_store4<DT>(a.dh, (uint64_t)a.idx[a.lo + i] * a.ld_dh + d, o, a.D - d, a.D % 4u == 0u && a.ld_dh % 4u == 0u && ((uintptr_t)a.dh & 15u) == 0u);
 }
 
-// Gradient of the weight, 256 columns (m) of 256 ids (n), over the piece's rows.
-template <int DT>
-__global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_dweight(ce_args a) {
-    typedef ce_tile<DT, false, true, true> T;
+// Gradient of the weight, a tile of columns (m) of ids (n), over the piece's rows.
+// (Of few rows there is little to multiply and much to write: three workgroups of
+// 128 x 128 a CU.)
+template <int DT, bool THIN>
+__global__ __launch_bounds__(CE_NT, THIN ? 3 : 1) void zs_k_ce_dweight(ce_args a) {
+    typedef tp_tile<DT, THIN ? 2 : 4, THIN ? 2 : 4, 2, true, true> T;
     const uint32_t n = ce_rows(a), mt = ce_over(a.D, T::BM), nt = a.Vp / T::BN, t = tp_place(blockIdx.x, mt * nt);
     if (t == ~0u) return;
     const uint2 at = tp_order(t, mt, nt);
     const tp_mat mh = ce_mat_h(a, true), md = ce_mat_dl(a, true);
     T tile(mh, md, at.x, at.y);
-    tp_acc c[4][4];
+    tp_acc c[T::M][T::N];
     ce_none(c);
     tile.run(0, ce_over(n, TP_KROUND) * (TP_KROUND / TP_KSTEP), c);
     const float un = ldexpf(1.0f, -ce_shift<DT>(a));
     if constexpr (DT == ZS_F16) {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < T::M; i++)
 #pragma unroll
-            for (int j = 0; j < 4; j++)
+            for (int j = 0; j < T::N; j++)
 #pragma unroll
                 for (int q = 0; q < 16; q++) c[i][j][q] *= un;
     }
     if (!a.first || !a.last || DT == ZS_F32) {
         const bool vec = a.D % 4u == 0u && a.ld_dw % 4u == 0u && ((uintptr_t)a.dw & 15u) == 0u;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < T::N; j++) {
             const uint32_t id = tile.n_of(j);
             if (id >= a.V) continue;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < T::M; i++)
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
                     const uint32_t d = tile.m_of(i, q);
@@ -536,8 +578,8 @@ __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_dweight(ce_args a) {
         return;
     }
     if constexpr (DT != ZS_F32) {
-        const uint32_t id0 = tile.n0 + T::wn() * 128u;
-        ce_out<DT>(tile, a.dw, a.ld_dw, a.D, tile.m0 + T::wm() * 128u,
+        const uint32_t id0 = tile.n0 + T::wn() * (32 * T::N);
+        ce_out<DT>(tile, a.dw, a.ld_dw, a.D, tile.m0 + T::wm() * (32 * T::M),
                    [&](int i, int j, int q) {
                        return make_uint2(hd_pack2<DT>(c[i][j][4 * q], c[i][j][4 * q + 1]), hd_pack2<DT>(c[i][j][4 * q + 2], c[i][j][4 * q + 3]));
                    },
@@ -563,15 +605,15 @@ static void ce_products(const ce_args& a, hipStream_t stream) {
         hipLaunchKernelGGL((zs_k_ce_join<DT, THIN>), dim3(a.R, (a.D + 255u) / 256u), wg, 0, stream, a);
     }
     if (a.want & CE_DW) {
-        const uint32_t tiles = (a.D + CE_TILE - 1u) / CE_TILE * (a.Vp / CE_TILE);
-        hipLaunchKernelGGL(zs_k_ce_dweight<DT>, dim3(tp_places(tiles)), wg, 0, stream, a);
+        constexpr uint32_t E = THIN ? CE_THIN_M : CE_TILE;
+        hipLaunchKernelGGL((zs_k_ce_dweight<DT, THIN>), dim3(tp_places((a.D + E - 1u) / E * (a.Vp / E))), wg, 0, stream, a);
     }
 }
 template <int DT>
 static void ce_go(ce_args a, hipStream_t stream) {
     const dim3 wg(CE_NT);
-    hipLaunchKernelGGL(zs_k_ce_rows, dim3(1), dim3(1024), 0, stream, a);
-    if (a.w) hipLaunchKernelGGL(zs_k_ce_weight<DT>, dim3(a.V < 16384u ? a.V : 16384u), wg, 0, stream, a);
+    if (a.N > CE_SELF) hipLaunchKernelGGL(zs_k_ce_rows, dim3(1), dim3(1024), 0, stream, a);
+    if (a.w) hipLaunchKernelGGL(zs_k_ce_weight<DT>, dim3(8192, (a.V + 65535u) / 65536u), wg, 0, stream, a);
     for (uint32_t p = 0; p < a.pieces; p++) {
         a.lo = p * a.R;
         a.first = p == 0u;

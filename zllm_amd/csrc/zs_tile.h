@@ -269,47 +269,70 @@ struct tp_tile {
         tp_arrived<0, true>();
     }
     // A wave's values as 16-bit numbers, whole rows n at a time. A lane has four
-    // values of 32 rows next to each other's rows, so written from there a row's
-    // 256 bytes would go out in 16-byte pieces (2048 x 1024 x 50257: the logits'
-    // kernel 208 us so, TODO from here). put gives the two words of (i, j, q);
-    // row(r, m, v) takes eight values of the wave's row r from its column m on
-    // or, where EACH, a single one, a row's next to each other.
-    // begin(j) and end(j) come before and behind the values of 32 rows.
-    template <bool EACH, class J, class P, class E, class R>
-    __device__ __forceinline__ void rows(const J& begin, const P& put, const E& end, const R& row) const {
-        constexpr uint32_t C = 4 * MT, B = 64 * MT;   // 16-byte pieces and bytes of a row
+    // values of each of its rows, so written from there a row's 256 bytes would go
+    // out in 16-byte pieces. begin(j) and end(j) come before and behind the values
+    // of 32 rows; put(i, j, q) gives the two words of four values.
+    template <uint32_t STEP, bool PLAIN, class P>
+    __device__ __forceinline__ void turn(tp_lds* s, int j, const P& put) const {
         typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) u2 l2;
-        typedef __attribute__((address_space(3))) u4 l4;
-        typedef __attribute__((address_space(3))) uint16_t l1;
-        static_assert(32 * B <= STAGE / 2, "a wave's values fit its share of the memory");
-        const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane(zs_wid());
-        tp_lds* s = stage(w >> 1) + (w & 1u) * (STAGE / 2);   // (32 rows of the wave's at a time)
         const uint32_t l = (uint32_t)zs_lane(), n = l & 31u;
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const uint2 v = put(i, j, q);
+                const uint32_t c = i * 4u + q;
+                *(l2*)(s + n * STEP + (PLAIN ? c : c ^ (n & (4u * MT - 1u))) * 16u + (l >> 5) * 8u) = u2{v.x, v.y};
+            }
+    }
+    __device__ __forceinline__ static tp_lds* mine() {   // the wave's share of the memory, room for 32 rows
+        static_assert(32 * (64 * MT + 16) <= STAGE / 2, "32 rows of a wave's values fit its share of the memory");
+        const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane(zs_wid());
+        return stage(w >> 1) + (w & 1u) * (STAGE / 2);
+    }
+    // row(r, m, v) takes eight values of the wave's row r from its column m on
+    template <class J, class P, class E, class R>
+    __device__ __forceinline__ void rows(const J& begin, const P& put, const E& end, const R& row) const {
+        constexpr uint32_t C = 4 * MT;   // 16-byte pieces of a row
+        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) u4 l4;
+        tp_lds* s = mine();
+        const uint32_t l = (uint32_t)zs_lane();
 #pragma unroll
         for (int j = 0; j < NT; j++) {
             begin(j);
-#pragma unroll
-            for (int i = 0; i < MT; i++)
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const uint2 v = put(i, j, q);
-                    tp_lds* at = s + n * B + ((i * 4u + q) ^ (n & (C - 1u))) * 16u + (l >> 5) * 8u;
-                    *(l2*)at = u2{v.x, v.y};
-                }
+            turn<64 * MT, false>(s, j, put);
             end(j);
-            if constexpr (EACH) {
-#pragma unroll 4
-                for (uint32_t r = 0; r < 32u; r++)
-                    for (uint32_t m = l; m < 32u * MT; m += 64u)
-                        row(j * 32u + r, m, *(const l1*)(s + r * B + ((m >> 3) ^ (r & (C - 1u))) * 16u + (m & 7u) * 2u));
-            } else {
 #pragma unroll
-                for (uint32_t t = 0; t < 32u; t += 64u / C) {
-                    const uint32_t r = t + l / C, c = l % C;
-                    row(j * 32u + r, c * 8u, *(const l4*)(s + r * B + (c ^ (r & (C - 1u))) * 16u));
-                }
+            for (uint32_t t = 0; t < 32u; t += 64u / C) {
+                const uint32_t r = t + l / C, c = l % C;
+                row(j * 32u + r, c * 8u, *(const l4*)(s + r * (64 * MT) + (c ^ (r & (C - 1u))) * 16u));
+            }
+        }
+    }
+    // The same to rows at any element: at(r) is where the wave's row r begins (the
+    // same for all lanes), NULL for none, `count` how many of its values go there. A lane
+    // stores two at a time, from the first that lies at four bytes.
+    template <class P, class R>
+    __device__ __forceinline__ void rows_any(const P& put, const R& at, uint32_t count) const {
+        typedef uint32_t u1 __attribute__((aligned(2)));
+        typedef __attribute__((address_space(3))) u1 l1;
+        constexpr uint32_t STEP = 64 * MT + 16;
+        tp_lds* s = mine();
+        const uint32_t l = (uint32_t)zs_lane();
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            turn<STEP, true>(s, j, put);
+#pragma unroll 4
+            for (uint32_t r = 0; r < 32u; r++) {
+                uint16_t* p = at(j * 32u + r);
+                if (!p) continue;
+                const uint32_t o = (uint32_t)((uintptr_t)p >> 1) & 1u, m = 2u * l + o;
+                const uint32_t v = *(const l1*)(s + r * STEP + m * 2u);
+                if (m + 1u < count) *(uint32_t*)(p + m) = v;
+                else if (m < count) p[m] = (uint16_t)v;
+                if (o && l == 0u) p[0] = *(const __attribute__((address_space(3))) uint16_t*)(s + r * STEP);
             }
         }
     }
