@@ -552,10 +552,14 @@ int zs_distill_loss_grad(zs_ctx* ctx, const zs_distill* args, void* stream);
  *     loss[r] = L - z[label] + z_weight * L^2,   lse[r] = L
  *     d_v = row_grad[r] * ((1 + 2 z_weight L) exp(z_v - L) - [v is the label])
  *     dhidden[r] = sum_v d_v W_v,   dweight_v = sum_r d_v h_r
- * hidden, weight and the gradients are of one type, sums in f32, z in f32 (of
- * f32 operands to 2^-26 of the sum of |h W_v|'s terms per product); d is
- * rounded to the type on its way into the gradients' products (f16: scaled so
- * that its largest factor is near 2^15; f32: kept whole), the gradients once.
+ * hidden, weight and the gradients are of one type, sums in f32. Products of
+ * 16-bit numbers are exact; d is rounded to their type on its way into the
+ * gradients' products (f16: scaled so that its largest factor is near 2^15).
+ * f32 numbers are multiplied as sums of two f16 of the number scaled by a power
+ * of two, of the whole weight, of a row of hidden states and of a row of d: to
+ * 3 * 2^-22 of each product, and a number below 2^-18 of the largest to 2^-40 of
+ * that; in the weight's gradient, whose rows differ in size by any factor, as
+ * sums of three bf16, to 2^-26. The gradients are rounded once.
  * A row whose label is ignore_index has loss, lse and gradient 0, and its
  * hidden state, whatever it holds, is in no sum; a label outside [0, V)
  * otherwise gives NaN. What is not finite comes out as not finite.

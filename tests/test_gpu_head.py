@@ -2,8 +2,8 @@
 in 64 bits, the gradients against differences too.
 
 Tolerances. With A the row's largest sum of |h_d W_vd| over d, a logit is a sum
-of D exact products (f32 operands: of products within 2^-24) added in f32: it is
-within ez = (D + 8) 2^-24 A of itself. The normaliser is the logarithm of a sum
+of D exact products (f32 operands: of products within 3 * 2^-22, two f16 each)
+added in f32: it is within ez = (D + 8) 2^-24 A of itself (f32: D + 20). The normaliser is the logarithm of a sum
 of exponentials, each within 2^-21 + ez, added in chains of 64 at most:
 el = ez + 2^-17. The loss is normaliser - logit of the label + z_weight * its
 square, rounded once: el (1 + 2 z |L|) + ez + 2^-23 |loss|. A gradient of a
@@ -12,7 +12,8 @@ of itself, 16-bit types a rounding of the exponential (2^-11) and of d (EPS)
 more and, below f16's normal numbers, 2^-39 of the largest factor. (Exponentials
 are kept as f16 of 2^15 e, e <= 1: under 2^-29 in steps of 2^-24 / 2^15, so
 within 2^-40, and a factor of at most |g k| takes them to d.) The sums over ids
-or rows are of as many f32 additions as terms, then rounded to the type."""
+or rows are of as many f32 additions as terms (f32 states' gradient: of products
+within 3 * 2^-22), then rounded to the type."""
 import numpy as np
 import pytest
 import torch
@@ -63,7 +64,8 @@ def oracle(h, W, labels, g, z, ignore=-100):
     loss, lse = (torch.zeros(N, dtype=torch.float64, device="cuda") for _ in range(2))
     tl, te = torch.zeros_like(loss), torch.zeros_like(loss)
     loss[keep], lse[keep] = L - yl + z * L * L, L
-    ez = (D + 8) * 2.0 ** -24 * A
+    wide = 12 if dtype == "f32" else 0           # (3 * 2^-22, in 2^-24)
+    ez = (D + 8 + wide) * 2.0 ** -24 * A
     el = ez + 2.0 ** -17
     tl[keep] = el * (1 + 2 * z * L.abs()) + ez + 2.0 ** -23 * loss[keep].abs()
     te[keep] = el + 2.0 ** -23 * L.abs()
@@ -81,7 +83,7 @@ def oracle(h, W, labels, g, z, ignore=-100):
         e += 2.0 ** -39 * (gg.abs() * k.abs().clamp_min(1.0)).max()
     dh, th = torch.zeros((N, D), dtype=torch.float64, device="cuda"), torch.zeros((N, D), dtype=torch.float64, device="cuda")
     dh[keep] = d @ Wd
-    th[keep] = e @ Wd.abs() + V * 2.0 ** -24 * (d.abs() @ Wd.abs())
+    th[keep] = e @ Wd.abs() + (V + wide) * 2.0 ** -24 * (d.abs() @ Wd.abs())
     dw = d.T @ hd
     tw = e.T @ hd.abs() + n * 2.0 ** -24 * (d.abs().T @ hd.abs())
     th += EPS[dtype] * dh.abs() + TINY[dtype]

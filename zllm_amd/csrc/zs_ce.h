@@ -24,7 +24,9 @@ struct ce_state {           // what the device finds out
 struct ce_row {             // of a piece
     float fix;              // the gradient at the label
     uint32_t label;
+    int32_t sh, sd;         // f32: the powers of two that its hidden state and its gradient of the logits are scaled by
 };
+#define CE_MAXIMA 512u      // parts of an f32 weight whose largest numbers are taken
 struct ce_args {
     const void *hidden, *weight;
     uint64_t ld_h, ld_w;
@@ -47,10 +49,12 @@ struct ce_args {
     ce_row* row;                 // [R]
     float2* stat;                // [R][subs] of `sub` ids each: maximum and sum of exponentials
     float* fac;                  // [R][subs] of an exponential in the gradient
-    uint16_t* h;                 // [planes][R][Dp] rows with a label, zeros behind them
-    uint16_t* w;                 // [planes][V][Dp], where the weight itself does not serve
+    uint16_t* h;                 // [R][Dp] rows with a label, zeros behind them (f32: three planes, the weight's gradient's)
+    uint16_t* w;                 // [V][Dp], where the weight itself does not serve (f32: two planes)
     void* e;                     // [R][Vp] f16 (f32: f32) exponentials
-    uint16_t* dl;                // [planes][R][Vp] gradient of the logits (16-bit types: e itself)
+    uint16_t* dl;                // [R][Vp] gradient of the logits, in their place (f32: three planes, the weight's gradient's)
+    uint16_t *h2, *dl2;          // f32: the same as two planes of scaled rows, the logits' and the hidden states' gradient's
+    float* wmax;                 // [CE_MAXIMA] f32: the weight's largest numbers
     float* part;                 // the hidden states' gradient over parts of the vocabulary (ce_parts)
     float* acc;                  // [V][Dm] the weight's gradient so far (more than one piece)
 };
@@ -62,6 +66,7 @@ inline uint64_t ce_up(uint64_t n, uint64_t to) { return (n + to - 1u) / to * to;
 inline uint64_t ce_work(ce_args& a, uint32_t dtype, void* work) {
     const bool wide = dtype == ZS_F32, grad = (a.want & (CE_DH | CE_DW)) != 0;
     const uint64_t planes = wide ? 3u : 1u;
+    const bool dh = (a.want & CE_DH) != 0, dw = (a.want & CE_DW) != 0;
     a.Dp = (uint32_t)ce_up(a.D, TP_KROUND);
     a.Vp = (uint32_t)ce_up(a.V, CE_TILE);
     a.Dm = (uint32_t)ce_up(a.D, 4);
@@ -70,7 +75,7 @@ inline uint64_t ce_work(ce_args& a, uint32_t dtype, void* work) {
     a.thin = a.N <= CE_THIN;
     a.sub = a.thin ? 32u : 128u;
     a.subs = a.Vp / a.sub;
-    uint64_t R = CE_ROOM / ((uint64_t)a.Vp * (wide ? 10u : 2u)) / CE_TILE * CE_TILE;
+    uint64_t R = CE_ROOM / ((uint64_t)a.Vp * (wide ? 4u + (dw ? 6u : 0u) + (dh ? 4u : 0u) : 2u)) / CE_TILE * CE_TILE;
     const uint64_t most = grad ? 65280u : 16384u;   // (a launch's y; 1187 parts of 8 bytes a row at 151936 ids)
     if (!grad || R > most) R = most;
     if (R < CE_TILE) R = CE_TILE;
@@ -84,14 +89,19 @@ inline uint64_t ce_work(ce_args& a, uint32_t dtype, void* work) {
     a.at = (float*)take(a.R * 4ull);
     a.row = (ce_row*)take(a.R * sizeof(ce_row));
     a.stat = (float2*)take((uint64_t)a.R * a.subs * 8u);
-    a.h = (uint16_t*)take(planes * a.R * a.Dp * 2u);
-    if (wide || (a.want & CE_COPY)) a.w = (uint16_t*)take(planes * a.V * a.Dp * 2u);
+    if (!wide || dw) a.h = (uint16_t*)take(planes * a.R * a.Dp * 2u);
+    if (wide || (a.want & CE_COPY)) a.w = (uint16_t*)take((wide ? 2u : 1u) * (uint64_t)a.V * a.Dp * 2u);
+    if (wide) {
+        a.h2 = (uint16_t*)take(2u * (uint64_t)a.R * a.Dp * 2u);
+        a.wmax = (float*)take(CE_MAXIMA * 4u);
+    }
     if (grad) {
         a.fac = (float*)take((uint64_t)a.R * a.subs * 4u);
         a.e = take((uint64_t)a.R * a.Vp * (wide ? 4u : 2u));
-        a.dl = wide ? (uint16_t*)take(planes * a.R * a.Vp * 2u) : (uint16_t*)a.e;
-        if (a.want & CE_DH) a.part = (float*)take((uint64_t)a.units * (a.thin ? CE_THIN_M * CE_THIN : CE_TILE * CE_TILE) * 4u);
-        if ((a.want & CE_DW) && a.pieces > 1u) a.acc = (float*)take((uint64_t)a.V * a.Dm * 4u);
+        a.dl = !wide ? (uint16_t*)a.e : dw ? (uint16_t*)take(planes * a.R * a.Vp * 2u) : nullptr;
+        if (wide && dh) a.dl2 = (uint16_t*)take(2u * (uint64_t)a.R * a.Vp * 2u);
+        if (dh) a.part = (float*)take((uint64_t)a.units * (a.thin ? CE_THIN_M * CE_THIN : CE_TILE * CE_TILE) * 4u);
+        if (dw && a.pieces > 1u) a.acc = (float*)take((uint64_t)a.V * a.Dm * 4u);
     }
     return (uint64_t)(p - (char*)work);
 }

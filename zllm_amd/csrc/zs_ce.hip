@@ -101,6 +101,7 @@ __global__ __launch_bounds__(1024) void zs_k_ce_rows(ce_args a) {
 template <int DT>
 __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
     __shared__ double sh[CE_NT / 64];
+    __shared__ float shf[CE_NT / 64];
     const uint32_t i = blockIdx.x, t = threadIdx.x;
     const uint64_t plane = (uint64_t)a.R * a.Dp;
     uint16_t* o = a.h + (uint64_t)i * a.Dp;
@@ -131,8 +132,14 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
         if (a.lo + (uint64_t)i < a.N) mine = a.idx[a.lo + i];
     }
     if (i >= n) {
-        if (i < (n + CE_TILE - 1u) / CE_TILE * CE_TILE)
-            for (int p = 0; p < (DT == ZS_F32 ? 3 : 1); p++) ce_zero<ZS_F16>(o + p * plane, a.Dp);
+        if (i < (n + CE_TILE - 1u) / CE_TILE * CE_TILE) {
+            if (a.h)
+                for (int p = 0; p < (DT == ZS_F32 ? 3 : 1); p++) ce_zero<ZS_F16>(o + p * plane, a.Dp);
+            if constexpr (DT == ZS_F32) {
+                for (int p = 0; p < 2; p++) ce_zero<ZS_F16>(a.h2 + p * plane + (uint64_t)i * a.Dp, a.Dp);
+                if (t == 0u) a.row[i].sh = 0;
+            }
+        }
         if (a.lo + (uint64_t)i < a.N) {
             const uint64_t r = mine;
             if (t == 0u) a.loss[r] = a.lse[r] = 0.0f;
@@ -145,12 +152,23 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
     const bool bad = label < 0 || label >= (int64_t)a.V;
     const uint64_t hr = r * a.ld_h, wr = (bad ? 0u : (uint64_t)label) * a.ld_w;
     double dot = 0.0;
+    int sh2 = 0;
+    if constexpr (DT == ZS_F32) {
+        float top = 0.0f;
+        for (uint32_t d = t; d < a.D; d += CE_NT) top = fmaxf(top, fabsf(ce_load<DT>(a.hidden, hr + d)));
+        sh2 = zs_split2_of(block_max_f<CE_NT>(top, shf));
+        if (t == 0u) a.row[i].sh = sh2;
+    }
     for (uint32_t d = t; d < a.Dp; d += CE_NT) {
         const float x = d < a.D ? ce_load<DT>(a.hidden, hr + d) : 0.0f;
         if constexpr (DT == ZS_F32) {
-            uint16_t p[3];
-            zs_split3(x, p);
-            for (int k = 0; k < 3; k++) o[k * plane + d] = p[k];
+            uint16_t p[3], p2[2];
+            if (a.h) {
+                zs_split3(x, p);
+                for (int k = 0; k < 3; k++) o[k * plane + d] = p[k];
+            }
+            zs_split2(x, sh2, p2);
+            for (int k = 0; k < 2; k++) a.h2[k * plane + (uint64_t)i * a.Dp + d] = p2[k];
         } else {
             o[d] = d < a.D ? ((const uint16_t*)a.hidden)[hr + d] : (uint16_t)0;
         }
@@ -163,12 +181,39 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
     }
 }
 
+// The largest numbers of the parts of an f32 weight, and by them the power of two
+// that it is scaled by.
+__global__ __launch_bounds__(CE_NT) void zs_k_ce_max(ce_args a) {
+    __shared__ float sh[CE_NT / 64];
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));   // (a row's float4 may lie anywhere)
+    float top = 0.0f;
+    for (uint64_t v = blockIdx.x * (CE_NT / 64) + zs_wid(); v < a.V; v += CE_MAXIMA * (CE_NT / 64)) {
+        const float* row = (const float*)a.weight + v * a.ld_w;
+        const uint32_t whole = a.D & ~3u;
+#pragma unroll 4
+        for (uint32_t d = zs_lane() * 4u; d < whole; d += 256u) {
+            const f4 x = zs_gload((const f4*)(row + d));
+            top = fmaxf(top, fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+        }
+        if (whole + zs_lane() < a.D) top = fmaxf(top, fabsf(row[whole + zs_lane()]));
+    }
+    top = block_max_f<CE_NT>(top, sh);
+    if (threadIdx.x == 0u) a.wmax[blockIdx.x] = top;
+}
+__device__ __forceinline__ int ce_weight_shift(const ce_args& a) {   // (by whole waves)
+    float top = 0.0f;
+#pragma unroll
+    for (uint32_t k = 0; k < CE_MAXIMA / 64u; k++) top = fmaxf(top, a.wmax[k * 64u + zs_lane()]);
+    return zs_split2_of(wave_max_f(top));
+}
 // The weight in rows of Dp, its planes apart, where its own rows do not serve.
 // A row may begin at any element: 16-bit rows are read as the aligned 16 bytes
 // that hold them, eight values of a row put together from two of those.
 template <int DT>
 __global__ __launch_bounds__(CE_NT) void zs_k_ce_weight(ce_args a) {
     const uint64_t plane = (uint64_t)a.V * a.Dp;
+    int sw = 0;
+    if constexpr (DT == ZS_F32) sw = ce_weight_shift(a);
     const uint32_t per = a.Dp / 8u;   // (at most 2^33 of them in all: the ids go over y where they are many)
     for (uint64_t v0 = (uint64_t)blockIdx.y * 65536u; v0 < a.V; v0 += (uint64_t)gridDim.y * 65536u) {
         const uint32_t ids = (uint32_t)(a.V - v0 < 65536u ? a.V - v0 : 65536u);
@@ -179,18 +224,18 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_weight(ce_args a) {
             uint16_t* o = a.w + v * a.Dp + j * 8u;
             const uint32_t d0 = j * 8u;
             if constexpr (DT == ZS_F32) {
-                uint16_t p[8][3];
+                uint16_t p[8][2];
                 if (d0 + 8u <= a.D) {
                     typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));   // (a row's float4 may lie anywhere)
                     const f4 x = zs_gload((const f4*)(row.row + d0)), y = zs_gload((const f4*)(row.row + d0 + 4u));
 #pragma unroll
-                    for (int k = 0; k < 4; k++) zs_split3(x[k], p[k]), zs_split3(y[k], p[k + 4]);
+                    for (int k = 0; k < 4; k++) zs_split2(x[k], sw, p[k]), zs_split2(y[k], sw, p[k + 4]);
                 } else {
 #pragma unroll
-                    for (uint32_t k = 0; k < 8u; k++) zs_split3(d0 + k < a.D ? row.at(d0 + k) : 0.0f, p[k]);
+                    for (uint32_t k = 0; k < 8u; k++) zs_split2(d0 + k < a.D ? row.at(d0 + k) : 0.0f, sw, p[k]);
                 }
 #pragma unroll
-                for (int q = 0; q < 3; q++) {
+                for (int q = 0; q < 2; q++) {
                     hd_u4 u;
 #pragma unroll
                     for (int k = 0; k < 4; k++) u[k] = (uint32_t)p[2 * k][q] | (uint32_t)p[2 * k + 1][q] << 16;
@@ -226,20 +271,26 @@ __device__ __forceinline__ tp_mat ce_mat_w(const ce_args& a, bool slow) {
     tp_mat m = {{p, p + plane, p + 2 * plane}, own ? a.Dp : a.ld_w, slow ? d : a.V, slow ? a.V : d};
     return m;
 }
+// (f32: the weight's gradient, whose rows of the other operands differ in size by any
+// factor, by three planes each; the others by two)
+template <int DT>
 __device__ __forceinline__ tp_mat ce_mat_h(const ce_args& a, bool slow) {
     const uint64_t plane = (uint64_t)a.R * a.Dp;
-    tp_mat m = {{a.h, a.h + plane, a.h + 2 * plane}, a.Dp, slow ? a.Dp : a.R, slow ? a.R : a.Dp};
+    const uint16_t* p = DT == ZS_F32 && !slow ? a.h2 : a.h;
+    tp_mat m = {{p, p + plane, p + 2 * plane}, a.Dp, slow ? a.Dp : a.R, slow ? a.R : a.Dp};
     return m;
 }
+template <int DT>
 __device__ __forceinline__ tp_mat ce_mat_dl(const ce_args& a, bool slow) {
     const uint64_t plane = (uint64_t)a.R * a.Vp;
-    tp_mat m = {{a.dl, a.dl + plane, a.dl + 2 * plane}, a.Vp, slow ? a.Vp : a.R, slow ? a.R : a.Vp};
+    const uint16_t* p = DT == ZS_F32 && !slow ? a.dl2 : a.dl;
+    tp_mat m = {{p, p + plane, p + 2 * plane}, a.Vp, slow ? a.Vp : a.R, slow ? a.R : a.Vp};
     return m;
 }
 
 // The tiles of the products: 256 x 256, or 128 x 64 where there are few rows.
 template <int DT, bool THIN, bool AS, bool BS>
-using ce_tile = tp_tile<DT, THIN ? 1 : 4, THIN ? 2 : 4, THIN ? 4 : 2, AS, BS>;
+using ce_tile = tp_tile<DT == ZS_F32 ? TP_TWO : DT, THIN ? 1 : 4, THIN ? 2 : 4, THIN ? 4 : 2, AS, BS>;
 template <int MT, int NT>
 __device__ __forceinline__ void ce_none(tp_acc (&c)[MT][NT]) {
 #pragma unroll
@@ -262,11 +313,22 @@ __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_logits(ce_args a) {
     const uint32_t n = ce_rows(a), mt = a.Vp / T::BM, nt = ce_over(n, T::BN), t = tp_place(blockIdx.x, mt * nt);
     if (t == ~0u) return;
     const uint2 at = tp_order(t, mt, nt);
-    const tp_mat mw = ce_mat_w<DT>(a, false), mh = ce_mat_h(a, false);
+    const tp_mat mw = ce_mat_w<DT>(a, false), mh = ce_mat_h<DT>(a, false);
     T tile(mw, mh, at.x, at.y);
     tp_acc c[MT][NT];
     ce_none(c);
     tile.run(0, a.Dp / TP_KSTEP, c);
+    if constexpr (DT == ZS_F32) {
+        const int sw = ce_weight_shift(a);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const int back = -sw - a.row[tile.n_of(j)].sh;
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int q = 0; q < 16; q++) c[i][j][q] = ldexpf(c[i][j][q], back);
+        }
+    }
     const uint32_t sub = at.x * (T::BM / (32 * MT)) + T::wm();
     if (tile.m0 + T::BM > a.V) {
 #pragma unroll
@@ -359,7 +421,8 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_loss(ce_args a) {
         for (uint32_t k = t; k < a.subs; k += CE_NT) a.fac[(uint64_t)i * a.subs + k] = f * ce_exp<DT>(st[k].x - m0);
         if (t == 0u) {
             a.row[i].fix = (float)((double)bad * ((double)k1 * exp(at - lse) - 1.0));
-            const float top = fabsf(g) * fmaxf(1.0f, fabsf(k1));
+            const float top = fabsf(g) * (k1 >= 0.0f ? fmaxf(1.0f, k1) : 1.0f - k1);   // at least |g (k1 p - [label])|
+            a.row[i].sd = zs_split2_of(top);
             if (DT == ZS_F16 && top < INFINITY) atomicMax(&a.st->amax[i & 63u], __float_as_uint(top));
         }
     }
@@ -396,12 +459,24 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_grad(ce_args a) {
     }
     if constexpr (DT == ZS_F32) {
         const uint64_t plane = (uint64_t)a.R * a.Vp;
-        uint16_t p[8][3];
-        for (int k = 0; k < 8; k++) zs_split3(x[k], p[k]);
-        for (int q = 0; q < 3; q++) {
-            hd_u4 o;
-            for (int k = 0; k < 4; k++) o[k] = (uint32_t)p[2 * k][q] | (uint32_t)p[2 * k + 1][q] << 16;
-            *(hd_u4*)(a.dl + q * plane + at) = o;
+        if (a.dl) {
+            uint16_t p[8][3];
+            for (int k = 0; k < 8; k++) zs_split3(x[k], p[k]);
+            for (int q = 0; q < 3; q++) {
+                hd_u4 o;
+                for (int k = 0; k < 4; k++) o[k] = (uint32_t)p[2 * k][q] | (uint32_t)p[2 * k + 1][q] << 16;
+                *(hd_u4*)(a.dl + q * plane + at) = o;
+            }
+        }
+        if (a.dl2) {
+            uint16_t p[8][2];
+            const int sd = i < n ? a.row[i].sd : 0;
+            for (int k = 0; k < 8; k++) zs_split2(x[k], sd, p[k]);
+            for (int q = 0; q < 2; q++) {
+                hd_u4 o;
+                for (int k = 0; k < 4; k++) o[k] = (uint32_t)p[2 * k][q] | (uint32_t)p[2 * k + 1][q] << 16;
+                *(hd_u4*)(a.dl2 + q * plane + at) = o;
+            }
         }
     } else {
         hd_u4 o;
@@ -464,12 +539,23 @@ __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_dhidden(ce_args a) {
     if (u == ~0u) return;
     const uint32_t part = u / tiles, k0 = part * p.steps, all = a.Vp / TP_KSTEP;
     const uint2 at = tp_order(u - part * tiles, p.mt, p.nt);
-    const tp_mat mw = ce_mat_w<DT>(a, true), md = ce_mat_dl(a, false);
+    const tp_mat mw = ce_mat_w<DT>(a, true), md = ce_mat_dl<DT>(a, false);
     T tile(mw, md, at.x, at.y);
     tp_acc c[MT][NT];
     ce_none(c);
     tile.run(k0, all - k0 < p.steps ? all - k0 : p.steps, c);
     const float un = ldexpf(1.0f, -ce_shift<DT>(a));
+    if constexpr (DT == ZS_F32) {
+        const int sw = ce_weight_shift(a);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const int back = -sw - a.row[tile.n_of(j)].sd;   // (rows past the last are not stored)
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int q = 0; q < 16; q++) c[i][j][q] = ldexpf(c[i][j][q], back);
+        }
+    }
     if (DT == ZS_F32 || p.parts > 1u) {
         const bool vec = a.D % 4u == 0u && a.ld_dh % 4u == 0u && ((uintptr_t)a.dh & 15u) == 0u;
 #pragma unroll
@@ -535,11 +621,11 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_join(ce_args a) {
 // 128 x 128 a CU.)
 template <int DT, bool THIN>
 __global__ __launch_bounds__(CE_NT, THIN ? 3 : 1) void zs_k_ce_dweight(ce_args a) {
-    typedef tp_tile<DT, THIN ? 2 : 4, THIN ? 2 : 4, 2, true, true> T;
+    typedef tp_tile<DT == ZS_F32 ? TP_THREE : DT, THIN ? 2 : 4, THIN ? 2 : 4, 2, true, true> T;
     const uint32_t n = ce_rows(a), mt = ce_over(a.D, T::BM), nt = a.Vp / T::BN, t = tp_place(blockIdx.x, mt * nt);
     if (t == ~0u) return;
     const uint2 at = tp_order(t, mt, nt);
-    const tp_mat mh = ce_mat_h(a, true), md = ce_mat_dl(a, true);
+    const tp_mat mh = ce_mat_h<DT>(a, true), md = ce_mat_dl<DT>(a, true);
     T tile(mh, md, at.x, at.y);
     tp_acc c[T::M][T::N];
     ce_none(c);
@@ -613,6 +699,7 @@ template <int DT>
 static void ce_go(ce_args a, hipStream_t stream) {
     const dim3 wg(CE_NT);
     if (a.N > CE_SELF) hipLaunchKernelGGL(zs_k_ce_rows, dim3(1), dim3(1024), 0, stream, a);
+    if (DT == ZS_F32) hipLaunchKernelGGL(zs_k_ce_max, dim3(CE_MAXIMA), wg, 0, stream, a);
     if (a.w) hipLaunchKernelGGL(zs_k_ce_weight<DT>, dim3(8192, (a.V + 65535u) / 65536u), wg, 0, stream, a);
     for (uint32_t p = 0; p < a.pieces; p++) {
         a.lo = p * a.R;

@@ -69,6 +69,19 @@ __device__ __forceinline__ void zs_split3(float x, uint16_t (&p)[3]) {
     p[2] = zs_bf16(r - hd_float(p[1]));
 }
 
+// x 2^s as a sum of two f16, each the nearest to what is left (22 bits in all down to
+// 2^-3, in steps of 2^-24 below); s from zs_split2_of of numbers no smaller than x.
+__device__ __forceinline__ int zs_split2_of(float top) {   // brings them to at most 2^15
+    const uint32_t b = __float_as_uint(top) & 0x7fffffffu;
+    return b == 0u ? 0 : b < 0x00800000u ? 141 : 15 - ((int)(b >> 23) - 126);
+}
+__device__ __forceinline__ void zs_split2(float x, int s, uint16_t (&p)[2]) {
+    const float y = ldexpf(x, s);
+    const _Float16 a = (_Float16)y, b = (_Float16)(y - (float)a);
+    p[0] = __builtin_bit_cast(uint16_t, a);
+    p[1] = __builtin_bit_cast(uint16_t, b);
+}
+
 template <int DT>
 struct hd_row {
     typedef typename hd_elem<DT>::T T;

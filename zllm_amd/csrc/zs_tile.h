@@ -6,7 +6,7 @@
 #include "zs_dev.h"
 
 // An operand lies k-fast (rows of A or B, k along a row) or k-slow (rows of k,
-// m or n along a row). It may have planes: bf16 matrices whose sum it is.
+// m or n along a row). It may have planes: matrices whose sum it is.
 struct tp_mat {
     const uint16_t* p[3];
     uint64_t ld;          // elements from row to row, a multiple of 8, at most TP_LD
@@ -24,10 +24,10 @@ typedef float tp_acc __attribute__((ext_vector_type(16)));
 typedef short tp_s4 __attribute__((ext_vector_type(4)));
 typedef short tp_s8 __attribute__((ext_vector_type(8)));
 
-template <int DT>
+template <int KIND>
 __device__ __forceinline__ tp_acc tp_mfma(tp_s8 a, tp_s8 b, tp_acc c) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    if constexpr (DT == ZS_F16) {
+    if constexpr (KIND == ZS_F16 || KIND == 3) {
         typedef _Float16 h8 __attribute__((ext_vector_type(8)));
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
     } else {
@@ -156,19 +156,36 @@ struct tp_side {
     }
 };
 
-// Which planes' products make an f32 product, the smallest first: with x = x0 + x1
-// + x2, each the bf16 nearest to what those before it leave, x1 y2, x2 y1 and
-// x2 y2 are left out (at most 2^-26 of |x y| together).
-#define TP_PAIRS 6
-__device__ __forceinline__ int tp_plane_a(int s) { return (int)(0x001102u >> (4 * s)) & 15; }
-__device__ __forceinline__ int tp_plane_b(int s) { return (int)(0x010120u >> (4 * s)) & 15; }
+// What operands are: 16-bit numbers (ZS_F16, ZS_BF16), or f32 numbers as planes
+// whose products make theirs, the smallest first:
+//   TP_TWO    f16 x0 + x1 of x scaled by a power of two (zs_split2): x1 y0, x0 y1,
+//             x0 y0. What x0 + x1 leaves of x and the product left out, x1 y1, are
+//             each at most 2^-22 of theirs: 3 * 2^-22 |x y| in all. Numbers below
+//             2^-18 of the largest that fits have less than 22 bits, to 2^-40 of it.
+//   TP_THREE  bf16 x0 + x1 + x2 (zs_split3), of any size: x2 y0, x0 y2, x1 y1, x1 y0,
+//             x0 y1, x0 y0. Left out are at most 2^-26 of |x y|.
+#define TP_TWO 3
+#define TP_THREE 4
+template <int KIND> struct tp_planes {
+    static constexpr int PAIRS = 1;
+    static constexpr uint32_t A = 0, B = 0;   // the planes of pair s at 4 s
+};
+template <> struct tp_planes<TP_TWO> {
+    static constexpr int PAIRS = 3;
+    static constexpr uint32_t A = 0x001u, B = 0x010u;
+};
+template <> struct tp_planes<TP_THREE> {
+    static constexpr int PAIRS = 6;
+    static constexpr uint32_t A = 0x001102u, B = 0x010120u;
+};
 
 // A tile of BM x BN = (32 MT WM) x (32 NT WN) by four waves, WM along m.
-template <int DT, int MT, int NT, int WM, bool AS, bool BS>
+template <int KIND, int MT, int NT, int WM, bool AS, bool BS>
 struct tp_tile {
     static constexpr int M = MT, N = NT, WN = 4 / WM, BM = 32 * MT * WM, BN = 32 * NT * WN;
     static constexpr int SA = BM * 64, STAGE = (BM + BN) * 64;
-    static constexpr int PAIRS = DT == ZS_F32 ? TP_PAIRS : 1;
+    typedef tp_planes<KIND> planes_of;
+    static constexpr int PAIRS = planes_of::PAIRS;
     typedef tp_side<BM, AS> A;
     typedef tp_side<BN, BS> B;
     static constexpr int LOADS = A::LOADS + B::LOADS;
@@ -210,7 +227,7 @@ struct tp_tile {
 #pragma unroll
         for (int i = 0; i < MT; i++)
 #pragma unroll
-            for (int j = 0; j < NT; j++) c[i][j] = tp_mfma<DT>(r.a[i], r.b[j], c[i][j]);
+            for (int j = 0; j < NT; j++) c[i][j] = tp_mfma<KIND>(r.a[i], r.b[j], c[i][j]);
     }
     // the next step's values; past the last the last again, which nobody reads
     __device__ __forceinline__ void put(tp_lds* s) {
@@ -226,8 +243,8 @@ struct tp_tile {
         }
     }
     __device__ __forceinline__ void planes() {
-        a.plane(ma, PAIRS > 1 ? tp_plane_a(pair) : 0, m0);
-        b.plane(mb, PAIRS > 1 ? tp_plane_b(pair) : 0, n0);
+        a.plane(ma, (int)(planes_of::A >> (4 * pair)) & 15, m0);
+        b.plane(mb, (int)(planes_of::B >> (4 * pair)) & 15, n0);
     }
     // c += A B over steps k0 .. k0 + n - 1
     __device__ __forceinline__ void run(uint32_t k0, uint32_t n, tp_acc (&c)[MT][NT]) {
