@@ -96,12 +96,12 @@ __global__ __launch_bounds__(1024) void zs_k_ce_rows(ce_args a) {
     if (t == 0u) a.st->rows = done;
 }
 
-// Row lo + i: its hidden state to the operand (zeros behind the last row), the
-// logit of its label; rows without one get their zeros.
+// Row lo + i: its hidden state to the operand (zeros behind the last row), its label
+// and (16-bit types) that one's logit; rows without one get their zeros.
 template <int DT>
 __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
-    __shared__ double sh[CE_NT / 64];
     __shared__ float shf[CE_NT / 64];
+    __shared__ double shd[CE_NT / 64];
     const uint32_t i = blockIdx.x, t = threadIdx.x;
     const uint64_t plane = (uint64_t)a.R * a.Dp;
     uint16_t* o = a.h + (uint64_t)i * a.Dp;
@@ -171,13 +171,14 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
             for (int k = 0; k < 2; k++) a.h2[k * plane + (uint64_t)i * a.Dp + d] = p2[k];
         } else {
             o[d] = d < a.D ? ((const uint16_t*)a.hidden)[hr + d] : (uint16_t)0;
+            if (d < a.D) dot += (double)x * (double)ce_load<DT>(a.weight, wr + d);
         }
-        if (d < a.D) dot += (double)x * (double)ce_load<DT>(a.weight, wr + d);
     }
-    dot = block_sum_d<CE_NT>(dot, sh);
+    if constexpr (DT != ZS_F32) dot = block_sum_d<CE_NT>(dot, shd);
     if (t == 0u) {
-        a.at[i] = bad ? NAN : (float)dot;
         a.row[i].label = bad ? ~0u : (uint32_t)label;
+        if (bad) a.at[i] = NAN;
+        else if (DT != ZS_F32) a.at[i] = (float)dot;
     }
 }
 
@@ -327,6 +328,23 @@ __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_logits(ce_args a) {
             for (int i = 0; i < MT; i++)
 #pragma unroll
                 for (int q = 0; q < 16; q++) c[i][j][q] = ldexpf(c[i][j][q], back);
+        }
+    }
+    // The label's logit, of the very products that the sum is of: where it is most of
+    // the sum, their errors then leave p - 1 as they leave the sum. (16-bit gradients
+    // show nothing of that: zs_k_ce_pack has theirs for less.)
+    if constexpr (DT == ZS_F32) {
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const uint32_t r = tile.n_of(j), v = (r < n ? a.row[r].label : ~0u) - tile.m_of(0, 0);   // (from the lane's first id on)
+            if (__ballot(v < 32u * MT)) {
+                float z = 0.0f;
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int q = 0; q < 16; q++) z = v == (uint32_t)(i * 32 + q / 4 * 8 + q % 4) ? c[i][j][q] : z;
+                if (v < 32u * MT && !(v & 4u)) a.at[r] = z;   // (the ids with that bit are the other half's)
+            }
         }
     }
     const uint32_t sub = at.x * (T::BM / (32 * MT)) + T::wm();
