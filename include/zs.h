@@ -607,8 +607,9 @@ int zs_ce_loss_grad(zs_ctx* ctx, const zs_ce* args, void* stream);
  * D is a multiple of group. The codes are laid out once for the kernels
  * (zs_q4_pack, into d_head of zs_q4_bytes bytes); logits are
  *     logits[r][v] = sum_d hidden[r][d] W_vd
- * in f32: codes and hidden states (f32: as three bf16, to 2^-26) multiplied
- * exactly, summed in f32 over a group, scaled, and summed in f32. They are what
+ * in f32: codes and hidden states (f32: as two f16 of the number scaled by a power
+ * of two of the row, to 2^-22, numbers below 2^-18 of the row's largest to 2^-40 of
+ * that) multiplied exactly, summed in f32 over a group, scaled, and summed in f32. They are what
  * zs_sample, zs_lane_step, zs_beam_select and the others read (those that ask
  * for it with ld % 4 == 0).
  *   zs_q4_quantize    codes and scales of a weight of any of the three types:

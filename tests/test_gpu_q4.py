@@ -5,7 +5,8 @@ Tolerance. In a group, products of x by numbers of at most 31 and 24 are exact
 and summed in f32, 2 G additions under partial sums of at most 55 X_g (X_g = sum
 |x|): (2 G + 8) 2^-24 55 X_g, times the scale. The groups' sums are then added,
 each under the whole's 15 s_g X_g + |min_g| X_g: (groups + 8) 2^-24 of that. f32
-states are multiplied as three bf16: 2^-26 of 31 s_g X_g more."""
+states are multiplied as two f16: 2^-22 of 31 s_g X_g more (numbers below 2^-18 of
+the row's largest: 2^-40 of that, G times a group)."""
 import numpy as np
 import pytest
 import torch
@@ -41,8 +42,11 @@ def bound(h, scales, mins, group):
     x = h.double().abs().view(h.shape[0], n, G).sum(2)
     s = scales.double().abs()
     whole = 15 * s + (mins.double().abs() if mins is not None else 0.0)
-    split = 31 * 2.0 ** -26 if h.dtype == torch.float32 else 0.0
-    return x @ (s * ((2 * G + 8) * 55 * 2.0 ** -24 + split) + (n + 8) * 2.0 ** -24 * whole).T
+    wide = h.dtype == torch.float32
+    tol = x @ (s * ((2 * G + 8) * 55 * 2.0 ** -24 + (31 * 2.0 ** -22 if wide else 0.0)) + (n + 8) * 2.0 ** -24 * whole).T
+    if wide:
+        tol += 2.0 ** -40 * h.double().abs().nan_to_num(0.0, 0.0, 0.0).amax(1, keepdim=True) * G * 31 * s.sum(1)
+    return tol
 
 
 def states(B, D, dtype, shift=0, pad=0, seed=1):

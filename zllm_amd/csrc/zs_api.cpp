@@ -1441,7 +1441,7 @@ extern "C" int zs_q4_logits(zs_ctx* ctx, const zs_q4* b, void* stream) {
     a.hidden = copy ? x.out : b->d_hidden;
     a.ld_h = copy ? b->D : b->ld_hidden;
     a.plane = (uint64_t)b->B * b->D;
-    a.sums = x.sums; a.Bp = x.Bp;
+    a.sums = x.sums; a.Bp = x.Bp; a.shift = x.shift;
     a.logits = b->d_logits; a.ld = b->ld;
     const int prev = zs_device_guard_begin(ctx);
     rc = q4_logits(a, x.out || x.sums ? &x : nullptr, b->dtype, b->group, b->flags & ZS_Q4_MINS, (hipStream_t)stream);

@@ -52,7 +52,7 @@ struct ce_args {
     uint16_t* h;                 // [R][Dp] rows with a label, zeros behind them (f32: three planes, the weight's gradient's)
     uint16_t* w;                 // [V][Dp], where the weight itself does not serve (f32: two planes)
     void* e;                     // [R][Vp] f16 (f32: f32) exponentials
-    uint16_t* dl;                // [R][Vp] gradient of the logits, in their place (f32: three planes, the weight's gradient's)
+    uint16_t* dl;                // [R][Vp] gradient of the logits, in their place (of few rows a second plane; f32: three, the weight's gradient's)
     uint16_t *h2, *dl2;          // f32: the same as two planes of scaled rows, the logits' and the hidden states' gradient's
     float* wmax;                 // [CE_MAXIMA] f32: the weight's largest numbers
     float* part;                 // the hidden states' gradient over parts of the vocabulary (ce_parts)
@@ -67,7 +67,7 @@ inline uint64_t ce_work(ce_args& a, uint32_t dtype, void* work) {
     const bool wide = dtype == ZS_F32, grad = (a.want & (CE_DH | CE_DW)) != 0;
     const uint64_t planes = wide ? 3u : 1u;
     const bool dh = (a.want & CE_DH) != 0, dw = (a.want & CE_DW) != 0;
-    a.Dp = (uint32_t)ce_up(a.D, TP_KROUND);
+    a.Dp = (uint32_t)ce_up(a.D, TP_KSTEP);
     a.Vp = (uint32_t)ce_up(a.V, CE_TILE);
     a.Dm = (uint32_t)ce_up(a.D, 4);
     // A tile of 256 rows is 192 of them for nothing where there are 64: us of the
@@ -97,7 +97,7 @@ inline uint64_t ce_work(ce_args& a, uint32_t dtype, void* work) {
     }
     if (grad) {
         a.fac = (float*)take((uint64_t)a.R * a.subs * 4u);
-        a.e = take((uint64_t)a.R * a.Vp * (wide ? 4u : 2u));
+        a.e = take((uint64_t)a.R * a.Vp * (wide || a.thin ? 4u : 2u));   // (thin: a plane more behind it)
         a.dl = !wide ? (uint16_t*)a.e : dw ? (uint16_t*)take(planes * a.R * a.Vp * 2u) : nullptr;
         if (wide && dh) a.dl2 = (uint16_t*)take(2u * (uint64_t)a.R * a.Vp * 2u);
         if (dh) a.part = (float*)take((uint64_t)a.units * (a.thin ? CE_THIN_M * CE_THIN : CE_TILE * CE_TILE) * 4u);

@@ -290,8 +290,15 @@ __device__ __forceinline__ tp_mat ce_mat_dl(const ce_args& a, bool slow) {
 }
 
 // The tiles of the products: 256 x 256, or 128 x 64 where there are few rows.
-template <int DT, bool THIN, bool AS, bool BS>
-using ce_tile = tp_tile<DT == ZS_F32 ? TP_TWO : DT, THIN ? 1 : 4, THIN ? 2 : 4, THIN ? 4 : 2, AS, BS>;
+// The logits' gradient d in 16 bits is off by half a step of the type. Over many rows
+// and ids that adds 0.7 of the outputs' own rounding to their error; in few rows, where
+// one d is most of a gradient's row, it may be the double. There the products wait for
+// memory, and what the rounding leaves is multiplied too.
+constexpr int ce_kind(int dt, bool thin, bool weight) {
+    return dt == ZS_F32 ? (weight ? TP_THREE : TP_TWO) : !thin ? dt : dt == ZS_F16 ? TP_REST_F16 : TP_REST_BF16;
+}
+template <int KIND, bool THIN, bool AS, bool BS>
+using ce_tile = tp_tile<KIND, THIN ? 1 : 4, THIN ? 2 : 4, THIN ? 4 : 2, AS, BS>;
 template <int MT, int NT>
 __device__ __forceinline__ void ce_none(tp_acc (&c)[MT][NT]) {
 #pragma unroll
@@ -309,7 +316,7 @@ __device__ __forceinline__ uint32_t ce_over(uint32_t n, uint32_t d) { return (n 
 // exponentials.
 template <int DT, bool GRAD, bool THIN>
 __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_logits(ce_args a) {
-    typedef ce_tile<DT, THIN, false, false> T;
+    typedef ce_tile<DT == ZS_F32 ? TP_TWO : DT, THIN, false, false> T;
     constexpr int MT = T::M, NT = T::N;
     const uint32_t n = ce_rows(a), mt = a.Vp / T::BM, nt = ce_over(n, T::BN), t = tp_place(blockIdx.x, mt * nt);
     if (t == ~0u) return;
@@ -452,7 +459,7 @@ template <int DT>
 __global__ __launch_bounds__(CE_NT) void zs_k_ce_grad(ce_args a) {
     const uint32_t i = blockIdx.y, n = ce_rows(a), v0 = (blockIdx.x * CE_NT + threadIdx.x) * 8u;
     const int sh = ce_shift<DT>(a);   // (by whole waves)
-    if (i >= (n + TP_KROUND - 1u) / TP_KROUND * TP_KROUND || v0 >= a.Vp) return;
+    if (i >= (n + TP_KSTEP - 1u) / TP_KSTEP * TP_KSTEP || v0 >= a.Vp) return;
     const uint64_t at = (uint64_t)i * a.Vp + v0;
     float x[8];
     if (i < n) {
@@ -500,6 +507,12 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_grad(ce_args a) {
         hd_u4 o;
         for (int k = 0; k < 4; k++) o[k] = hd_pack2<DT>(x[2 * k], x[2 * k + 1]);
         *(hd_u4*)(a.dl + at) = o;
+        if (a.thin) {
+            float y[8];
+            hd_unpack<DT>(o, y);
+            for (int k = 0; k < 4; k++) o[k] = hd_pack2<DT>(x[2 * k] - y[2 * k], x[2 * k + 1] - y[2 * k + 1]);
+            *(hd_u4*)(a.dl + (uint64_t)a.R * a.Vp + at) = o;
+        }
     }
 }
 
@@ -550,7 +563,7 @@ __device__ __forceinline__ ce_cut ce_parts(const ce_args& a) {
 // vocabulary or a part of it.
 template <int DT, bool THIN>
 __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_dhidden(ce_args a) {
-    typedef ce_tile<DT, THIN, true, false> T;
+    typedef ce_tile<ce_kind(DT, THIN, false), THIN, true, false> T;
     constexpr int MT = T::M, NT = T::N;
     const ce_cut p = ce_parts<T>(a);
     const uint32_t n = ce_rows(a), tiles = p.mt * p.nt, u = tp_place(blockIdx.x, tiles * p.parts);
@@ -608,7 +621,7 @@ __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_dhidden(ce_args a) {
 // times over the parts.
 template <int DT, bool THIN>
 __global__ __launch_bounds__(CE_NT) void zs_k_ce_join(ce_args a) {
-    typedef ce_tile<DT, THIN, true, false> T;
+    typedef ce_tile<ce_kind(DT, THIN, false), THIN, true, false> T;
     __shared__ float4 sh[3][64];
     const uint32_t i = blockIdx.x, l = threadIdx.x & 63u, w = threadIdx.x >> 6, d = (blockIdx.y * 64u + l) * 4u;
     const ce_cut p = ce_parts<T>(a);
@@ -639,7 +652,7 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_join(ce_args a) {
 // 128 x 128 a CU.)
 template <int DT, bool THIN>
 __global__ __launch_bounds__(CE_NT, THIN ? 3 : 1) void zs_k_ce_dweight(ce_args a) {
-    typedef tp_tile<DT == ZS_F32 ? TP_THREE : DT, THIN ? 2 : 4, THIN ? 2 : 4, 2, true, true> T;
+    typedef tp_tile<ce_kind(DT, THIN, true), THIN ? 2 : 4, THIN ? 2 : 4, 2, true, true> T;
     const uint32_t n = ce_rows(a), mt = ce_over(a.D, T::BM), nt = a.Vp / T::BN, t = tp_place(blockIdx.x, mt * nt);
     if (t == ~0u) return;
     const uint2 at = tp_order(t, mt, nt);
@@ -647,7 +660,7 @@ __global__ __launch_bounds__(CE_NT, THIN ? 3 : 1) void zs_k_ce_dweight(ce_args a
     T tile(mh, md, at.x, at.y);
     tp_acc c[T::M][T::N];
     ce_none(c);
-    tile.run(0, ce_over(n, TP_KROUND) * (TP_KROUND / TP_KSTEP), c);
+    tile.run(0, ce_over(n, TP_KSTEP), c);
     const float un = ldexpf(1.0f, -ce_shift<DT>(a));
     if constexpr (DT == ZS_F16) {
 #pragma unroll

@@ -34,6 +34,7 @@ struct q4_args {
     uint64_t ld_h, plane;        // elements
     const float* sums;           // of groups of more than Q4_FEW rows (q4_x_args)
     uint32_t Bp;
+    const int32_t* shift;        // f32: of each row (q4_x_args)
     float* logits;
     uint64_t ld;
 };
@@ -52,6 +53,7 @@ struct q4_x_args {               // hidden states to rows the kernels take
     uint64_t ld_h;
     uint32_t B, D, group, Bp;
     float off;                   // what codes are moved by as operands: -24, with minima -16
+    int32_t* shift;              // [B] f32: the powers of two the rows are scaled by
     uint16_t* out;               // [planes][B][D], or NULL: they serve as they are
     float* sums;                 // [D / group][Bp], or NULL
 };
@@ -61,7 +63,11 @@ inline uint64_t q4_work(q4_x_args& x, uint32_t dtype, bool copy, void* work) {
     const bool wide = dtype == ZS_F32;
     if (copy || wide) {
         x.out = (uint16_t*)p;
-        p += hd_pad((uint64_t)x.B * x.D * (wide ? 6u : 2u));
+        p += hd_pad((uint64_t)x.B * x.D * (wide ? 4u : 2u));
+    }
+    if (wide) {
+        x.shift = (int32_t*)p;
+        p += hd_pad(x.B * 4ull);
     }
     if (x.B > Q4_FEW) {
         x.sums = (float*)p;

@@ -87,13 +87,23 @@ __global__ __launch_bounds__(64) void zs_k_q4_pack(q4_pack_args a) {
 }
 
 // ------------------------------------------------------------------ hidden states
-// Rows at 16 bytes each where they are not (COPY; f32 as three bf16 whose sum is
-// the value to 2^-26 of it), and their sums over the groups, times what
-// zs_k_q4_batch starts from. One wave a row's 128 columns.
-template <int DT, bool COPY>
+// A wave's part of a row: 128 columns, two a lane, to the rows the kernels take and
+// to their sums over the groups, times what zs_k_q4_batch starts from.
+__device__ __forceinline__ void q4_sums(const q4_x_args& a, uint64_t r, uint32_t b, float x, float y, int s) {
+    const uint32_t l = zs_lane(), per = 128u / a.group;
+    double t = (double)x + (double)y;
+    t += zs_lane_xor<1>(t);
+    t += zs_lane_xor<2>(t);
+    t += zs_lane_xor<4>(t);
+    t += zs_lane_xor<8>(t);
+    if (a.group > 32u) t += zs_lane_xor<16>(t);
+    if (a.group > 64u) t += zs_lane_xor<32>(t);
+    if (l % (a.group / 2u) == 0u) a.sums[((uint64_t)b * per + l / (a.group / 2u)) * a.Bp + r] = ldexpf((float)(t * (double)a.off), s);
+}
+template <int DT>
 __global__ __launch_bounds__(Q4_NT) void zs_k_q4_rows(q4_x_args a) {
-    const uint32_t l = zs_lane(), blocks = (a.D + 127u) / 128u, per = 128u / a.group;
-    const uint64_t n = (uint64_t)a.B * a.D, all = (uint64_t)a.B * blocks;
+    const uint32_t l = zs_lane(), blocks = (a.D + 127u) / 128u;
+    const uint64_t all = (uint64_t)a.B * blocks;
     for (uint64_t i = (uint64_t)blockIdx.x * (Q4_NT / 64) + zs_wid(); i < all; i += (uint64_t)gridDim.x * (Q4_NT / 64)) {
         const uint64_t r = i / blocks;
         const uint32_t b = (uint32_t)(i - r * blocks), d = b * 128u + l * 2u;
@@ -102,27 +112,34 @@ __global__ __launch_bounds__(Q4_NT) void zs_k_q4_rows(q4_x_args a) {
         if (d < a.D)
             for (int k = 0; k < 2; k++) {
                 v[k] = hd_float(x[k]);
-                if constexpr (COPY) {
-                    const uint64_t to = r * a.D + d + k;
-                    if constexpr (DT == ZS_F32) {
-                        uint16_t p[3];
-                        zs_split3(v[k], p);
-                        for (int q = 0; q < 3; q++) a.out[q * n + to] = p[q];
-                    } else {
-                        a.out[to] = __builtin_bit_cast(uint16_t, x[k]);
-                    }
-                }
+                if (a.out) a.out[r * a.D + d + k] = __builtin_bit_cast(uint16_t, x[k]);
             }
-        if (!a.sums) continue;
-        double t = (double)v[0] + (double)v[1];
-        t += zs_lane_xor<1>(t);
-        t += zs_lane_xor<2>(t);
-        t += zs_lane_xor<4>(t);
-        t += zs_lane_xor<8>(t);
-        if (a.group > 32u) t += zs_lane_xor<16>(t);
-        if (a.group > 64u) t += zs_lane_xor<32>(t);
-        const uint32_t g = l / (a.group / 2u);
-        if (l % (a.group / 2u) == 0u) a.sums[((uint64_t)b * per + g) * a.Bp + r] = (float)(t * (double)a.off);
+        if (a.sums) q4_sums(a, r, b, v[0], v[1], 0);
+    }
+}
+// f32 rows as two f16 of the number scaled by a power of two of the row (zs_split2),
+// by which the logits are scaled back.
+__global__ __launch_bounds__(Q4_NT) void zs_k_q4_rows_f32(q4_x_args a) {
+    __shared__ float sh[Q4_NT / 64];
+    const uint32_t l = zs_lane(), blocks = (a.D + 127u) / 128u;
+    const uint64_t r = blockIdx.x, n = (uint64_t)a.B * a.D;
+    const float* x = (const float*)a.hidden + r * a.ld_h;
+    float top = 0.0f;
+    for (uint32_t d = threadIdx.x; d < a.D; d += Q4_NT) top = fmaxf(top, fabsf(x[d]));
+    const int s = zs_split2_of(block_max_f<Q4_NT>(top, sh));
+    if (threadIdx.x == 0u) a.shift[r] = s;
+    for (uint32_t b = zs_wid(); b < blocks; b += Q4_NT / 64) {
+        const uint32_t d = b * 128u + l * 2u;
+        float v[2] = {0.0f, 0.0f};
+        if (d < a.D) {
+            uint16_t p[2][2];
+            for (int k = 0; k < 2; k++) {
+                v[k] = x[d + k];
+                zs_split2(v[k], s, p[k]);
+            }
+            for (int q = 0; q < 2; q++) *(uint32_t*)(a.out + q * n + r * a.D + d) = (uint32_t)p[0][q] | (uint32_t)p[1][q] << 16;
+        }
+        if (a.sums) q4_sums(a, r, b, v[0], v[1], s);
     }
 }
 
@@ -133,9 +150,9 @@ __global__ __launch_bounds__(Q4_NT) void zs_k_q4_rows(q4_x_args a) {
 // sum the products start from. Operand register j holds columns 2 j, 2 j + 1.
 template <int DT>
 struct q4_num {
-    static constexpr uint32_t ONE = DT == ZS_F16 ? 6 : 3;                                   // log2 of a unit's bits
-    static constexpr uint32_t BASE = DT == ZS_F16 ? 0x4c004c00u : 0x41804180u, MASK = 0x000f000fu << ONE;
-    static constexpr uint32_t M16 = DT == ZS_F16 ? 0xcc00cc00u : 0xc180c180u, M24 = DT == ZS_F16 ? 0xce00ce00u : 0xc1c0c1c0u;
+    static constexpr uint32_t ONE = DT != ZS_BF16 ? 6 : 3;                                   // log2 of a unit's bits
+    static constexpr uint32_t BASE = DT != ZS_BF16 ? 0x4c004c00u : 0x41804180u, MASK = 0x000f000fu << ONE;
+    static constexpr uint32_t M16 = DT != ZS_BF16 ? 0xcc00cc00u : 0xc180c180u, M24 = DT != ZS_BF16 ? 0xce00ce00u : 0xc1c0c1c0u;
     uint32_t mask, base;
     __device__ __forceinline__ q4_num() {
         // in a scalar and a vector register, which one and-or takes: of two
@@ -154,7 +171,7 @@ struct q4_num {
     }
     static __device__ __forceinline__ q4_f4 mul(q4_u4 a, q4_u4 b, q4_f4 c) {
 #if defined(__HIP_DEVICE_COMPILE__)
-        if constexpr (DT == ZS_F16) {
+        if constexpr (DT != ZS_BF16) {
             typedef _Float16 h8 __attribute__((ext_vector_type(8)));
             return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
         } else {
@@ -175,7 +192,7 @@ struct q4_num {
 // of their lane, up to 8 the first two.
 template <int DT, int G, bool MINS, int T, int NI>
 struct q4_few {
-    static constexpr int P = DT == ZS_F32 ? 3 : 1, PER = 128 / G;
+    static constexpr int P = DT == ZS_F32 ? 2 : 1, PER = 128 / G;
     typedef q4_num<DT> num;
     typedef _Float16 hv __attribute__((ext_vector_type(PER)));
     struct regs {
@@ -238,7 +255,7 @@ struct q4_few {
 #pragma unroll
             for (int k = q * (G / 32); k < (q + 1) * (G / 32); k++)
 #pragma unroll
-                for (int p = P - 1; p >= 0; p--) c0[q] = num::mul(g.x[p][k], off, c0[q]);
+                for (int p = 0; p < P; p++) c0[q] = num::mul(g.x[p][k], off, c0[q]);
         }
 #pragma unroll
         for (int q = 0; q < PER; q++) {
@@ -248,7 +265,7 @@ struct q4_few {
                 for (int t = 0; t < T; t++) {
                     const q4_u4 op = nm.operand(g.w[t][k]);
 #pragma unroll
-                    for (int p = P - 1; p >= 0; p--) d[q][t] = num::mul(g.x[p][k], op, k == q * (G / 32) && p == P - 1 ? c0[q] : d[q][t]);
+                    for (int p = 0; p < P; p++) d[q][t] = num::mul(g.x[p][k], op, k == q * (G / 32) && p == 0 ? c0[q] : d[q][t]);
                 }
             if (q > 0) scaled(q - 1);
         }
@@ -287,7 +304,7 @@ __global__ __launch_bounds__(KS * 64) void zs_k_q4_logits(q4_args a) {
 #pragma unroll
         for (uint32_t i = 0; i < NI; i++) {
             const uint32_t row = i * 4u + (q.l >> 4);
-            if (row < a.B) a.logits[row * a.ld + id] = v[i];
+            if (row < a.B) a.logits[row * a.ld + id] = DT == ZS_F32 ? ldexpf(v[i], -a.shift[row]) : v[i];
         }
     }
 }
@@ -298,7 +315,7 @@ __global__ __launch_bounds__(KS * 64) void zs_k_q4_logits(q4_args a) {
 // and the waves' codes and scales to registers likewise.
 template <int DT, int G, bool MINS, int T, int RT>
 struct q4_batch {
-    static constexpr int P = DT == ZS_F32 ? 3 : 1, PER = 128 / G, PIECES = P * RT * 4;
+    static constexpr int P = DT == ZS_F32 ? 2 : 1, PER = 128 / G, PIECES = P * RT * 4;
     static constexpr int LOADS = T * (MINS ? 3 : 2) + P * RT + 1, STAGE = PIECES * 1024 + 1024;
     typedef q4_num<DT> num;
     typedef _Float16 hv __attribute__((ext_vector_type(PER)));
@@ -389,9 +406,9 @@ struct q4_batch {
                 for (int t = 0; t < T; t++) {
                     const q4_u4 op = nm.operand(g.w[t][k]);
 #pragma unroll
-                    for (int p = P - 1; p >= 0; p--)
+                    for (int p = 0; p < P; p++)
 #pragma unroll
-                        for (int r = 0; r < RT; r++) d[t][r] = num::mul(f[p][r], op, first && p == P - 1 ? c0[r] : d[t][r]);
+                        for (int r = 0; r < RT; r++) d[t][r] = num::mul(f[p][r], op, first && p == 0 ? c0[r] : d[t][r]);
                     if (last && t > 0) scaled(t - 1);
                 }
                 if (last) scaled(T - 1);
@@ -442,7 +459,7 @@ __global__ __launch_bounds__(Q4_NT, 2) void zs_k_q4_batch(q4_args a, uint32_t pa
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const uint32_t row = r0 + r * 16u + (q.l >> 4) * 4u + i;
-                if (row < a.B) a.logits[row * a.ld + id] = q.acc[t][r][i];
+                if (row < a.B) a.logits[row * a.ld + id] = DT == ZS_F32 ? ldexpf(q.acc[t][r][i], -a.shift[row]) : q.acc[t][r][i];
             }
     }
 }
@@ -503,11 +520,9 @@ int q4_logits(const q4_args& a, const q4_x_args* x, uint32_t dtype, uint32_t gro
     if (x) {
         const uint64_t n = ((uint64_t)x->B * ((x->D + 127u) / 128u) + Q4_NT / 64 - 1u) / (Q4_NT / 64);
         const dim3 grid(n < 4096u ? (uint32_t)n : 4096u), wg(Q4_NT);
-        if (dtype == ZS_F32) hipLaunchKernelGGL((zs_k_q4_rows<ZS_F32, true>), grid, wg, 0, stream, *x);
-        else if (dtype == ZS_F16 && x->out) hipLaunchKernelGGL((zs_k_q4_rows<ZS_F16, true>), grid, wg, 0, stream, *x);
-        else if (dtype == ZS_F16) hipLaunchKernelGGL((zs_k_q4_rows<ZS_F16, false>), grid, wg, 0, stream, *x);
-        else if (x->out) hipLaunchKernelGGL((zs_k_q4_rows<ZS_BF16, true>), grid, wg, 0, stream, *x);
-        else hipLaunchKernelGGL((zs_k_q4_rows<ZS_BF16, false>), grid, wg, 0, stream, *x);
+        if (dtype == ZS_F32) hipLaunchKernelGGL(zs_k_q4_rows_f32, dim3(x->B), wg, 0, stream, *x);
+        else if (dtype == ZS_F16) hipLaunchKernelGGL(zs_k_q4_rows<ZS_F16>, grid, wg, 0, stream, *x);
+        else hipLaunchKernelGGL(zs_k_q4_rows<ZS_BF16>, grid, wg, 0, stream, *x);
     }
     if (dtype == ZS_F32) q4_group<ZS_F32>(a, group, mins, stream);
     else if (dtype == ZS_F16) q4_group<ZS_F16>(a, group, mins, stream);

@@ -16,7 +16,6 @@ struct tp_mat {
 };
 #define TP_LD (1u << 22)
 #define TP_KSTEP 32       // k of a step
-#define TP_KROUND 128     // k are a multiple of
 
 typedef __attribute__((address_space(3))) char tp_lds;
 typedef __attribute__((address_space(1))) const char tp_glb;
@@ -27,7 +26,7 @@ typedef short tp_s8 __attribute__((ext_vector_type(8)));
 template <int KIND>
 __device__ __forceinline__ tp_acc tp_mfma(tp_s8 a, tp_s8 b, tp_acc c) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    if constexpr (KIND == ZS_F16 || KIND == 3) {
+    if constexpr (KIND == ZS_F16 || KIND == 3 || KIND == 5) {
         typedef _Float16 h8 __attribute__((ext_vector_type(8)));
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
     } else {
@@ -164,8 +163,12 @@ struct tp_side {
 //             2^-18 of the largest that fits have less than 22 bits, to 2^-40 of it.
 //   TP_THREE  bf16 x0 + x1 + x2 (zs_split3), of any size: x2 y0, x0 y2, x1 y1, x1 y0,
 //             x0 y1, x0 y0. Left out are at most 2^-26 of |x y|.
+// or 16-bit numbers A with a B of two planes, B1 what B0 leaves:
+//   TP_REST_F16, TP_REST_BF16   x y1, x y0
 #define TP_TWO 3
 #define TP_THREE 4
+#define TP_REST_F16 5
+#define TP_REST_BF16 6
 template <int KIND> struct tp_planes {
     static constexpr int PAIRS = 1;
     static constexpr uint32_t A = 0, B = 0;   // the planes of pair s at 4 s
@@ -174,6 +177,11 @@ template <> struct tp_planes<TP_TWO> {
     static constexpr int PAIRS = 3;
     static constexpr uint32_t A = 0x001u, B = 0x010u;
 };
+template <> struct tp_planes<TP_REST_F16> {
+    static constexpr int PAIRS = 2;
+    static constexpr uint32_t A = 0x00u, B = 0x01u;
+};
+template <> struct tp_planes<TP_REST_BF16> : tp_planes<TP_REST_F16> {};
 template <> struct tp_planes<TP_THREE> {
     static constexpr int PAIRS = 6;
     static constexpr uint32_t A = 0x001102u, B = 0x010120u;
