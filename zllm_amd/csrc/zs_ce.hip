@@ -159,7 +159,24 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
         sh2 = zs_split2_of(block_max_f<CE_NT>(top, shf));
         if (t == 0u) a.row[i].sh = sh2;
     }
-    for (uint32_t d = t; d < a.Dp; d += CE_NT) {
+    const bool vec = DT != ZS_F32 && a.D % 8u == 0u && a.ld_h % 8u == 0u && a.ld_w % 8u == 0u &&
+                     (((uintptr_t)a.hidden | (uintptr_t)a.weight) & 15u) == 0u;
+    if constexpr (DT != ZS_F32) {
+        if (vec)
+            for (uint32_t d = t * 8u; d < a.Dp; d += CE_NT * 8u) {
+                hd_u4 u = {0u, 0u, 0u, 0u};
+                if (d < a.D) {
+                    u = zs_gload((const hd_u4*)((const uint16_t*)a.hidden + hr + d));
+                    float x[8], y[8];
+                    hd_unpack<DT>(u, x);
+                    hd_unpack<DT>(zs_gload((const hd_u4*)((const uint16_t*)a.weight + wr + d)), y);
+#pragma unroll
+                    for (int k = 0; k < 8; k++) dot += (double)x[k] * (double)y[k];
+                }
+                *(hd_u4*)(o + d) = u;
+            }
+    }
+    for (uint32_t d = vec ? a.Dp : t; d < a.Dp; d += CE_NT) {
         const float x = d < a.D ? ce_load<DT>(a.hidden, hr + d) : 0.0f;
         if constexpr (DT == ZS_F32) {
             uint16_t p[3], p2[2];
