@@ -555,11 +555,11 @@ int zs_distill_loss_grad(zs_ctx* ctx, const zs_distill* args, void* stream);
  * hidden, weight and the gradients are of one type, sums in f32. Products of
  * 16-bit numbers are exact; d is rounded to their type on its way into the
  * gradients' products (f16: scaled so that its largest factor is near 2^15).
- * f32 numbers are multiplied as sums of two f16 of the number scaled by a power
- * of two, of the whole weight, of a row of hidden states and of a row of d: to
- * 3 * 2^-22 of each product, and a number below 2^-18 of the largest to 2^-40 of
- * that; in the weight's gradient, whose rows differ in size by any factor, as
- * sums of three bf16, to 2^-26. The gradients are rounded once.
+ * f32 numbers are multiplied as sums of three bf16, to 2^-26 of each product; for
+ * logits and dhidden of more than 256 rows (or a weight that is FAR) as sums of
+ * two f16 of the number scaled by a power of two, of the whole weight, of a row of
+ * hidden states and of a row of d: to 3 * 2^-22, and a number below 2^-18 of the
+ * largest to 2^-40 of that. The gradients are rounded once.
  * A row whose label is ignore_index has loss, lse and gradient 0, and its
  * hidden state, whatever it holds, is in no sum; a label outside [0, V)
  * otherwise gives NaN. What is not finite comes out as not finite.
@@ -568,14 +568,16 @@ int zs_distill_loss_grad(zs_ctx* ctx, const zs_distill* args, void* stream);
  *   zs_ce_loss_grad  also d_dhidden and d_dweight (either may be NULL: not
  *                    wanted), which overlap none of the other arrays
  * row_grad_stride 0 reads one value for all rows. `want` of zs_ce_work says
- * which gradients a call will have and whether rows of the weight do not all
- * begin at 16 bytes or are longer than ZS_CE_LD values (they are then copied;
- * as are f32 weights always). */
+ * which gradients a call will have, (COPY) whether the weight's rows do not all
+ * begin and end at 16 bytes and (FAR) whether they lie further apart than ZS_CE_LD
+ * values (16-bit weights are then copied; f32 weights of more than 256 rows and
+ * those that are FAR). */
 #define ZS_CE_MAX_HIDDEN 65536u
 #define ZS_CE_LD 4194304u
 #define ZS_CE_DHIDDEN 1u
 #define ZS_CE_DWEIGHT 2u
 #define ZS_CE_COPY 4u
+#define ZS_CE_FAR 8u
 typedef struct zs_ce {
     uint32_t N, V, D, dtype;
     uint64_t ld_hidden, ld_weight;

@@ -1309,7 +1309,7 @@ extern "C" int zs_distill_loss_grad(zs_ctx* ctx, const zs_distill* args, void* s
 
 // ---- cross entropy of the vocabulary head
 extern "C" int zs_ce_work(uint32_t N, uint32_t V, uint32_t D, uint32_t dtype, uint32_t want, uint64_t* bytes) {
-    if (!bytes || dtype > ZS_BF16 || V == 0 || V > ZS_HEAD_MAX_VOCAB || D == 0 || D > ZS_CE_MAX_HIDDEN || want > 7u) return ZS_EINVAL;
+    if (!bytes || dtype > ZS_BF16 || V == 0 || V > ZS_HEAD_MAX_VOCAB || D == 0 || D > ZS_CE_MAX_HIDDEN || want > 15u) return ZS_EINVAL;
     *bytes = 0;
     if (N == 0) return ZS_OK;
     ce_args a{};
@@ -1351,8 +1351,8 @@ static int ce_call(zs_ctx* ctx, const zs_ce* b, bool grad, const char* who, void
         a.dh = b->N ? b->d_dhidden : nullptr; a.dw = b->d_dweight; a.ld_dh = b->ld_dhidden; a.ld_dw = b->ld_dweight;
         a.want = (a.dh ? CE_DH : 0u) | (a.dw ? CE_DW : 0u);
     }
-    if (((uintptr_t)b->d_weight & 15u) || b->D % 8u || (b->V > 1u && b->ld_weight % 8u) || b->ld_weight > ZS_CE_LD || size == 4u)
-        a.want |= CE_COPY;
+    if (((uintptr_t)b->d_weight & 15u) || b->D * size % 16u || (b->V > 1u && b->ld_weight * size % 16u)) a.want |= CE_COPY;
+    if (b->ld_weight > ZS_CE_LD) a.want |= CE_FAR;
     const int prev = zs_device_guard_begin(ctx);
     if (b->N == 0) {
         rc = ce_clear(b->d_dweight, b->V, b->D, b->ld_dweight, b->dtype, (hipStream_t)stream);

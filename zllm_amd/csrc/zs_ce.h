@@ -8,11 +8,15 @@
 #define CE_TILE 256         // ids, rows or columns of a product's tile; of few rows:
 #define CE_THIN_M 128       // ids or columns
 #define CE_THIN 64          // rows
+// f32 weights are multiplied as they lie up to so many rows, and as two planes that are
+// made of them once above: us TODO
+#define CE_RAW 192u
 #define CE_ROOM (4ull << 30)   // bytes of exponentials kept at once (a piece of the rows)
 
 #define CE_DH 1u            // the gradient of the hidden states is wanted
 #define CE_DW 2u            // the weight's
-#define CE_COPY 4u          // the weight's rows do not begin at 16 bytes each: they are copied
+#define CE_COPY 4u          // the weight's rows do not begin and end at 16 bytes each: they are copied (f32: only where CE_RAW says so)
+#define CE_FAR 8u           // they lie further apart than the products' offsets reach: they are copied
 #define CE_E_SHIFT 15.0f
 #define CE_E_SCALE 32768.0f // exponentials are kept as f16 of e * 2^15: 11 bits down to 2^-29 of their maximum
 
@@ -40,7 +44,7 @@ struct ce_args {
     void *dh, *dw;
     uint64_t ld_dh, ld_dw;
     // the plan
-    uint32_t Dp, Vp, R, pieces, sub, subs, thin, units, Dm;
+    uint32_t Dp, Vp, R, pieces, sub, subs, thin, raw, units, Dm;   // raw: an f32 weight is multiplied as it lies, 1 by 16 bytes, 2 by 4
     uint32_t lo, first, last;    // the piece at hand: its first row; whether it is the first, the last
     // scratch
     ce_state* st;
@@ -72,7 +76,8 @@ inline uint64_t ce_work(ce_args& a, uint32_t dtype, void* work) {
     a.Dm = (uint32_t)ce_up(a.D, 4);
     // A tile of 256 rows is 192 of them for nothing where there are 64: us of the
     // logits TODO
-    a.thin = a.N <= CE_THIN;
+    a.raw = !wide || (a.want & CE_FAR) || a.N > CE_RAW ? 0u : a.want & CE_COPY ? 2u : 1u;
+    a.thin = a.raw || a.N <= CE_THIN;
     a.sub = a.thin ? 32u : 128u;
     a.subs = a.Vp / a.sub;
     uint64_t R = CE_ROOM / ((uint64_t)a.Vp * (wide ? 4u + (dw ? 6u : 0u) + (dh ? 4u : 0u) : 2u)) / CE_TILE * CE_TILE;
@@ -89,17 +94,17 @@ inline uint64_t ce_work(ce_args& a, uint32_t dtype, void* work) {
     a.at = (float*)take(a.R * 4ull);
     a.row = (ce_row*)take(a.R * sizeof(ce_row));
     a.stat = (float2*)take((uint64_t)a.R * a.subs * 8u);
-    if (!wide || dw) a.h = (uint16_t*)take(planes * a.R * a.Dp * 2u);
-    if (wide || (a.want & CE_COPY)) a.w = (uint16_t*)take((wide ? 2u : 1u) * (uint64_t)a.V * a.Dp * 2u);
-    if (wide) {
+    if (!wide || dw || a.raw) a.h = (uint16_t*)take(planes * a.R * a.Dp * 2u);
+    if (wide ? !a.raw : (a.want & (CE_COPY | CE_FAR)) != 0) a.w = (uint16_t*)take((wide ? 2u : 1u) * (uint64_t)a.V * a.Dp * 2u);
+    if (wide && !a.raw) {
         a.h2 = (uint16_t*)take(2u * (uint64_t)a.R * a.Dp * 2u);
         a.wmax = (float*)take(CE_MAXIMA * 4u);
     }
     if (grad) {
         a.fac = (float*)take((uint64_t)a.R * a.subs * 4u);
         a.e = take((uint64_t)a.R * a.Vp * (wide || a.thin ? 4u : 2u));   // (thin: a plane more behind it)
-        a.dl = !wide ? (uint16_t*)a.e : dw ? (uint16_t*)take(planes * a.R * a.Vp * 2u) : nullptr;
-        if (wide && dh) a.dl2 = (uint16_t*)take(2u * (uint64_t)a.R * a.Vp * 2u);
+        a.dl = !wide ? (uint16_t*)a.e : dw || a.raw ? (uint16_t*)take(planes * a.R * a.Vp * 2u) : nullptr;
+        if (wide && dh && !a.raw) a.dl2 = (uint16_t*)take(2u * (uint64_t)a.R * a.Vp * 2u);
         if (dh) a.part = (float*)take((uint64_t)a.units * (a.thin ? CE_THIN_M * CE_THIN : CE_TILE * CE_TILE) * 4u);
         if (dw && a.pieces > 1u) a.acc = (float*)take((uint64_t)a.V * a.Dm * 4u);
     }

@@ -135,7 +135,7 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
         if (i < (n + CE_TILE - 1u) / CE_TILE * CE_TILE) {
             if (a.h)
                 for (int p = 0; p < (DT == ZS_F32 ? 3 : 1); p++) ce_zero<ZS_F16>(o + p * plane, a.Dp);
-            if constexpr (DT == ZS_F32) {
+            if (DT == ZS_F32 && a.h2) {
                 for (int p = 0; p < 2; p++) ce_zero<ZS_F16>(a.h2 + p * plane + (uint64_t)i * a.Dp, a.Dp);
                 if (t == 0u) a.row[i].sh = 0;
             }
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
     const uint64_t hr = r * a.ld_h, wr = (bad ? 0u : (uint64_t)label) * a.ld_w;
     double dot = 0.0;
     int sh2 = 0;
-    if constexpr (DT == ZS_F32) {
+    if (DT == ZS_F32 && a.h2) {
         float top = 0.0f;
         for (uint32_t d = t; d < a.D; d += CE_NT) top = fmaxf(top, fabsf(ce_load<DT>(a.hidden, hr + d)));
         sh2 = zs_split2_of(block_max_f<CE_NT>(top, shf));
@@ -184,6 +184,7 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
                 zs_split3(x, p);
                 for (int k = 0; k < 3; k++) o[k * plane + d] = p[k];
             }
+            if (!a.h2) continue;
             zs_split2(x, sh2, p2);
             for (int k = 0; k < 2; k++) a.h2[k * plane + (uint64_t)i * a.Dp + d] = p2[k];
         } else {
@@ -289,19 +290,23 @@ __device__ __forceinline__ tp_mat ce_mat_w(const ce_args& a, bool slow) {
     tp_mat m = {{p, p + plane, p + 2 * plane}, own ? a.Dp : a.ld_w, slow ? d : a.V, slow ? a.V : d};
     return m;
 }
+__device__ __forceinline__ tp_mat ce_mat_raw(const ce_args& a, bool slow) {   // f32, as it lies
+    tp_mat m = {{(const uint16_t*)a.weight}, a.ld_w, slow ? a.D : a.V, slow ? a.V : a.D};
+    return m;
+}
 // (f32: the weight's gradient, whose rows of the other operands differ in size by any
 // factor, by three planes each; the others by two)
 template <int DT>
 __device__ __forceinline__ tp_mat ce_mat_h(const ce_args& a, bool slow) {
     const uint64_t plane = (uint64_t)a.R * a.Dp;
-    const uint16_t* p = DT == ZS_F32 && !slow ? a.h2 : a.h;
+    const uint16_t* p = DT == ZS_F32 && !slow && !a.raw ? a.h2 : a.h;
     tp_mat m = {{p, p + plane, p + 2 * plane}, a.Dp, slow ? a.Dp : a.R, slow ? a.R : a.Dp};
     return m;
 }
 template <int DT>
 __device__ __forceinline__ tp_mat ce_mat_dl(const ce_args& a, bool slow) {
     const uint64_t plane = (uint64_t)a.R * a.Vp;
-    const uint16_t* p = DT == ZS_F32 && !slow ? a.dl2 : a.dl;
+    const uint16_t* p = DT == ZS_F32 && !slow && !a.raw ? a.dl2 : a.dl;
     tp_mat m = {{p, p + plane, p + 2 * plane}, a.Vp, slow ? a.Vp : a.R, slow ? a.R : a.Vp};
     return m;
 }
@@ -316,6 +321,8 @@ constexpr int ce_kind(int dt, bool thin, bool weight) {
 }
 template <int KIND, bool THIN, bool AS, bool BS>
 using ce_tile = tp_tile<KIND, THIN ? 1 : 4, THIN ? 2 : 4, THIN ? 4 : 2, AS, BS>;
+template <int RAW, class T, bool SLOW> struct ce_or_raw { typedef tp_raw_tile<SLOW, RAW == 2> type; };
+template <class T, bool SLOW> struct ce_or_raw<0, T, SLOW> { typedef T type; };
 template <int MT, int NT>
 __device__ __forceinline__ void ce_none(tp_acc (&c)[MT][NT]) {
 #pragma unroll
@@ -331,19 +338,19 @@ __device__ __forceinline__ uint32_t ce_over(uint32_t n, uint32_t d) { return (n 
 // vocabulary needs leaves the registers: per row and wave (128 ids, or 32) their
 // maximum and the sum of exponentials relative to it, and for the gradient the
 // exponentials.
-template <int DT, bool GRAD, bool THIN>
+template <int DT, bool GRAD, bool THIN, int RAW>
 __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_logits(ce_args a) {
-    typedef ce_tile<DT == ZS_F32 ? TP_TWO : DT, THIN, false, false> T;
+    typedef typename ce_or_raw<RAW, ce_tile<DT == ZS_F32 ? TP_TWO : DT, THIN, false, false>, false>::type T;
     constexpr int MT = T::M, NT = T::N;
     const uint32_t n = ce_rows(a), mt = a.Vp / T::BM, nt = ce_over(n, T::BN), t = tp_place(blockIdx.x, mt * nt);
     if (t == ~0u) return;
     const uint2 at = tp_order(t, mt, nt);
-    const tp_mat mw = ce_mat_w<DT>(a, false), mh = ce_mat_h<DT>(a, false);
+    const tp_mat mw = RAW ? ce_mat_raw(a, false) : ce_mat_w<DT>(a, false), mh = ce_mat_h<DT>(a, false);
     T tile(mw, mh, at.x, at.y);
     tp_acc c[MT][NT];
     ce_none(c);
     tile.run(0, a.Dp / TP_KSTEP, c);
-    if constexpr (DT == ZS_F32) {
+    if constexpr (DT == ZS_F32 && !RAW) {
         const int sw = ce_weight_shift(a);
 #pragma unroll
         for (int j = 0; j < NT; j++) {
@@ -578,22 +585,22 @@ __device__ __forceinline__ ce_cut ce_parts(const ce_args& a) {
 
 // Gradient of the hidden states, a tile of columns (m) and rows (n), over the
 // vocabulary or a part of it.
-template <int DT, bool THIN>
+template <int DT, bool THIN, int RAW>
 __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_dhidden(ce_args a) {
-    typedef ce_tile<ce_kind(DT, THIN, false), THIN, true, false> T;
+    typedef typename ce_or_raw<RAW, ce_tile<ce_kind(DT, THIN, false), THIN, true, false>, true>::type T;
     constexpr int MT = T::M, NT = T::N;
     const ce_cut p = ce_parts<T>(a);
     const uint32_t n = ce_rows(a), tiles = p.mt * p.nt, u = tp_place(blockIdx.x, tiles * p.parts);
     if (u == ~0u) return;
     const uint32_t part = u / tiles, k0 = part * p.steps, all = a.Vp / TP_KSTEP;
     const uint2 at = tp_order(u - part * tiles, p.mt, p.nt);
-    const tp_mat mw = ce_mat_w<DT>(a, true), md = ce_mat_dl<DT>(a, false);
+    const tp_mat mw = RAW ? ce_mat_raw(a, true) : ce_mat_w<DT>(a, true), md = ce_mat_dl<DT>(a, false);
     T tile(mw, md, at.x, at.y);
     tp_acc c[MT][NT];
     ce_none(c);
     tile.run(k0, all - k0 < p.steps ? all - k0 : p.steps, c);
     const float un = ldexpf(1.0f, -ce_shift<DT>(a));
-    if constexpr (DT == ZS_F32) {
+    if constexpr (DT == ZS_F32 && !RAW) {
         const int sw = ce_weight_shift(a);
 #pragma unroll
         for (int j = 0; j < NT; j++) {
@@ -721,21 +728,21 @@ __global__ __launch_bounds__(CE_NT, THIN ? 3 : 1) void zs_k_ce_dweight(ce_args a
     }
 }
 
-template <int DT, bool THIN>
+template <int DT, bool THIN, int RAW>
 static void ce_products(const ce_args& a, hipStream_t stream) {
     const dim3 wg(CE_NT);
-    const uint32_t bm = THIN ? CE_THIN_M : CE_TILE, rt = THIN ? 1u : a.R / CE_TILE, vt = a.Vp / bm, dt = (a.D + bm - 1u) / bm;
+    const uint32_t bm = THIN ? CE_THIN_M : CE_TILE, rt = THIN ? (a.N + CE_THIN - 1u) / CE_THIN : a.R / CE_TILE, vt = a.Vp / bm, dt = (a.D + bm - 1u) / bm;
     const dim3 grid(tp_places(vt * rt));
     if (!(a.want & (CE_DH | CE_DW))) {
-        hipLaunchKernelGGL((zs_k_ce_logits<DT, false, THIN>), grid, wg, 0, stream, a);
+        hipLaunchKernelGGL((zs_k_ce_logits<DT, false, THIN, RAW>), grid, wg, 0, stream, a);
         hipLaunchKernelGGL((zs_k_ce_loss<DT, false>), dim3(a.R), wg, 0, stream, a);
         return;
     }
-    hipLaunchKernelGGL((zs_k_ce_logits<DT, true, THIN>), grid, wg, 0, stream, a);
+    hipLaunchKernelGGL((zs_k_ce_logits<DT, true, THIN, RAW>), grid, wg, 0, stream, a);
     hipLaunchKernelGGL((zs_k_ce_loss<DT, true>), dim3(a.R), wg, 0, stream, a);
     hipLaunchKernelGGL(zs_k_ce_grad<DT>, dim3((a.Vp / 8u + CE_NT - 1u) / CE_NT, a.R), wg, 0, stream, a);
     if (a.want & CE_DH) {
-        hipLaunchKernelGGL((zs_k_ce_dhidden<DT, THIN>), dim3(tp_places(dt * rt > a.units ? dt * rt : a.units)), wg, 0, stream, a);
+        hipLaunchKernelGGL((zs_k_ce_dhidden<DT, THIN, RAW>), dim3(tp_places(dt * rt > a.units ? dt * rt : a.units)), wg, 0, stream, a);
         hipLaunchKernelGGL((zs_k_ce_join<DT, THIN>), dim3(a.R, (a.D + 255u) / 256u), wg, 0, stream, a);
     }
     if (a.want & CE_DW) {
@@ -747,15 +754,18 @@ template <int DT>
 static void ce_go(ce_args a, hipStream_t stream) {
     const dim3 wg(CE_NT);
     if (a.N > CE_SELF) hipLaunchKernelGGL(zs_k_ce_rows, dim3(1), dim3(1024), 0, stream, a);
-    if (DT == ZS_F32) hipLaunchKernelGGL(zs_k_ce_max, dim3(CE_MAXIMA), wg, 0, stream, a);
+    if (DT == ZS_F32 && a.w) hipLaunchKernelGGL(zs_k_ce_max, dim3(CE_MAXIMA), wg, 0, stream, a);
     if (a.w) hipLaunchKernelGGL(zs_k_ce_weight<DT>, dim3(8192, (a.V + 65535u) / 65536u), wg, 0, stream, a);
     for (uint32_t p = 0; p < a.pieces; p++) {
         a.lo = p * a.R;
         a.first = p == 0u;
         a.last = p + 1u == a.pieces;
         hipLaunchKernelGGL(zs_k_ce_pack<DT>, dim3(a.R), wg, 0, stream, a);
-        if (a.thin) ce_products<DT, true>(a, stream);
-        else ce_products<DT, false>(a, stream);
+        constexpr int ONE = DT == ZS_F32 ? 1 : 0;   // (f32 alone has them)
+        if (a.raw == 1u) ce_products<DT, true, ONE>(a, stream);
+        else if (a.raw) ce_products<DT, true, 2 * ONE>(a, stream);
+        else if (a.thin) ce_products<DT, true, false>(a, stream);
+        else ce_products<DT, false, false>(a, stream);
     }
 }
 int ce_launch(const ce_args& a, uint32_t dtype, hipStream_t stream) {

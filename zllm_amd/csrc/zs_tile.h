@@ -375,6 +375,182 @@ struct tp_tile {
     }
 };
 
+// The same product with an f32 A that lies in memory as it is (ANY: its rows at any
+// number, fetched one by one, not by 16 bytes) and three planes of B: 128 x 64 a
+// workgroup, each wave's 32 rows of A split into planes in its registers (44
+// instructions for 16 columns of 32 rows, beside 12 products of them). Where there
+// are few n: nothing of A is written and read again. ld, k and rows of A's tp_mat
+// count f32 numbers.
+template <bool SLOW, bool ANY>
+struct tp_raw_tile {
+    static constexpr int M = 1, N = 2, BM = 128, BN = 64;
+    static constexpr int SA = BM * 128, SB = BN * 64, STAGE = SA + 3 * SB;
+    typedef tp_side<BN, false> B;
+    const tp_mat &ma, &mb;
+    B b;
+    const char* base;
+    static constexpr int L = ANY ? 16 : 4, G = ANY ? 4 : 16;   // a lane's loads of A a step, bytes of each
+    uint32_t m0, n0, off[SLOW && ANY ? 2 : SLOW ? 4 : L], ka, kmax, ld4, rd;
+
+    __device__ __forceinline__ static uint32_t wm() { return (uint32_t)__builtin_amdgcn_readfirstlane(zs_wid()); }
+    __device__ __forceinline__ static uint32_t wn() { return 0; }
+    __device__ __forceinline__ uint32_t n_of(int j) const { return n0 + (uint32_t)j * 32u + ((uint32_t)zs_lane() & 31u); }
+    __device__ __forceinline__ uint32_t m_of(int i, int q) const {
+        return m0 + wm() * 32u + (uint32_t)i * 32u + (uint32_t)q * 8u + ((uint32_t)zs_lane() >> 5) * 4u;
+    }
+    __device__ __forceinline__ tp_raw_tile(const tp_mat& ma_, const tp_mat& mb_, uint32_t m, uint32_t n) : ma(ma_), mb(mb_), m0(m * BM), n0(n * BN) {
+        const uint32_t l = (uint32_t)zs_lane(), w = wm(), r = l & 31u, h = l >> 5;
+        b.start(mb, n0, 0);
+        ld4 = (uint32_t)ma.ld * 4u;
+        if constexpr (!SLOW) {
+            // row r's eight 16-byte pieces at r * 128 B, piece c in place c ^ (r & 7)
+            const uint32_t x = m0 < ma.rows ? m0 : ma.rows - 1u;
+            base = (const char*)ma.p[0] + (uint64_t)x * ld4;
+            // load i of wave w fetches rows from (i * 4 + w) * R on, R a load
+            constexpr uint32_t R = 64u * G / 128u, PER = 64u / R;
+            kmax = ma.k * 4u - G;
+            const uint32_t rl = l / PER;
+            // (a row's place among eight, the same for all i)
+            const uint32_t r7 = ANY ? (w * 2u + rl) & 7u : rl & 7u;
+            ka = ANY ? ((((l & 31u) >> 2) ^ r7) * 4u + (l & 3u)) * 4u : ((l & 7u) ^ r7) * 16u;
+#pragma unroll
+            for (int i = 0; i < L; i++) {
+                uint32_t row = m0 + ((uint32_t)i * 4u + w) * R + rl;
+                row = row < ma.rows ? row : ma.rows - 1u;
+                off[i] = (row - x) * ld4;
+            }
+            rd = (w * 32u + r) * 128u + (r & 7u) * 16u;      // (place of piece 0; piece c's is that ^ 16 c)
+        } else {
+            // row k's 32 pieces at k * 512 B, piece c in place c ^ (k & 8)
+            base = (const char*)ma.p[0] + (uint64_t)m0 * 4u;
+            if constexpr (!ANY) {
+                const uint32_t last = (ma.rows >> 2) - 1u - (m0 >> 2);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t k = (uint32_t)i * 8u + w * 2u + h;
+                    const uint32_t c = (l & 31u) ^ (k & 8u);
+                    off[i] = (c < last ? c : last) * 16u;
+                }
+            } else {
+                // a load: half of a row, k = (i * 4 + w) / 2; pieces moved by 8 are the other 32 numbers of the half
+                const uint32_t last = ma.rows - 1u - m0;
+#pragma unroll
+                for (int z = 0; z < 2; z++) {
+                    const uint32_t e = ((w & 1u) * 64u + l) ^ (uint32_t)z * 32u;
+                    off[z] = (e < last ? e : last) * 4u;
+                }
+            }
+            ka = ANY ? w >> 1 : w * 2u + h;
+            kmax = ma.k;
+            rd = h * 8u * 512u + ((w * 32u + r) * 4u ^ h * 128u);
+        }
+    }
+    __device__ __forceinline__ static tp_lds* stage(uint32_t i) {
+        __shared__ char s0_[STAGE], s1_[STAGE];
+        return i == 0u ? (tp_lds*)s0_ : (tp_lds*)s1_;
+    }
+    __device__ __forceinline__ static void fetch(const char* p, tp_lds* s) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        // (the size has to be a number as it stands)
+        if constexpr (ANY) __builtin_amdgcn_global_load_lds((tp_glb*)p, s, 4, 0, 0);
+        else __builtin_amdgcn_global_load_lds((tp_glb*)p, s, 16, 0, 0);
+#endif
+    }
+    __device__ __forceinline__ void put(uint32_t kt, tp_lds* s) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        const uint32_t w = wm();
+        if constexpr (!SLOW) {
+            uint32_t k = kt * 128u + ka;
+            k = k < kmax ? k : kmax;
+#pragma unroll
+            for (int i = 0; i < L; i++) fetch(base + (off[i] + k), s + (i * 256 * G + w * 64u * G));
+        } else {
+            const uint32_t k0 = kt * 32u < kmax ? kt * 32u : kmax - 1u, end = kmax - 1u - k0;
+            const char* p = base + (uint64_t)k0 * ld4;
+#pragma unroll
+            for (int i = 0; i < L; i++) {
+                uint32_t k = ka + (uint32_t)i * (ANY ? 2u : 8u);
+                // (a row's number is that of its place: the clamped one's pieces stay where the row's own would)
+                const uint32_t o = ANY ? off[(i >> 2) & 1] : off[i & 3];
+                k = k < end ? k : end;
+                fetch(p + (uint64_t)k * ld4 + o, s + (i * 256 * G + w * 64u * G));
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 3; q++) {
+            b.plane(mb, q, n0);
+            b.load(kt, s + SA + q * SB);
+        }
+#endif
+    }
+    // 16 columns ks of the wave's rows as planes: lane l has row l % 32, k (l / 32) * 8 on
+    __device__ __forceinline__ void split(const tp_lds* s, int ks, tp_s8 (&p)[3]) const {
+        typedef float f4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) f4 l4;
+        typedef __attribute__((address_space(3))) float l1;
+        float x[8];
+        if constexpr (!SLOW) {
+            const uint32_t h = (uint32_t)zs_lane() >> 5;
+            const uint32_t c = (uint32_t)ks * 4u + h * 2u;
+            const f4 u = *(const l4*)(s + (rd ^ (c * 16u))), v = *(const l4*)(s + (rd ^ ((c + 1u) * 16u)));
+#pragma unroll
+            for (int k = 0; k < 4; k++) x[k] = u[k], x[k + 4] = v[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++) x[k] = *(const l1*)(s + rd + (ks * 16 + k) * 512);
+        }
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int q = 0; q < 3; q++) {
+            u4 o;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const b2 v = {(__bf16)x[2 * k], (__bf16)x[2 * k + 1]};
+                o[k] = __builtin_bit_cast(uint32_t, v);
+                if (q < 2) {
+                    x[2 * k] -= __uint_as_float(o[k] << 16);
+                    x[2 * k + 1] -= __uint_as_float(o[k] & 0xffff0000u);
+                }
+            }
+            p[q] = __builtin_bit_cast(tp_s8, o);
+        }
+    }
+    __device__ __forceinline__ void mul(const tp_lds* s, tp_acc (&c)[1][2]) const {
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+            tp_s8 x[3];
+            split(s, ks, x);
+#pragma unroll
+            for (int e = 0; e < 6; e++) {
+                constexpr uint32_t A = tp_planes<TP_THREE>::A, P = tp_planes<TP_THREE>::B;
+                const int pa = (int)(A >> (4 * e)) & 15, pb = (int)(P >> (4 * e)) & 15;
+#pragma unroll
+                for (int j = 0; j < 2; j++) c[0][j] = tp_mfma<TP_THREE>(x[pa], b.frag(s + SA + pb * SB, j, ks), c[0][j]);
+            }
+        }
+    }
+    __device__ __forceinline__ void run(uint32_t k0, uint32_t n, tp_acc (&c)[1][2]) {
+        tp_lds *s0 = stage(0), *s1 = stage(1);
+        if (n == 0u) return;
+        put(k0, s0);
+        uint32_t k = 1u;
+        for (; k < n; k += 2u) {
+            tp_arrived<0, true>();
+            put(k0 + k, s1);
+            mul(s0, c);
+            tp_arrived<0, true>();
+            if (k + 1u < n) put(k0 + k + 1u, s0);
+            mul(s1, c);
+        }
+        if (k == n) {
+            tp_arrived<0, true>();
+            mul(s0, c);
+        }
+        tp_arrived<0, true>();
+    }
+};
+
 // Workgroup id's place among n pieces of work (~0: none). Workgroups id, id + 8,
 // ... run on one XCD: each XCD has a run of pieces of its own.
 __device__ __forceinline__ uint32_t tp_place(uint32_t id, uint32_t n) {

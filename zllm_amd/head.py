@@ -30,7 +30,7 @@ from .engine import Context, _check
 
 MAX_HIDDEN = 65536
 MAX_LD = 4194304
-_DHIDDEN, _DWEIGHT, _COPY = 1, 2, 4
+_DHIDDEN, _DWEIGHT, _COPY, _FAR = 1, 2, 4, 8
 # the arguments are packed to bytes, as zllm_amd.beam's
 _CE = struct.Struct("=4I2Q3QqfI10Q")
 _Q4 = struct.Struct("=4IQ2I6Q")
@@ -70,8 +70,11 @@ def _call(ctx, entry, what, hidden, weight, labels, cfg, row_grad=None, want=(Fa
     dw = torch.empty((V, D), dtype=hidden.dtype, device=dev) if want[1] else None
     bits = (_DHIDDEN if want[0] else 0) | (_DWEIGHT if want[1] else 0)
     at, ldw = weight.data_ptr(), _ld(weight)
-    if hidden.dtype == torch.float32 or at % 16 or D % 8 or (V > 1 and ldw % 8) or ldw > MAX_LD:
+    size = hidden.element_size()
+    if at % 16 or D * size % 16 or (V > 1 and ldw * size % 16):
         bits |= _COPY
+    if ldw > MAX_LD:
+        bits |= _FAR
     nbytes = _work_bytes("zs_ce_work", N, V, D, DTYPES[hidden.dtype], bits)
     work, work_at = _work(nbytes, dev)
     rg, rg_stride = (row_grad.data_ptr(), row_grad.stride(0) if row_grad.dim() else 0) if row_grad is not None else (0, 0)
