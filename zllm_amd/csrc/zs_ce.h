@@ -76,10 +76,14 @@ inline uint64_t ce_work(ce_args& a, uint32_t dtype, void* work) {
     a.Dp = (uint32_t)ce_up(a.D, TP_KSTEP);
     a.Vp = (uint32_t)ce_up(a.V, CE_TILE);
     a.Dm = (uint32_t)ce_up(a.D, 4);
-    // A tile of 256 rows is 192 of them for nothing where there are 64: us of the
-    // logits TODO
     a.raw = !wide || (a.want & CE_FAR) || a.N > CE_RAW ? 0u : a.want & CE_COPY ? 2u : 1u;
-    a.thin = a.raw || a.N <= CE_THIN;
+    // A tile of 256 rows is 192 of them for nothing where there are 64, but the thin
+    // tiles of 65 rows read the weight twice. us of a bf16 loss by thin tiles and by
+    // others, 896 x 151936: 64 rows 67 and 118, 128 rows 92 and 118, 160 rows 116 and
+    // 121; 4096 x 151936: 271 and 414, 389 and 424, 498 and 415; of a step, whose two
+    // other products a tile more costs as much each, 896 x 151936: 64 rows 326 and 351,
+    // 65 rows 421 and 357
+    a.thin = a.raw || a.N <= (grad ? CE_THIN : 2u * CE_THIN);
     a.sub = a.thin ? 32u : 128u;
     a.subs = a.Vp / a.sub;
     uint64_t R = CE_ROOM / ((uint64_t)a.Vp * (wide ? 4u + (dw ? 6u : 0u) + (dh ? 4u : 0u) : 2u)) / CE_TILE * CE_TILE;
