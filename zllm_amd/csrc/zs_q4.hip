@@ -428,17 +428,17 @@ struct q4_batch {
         put(1, g1, s1);
         tp_in_order();
         for (uint32_t b = 0; b < whole; b += 3u) {
-            tp_arrived<LOADS>();
+            tp_arrived<LOADS, true>();
             put(b + 2u, g2, s2);
             mul(g0, s0);
-            tp_arrived<LOADS>();
+            tp_arrived<LOADS, true>();
             put(b + 3u, g0, s0);
             mul(g1, s1);
-            tp_arrived<LOADS>();
+            tp_arrived<LOADS, true>();
             put(b + 4u, g1, s1);
             mul(g2, s2);
         }
-        tp_arrived<0>();
+        tp_arrived<0, true>();
         if (n - whole > 0u) mul(g0, s0);
         if (n - whole > 1u) mul(g1, s1);
     }
@@ -493,15 +493,25 @@ static void q4_few_go(const q4_args& a, hipStream_t stream) {
 template <int DT, int G, bool MINS>
 static void q4_go(const q4_args& a, hipStream_t stream) {
     if (a.B > 16u) {
-        // tiles a wave such that all workgroups find room at once, two a CU
-        const uint32_t t = (a.at.tiles + 2047u) / 2048u;
-        if constexpr (DT == ZS_F32) q4_batch_go<DT, G, MINS, 2, 2>(a, stream);
-        else if (a.B <= 32u) t <= 2u ? q4_batch_go<DT, G, MINS, 2, 2>(a, stream) : q4_batch_go<DT, G, MINS, 4, 2>(a, stream);
-        else if (a.B > 64u || t == 4u || t > (G == 32 && !MINS ? 5u : 4u)) q4_batch_go<DT, G, MINS, 4, 4>(a, stream);
-        else if (t == 1u) q4_batch_go<DT, G, MINS, 1, 4>(a, stream);
-        else if (t == 2u) q4_batch_go<DT, G, MINS, 2, 4>(a, stream);
-        else if (t == 3u) q4_batch_go<DT, G, MINS, 3, 4>(a, stream);
-        else if constexpr (G == 32 && !MINS) q4_batch_go<DT, G, MINS, 5, 4>(a, stream);
+        // Tiles of ids a wave: as many as let all workgroups find room at once, two a CU
+        // (one, where a workgroup a CU is all there is). us, 64 bf16 rows of 4096, groups
+        // of 32, by 1, 2, 3, 4 and 5 tiles: 16000 ids 29 and 37; 32000 ids 46, 40 and (4)
+        // 55; 90000 ids (2) 75, 70 and 84; 128256 ids (2) 117 and (4) 102; 151936 ids (2)
+        // 139, (4) 136 and 122. Up to 32 rows, of which a workgroup has 32 and not 64, two
+        // (17 rows by 2 and by as many as find room: 90000 ids 47 and 57, 128256 ids 66 and
+        // 68, 151936 ids 83 and 92; by 64 rows a workgroup 78, 95 and 126). Beyond 64 rows a
+        // part of the rows finds another's codes in the L2, and 4 serve. Of larger groups or
+        // with minima 5 do not fit the registers.
+        uint32_t t = (a.at.tiles + 2047u) / 2048u;
+        t = a.at.tiles <= 1024u ? 1u : t < 2u ? 2u : t;
+        if (DT == ZS_F32 || a.B <= 32u) q4_batch_go<DT, G, MINS, 2, 2>(a, stream);
+        else if constexpr (DT != ZS_F32) {
+            if (a.B > 64u || t == 4u || t > (G == 32 && !MINS ? 5u : 4u)) q4_batch_go<DT, G, MINS, 4, 4>(a, stream);
+            else if (t == 1u) q4_batch_go<DT, G, MINS, 1, 4>(a, stream);
+            else if (t == 2u) q4_batch_go<DT, G, MINS, 2, 4>(a, stream);
+            else if (t == 3u) q4_batch_go<DT, G, MINS, 3, 4>(a, stream);
+            else if constexpr (G == 32 && !MINS) q4_batch_go<DT, G, MINS, 5, 4>(a, stream);
+        }
         return;
     }
     // Waves along the columns where there are few ids: 4 against 1, us, 16 bf16
