@@ -258,6 +258,37 @@ def test_one_gradient_alone():
     assert torch.equal(check(*args, need_hidden=False)[2], both[2])
 
 
+@pytest.mark.parametrize("D,shift,pad", [(96, 0, 0), (100, 4, 4), (100, 1, 3), (97, 0, 0), (1, 0, 0), (3, 2, 0), (1030, 0, 2)])
+@pytest.mark.parametrize("N", [1, 64, 65, 129, 192, 193])
+def test_f32_rows_where_the_way_changes(N, D, shift, pad):
+    """A few rows take an f32 weight as it lies, by 16 bytes or number by number, more
+    of them a copy."""
+    check(*inputs(N, 1101, D, "f32", seed=N + D, shift=shift, pad=pad, ignored=0.1 if N > 1 else 0.0), what="f32 rows")
+
+
+@pytest.mark.parametrize("D", [64, 70])
+def test_one_gradient_of_few_f32_rows(D):
+    args = inputs(70, 700, D, "f32", seed=D)
+    both = check(*args)
+    assert torch.equal(check(*args, need_weight=False)[1], both[1])
+    assert torch.equal(check(*args, need_hidden=False)[2], both[2])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("N", [63, 65, 127, 128, 129])
+def test_rows_where_the_tiles_change(N, dtype):
+    check(*inputs(N, 2000, 136, dtype, seed=N), what="tiles")
+
+
+@pytest.mark.parametrize("N", [5, 300])
+def test_f32_rows_far_apart(N):
+    """Further than the products' offsets reach: copied whatever the rows' number."""
+    h, W, labels, g = inputs(N, 6, 64, "f32", seed=N)
+    buf = torch.full((6, 5_000_000), float("nan"), device="cuda")
+    buf[:, 100:164] = W
+    check(h, buf[:, 100:164], labels, g, what="far f32 weight")
+
+
 def test_same_results_every_time():
     args = inputs(700, 5000, 256, "bf16", seed=15, ignored=0.2)
     from zllm_amd.head import head_loss_grad

@@ -300,14 +300,14 @@ template <int DT>
 __device__ __forceinline__ tp_mat ce_mat_h(const ce_args& a, bool slow) {
     const uint64_t plane = (uint64_t)a.R * a.Dp;
     const uint16_t* p = DT == ZS_F32 && !slow && !a.raw ? a.h2 : a.h;
-    tp_mat m = {{p, p + plane, p + 2 * plane}, a.Dp, slow ? a.Dp : a.R, slow ? a.R : a.Dp};
+    tp_mat m = {{p, p + plane, p + 2 * plane}, a.Dp, slow ? a.Dp : ce_rows(a), slow ? a.R : a.Dp};
     return m;
 }
 template <int DT>
 __device__ __forceinline__ tp_mat ce_mat_dl(const ce_args& a, bool slow) {
     const uint64_t plane = (uint64_t)a.R * a.Vp;
     const uint16_t* p = DT == ZS_F32 && !slow && !a.raw ? a.dl2 : a.dl;
-    tp_mat m = {{p, p + plane, p + 2 * plane}, a.Vp, slow ? a.Vp : a.R, slow ? a.R : a.Vp};
+    tp_mat m = {{p, p + plane, p + 2 * plane}, a.Vp, slow ? a.Vp : ce_rows(a), slow ? a.R : a.Vp};
     return m;
 }
 
