@@ -226,8 +226,7 @@ __device__ __forceinline__ int ce_weight_shift(const ce_args& a) {   // (by whol
     return zs_split2_of(wave_max_f(top));
 }
 // The weight in rows of Dp, its planes apart, where its own rows do not serve.
-// A row may begin at any element: 16-bit rows are read as the aligned 16 bytes
-// that hold them, eight values of a row put together from two of those.
+// A row may begin at any element.
 template <int DT>
 __global__ __launch_bounds__(CE_NT) void zs_k_ce_weight(ce_args a) {
     const uint64_t plane = (uint64_t)a.V * a.Dp;
@@ -261,19 +260,17 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_weight(ce_args a) {
                     *(hd_u4*)(o + q * plane) = u;
                 }
             } else {
-                const hd_u4 lo = j < row.nvec ? row.raw(j) : hd_row<DT>::none(), hi = j + 1u < row.nvec ? row.raw(j + 1u) : hd_row<DT>::none();
-                const uint32_t w[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                uint32_t u[5];
-                // from word shift / 2 on (the row's own shift: the same for all lanes)
-#pragma unroll
-                for (int k = 0; k < 5; k++) u[k] = row.shift < 2u ? w[k] : row.shift < 4u ? w[k + 1] : row.shift < 6u ? w[k + 2] : w[(k + 3) & 7];
+                typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));   // (a row's eight values may lie anywhere)
                 hd_u4 x;
+                if (d0 + 8u <= a.D) {
+                    x = zs_gload((const u4*)(row.row + d0));
+                } else {
+                    const uint16_t* r = (const uint16_t*)row.row;
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    x[k] = row.shift & 1u ? u[k] >> 16 | u[k + 1] << 16 : u[k];
-                    // values past the row are none of it
-                    const uint32_t d = d0 + 2u * k;
-                    x[k] = d + 1u < a.D ? x[k] : d < a.D ? x[k] & 0xffffu : 0u;
+                    for (uint32_t k = 0; k < 4u; k++) {
+                        const uint32_t d = d0 + 2u * k;
+                        x[k] = (d < a.D ? (uint32_t)r[d] : 0u) | (d + 1u < a.D ? (uint32_t)r[d + 1u] << 16 : 0u);
+                    }
                 }
                 *(hd_u4*)o = x;
             }
