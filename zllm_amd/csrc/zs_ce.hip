@@ -548,20 +548,22 @@ template <int DT, class T, class P, class I>
 __device__ __forceinline__ void ce_out(const T& tile, void* out, uint64_t ld, uint32_t D, uint32_t d0, const P& put, const I& row) {
     uint16_t* o = (uint16_t*)out;
     if (d0 >= D) return;
-    if (D % 8u == 0u && ld % 8u == 0u && ((uintptr_t)out & 15u) == 0u) {
-        const auto none = [](int) {};
+    typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));   // (a row may begin at any element)
+    const auto none = [](int) {};
+    if (D % 8u == 0u) {
         tile.rows(none, put, none, [&](uint32_t r, uint32_t m, hd_u4 v) {
             const uint64_t to = row(r);
-            if (to != ~0ull && d0 + m < D) *(hd_u4*)(o + to * ld + d0 + m) = v;
+            if (to != ~0ull && d0 + m < D) *(u4*)(o + to * ld + d0 + m) = v;
         });
     } else {
-        tile.rows_any(
-            put,
-            [&](uint32_t r) {
-                const uint64_t to = row(r);
-                return to == ~0ull ? (uint16_t*)nullptr : o + to * ld + d0;
-            },
-            D - d0 < 32u * T::M ? D - d0 : 32u * T::M);
+        tile.rows(none, put, none, [&](uint32_t r, uint32_t m, hd_u4 v) {
+            const uint64_t to = row(r);
+            if (to == ~0ull || d0 + m >= D) return;
+            uint16_t* p = o + to * ld + d0 + m;
+            if (d0 + m + 8u <= D) *(u4*)p = v;
+            else
+                for (uint32_t k = 0; k < D - d0 - m; k++) p[k] = (uint16_t)(v[k >> 1] >> (k & 1u) * 16u);
+        });
     }
 }
 

@@ -305,7 +305,7 @@ struct tp_tile {
     // values of each of its rows, so written from there a row's 256 bytes would go
     // out in 16-byte pieces. begin(j) and end(j) come before and behind the values
     // of 32 rows; put(i, j, q) gives the two words of four values.
-    template <uint32_t STEP, bool PLAIN, class P>
+    template <class P>
     __device__ __forceinline__ void turn(tp_lds* s, int j, const P& put) const {
         typedef uint32_t u2 __attribute__((ext_vector_type(2)));
         typedef __attribute__((address_space(3))) u2 l2;
@@ -316,11 +316,11 @@ struct tp_tile {
             for (int q = 0; q < 4; q++) {
                 const uint2 v = put(i, j, q);
                 const uint32_t c = i * 4u + q;
-                *(l2*)(s + n * STEP + (PLAIN ? c : c ^ (n & (4u * MT - 1u))) * 16u + (l >> 5) * 8u) = u2{v.x, v.y};
+                *(l2*)(s + n * (64 * MT) + (c ^ (n & (4u * MT - 1u))) * 16u + (l >> 5) * 8u) = u2{v.x, v.y};
             }
     }
     __device__ __forceinline__ static tp_lds* mine() {   // the wave's share of the memory, room for 32 rows
-        static_assert(32 * (64 * MT + 16) <= STAGE / 2, "32 rows of a wave's values fit its share of the memory");
+        static_assert(32 * 64 * MT <= STAGE / 2 && 32 * 128 <= STAGE / 2, "32 rows of a wave's values fit its share of the memory");
         const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane(zs_wid());
         return stage(w >> 1) + (w & 1u) * (STAGE / 2);
     }
@@ -335,37 +335,12 @@ struct tp_tile {
 #pragma unroll
         for (int j = 0; j < NT; j++) {
             begin(j);
-            turn<64 * MT, false>(s, j, put);
+            turn(s, j, put);
             end(j);
 #pragma unroll
             for (uint32_t t = 0; t < 32u; t += 64u / C) {
                 const uint32_t r = t + l / C, c = l % C;
                 row(j * 32u + r, c * 8u, *(const l4*)(s + r * (64 * MT) + (c ^ (r & (C - 1u))) * 16u));
-            }
-        }
-    }
-    // The same to rows at any element: at(r) is where the wave's row r begins (the
-    // same for all lanes), NULL for none, `count` how many of its values go there. A lane
-    // stores two at a time, from the first that lies at four bytes.
-    template <class P, class R>
-    __device__ __forceinline__ void rows_any(const P& put, const R& at, uint32_t count) const {
-        typedef uint32_t u1 __attribute__((aligned(2)));
-        typedef __attribute__((address_space(3))) u1 l1;
-        constexpr uint32_t STEP = 64 * MT + 16;
-        tp_lds* s = mine();
-        const uint32_t l = (uint32_t)zs_lane();
-#pragma unroll
-        for (int j = 0; j < NT; j++) {
-            turn<STEP, true>(s, j, put);
-#pragma unroll 4
-            for (uint32_t r = 0; r < 32u; r++) {
-                uint16_t* p = at(j * 32u + r);
-                if (!p) continue;
-                const uint32_t o = (uint32_t)((uintptr_t)p >> 1) & 1u, m = 2u * l + o;
-                const uint32_t v = *(const l1*)(s + r * STEP + m * 2u);
-                if (m + 1u < count) *(uint32_t*)(p + m) = v;
-                else if (m < count) p[m] = (uint16_t)v;
-                if (o && l == 0u) p[0] = *(const __attribute__((address_space(3))) uint16_t*)(s + r * STEP);
             }
         }
     }
