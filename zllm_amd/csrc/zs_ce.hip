@@ -703,8 +703,8 @@ __global__ __launch_bounds__(CE_NT, THIN ? 3 : 1) void zs_k_ce_dweight(ce_args a
 #pragma unroll
                 for (int q = 0; q < 16; q++) c[i][j][q] *= un;
     }
-    const bool vec = a.D % 4u == 0u && a.ld_dw % 4u == 0u && ((uintptr_t)a.dw & 15u) == 0u;
     if (!a.first || !a.last) {
+        const bool vec = a.D % 4u == 0u && a.ld_dw % 4u == 0u && ((uintptr_t)a.dw & 15u) == 0u;
 #pragma unroll
         for (int j = 0; j < T::N; j++) {
             const uint32_t id = tile.n_of(j);
@@ -733,7 +733,7 @@ __global__ __launch_bounds__(CE_NT, THIN ? 3 : 1) void zs_k_ce_dweight(ce_args a
         if (d0 >= a.D) return;
         tile.words(
             [&](int i, int j, int q) { return make_float4(c[i][j][4 * q], c[i][j][4 * q + 1], c[i][j][4 * q + 2], c[i][j][4 * q + 3]); },
-            [&](uint32_t r) { return id0 + r < a.V ? (float*)a.dw + (uint64_t)(id0 + r) * a.ld_dw + d0 : (float*)nullptr; }, a.D - d0, vec);
+            [&](uint32_t r) { return id0 + r < a.V ? (float*)a.dw + (uint64_t)(id0 + r) * a.ld_dw + d0 : (float*)nullptr; }, a.D - d0);
     } else {
         ce_out<DT>(tile, a.dw, a.ld_dw, a.D, tile.m0 + T::wm() * (32 * T::M),
                    [&](int i, int j, int q) {

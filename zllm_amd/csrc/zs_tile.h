@@ -345,14 +345,14 @@ struct tp_tile {
         }
     }
     // The same of f32 numbers, 32 x 32 at a time: get(i, j, q) gives four values,
-    // at(r) is where the wave's row r goes, NULL for nowhere (vec: all rows and their
-    // `count` columns by 16 bytes): of the gradient of 58134 x 3456 weights 337 ->
-    // 241 us, where rows begin at any number (140910 x 869) 414 -> 205.
+    // at(r) is where the wave's row r goes with its `count` columns, NULL for nowhere.
+    // (One f32 row's gradient of 58134 x 3456 weights, from the lanes as they have the
+    // values and so: 337 and 241 us.)
     template <class P, class R>
-    __device__ __forceinline__ void words(const P& get, const R& at, uint32_t count, bool vec) const {
+    __device__ __forceinline__ void words(const P& get, const R& at, uint32_t count) const {
         typedef float f4 __attribute__((ext_vector_type(4)));
+        typedef float f4a __attribute__((ext_vector_type(4), aligned(4)));   // (a row may begin at any number)
         typedef __attribute__((address_space(3))) f4 l4;
-        typedef __attribute__((address_space(3))) float l1;
         tp_lds* s = mine();
         const uint32_t l = (uint32_t)zs_lane(), n = l & 31u;
 #pragma unroll
@@ -364,22 +364,15 @@ struct tp_tile {
                     const float4 v = get(i, j, q);
                     *(l4*)(s + n * 128u + (((uint32_t)q * 2u + (l >> 5)) ^ (n & 7u)) * 16u) = f4{v.x, v.y, v.z, v.w};
                 }
-                if (vec) {
 #pragma unroll
-                    for (uint32_t t = 0; t < 4u; t++) {
-                        const uint32_t r = t * 8u + (l >> 3), c = l & 7u, m = (uint32_t)i * 32u + c * 4u;
-                        float* p = at((uint32_t)j * 32u + r);
-                        const f4 v = *(const l4*)(s + r * 128u + (c ^ (r & 7u)) * 16u);
-                        if (p && m < count) *(f4*)(p + m) = v;
-                    }
-                } else {
-#pragma unroll 4
-                    for (uint32_t t = 0; t < 16u; t++) {
-                        const uint32_t r = t * 2u + (l >> 5), m = (uint32_t)i * 32u + n;
-                        float* p = at((uint32_t)j * 32u + r);
-                        const float v = *(const l1*)(s + r * 128u + ((n >> 2) ^ (r & 7u)) * 16u + (n & 3u) * 4u);
-                        if (p && m < count) p[m] = v;
-                    }
+                for (uint32_t t = 0; t < 4u; t++) {
+                    const uint32_t r = t * 8u + (l >> 3), c = l & 7u, m = (uint32_t)i * 32u + c * 4u;
+                    float* p = at((uint32_t)j * 32u + r);
+                    const f4 v = *(const l4*)(s + r * 128u + (c ^ (r & 7u)) * 16u);
+                    if (!p) continue;
+                    if (m + 4u <= count) *(f4a*)(p + m) = v;
+                    else
+                        for (uint32_t k = 0; m + k < count; k++) p[m + k] = v[k];
                 }
             }
     }
