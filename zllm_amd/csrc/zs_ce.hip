@@ -543,7 +543,9 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_grad(ce_args a) {
 }
 
 // A gradient's tile of 16-bit values, whole rows at a time: out[row(r)] for the
-// wave's rows r, from column d0 on, columns before D.
+// wave's rows r, from column d0 on, columns before D. (Not read again here: stored
+// past the caches, one row's step over 151936 x 4096 bf16 weights takes 1010 us for
+// 1087, over 58134 x 3456 f32 ones 611 for 696.)
 template <int DT, class T, class P, class I>
 __device__ __forceinline__ void ce_out(const T& tile, void* out, uint64_t ld, uint32_t D, uint32_t d0, const P& put, const I& row) {
     uint16_t* o = (uint16_t*)out;
@@ -553,14 +555,14 @@ __device__ __forceinline__ void ce_out(const T& tile, void* out, uint64_t ld, ui
     if (D % 8u == 0u) {
         tile.rows(none, put, none, [&](uint32_t r, uint32_t m, hd_u4 v) {
             const uint64_t to = row(r);
-            if (to != ~0ull && d0 + m < D) *(u4*)(o + to * ld + d0 + m) = v;
+            if (to != ~0ull && d0 + m < D) __builtin_nontemporal_store((u4)v, (u4*)(o + to * ld + d0 + m));
         });
     } else {
         tile.rows(none, put, none, [&](uint32_t r, uint32_t m, hd_u4 v) {
             const uint64_t to = row(r);
             if (to == ~0ull || d0 + m >= D) return;
             uint16_t* p = o + to * ld + d0 + m;
-            if (d0 + m + 8u <= D) *(u4*)p = v;
+            if (d0 + m + 8u <= D) __builtin_nontemporal_store((u4)v, (u4*)p);
             else
                 for (uint32_t k = 0; k < D - d0 - m; k++) p[k] = (uint16_t)(v[k >> 1] >> (k & 1u) * 16u);
         });

@@ -370,7 +370,7 @@ struct tp_tile {
                     float* p = at((uint32_t)j * 32u + r);
                     const f4 v = *(const l4*)(s + r * 128u + (c ^ (r & 7u)) * 16u);
                     if (!p) continue;
-                    if (m + 4u <= count) *(f4a*)(p + m) = v;
+                    if (m + 4u <= count) __builtin_nontemporal_store((f4a)v, (f4a*)(p + m));
                     else
                         for (uint32_t k = 0; m + k < count; k++) p[m + k] = v[k];
                 }
