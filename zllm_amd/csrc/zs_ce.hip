@@ -545,7 +545,9 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_grad(ce_args a) {
 // A gradient's tile of 16-bit values, whole rows at a time: out[row(r)] for the
 // wave's rows r, from column d0 on, columns before D. (Not read again here: stored
 // past the caches, one row's step over 151936 x 4096 bf16 weights takes 1010 us for
-// 1087, over 58134 x 3456 f32 ones 611 for 696.)
+// 1087, over 58134 x 3456 f32 ones 611 for 696. Rows at
+// any element share their lines' ends and are left to the caches: 7 rows' step over
+// 140910 x 869 f32 weights takes 664 past them, 590 so.)
 template <int DT, class T, class P, class I>
 __device__ __forceinline__ void ce_out(const T& tile, void* out, uint64_t ld, uint32_t D, uint32_t d0, const P& put, const I& row) {
     uint16_t* o = (uint16_t*)out;
@@ -562,7 +564,7 @@ __device__ __forceinline__ void ce_out(const T& tile, void* out, uint64_t ld, ui
             const uint64_t to = row(r);
             if (to == ~0ull || d0 + m >= D) return;
             uint16_t* p = o + to * ld + d0 + m;
-            if (d0 + m + 8u <= D) __builtin_nontemporal_store((u4)v, (u4*)p);
+            if (d0 + m + 8u <= D) *(u4*)p = v;
             else
                 for (uint32_t k = 0; k < D - d0 - m; k++) p[k] = (uint16_t)(v[k >> 1] >> (k & 1u) * 16u);
         });
@@ -705,8 +707,8 @@ __global__ __launch_bounds__(CE_NT, THIN ? 3 : 1) void zs_k_ce_dweight(ce_args a
 #pragma unroll
                 for (int q = 0; q < 16; q++) c[i][j][q] *= un;
     }
+    const bool vec = a.D % 4u == 0u && a.ld_dw % 4u == 0u && ((uintptr_t)a.dw & 15u) == 0u;
     if (!a.first || !a.last) {
-        const bool vec = a.D % 4u == 0u && a.ld_dw % 4u == 0u && ((uintptr_t)a.dw & 15u) == 0u;
 #pragma unroll
         for (int j = 0; j < T::N; j++) {
             const uint32_t id = tile.n_of(j);
@@ -733,9 +735,10 @@ __global__ __launch_bounds__(CE_NT, THIN ? 3 : 1) void zs_k_ce_dweight(ce_args a
     if constexpr (DT == ZS_F32) {
         const uint32_t d0 = tile.m0 + T::wm() * (32 * T::M);
         if (d0 >= a.D) return;
-        tile.words(
-            [&](int i, int j, int q) { return make_float4(c[i][j][4 * q], c[i][j][4 * q + 1], c[i][j][4 * q + 2], c[i][j][4 * q + 3]); },
-            [&](uint32_t r) { return id0 + r < a.V ? (float*)a.dw + (uint64_t)(id0 + r) * a.ld_dw + d0 : (float*)nullptr; }, a.D - d0);
+        const auto get = [&](int i, int j, int q) { return make_float4(c[i][j][4 * q], c[i][j][4 * q + 1], c[i][j][4 * q + 2], c[i][j][4 * q + 3]); };
+        const auto row = [&](uint32_t r) { return id0 + r < a.V ? (float*)a.dw + (uint64_t)(id0 + r) * a.ld_dw + d0 : (float*)nullptr; };
+        if (vec) tile.template words<true>(get, row, a.D - d0);
+        else tile.template words<false>(get, row, a.D - d0);
     } else {
         ce_out<DT>(tile, a.dw, a.ld_dw, a.D, tile.m0 + T::wm() * (32 * T::M),
                    [&](int i, int j, int q) {

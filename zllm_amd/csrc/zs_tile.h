@@ -345,10 +345,11 @@ struct tp_tile {
         }
     }
     // The same of f32 numbers, 32 x 32 at a time: get(i, j, q) gives four values,
-    // at(r) is where the wave's row r goes with its `count` columns, NULL for nowhere.
+    // at(r) is where the wave's row r goes with its `count` columns, NULL for nowhere;
+    // PAST: past the caches (of two stores at run time the compiler makes an ordinary one).
     // (One f32 row's gradient of 58134 x 3456 weights, from the lanes as they have the
     // values and so: 337 and 241 us.)
-    template <class P, class R>
+    template <bool PAST, class P, class R>
     __device__ __forceinline__ void words(const P& get, const R& at, uint32_t count) const {
         typedef float f4 __attribute__((ext_vector_type(4)));
         typedef float f4a __attribute__((ext_vector_type(4), aligned(4)));   // (a row may begin at any number)
@@ -370,8 +371,10 @@ struct tp_tile {
                     float* p = at((uint32_t)j * 32u + r);
                     const f4 v = *(const l4*)(s + r * 128u + (c ^ (r & 7u)) * 16u);
                     if (!p) continue;
-                    if (m + 4u <= count) __builtin_nontemporal_store((f4a)v, (f4a*)(p + m));
-                    else
+                    if (m + 4u <= count) {
+                        if constexpr (PAST) __builtin_nontemporal_store((f4a)v, (f4a*)(p + m));
+                        else *(f4a*)(p + m) = v;
+                    } else
                         for (uint32_t k = 0; m + k < count; k++) p[m + k] = v[k];
                 }
             }
