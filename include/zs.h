@@ -556,7 +556,7 @@ int zs_distill_loss_grad(zs_ctx* ctx, const zs_distill* args, void* stream);
  * 16-bit numbers are exact; d is rounded to their type on its way into the
  * gradients' products (f16: scaled so that its largest factor is near 2^15).
  * f32 numbers are multiplied as sums of three bf16, to 2^-26 of each product; for
- * logits and dhidden of more than 256 rows (or a weight that is FAR) as sums of
+ * logits and dhidden of more than 192 rows (or a weight that is FAR) as sums of
  * two f16 of the number scaled by a power of two, of the whole weight, of a row of
  * hidden states and of a row of d: to 3 * 2^-22, and a number below 2^-18 of the
  * largest to 2^-40 of that. The gradients are rounded once.
@@ -570,7 +570,7 @@ int zs_distill_loss_grad(zs_ctx* ctx, const zs_distill* args, void* stream);
  * row_grad_stride 0 reads one value for all rows. `want` of zs_ce_work says
  * which gradients a call will have, (COPY) whether the weight's rows do not all
  * begin and end at 16 bytes and (FAR) whether they lie further apart than ZS_CE_LD
- * values (16-bit weights are then copied; f32 weights of more than 256 rows and
+ * values (16-bit weights are then copied; f32 weights of more than 192 rows and
  * those that are FAR). */
 #define ZS_CE_MAX_HIDDEN 65536u
 #define ZS_CE_LD 4194304u

@@ -7,6 +7,8 @@ each time it is called.
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -23,27 +25,34 @@ FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     # IEEE f32 behaviour the exact paths rely on: keep denormals, no contraction
     "-fno-gpu-flush-denormals-to-zero",
     "-ffp-contract=off",
     "-fno-fast-math",
-    # packed fp32 VALU ops are disabled for correctness on this pool
+    # some forms of packed fp32 VALU ops have given wrong results
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-I" + os.path.join(ROOT, "include"),
     "-Wno-unused-result",
 ]
 
 
-def build(verbose=False):
-    srcs = [os.path.join(CSRC, s) for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
-    cmd = [HIPCC] + FLAGS + srcs + ["-o", LIB + ".tmp"]
+def _run(cmd, verbose):
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)
         raise RuntimeError("hipcc failed building libzs.so")
+
+
+def build(verbose=False):
+    """The sources side by side (one behind the other they take four minutes), then the library."""
+    with tempfile.TemporaryDirectory(dir=HERE, prefix=".build") as tmp, ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
+        objs = [os.path.join(tmp, s + ".o") for s in SOURCES]
+        # (the longest first)
+        list(pool.map(lambda s: _run([HIPCC] + FLAGS + ["-c", os.path.join(CSRC, s), "-o", os.path.join(tmp, s + ".o")], verbose),
+                      reversed(SOURCES)))
+        _run([HIPCC, "--offload-arch=gfx950", "-fPIC", "-shared"] + objs + ["-o", LIB + ".tmp"], verbose)
     os.replace(LIB + ".tmp", LIB)
     return LIB
 

@@ -10,8 +10,8 @@
 #define CE_THIN 64          // rows
 // f32 weights are multiplied as they lie up to so many rows, and as two planes that
 // are made of them once above. us of the loss / of a step as they lie and as planes,
-// 3456 x 58134: 1 row 234 / 807 and 722 / 1372, 128 rows 408 / 1372 and 778 / 1802, 256
-// rows 738 / 2380 and 788 / 2124, 512 rows 1380 / 4485 and 1086 / 3191
+// 3456 x 58134: 1 row 218 / 610 and 700 / 1119, 128 rows 428 / 1260 and 819 / 1573, 192
+// rows 583 / 1750 and 785 / 1745, 256 rows 768 / 2280 and 793 / 1910
 #define CE_RAW 192u
 #define CE_ROOM (4ull << 30)   // bytes of exponentials kept at once (a piece of the rows)
 
