@@ -135,7 +135,9 @@ class HeadLoss(torch.nn.Module):
     """Loss per row, differentiable by the hidden states and the weight. Keeps
     neither logits nor exponentials between the passes: the backward pass makes
     the logits again, in pieces. (Where the rows' weights are known before the
-    loss, head_loss_grad makes them once.)"""
+    loss, head_loss_grad makes them once; it is also what belongs into a captured
+    HIP graph: autograd's own bookkeeping of leaves that an eager graph holds too
+    does not.)"""
 
     def __init__(self, ctx: Context, cfg: HeadLossConfig = HeadLossConfig()):
         super().__init__()
@@ -204,7 +206,8 @@ class Q4Head:
     def logits(self, hidden: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """float32 [B, V] for hidden [B, D] of any of the three types and any
         row stride. Without out the rows lie 4 values' multiples apart, as
-        zs_sample and zs_lane_step take them. No host sync."""
+        zs_sample and zs_lane_step take them. Not differentiable. No host
+        sync."""
         what = "Q4Head.logits"
         _matrix(self.ctx, hidden, what, "hidden")
         B, dev = hidden.shape[0], hidden.device
