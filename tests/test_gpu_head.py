@@ -280,7 +280,7 @@ def test_rows_where_the_tiles_change(N, dtype):
     check(*inputs(N, 2000, 136, dtype, seed=N), what="tiles")
 
 
-@pytest.mark.parametrize("N", [5, 300])
+@pytest.mark.parametrize("N", [5, 100, 300])
 def test_f32_rows_far_apart(N):
     """Further than the products' offsets reach: copied whatever the rows' number."""
     h, W, labels, g = inputs(N, 6, 64, "f32", seed=N)
