@@ -179,7 +179,11 @@ class Q4Head:
     """A head held in 4 bits: codes uint8 [V, D / 2] (0 to 15, the even
     column's in the low half of a byte), scales float16 [V, D / group] and
     perhaps minima likewise; w = scale * (code - 8), or scale * code + min. The
-    codes are laid out once, when it is made; what it is made from is not kept."""
+    codes are laid out once, when it is made; what it is made from is not kept.
+    That is done when the constructor returns (a host sync, but in a captured
+    graph), so logits may be asked for on any stream from then on, and a head
+    that is dropped keeps its memory until the streams that it was called on are
+    through. A captured graph has its address: keep the head as long as that."""
 
     def __init__(self, ctx: Context, codes: torch.Tensor, scales: torch.Tensor, mins: Optional[torch.Tensor] = None):
         what = "Q4Head"
@@ -198,6 +202,19 @@ class Q4Head:
                               self.group, self._data.data_ptr(), _stream(dev))
         if rc:
             _check(ctx.h, rc, what)
+        self._streams = {_stream(dev)}
+        with torch.cuda.device(dev):
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream().synchronize()
+
+    def _called_on(self, stream: int, dev) -> None:
+        """Another stream than those so far: torch's allocator is told of it, or
+        it would give the memory of a dropped head to the first stream's next
+        tensor while this one still reads it."""
+        with torch.cuda.device(dev):
+            if not torch.cuda.is_current_stream_capturing():
+                self._data.record_stream(torch.cuda.current_stream())
+                self._streams.add(stream)
 
     @classmethod
     def quantize(cls, ctx: Context, weight: torch.Tensor, group: int = 32, mins: bool = False) -> "Q4Head":
@@ -227,7 +244,10 @@ class Q4Head:
         work, work_at = _work(nbytes, dev)
         raw = _Q4.pack(self.V, self.D, self.group, int(self.mins), self._data.data_ptr(), B, DTYPES[hidden.dtype], at, ld,
                        out.data_ptr(), _ld(out), work_at, nbytes)
-        rc = lib().zs_q4_logits(self.ctx.h, raw, _stream(dev))
+        stream = _stream(dev)
+        if stream not in self._streams:
+            self._called_on(stream, dev)
+        rc = lib().zs_q4_logits(self.ctx.h, raw, stream)
         if rc:
             _check(self.ctx.h, rc, what)
         if given:
