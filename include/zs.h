@@ -554,7 +554,10 @@ int zs_distill_loss_grad(zs_ctx* ctx, const zs_distill* args, void* stream);
  *     dhidden[r] = sum_v d_v W_v,   dweight_v = sum_r d_v h_r
  * hidden, weight and the gradients are of one type, sums in f32. Products of
  * 16-bit numbers are exact; d is rounded to their type on its way into the
- * gradients' products (f16: scaled so that its largest factor is near 2^15).
+ * gradients' products (f16: scaled so that its largest is near 2^15). The loss and
+ * the label's d are made of sums of the other ids' exponentials, relative to the
+ * label's logit of the same products: of a row that is all but certain both keep
+ * their digits, and neither has the wrong sign.
  * f32 numbers are multiplied as sums of three bf16, to 2^-26 of each product; for
  * logits and dhidden of more than 192 rows (or a weight that is FAR) as sums of
  * two f16 of the number scaled by a power of two, of the whole weight, of a row of

@@ -30,6 +30,7 @@ struct ce_state {           // what the device finds out
 struct ce_row {             // of a piece
     float fix;              // the gradient at the label
     uint32_t label;
+    float fac, m;           // of an exponential in the gradient, relative to the row's largest logit m
     int32_t sh, sd;         // f32: the powers of two that its hidden state and its gradient of the logits are scaled by
 };
 #define CE_MAXIMA 512u      // parts of an f32 weight whose largest numbers are taken
@@ -51,7 +52,7 @@ struct ce_args {
     // scratch
     ce_state* st;
     uint32_t* idx;               // [N] the rows with a label in order, behind them the others
-    float* at;                   // [R] logit of the label
+    float* own;                  // [R][sub] logits of the `sub` ids that have the label among them
     ce_row* row;                 // [R]
     float2* stat;                // [R][subs] of `sub` ids each: maximum and sum of exponentials
     float* fac;                  // [R][subs] of an exponential in the gradient
@@ -97,7 +98,7 @@ inline uint64_t ce_work(ce_args& a, uint32_t dtype, void* work) {
     auto take = [&](uint64_t bytes) { char* at = p; p += hd_pad(bytes); return (void*)at; };
     a.st = (ce_state*)take(sizeof(ce_state));
     a.idx = (uint32_t*)take(a.N * 4ull);
-    a.at = (float*)take(a.R * 4ull);
+    a.own = (float*)take((uint64_t)a.R * a.sub * 4u);
     a.row = (ce_row*)take(a.R * sizeof(ce_row));
     a.stat = (float2*)take((uint64_t)a.R * a.subs * 8u);
     if (!wide || dw || a.raw) a.h = (uint16_t*)take(planes * a.R * a.Dp * 2u);

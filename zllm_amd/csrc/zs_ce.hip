@@ -40,6 +40,7 @@ __device__ __forceinline__ uint32_t ce_rows(const ce_args& a) {   // of the piec
     const uint32_t n = a.st->rows;
     return n <= a.lo ? 0u : n - a.lo < a.R ? n - a.lo : a.R;
 }
+__device__ __forceinline__ uint32_t ce_sub(const ce_args& a, uint32_t id) { return id >> (31 - __builtin_clz(a.sub)); }   // the part that has it
 template <int DT>
 __device__ __forceinline__ float ce_load(const void* p, uint64_t i) {
     return hd_float(reinterpret_cast<const typename hd_elem<DT>::T*>(p)[i]);
@@ -96,12 +97,11 @@ __global__ __launch_bounds__(1024) void zs_k_ce_rows(ce_args a) {
     if (t == 0u) a.st->rows = done;
 }
 
-// Row lo + i: its hidden state to the operand (zeros behind the last row), its label
-// and (16-bit types) that one's logit; rows without one get their zeros.
+// Row lo + i: its hidden state to the operand (zeros behind the last row), and its
+// label; rows without one get their zeros.
 template <int DT>
 __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
     __shared__ float shf[CE_NT / 64];
-    __shared__ double shd[CE_NT / 64];
     const uint32_t i = blockIdx.x, t = threadIdx.x;
     const uint64_t plane = (uint64_t)a.R * a.Dp;
     uint16_t* o = a.h + (uint64_t)i * a.Dp;
@@ -150,8 +150,7 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
     const uint64_t r = mine;
     const int64_t label = a.labels[r];
     const bool bad = label < 0 || label >= (int64_t)a.V;
-    const uint64_t hr = r * a.ld_h, wr = (bad ? 0u : (uint64_t)label) * a.ld_w;
-    double dot = 0.0;
+    const uint64_t hr = r * a.ld_h;
     int sh2 = 0;
     if (DT == ZS_F32 && a.h2) {
         float top = 0.0f;
@@ -159,26 +158,16 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
         sh2 = zs_split2_of(block_max_f<CE_NT>(top, shf));
         if (t == 0u) a.row[i].sh = sh2;
     }
-    const bool vec = DT != ZS_F32 && a.D % 8u == 0u && a.ld_h % 8u == 0u && a.ld_w % 8u == 0u &&
-                     (((uintptr_t)a.hidden | (uintptr_t)a.weight) & 15u) == 0u;
-    if constexpr (DT != ZS_F32) {
-        if (vec)
-            for (uint32_t d = t * 8u; d < a.Dp; d += CE_NT * 8u) {
-                hd_u4 u = {0u, 0u, 0u, 0u};
-                if (d < a.D) {
-                    u = zs_gload((const hd_u4*)((const uint16_t*)a.hidden + hr + d));
-                    float x[8], y[8];
-                    hd_unpack<DT>(u, x);
-                    hd_unpack<DT>(zs_gload((const hd_u4*)((const uint16_t*)a.weight + wr + d)), y);
-#pragma unroll
-                    for (int k = 0; k < 8; k++) dot += (double)x[k] * (double)y[k];
-                }
-                *(hd_u4*)(o + d) = u;
-            }
-    }
+    const bool vec = DT != ZS_F32 && a.D % 8u == 0u && a.ld_h % 8u == 0u && ((uintptr_t)a.hidden & 15u) == 0u;
+    if (vec)
+        for (uint32_t d = t * 8u; d < a.Dp; d += CE_NT * 8u) {
+            hd_u4 u = {0u, 0u, 0u, 0u};
+            if (d < a.D) u = zs_gload((const hd_u4*)((const uint16_t*)a.hidden + hr + d));
+            *(hd_u4*)(o + d) = u;
+        }
     for (uint32_t d = vec ? a.Dp : t; d < a.Dp; d += CE_NT) {
-        const float x = d < a.D ? ce_load<DT>(a.hidden, hr + d) : 0.0f;
         if constexpr (DT == ZS_F32) {
+            const float x = d < a.D ? ce_load<DT>(a.hidden, hr + d) : 0.0f;
             uint16_t p[3], p2[2];
             if (a.h) {
                 zs_split3(x, p);
@@ -189,15 +178,9 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
             for (int k = 0; k < 2; k++) a.h2[k * plane + (uint64_t)i * a.Dp + d] = p2[k];
         } else {
             o[d] = d < a.D ? ((const uint16_t*)a.hidden)[hr + d] : (uint16_t)0;
-            if (d < a.D) dot += (double)x * (double)ce_load<DT>(a.weight, wr + d);
         }
     }
-    if constexpr (DT != ZS_F32) dot = block_sum_d<CE_NT>(dot, shd);
-    if (t == 0u) {
-        a.row[i].label = bad ? ~0u : (uint32_t)label;
-        if (bad) a.at[i] = NAN;
-        else if (DT != ZS_F32) a.at[i] = (float)dot;
-    }
+    if (t == 0u) a.row[i].label = bad ? ~0u : (uint32_t)label;
 }
 
 // The largest numbers of the parts of an f32 weight, and by them the power of two
@@ -333,8 +316,8 @@ __device__ __forceinline__ uint32_t ce_over(uint32_t n, uint32_t d) { return (n 
 
 // Logits of a tile of ids (m) and rows (n), of which only what a softmax over the
 // vocabulary needs leaves the registers: per row and wave (128 ids, or 32) their
-// maximum and the sum of exponentials relative to it, and for the gradient the
-// exponentials.
+// maximum and the sum of exponentials relative to it, for the gradient the
+// exponentials, and of the block of ids that has the row's label the logits.
 // Bound by the matrix cores (4096 rows of 4096, 151936 ids, bf16: 4150 us, 1230
 // TFLOP/s, 72 % of the clocks), with the exponentials behind each tile's products;
 // few rows by the weight's bytes (5 rows of 1024, 32000 ids: 12 us, 5.4 TB/s).
@@ -349,7 +332,14 @@ __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_logits(ce_args a) {
     T tile(mw, mh, at.x, at.y);
     tp_acc c[MT][NT];
     ce_none(c);
-    tile.run(0, a.Dp / TP_KSTEP, c);
+    const uint32_t block = tile.m0 + T::wm() * (32 * MT);
+    uint32_t lab[NT], own = 0u;   // own, a bit for each j: the block has the row's label (found out beside the first loads)
+#pragma unroll
+    for (int j = 0; j < NT; j++) lab[j] = tile.n_of(j) < n ? a.row[tile.n_of(j)].label : ~0u;
+    tile.run(0, a.Dp / TP_KSTEP, c, [&] {
+#pragma unroll
+        for (int j = 0; j < NT; j++) own |= lab[j] - block < 32u * MT ? 1u << j : 0u;
+    });
     if constexpr (DT == ZS_F32 && !RAW) {
         const int sw = ce_weight_shift(a);
 #pragma unroll
@@ -361,23 +351,22 @@ __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_logits(ce_args a) {
                 for (int q = 0; q < 16; q++) c[i][j][q] = ldexpf(c[i][j][q], back);
         }
     }
-    // The label's logit, of the very products that the sum is of: where it is most of
-    // the sum, their errors then leave p - 1 as they leave the sum. (16-bit gradients
-    // show nothing of that: zs_k_ce_pack has theirs for less.)
-    if constexpr (DT == ZS_F32) {
+    // The logits of the label's block, of which the row's loss and the block's gradient
+    // are made: errors that the label's products have in common with the others' cancel
+    // in the differences, and the others' exponentials, all there is of a certain row's
+    // loss and of p - 1, are kept from the label's. (Values that go out, not a sum without
+    // the label here: accumulators changed or read on a second way cost an evaluation of
+    // 4100 us 70 to 230.)
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
-            const uint32_t r = tile.n_of(j), v = (r < n ? a.row[r].label : ~0u) - tile.m_of(0, 0);   // (from the lane's first id on)
-            if (__ballot(v < 32u * MT)) {
-                float z = 0.0f;
+    for (int j = 0; j < NT; j++)
+        if (own >> j & 1u)
 #pragma unroll
-                for (int i = 0; i < MT; i++)
+            for (int i = 0; i < MT; i++)
 #pragma unroll
-                    for (int q = 0; q < 16; q++) z = v == (uint32_t)(i * 32 + q / 4 * 8 + q % 4) ? c[i][j][q] : z;
-                if (v < 32u * MT && !(v & 4u)) a.at[r] = z;   // (the ids with that bit are the other half's)
-            }
-        }
-    }
+                for (int q = 0; q < 4; q++) {
+                    const float v[4] = {c[i][j][4 * q], c[i][j][4 * q + 1], c[i][j][4 * q + 2], c[i][j][4 * q + 3]};
+                    ce_store4<ZS_F32>(a.own, (uint64_t)tile.n_of(j) * (32 * MT) + (tile.m_of(i, q) - block), v, 4, true);
+                }
     const uint32_t sub = at.x * (T::BM / (32 * MT)) + T::wm();
     if (tile.m0 + T::BM > a.V) {
 #pragma unroll
@@ -439,48 +428,64 @@ __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_logits(ce_args a) {
     }
 }
 
-// A row's normaliser and loss from its parts, and what its gradient goes by.
+// A row's normaliser and loss from its parts, and what its gradient goes by. With m
+// the row's largest logit, rest the others' exponentials relative to it and s = rest
+// + exp(z_label - m), 1 - p is rest / s and the loss ln s - (z_label - m), of two numbers
+// that are not negative: nothing cancels.
 template <int DT, bool GRAD>
 __global__ __launch_bounds__(CE_NT) void zs_k_ce_loss(ce_args a) {
-    __shared__ float shf[CE_NT / 64];
+    __shared__ float shf[CE_NT / 64], at_;
     __shared__ double shd[CE_NT / 64];
     const uint32_t i = blockIdx.x, t = threadIdx.x;
     if (i >= ce_rows(a)) return;
     const float2* st = a.stat + (uint64_t)i * a.subs;
-    float m = -INFINITY;
-    for (uint32_t k = t; k < a.subs; k += CE_NT) m = fmaxf(m, st[k].x);
+    const float y = t < a.sub ? a.own[(uint64_t)i * a.sub + t] : 0.0f;
+    const uint32_t label = a.row[i].label, own = ce_sub(a, label), id = own * a.sub + t;
+    const bool none = label == ~0u;   // (outside the vocabulary: it has no block)
+    const bool in = !none && t < a.sub && id < a.V;
+    if (t == (none ? 0u : (label & (a.sub - 1u)))) at_ = none ? -INFINITY : y;
+    float m = in ? y : -INFINITY;
+    for (uint32_t k = t; k < a.subs; k += CE_NT)
+        if (k != own) m = fmaxf(m, st[k].x);
     m = block_max_f<CE_NT>(m, shf);
     const float m0 = m > -INFINITY ? m : 0.0f;
-    double s = 0.0;
+    const float at = at_;   // (written in front of the maximum's barriers)
+    double rest = in && id != label ? (double)ce_exp<ZS_F32>(y - m0) : 0.0;
     for (uint32_t k = t; k < a.subs; k += CE_NT) {
         const float2 v = st[k];
-        s += (double)(v.y * ce_exp<DT>(v.x - m0));
+        if (k != own) rest += (double)(v.y * ce_exp<DT>(v.x - m0));
     }
-    s = block_sum_d<CE_NT>(s, shd);
-    const double lse = (double)m0 + log(s), at = (double)a.at[i];
+    rest = block_sum_d<CE_NT>(rest, shd);
+    const double below = (double)at - (double)m0, e = DT == ZS_F32 ? exp(below) : (double)ce_exp<ZS_F32>(at - m0);
+    const double s = rest + e, ln = log1p(below == 0.0 ? rest : s - 1.0), lse = (double)m0 + ln;
     const uint32_t r = a.idx[a.lo + i];
     if (t == 0u) {
         a.lse[r] = (float)lse;
-        a.loss[r] = (float)((lse - at) + (double)a.zw * lse * lse);
+        a.loss[r] = (float)((none ? NAN : ln - below) + (double)a.zw * lse * lse);
     }
     if constexpr (GRAD) {
-        const float g = a.row_grad[r * a.row_grad_stride], k1 = (float)(1.0 + 2.0 * (double)a.zw * lse);
-        const float bad = a.row[i].label == ~0u ? NAN : g;
-        const float f = (float)((double)bad * (double)k1 / s);
+        const float g = a.row_grad[r * a.row_grad_stride];
+        const double k1 = 1.0 + 2.0 * (double)a.zw * lse, bad = none ? NAN : g;
+        const float f = (float)(bad * k1 / s);
         for (uint32_t k = t; k < a.subs; k += CE_NT) a.fac[(uint64_t)i * a.subs + k] = f * ce_exp<DT>(st[k].x - m0);
         if (t == 0u) {
-            a.row[i].fix = (float)((double)bad * ((double)k1 * exp(at - lse) - 1.0));
-            const float top = fabsf(g) * (k1 >= 0.0f ? fmaxf(1.0f, k1) : 1.0f - k1);   // at least |g (k1 p - [label])|
+            // g (k1 p - 1) at the label, at most g k1 rest / s at the others
+            const double others = k1 * (rest / s);
+            const float fix = (float)(bad * (2.0 * (double)a.zw * lse - others));
+            const float top = fmaxf(fabsf(fix), fabsf((float)((double)g * others)));
+            a.row[i].fix = fix;
+            a.row[i].fac = f;
+            a.row[i].m = m0;
             a.row[i].sd = zs_split2_of(top);
             if (DT == ZS_F16 && top < INFINITY) atomicMax(&a.st->amax[i & 63u], __float_as_uint(top));
         }
     }
 }
 
-// Exponentials to the gradient of the logits, in their place (f32: to three
-// planes); zeros in the rows up to where the products over the rows end. Bound by
-// memory: 8192 x 151936 in 790 us, 6.4 TB/s. (A pass of its own, as a row's sum is
-// known only when all of its tiles are done.)
+// Exponentials (of the label's block the logits) to the gradient of the logits, in
+// their place (f32: to three planes); zeros in the rows up to where the products over
+// the rows end. Bound by memory: 8192 x 151936 in 795 us, 6.4 TB/s. (A pass of its own,
+// as a row's sum is known only when all of its tiles are done.)
 template <int DT>
 __global__ __launch_bounds__(CE_NT) void zs_k_ce_grad(ce_args a) {
     const uint32_t i = blockIdx.y, n = ce_rows(a), v0 = (blockIdx.x * CE_NT + threadIdx.x) * 8u;
@@ -489,21 +494,25 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_grad(ce_args a) {
     const uint64_t at = (uint64_t)i * a.Vp + v0;
     float x[8];
     if (i < n) {
-        const float f = ldexpf(a.fac[(uint64_t)i * a.subs + v0 / a.sub], sh) * (DT == ZS_F32 ? 1.0f : 1.0f / CE_E_SCALE);
         const ce_row row = a.row[i];
-        if constexpr (DT == ZS_F32) {
-            const float4 u = *(const float4*)((const float*)a.e + at), w = *(const float4*)((const float*)a.e + at + 4);
+        if ((row.label ^ v0) < a.sub) {
+            // the label's block, from its logits
+            const float* z = a.own + (uint64_t)i * a.sub + (v0 & (a.sub - 1u));
+            const float f = ldexpf(row.fac, sh), fix = ldexpf(row.fix, sh);
+            const float4 u = *(const float4*)z, w = *(const float4*)(z + 4);
             const float y[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
-            for (int k = 0; k < 8; k++) x[k] = y[k] * f;
+            for (uint32_t k = 0; k < 8u; k++) x[k] = v0 + k >= a.V ? 0.0f : v0 + k == row.label ? fix : f * ce_exp<ZS_F32>(y[k] - row.m);
         } else {
-            const hd_u4 u = *(const hd_u4*)((const uint16_t*)a.e + at);
-            hd_unpack<ZS_F16>(u, x);
-            for (int k = 0; k < 8; k++) x[k] *= f;
-        }
-        if (row.label - v0 < 8u) {
-            const float y = ldexpf(row.fix, sh);
-            for (uint32_t k = 0; k < 8u; k++)
-                if (row.label == v0 + k) x[k] = y;
+            const float f = ldexpf(a.fac[(uint64_t)i * a.subs + ce_sub(a, v0)], sh) * (DT == ZS_F32 ? 1.0f : 1.0f / CE_E_SCALE);
+            if constexpr (DT == ZS_F32) {
+                const float4 u = *(const float4*)((const float*)a.e + at), w = *(const float4*)((const float*)a.e + at + 4);
+                const float y[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+                for (int k = 0; k < 8; k++) x[k] = y[k] * f;
+            } else {
+                const hd_u4 u = *(const hd_u4*)((const uint16_t*)a.e + at);
+                hd_unpack<ZS_F16>(u, x);
+                for (int k = 0; k < 8; k++) x[k] *= f;
+            }
         }
     } else {
         for (int k = 0; k < 8; k++) x[k] = 0.0f;

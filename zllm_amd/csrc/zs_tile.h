@@ -187,6 +187,10 @@ template <> struct tp_planes<TP_THREE> {
     static constexpr uint32_t A = 0x001102u, B = 0x010120u;
 };
 
+struct tp_none {
+    __device__ __forceinline__ void operator()() const {}
+};
+
 // A tile of BM x BN = (32 MT WM) x (32 NT WN) by four waves, WM along m.
 // 256 x 256 has 128 x 128 a wave, all of its 256 accumulation registers: 16
 // instructions of 32 clocks for eight operands of 1 KB, so that the four waves ask
@@ -262,8 +266,9 @@ struct tp_tile {
         a.plane(ma, (int)(planes_of::A >> (4 * pair)) & 15, m0);
         b.plane(mb, (int)(planes_of::B >> (4 * pair)) & 15, n0);
     }
-    // c += A B over steps k0 .. k0 + n - 1
-    __device__ __forceinline__ void run(uint32_t k0, uint32_t n, tp_acc (&c)[MT][NT]) {
+    // c += A B over steps k0 .. k0 + n - 1; beside() is called while the first are on their way
+    template <class F = tp_none>
+    __device__ __forceinline__ void run(uint32_t k0, uint32_t n, tp_acc (&c)[MT][NT], const F& beside = F()) {
         tp_lds* const s[3] = {stage(0), stage(1), stage(2)};
         if (n == 0u) return;
         regs r0, r1;
@@ -277,6 +282,7 @@ struct tp_tile {
         tp_in_order();
         put(s[2]);
         tp_in_order();
+        beside();
         tp_arrived<2 * LOADS>();
         get(s[0], 0, r0);
         // A step: its first half's products while the second's operands are read;
@@ -548,10 +554,12 @@ struct tp_raw_tile {
             }
         }
     }
-    __device__ __forceinline__ void run(uint32_t k0, uint32_t n, tp_acc (&c)[1][2]) {
+    template <class F = tp_none>
+    __device__ __forceinline__ void run(uint32_t k0, uint32_t n, tp_acc (&c)[1][2], const F& beside = F()) {
         tp_lds *s0 = stage(0), *s1 = stage(1);
         if (n == 0u) return;
         put(k0, s0);
+        beside();
         uint32_t k = 1u;
         for (; k < n; k += 2u) {
             tp_arrived<0, true>();
