@@ -64,8 +64,9 @@ def _call(ctx, entry, what, hidden, weight, labels, cfg, row_grad=None, want=(Fa
     if not 1 <= V <= MAX_VOCAB or not 1 <= D <= MAX_HIDDEN:
         raise ValueError(f"{what}: V is 1 to {MAX_VOCAB}, D 1 to {MAX_HIDDEN}")
     lab = _like(labels, (N,), torch.int64, dev, what, "labels").data_ptr()
-    out = torch.empty((2, N), dtype=torch.float32, device=dev)
-    loss, lse = out.unbind(0)
+    # (each of its own: autograd lets no view of one of several be changed in place)
+    loss = torch.empty(N, dtype=torch.float32, device=dev)
+    lse = torch.empty(N, dtype=torch.float32, device=dev)
     dh = torch.empty((N, D), dtype=hidden.dtype, device=dev) if want[0] else None
     dw = torch.empty((V, D), dtype=hidden.dtype, device=dev) if want[1] else None
     bits = (_DHIDDEN if want[0] else 0) | (_DWEIGHT if want[1] else 0)
