@@ -89,16 +89,15 @@ __global__ __launch_bounds__(64) void zs_k_q4_pack(q4_pack_args a) {
 // ------------------------------------------------------------------ hidden states
 // A wave's part of a row: 128 columns, two a lane, to the rows the kernels take and
 // to their sums over the groups, times what zs_k_q4_batch starts from.
-__device__ __forceinline__ void q4_sums(const q4_x_args& a, uint64_t r, uint32_t b, float x, float y, int s) {
+__device__ __forceinline__ void q4_sums(const q4_x_args& a, uint64_t r, uint32_t b, double t) {
     const uint32_t l = zs_lane(), per = 128u / a.group;
-    double t = (double)x + (double)y;
     t += zs_lane_xor<1>(t);
     t += zs_lane_xor<2>(t);
     t += zs_lane_xor<4>(t);
     t += zs_lane_xor<8>(t);
     if (a.group > 32u) t += zs_lane_xor<16>(t);
     if (a.group > 64u) t += zs_lane_xor<32>(t);
-    if (l % (a.group / 2u) == 0u) a.sums[((uint64_t)b * per + l / (a.group / 2u)) * a.Bp + r] = ldexpf((float)(t * (double)a.off), s);
+    if (l % (a.group / 2u) == 0u) a.sums[((uint64_t)b * per + l / (a.group / 2u)) * a.Bp + r] = (float)(t * (double)a.off);
 }
 template <int DT>
 __global__ __launch_bounds__(Q4_NT) void zs_k_q4_rows(q4_x_args a) {
@@ -114,11 +113,12 @@ __global__ __launch_bounds__(Q4_NT) void zs_k_q4_rows(q4_x_args a) {
                 v[k] = hd_float(x[k]);
                 if (a.out) a.out[r * a.D + d + k] = __builtin_bit_cast(uint16_t, x[k]);
             }
-        if (a.sums) q4_sums(a, r, b, v[0], v[1], 0);
+        if (a.sums) q4_sums(a, r, b, (double)v[0] + (double)v[1]);
     }
 }
 // f32 rows as two f16 of the number scaled by a power of two of the row (zs_split2),
-// by which the logits are scaled back.
+// by which the logits are scaled back. Their sums are of what the two f16 hold: what
+// these leave of the number would otherwise be in the logits 24 (16) times.
 __global__ __launch_bounds__(Q4_NT) void zs_k_q4_rows_f32(q4_x_args a) {
     __shared__ float sh[Q4_NT / 64];
     const uint32_t l = zs_lane(), blocks = (a.D + 127u) / 128u;
@@ -130,16 +130,16 @@ __global__ __launch_bounds__(Q4_NT) void zs_k_q4_rows_f32(q4_x_args a) {
     if (threadIdx.x == 0u) a.shift[r] = s;
     for (uint32_t b = zs_wid(); b < blocks; b += Q4_NT / 64) {
         const uint32_t d = b * 128u + l * 2u;
-        float v[2] = {0.0f, 0.0f};
+        double v = 0.0;
         if (d < a.D) {
             uint16_t p[2][2];
             for (int k = 0; k < 2; k++) {
-                v[k] = x[d + k];
-                zs_split2(v[k], s, p[k]);
+                zs_split2(x[d + k], s, p[k]);
+                for (int q = 0; q < 2; q++) v += (double)__builtin_bit_cast(_Float16, p[k][q]);
             }
             for (int q = 0; q < 2; q++) *(uint32_t*)(a.out + q * n + r * a.D + d) = (uint32_t)p[0][q] | (uint32_t)p[1][q] << 16;
         }
-        if (a.sums) q4_sums(a, r, b, v[0], v[1], s);
+        if (a.sums) q4_sums(a, r, b, v);
     }
 }
 
