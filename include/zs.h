@@ -621,7 +621,9 @@ int zs_ce_loss_grad(zs_ctx* ctx, const zs_ce* args, void* stream);
  *                     scale = f16(max |w| / 7), code = round(w / scale) + 8; with
  *                     d_mins scale = f16((max - min) / 15), min = f16(min), code =
  *                     round((w - min) / scale); limited to 0 .. 15, halves to even,
- *                     a scale of 0 has w = 0 (min)
+ *                     a scale of 0 has w = 0 (min). A group with a NaN has a scale
+ *                     of NaN; with an infinity, or past f16's range, scale or
+ *                     minimum are infinite: that row's logits are not finite
  *   zs_q4_logits      B rows; scratch for f32 rows, for those that do not all
  *                     begin at 16 bytes (`copy`) and for more than 16 */
 #define ZS_Q4_MINS 1u

@@ -14,7 +14,8 @@ typedef uint32_t q4_u4 __attribute__((ext_vector_type(4)));
 // A group's scale and minimum from its extremes, then its codes, two to a byte.
 // Without minima w ~ scale * (code - 8) with scale = max |w| / 7; with them
 // w ~ scale * code + min with scale = (max - min) / 15. Both are rounded to f16
-// first and the codes taken by the rounded ones; a scale of 0 has codes of 0 (8).
+// first and the codes taken by the rounded ones; a scale of 0 has codes of 0 (8). A
+// group with a NaN or an infinity has a scale that is one, and so has its row's logits.
 template <int DT>
 __global__ __launch_bounds__(Q4_NT) void zs_k_q4_quantize(q4_pack_args a) {
     const uint32_t per = a.D / a.group, w = zs_wid(), l = zs_lane();
@@ -41,6 +42,8 @@ __global__ __launch_bounds__(Q4_NT) void zs_k_q4_quantize(q4_pack_args a) {
         } else {
             s = (_Float16)(fmaxf(fabsf(lo), fabsf(hi)) / 7.0f);
         }
+        // (the extremes pass over a NaN)
+        if (__ballot(y[0] != y[0] || y[1] != y[1])) s = (_Float16)NAN;
         const float sf = (float)s, mf = (float)m;
         uint32_t code = 0;
         for (int i = 0; i < 2; i++) {

@@ -158,7 +158,8 @@ def _group_of(V: int, D: int, groups: int, what: str) -> int:
 def q4_quantize(ctx: Context, weight: torch.Tensor, group: int = 32, mins: bool = False
                 ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
     """Codes (uint8 [V, D / 2]), scales and, asked for, minima (float16 [V, D /
-    group]) of a weight [V, D] of any of the three types (zs_q4_quantize)."""
+    group]) of a weight [V, D] of any of the three types (zs_q4_quantize). What
+    is not finite in a group makes its scale so, and its row's logits."""
     what = "q4_quantize"
     _matrix(ctx, weight, what, "weight")
     V, D = weight.shape
