@@ -558,11 +558,11 @@ int zs_distill_loss_grad(zs_ctx* ctx, const zs_distill* args, void* stream);
  * the label's d are made of sums of the other ids' exponentials, relative to the
  * label's logit of the same products: of a row that is all but certain both keep
  * their digits, and neither has the wrong sign.
- * f32 numbers are multiplied as sums of three bf16, to 2^-26 of each product; for
+ * f32 numbers are multiplied as sums of three bf16, to 2^-24 of each product; for
  * logits and dhidden of more than 192 rows (or a weight that is FAR) as sums of
  * two f16 of the number scaled by a power of two, of the whole weight, of a row of
  * hidden states and of a row of d: to 3 * 2^-22, and a number below 2^-18 of the
- * largest to 2^-40 of that. The gradients are rounded once.
+ * largest to 2^-39 of that. The gradients are rounded once.
  * A row whose label is ignore_index has loss, lse and gradient 0, and its
  * hidden state, whatever it holds, is in no sum; a label outside [0, V)
  * otherwise gives NaN. What is not finite comes out as not finite.
@@ -613,7 +613,7 @@ int zs_ce_loss_grad(zs_ctx* ctx, const zs_ce* args, void* stream);
  * (zs_q4_pack, into d_head of zs_q4_bytes bytes); logits are
  *     logits[r][v] = sum_d hidden[r][d] W_vd
  * in f32: codes and hidden states (f32: as two f16 of the number scaled by a power
- * of two of the row, to 2^-22, numbers below 2^-18 of the row's largest to 2^-40 of
+ * of two of the row, to 2^-22, numbers below 2^-18 of the row's largest to 2^-39 of
  * that) multiplied exactly, summed in f32 over a group, scaled, and summed in f32. They are what
  * zs_sample, zs_lane_step, zs_beam_select and the others read (those that ask
  * for it with ld % 4 == 0).

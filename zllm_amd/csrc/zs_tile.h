@@ -160,9 +160,11 @@ struct tp_side {
 //   TP_TWO    f16 x0 + x1 of x scaled by a power of two (zs_split2): x1 y0, x0 y1,
 //             x0 y0. What x0 + x1 leaves of x and the product left out, x1 y1, are
 //             each at most 2^-22 of theirs: 3 * 2^-22 |x y| in all. Numbers below
-//             2^-18 of the largest that fits have less than 22 bits, to 2^-40 of it.
+//             2^-18 of the largest have less than 22 bits: half of f16's smallest step,
+//             2^-25, is at most 2^-39 of a largest that is 2^14 or more.
 //   TP_THREE  bf16 x0 + x1 + x2 (zs_split3), of any size: x2 y0, x0 y2, x1 y1, x1 y0,
-//             x0 y1, x0 y0. Left out are at most 2^-26 of |x y|.
+//             x0 y1, x0 y0. |x1| is at most 2^-8 |x| and |x2| 2^-17 |x|, so that x1 y2, x2
+//             y1 and x2 y2, left out, are 2^-24 (1 + 2^-10) of |x y|.
 // or 16-bit numbers A with a B of two planes, B1 what B0 leaves:
 //   TP_REST_F16, TP_REST_BF16   x y1, x y0
 #define TP_TWO 3
