@@ -614,7 +614,9 @@ int zs_ce_loss_grad(zs_ctx* ctx, const zs_ce* args, void* stream);
  *     logits[r][v] = sum_d hidden[r][d] W_vd
  * in f32: codes and hidden states (f32: as two f16 of the number scaled by a power
  * of two of the row, to 2^-22, numbers below 2^-18 of the row's largest to 2^-39 of
- * that) multiplied exactly, summed in f32 over a group, scaled, and summed in f32. They are what
+ * that) multiplied exactly, summed in f32 over a group, scaled, and summed in f32. A
+ * code is multiplied as 16 + code, so 31 times a group's sum of |hidden| has to be an
+ * f32 number too (bf16 states past 2^120 over a group are not finite). They are what
  * zs_sample, zs_lane_step, zs_beam_select and the others read (those that ask
  * for it with ld % 4 == 0).
  *   zs_q4_quantize    codes and scales of a weight of any of the three types:

@@ -318,9 +318,9 @@ __device__ __forceinline__ uint32_t ce_over(uint32_t n, uint32_t d) { return (n 
 // vocabulary needs leaves the registers: per row and wave (128 ids, or 32) their
 // maximum and the sum of exponentials relative to it, for the gradient the
 // exponentials, and of the block of ids that has the row's label the logits.
-// Bound by the matrix cores (4096 rows of 4096, 151936 ids, bf16: 4150 us, 1230
-// TFLOP/s, 72 % of the clocks), with the exponentials behind each tile's products;
-// few rows by the weight's bytes (5 rows of 1024, 32000 ids: 12 us, 5.4 TB/s).
+// Bound by the matrix cores (4096 rows of 4096, 151936 ids, bf16: 4151 us, 1228
+// TFLOP/s, 70 % of the clocks), with the exponentials behind each tile's products;
+// few rows by the weight's bytes (5 rows of 1024, 32000 ids: 12.7 us, 5.2 TB/s).
 template <int DT, bool GRAD, bool THIN, int RAW>
 __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_logits(ce_args a) {
     typedef typename ce_or_raw<RAW, ce_tile<DT == ZS_F32 ? TP_TWO : DT, THIN, false, false>, false>::type T;
@@ -694,8 +694,10 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_join(ce_args a) {
 
 // Gradient of the weight, a tile of columns (m) of ids (n), over the piece's rows.
 // (Of few rows there is little to multiply and much to write: three workgroups of
-// 128 x 128 a CU.) 151936 x 4096 over 8192 rows: 7450 us, 1369 TFLOP/s; over one f32
-// row, 58134 x 3456: 185 us, 4.3 TB/s written.
+// 128 x 128 a CU. In f32 the planes' addresses, picked at run time, lie in private
+// memory: over a few rows, where a plane ends every step or two, the products wait for
+// them.) 151936 x 4096 over 8192 rows: 7344 us, 1388 TFLOP/s; over one f32 row, 58134 x
+// 3456: 185 us, 4.3 TB/s written.
 template <int DT, bool THIN>
 __global__ __launch_bounds__(CE_NT, THIN ? 3 : 1) void zs_k_ce_dweight(ce_args a) {
     typedef tp_tile<ce_kind(DT, THIN, true), THIN ? 2 : 4, THIN ? 2 : 4, 2, true, true> T;

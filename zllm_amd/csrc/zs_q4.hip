@@ -318,10 +318,12 @@ __global__ __launch_bounds__(KS * 64) void zs_k_q4_logits(q4_args a) {
 // The same for more rows: 16 RT rows by 64 T ids a workgroup, its waves side by
 // side along the ids. The hidden states of 128 columns at a time come to shared
 // memory as operands (lane l's 16 bytes at 16 l), two steps ahead of their use,
-// and the waves' codes and scales to registers likewise.
-// Bound by the instructions: 64 rows of 4096, 151936 ids, groups of 32, 121 us, the
-// vector units busy for 56 %, the matrix cores for 32 % of it, one beside the other
-// in part only; 320 rows, groups of 128, 410 us, 48 % each (970 TFLOP/s).
+// and the waves' codes and scales to registers likewise. (Groups of 32: one step in
+// three waits for all loads, as the compiler makes the next step's first operands
+// before that step begins.)
+// Bound by the instructions: 64 rows of 4096, 151936 ids, groups of 32, 119 us, the
+// vector units busy for 54 %, the matrix cores for 29 % of it, one beside the other
+// in part only; 320 rows, groups of 128, 411 us, 49 and 46 % (969 TFLOP/s).
 template <int DT, int G, bool MINS, int T, int RT>
 struct q4_batch {
     static constexpr int P = DT == ZS_F32 ? 2 : 1, PER = 128 / G, PIECES = P * RT * 4;
@@ -510,7 +512,8 @@ static void q4_go(const q4_args& a, hipStream_t stream) {
         // (17 rows by 2 and by as many as find room: 90000 ids 47 and 57, 128256 ids 66 and
         // 68, 151936 ids 83 and 92; by 64 rows a workgroup 78, 95 and 126). Beyond 64 rows a
         // part of the rows finds another's codes in the L2, and 4 serve. Of larger groups or
-        // with minima 5 do not fit the registers.
+        // with minima 5 do not fit the registers (of groups of 128 with minima 4 do but for
+        // 6 registers, which are spilled).
         uint32_t t = (a.at.tiles + 2047u) / 2048u;
         t = a.at.tiles <= 1024u ? 1u : t < 2u ? 2u : t;
         if (DT == ZS_F32 || a.B <= 32u) q4_batch_go<DT, G, MINS, 2, 2>(a, stream);

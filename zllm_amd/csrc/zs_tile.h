@@ -198,8 +198,9 @@ struct tp_none {
 // instructions of 32 clocks for eight operands of 1 KB, so that the four waves ask
 // for 64 of the some 230 bytes a clock that shared memory gives, and memory for 32
 // KB in 1024 clocks a CU. Bound by the matrix cores: 8192 x 4096 over 151936 in
-// 7313 us, 1395 TFLOP/s (the library's product 1574), the cores busy for 80 % of the
-// clocks there are under that load (1.6 to 1.9 GHz). Smaller tiles, two workgroups a
+// 7250 us, 1407 TFLOP/s (the library's product 1574), the cores busy for 82 % of the
+// clocks there are under that load (1.6 to 1.9 GHz). (Of what else is held 16 to 51
+// registers are spilled, outside the loop over the steps.) Smaller tiles, two workgroups a
 // CU, have one's begin and end beside the other's products, but read more: 256 x 128
 // took 5106 us of an evaluation's 4184.
 template <int KIND, int MT, int NT, int WM, bool AS, bool BS>

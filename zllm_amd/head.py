@@ -1,6 +1,6 @@
 """The vocabulary head over libzs: its cross entropy from hidden states, without
-logits, with the gradients; and a head held in 4 bits, whose logits the sampler,
-the lanes and beam search read.
+logits in memory, with the gradients; and a head held in 4 bits, whose logits the
+sampler, the lanes and beam search read.
 
     loss_of = HeadLoss(ctx)
     loss_of(hidden, head_weight, labels).mean().backward()
@@ -14,6 +14,13 @@ log-probabilities are -loss) and head_loss_grad;
 
 or head.logits(hidden). The formulas are in include/zs.h. The reference trains
 nothing; the loss has no counterpart.
+Scratch of a call, from torch's allocator: a loss keeps 8 bytes for each row and 128
+ids (32, of up to 128 rows). A step keeps an exponential for each row and id besides,
+2 bytes of 16-bit types (4 up to 64 rows) and 8 to 14 of float32, of at most 4 GiB of
+rows at a time: 8192 rows of 151936 ids take 2.5 GB. The gradients of more rows than
+that are made in pieces, the weight's summed in float32 (4 V D bytes). A float32
+weight is copied as well (4 V D) for more than 192 rows, a 16-bit one (2 V D) if its
+rows do not lie at 16 bytes each.
 torch holds the device memory and the stream; the computation is libzs's.
 """
 import ctypes as C
@@ -135,7 +142,7 @@ class _HeadLossFunction(torch.autograd.Function):
 class HeadLoss(torch.nn.Module):
     """Loss per row, differentiable by the hidden states and the weight. Keeps
     neither logits nor exponentials between the passes: the backward pass makes
-    the logits again, in pieces. (Where the rows' weights are known before the
+    the logits again, 8 N V D operations in all for head_loss_grad's 6. (Where the rows' weights are known before the
     loss, head_loss_grad makes them once; it is also what belongs into a captured
     HIP graph: autograd's own bookkeeping of leaves that an eager graph holds too
     does not.)"""
