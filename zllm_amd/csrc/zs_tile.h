@@ -402,9 +402,19 @@ struct tp_tile {
     }
 };
 
+// x within bf16's range (what is past it, or no number, shows in what is left of x)
+__device__ __forceinline__ float tp_bf16_below(float x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const float m = __uint_as_float(0x7f7f0000u);
+    return __builtin_amdgcn_fmed3f(x, -m, m);
+#else
+    return x;
+#endif
+}
+
 // The same product with an f32 A that lies in memory as it is (ANY: its rows at any
 // number, fetched one by one, not by 16 bytes) and three planes of B: 128 x 64 a
-// workgroup, each wave's 32 rows of A split into planes in its registers (44
+// workgroup, each wave's 32 rows of A split into planes in its registers (52
 // instructions for 16 columns of 32 rows, beside 12 products of them). Where there
 // are few n: nothing of A is written and read again. ld, k and rows of A's tp_mat
 // count f32 numbers.
@@ -533,7 +543,8 @@ struct tp_raw_tile {
             u4 o;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const b2 v = {(__bf16)x[2 * k], (__bf16)x[2 * k + 1]};
+                // (the first: of a number that bf16 would make infinite the one below it)
+                const b2 v = {(__bf16)(q ? x[2 * k] : tp_bf16_below(x[2 * k])), (__bf16)(q ? x[2 * k + 1] : tp_bf16_below(x[2 * k + 1]))};
                 o[k] = __builtin_bit_cast(uint32_t, v);
                 if (q < 2) {
                     x[2 * k] -= __uint_as_float(o[k] << 16);
