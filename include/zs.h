@@ -560,9 +560,10 @@ int zs_distill_loss_grad(zs_ctx* ctx, const zs_distill* args, void* stream);
  * their digits, and neither has the wrong sign.
  * f32 numbers are multiplied as sums of three bf16, to 2^-24 of each product; for
  * logits and dhidden of more than 192 rows (or a weight that is FAR) as sums of
- * two f16 of the number scaled by a power of two, of the whole weight, of a row of
- * hidden states and of a row of d: to 3 * 2^-22, and a number below 2^-18 of the
- * largest to 2^-39 of that. The gradients are rounded once.
+ * two f16 of the number scaled by a power of two, of a row of the weight, of a row of
+ * hidden states and of a row of d, whose d_v are first divided by the power of W_v: to
+ * 3 * 2^-22, and a number below 2^-18 of the largest to 2^-39 of that (there to 2^-38
+ * of the largest over its power). The gradients are rounded once.
  * A row whose label is ignore_index has loss, lse and gradient 0, and its
  * hidden state, whatever it holds, is in no sum; a label outside [0, V)
  * otherwise gives NaN. What is not finite comes out as not finite.

@@ -10,8 +10,8 @@
 #define CE_THIN 64          // rows
 // f32 weights are multiplied as they lie up to so many rows, and as two planes that
 // are made of them once above. us of the loss / of a step as they lie and as planes,
-// 3456 x 58134: 1 row 218 / 610 and 700 / 1119, 128 rows 428 / 1260 and 819 / 1573, 192
-// rows 583 / 1750 and 785 / 1745, 256 rows 768 / 2280 and 793 / 1910
+// 3456 x 58134: 1 row 268 / 704 and 628 / 1052, 128 rows 449 / 1291 and 743 / 1500, 192
+// rows 618 / 1798 and 714 / 1676, 256 rows 805 / 2399 and 721 / 1843
 #define CE_RAW 192u
 #define CE_ROOM (4ull << 30)   // bytes of exponentials kept at once (a piece of the rows)
 
@@ -31,9 +31,8 @@ struct ce_row {             // of a piece
     float fix;              // the gradient at the label
     uint32_t label;
     float fac, m;           // of an exponential in the gradient, relative to the row's largest logit m
-    int32_t sh, sd;         // f32: the powers of two that its hidden state and its gradient of the logits are scaled by
+    int32_t sh, sd;         // f32: the powers of two that its hidden state and its gradient of the logits (over the ids' own) are scaled by
 };
-#define CE_MAXIMA 512u      // parts of an f32 weight whose largest numbers are taken
 struct ce_args {
     const void *hidden, *weight;
     uint64_t ld_h, ld_w;
@@ -61,7 +60,8 @@ struct ce_args {
     void* e;                     // [R][Vp] f16 (f32: f32) exponentials
     uint16_t* dl;                // [R][Vp] gradient of the logits, in their place (of few rows a second plane; f32: three, the weight's gradient's)
     uint16_t *h2, *dl2;          // f32: the same as two planes of scaled rows, the logits' and the hidden states' gradient's
-    float* wmax;                 // [CE_MAXIMA] f32: the weight's largest numbers
+    int32_t* wsh;                // [Vp] f32: the powers of two that the weight's rows are scaled by
+    float* lead;                 // [R][subs] the largest exponential over its id's power of two (the hidden states' gradient is wanted)
     float* part;                 // the hidden states' gradient over parts of the vocabulary (ce_parts)
     float* acc;                  // [V][Dm] the weight's gradient so far (more than one piece)
 };
@@ -105,13 +105,16 @@ inline uint64_t ce_work(ce_args& a, uint32_t dtype, void* work) {
     if (wide ? !a.raw : (a.want & (CE_COPY | CE_FAR)) != 0) a.w = (uint16_t*)take((wide ? 2u : 1u) * (uint64_t)a.V * a.Dp * 2u);
     if (wide && !a.raw) {
         a.h2 = (uint16_t*)take(2u * (uint64_t)a.R * a.Dp * 2u);
-        a.wmax = (float*)take(CE_MAXIMA * 4u);
+        a.wsh = (int32_t*)take(a.Vp * 4ull);
     }
     if (grad) {
         a.fac = (float*)take((uint64_t)a.R * a.subs * 4u);
         a.e = take((uint64_t)a.R * a.Vp * (wide || a.thin ? 4u : 2u));   // (thin: a plane more behind it)
         a.dl = !wide ? (uint16_t*)a.e : dw || a.raw ? (uint16_t*)take(planes * a.R * a.Vp * 2u) : nullptr;
-        if (wide && dh && !a.raw) a.dl2 = (uint16_t*)take(2u * (uint64_t)a.R * a.Vp * 2u);
+        if (wide && dh && !a.raw) {
+            a.dl2 = (uint16_t*)take(2u * (uint64_t)a.R * a.Vp * 2u);
+            a.lead = (float*)take((uint64_t)a.R * a.subs * 4u);
+        }
         if (dh) a.part = (float*)take((uint64_t)a.units * (a.thin ? CE_THIN_M * CE_THIN : CE_TILE * CE_TILE) * 4u);
         if (dw && a.pieces > 1u) a.acc = (float*)take((uint64_t)a.V * a.Dm * 4u);
     }

@@ -183,38 +183,56 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_pack(ce_args a) {
     if (t == 0u) a.row[i].label = bad ? ~0u : (uint32_t)label;
 }
 
-// The largest numbers of the parts of an f32 weight, and by them the power of two
-// that it is scaled by.
-__global__ __launch_bounds__(CE_NT) void zs_k_ce_max(ce_args a) {
-    __shared__ float sh[CE_NT / 64];
-    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));   // (a row's float4 may lie anywhere)
-    float top = 0.0f;
-    for (uint64_t v = blockIdx.x * (CE_NT / 64) + zs_wid(); v < a.V; v += CE_MAXIMA * (CE_NT / 64)) {
+// An f32 weight as two planes, row by row (each by a wave): its largest number, by that
+// the power of two that it is scaled by, and its numbers once more, from the caches.
+// (One power for the whole weight would leave nothing of the others where one row has
+// a number that bans it.)
+__global__ __launch_bounds__(CE_NT) void zs_k_ce_split(ce_args a) {
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));   // (a row may begin at any number)
+    const uint64_t plane = (uint64_t)a.V * a.Dp;
+    const uint32_t l = (uint32_t)zs_lane(), whole = a.D & ~3u;
+    for (uint32_t v = blockIdx.x * (CE_NT / 64) + zs_wid(); v < a.Vp; v += gridDim.x * (CE_NT / 64)) {
+        if (v >= a.V) {
+            if (l == 0u) a.wsh[v] = 0;
+            continue;
+        }
         const float* row = (const float*)a.weight + v * a.ld_w;
-        const uint32_t whole = a.D & ~3u;
+        float top = 0.0f;
 #pragma unroll 4
-        for (uint32_t d = zs_lane() * 4u; d < whole; d += 256u) {
-            const f4 x = zs_gload((const f4*)(row + d));
+        for (uint32_t d = l * 4u; d < whole; d += 256u) {
+            const f4 x = *(const f4*)(row + d);
             top = fmaxf(top, fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
         }
-        if (whole + zs_lane() < a.D) top = fmaxf(top, fabsf(row[whole + zs_lane()]));
-    }
-    top = block_max_f<CE_NT>(top, sh);
-    if (threadIdx.x == 0u) a.wmax[blockIdx.x] = top;
-}
-__device__ __forceinline__ int ce_weight_shift(const ce_args& a) {   // (by whole waves)
-    float top = 0.0f;
+        if (whole + l < a.D) top = fmaxf(top, fabsf(row[whole + l]));
+        top = wave_max_f(top);
+        const int sw = top == 0.0f ? 141 : zs_split2_of(top);   // (a row of zeros: as the smallest, or its entry over it would be the largest)
+        if (l == 0u) a.wsh[v] = sw;
+        uint16_t* o = a.w + (uint64_t)v * a.Dp;
+#pragma unroll 2
+        for (uint32_t d = l * 8u; d < a.Dp; d += 512u) {
+            uint16_t p[8][2];
+            if (d + 8u <= a.D) {
+                const f4 x = *(const f4*)(row + d), y = *(const f4*)(row + d + 4u);
 #pragma unroll
-    for (uint32_t k = 0; k < CE_MAXIMA / 64u; k++) top = fmaxf(top, a.wmax[k * 64u + zs_lane()]);
-    return zs_split2_of(wave_max_f(top));
+                for (int k = 0; k < 4; k++) zs_split2(x[k], sw, p[k]), zs_split2(y[k], sw, p[k + 4]);
+            } else {
+#pragma unroll
+                for (uint32_t k = 0; k < 8u; k++) zs_split2(d + k < a.D ? row[d + k] : 0.0f, sw, p[k]);
+            }
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                hd_u4 u;
+#pragma unroll
+                for (int k = 0; k < 4; k++) u[k] = (uint32_t)p[2 * k][q] | (uint32_t)p[2 * k + 1][q] << 16;
+                *(hd_u4*)(o + q * plane + d) = u;
+            }
+        }
+    }
 }
-// The weight in rows of Dp, its planes apart, where its own rows do not serve.
-// A row may begin at any element.
+// A 16-bit weight in rows of Dp, where its own rows do not serve. A row may begin at
+// any element.
 template <int DT>
 __global__ __launch_bounds__(CE_NT) void zs_k_ce_weight(ce_args a) {
-    const uint64_t plane = (uint64_t)a.V * a.Dp;
-    int sw = 0;
-    if constexpr (DT == ZS_F32) sw = ce_weight_shift(a);
     const uint32_t per = a.Dp / 8u;   // (at most 2^33 of them in all: the ids go over y where they are many)
     for (uint64_t v0 = (uint64_t)blockIdx.y * 65536u; v0 < a.V; v0 += (uint64_t)gridDim.y * 65536u) {
         const uint32_t ids = (uint32_t)(a.V - v0 < 65536u ? a.V - v0 : 65536u);
@@ -222,41 +240,20 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_weight(ce_args a) {
             const uint64_t v = v0 + i / per;
             const uint32_t j = i % per;
             const hd_row<DT> row(a.weight, a.ld_w, v, a.D);
-            uint16_t* o = a.w + v * a.Dp + j * 8u;
             const uint32_t d0 = j * 8u;
-            if constexpr (DT == ZS_F32) {
-                uint16_t p[8][2];
-                if (d0 + 8u <= a.D) {
-                    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));   // (a row's float4 may lie anywhere)
-                    const f4 x = zs_gload((const f4*)(row.row + d0)), y = zs_gload((const f4*)(row.row + d0 + 4u));
-#pragma unroll
-                    for (int k = 0; k < 4; k++) zs_split2(x[k], sw, p[k]), zs_split2(y[k], sw, p[k + 4]);
-                } else {
-#pragma unroll
-                    for (uint32_t k = 0; k < 8u; k++) zs_split2(d0 + k < a.D ? row.at(d0 + k) : 0.0f, sw, p[k]);
-                }
-#pragma unroll
-                for (int q = 0; q < 2; q++) {
-                    hd_u4 u;
-#pragma unroll
-                    for (int k = 0; k < 4; k++) u[k] = (uint32_t)p[2 * k][q] | (uint32_t)p[2 * k + 1][q] << 16;
-                    *(hd_u4*)(o + q * plane) = u;
-                }
+            typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));   // (a row's eight values may lie anywhere)
+            hd_u4 x;
+            if (d0 + 8u <= a.D) {
+                x = zs_gload((const u4*)(row.row + d0));
             } else {
-                typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));   // (a row's eight values may lie anywhere)
-                hd_u4 x;
-                if (d0 + 8u <= a.D) {
-                    x = zs_gload((const u4*)(row.row + d0));
-                } else {
-                    const uint16_t* r = (const uint16_t*)row.row;
+                const uint16_t* r = (const uint16_t*)row.row;
 #pragma unroll
-                    for (uint32_t k = 0; k < 4u; k++) {
-                        const uint32_t d = d0 + 2u * k;
-                        x[k] = (d < a.D ? (uint32_t)r[d] : 0u) | (d + 1u < a.D ? (uint32_t)r[d + 1u] << 16 : 0u);
-                    }
+                for (uint32_t k = 0; k < 4u; k++) {
+                    const uint32_t d = d0 + 2u * k;
+                    x[k] = (d < a.D ? (uint32_t)r[d] : 0u) | (d + 1u < a.D ? (uint32_t)r[d + 1u] << 16 : 0u);
                 }
-                *(hd_u4*)o = x;
             }
+            *(hd_u4*)(a.w + v * a.Dp + d0) = x;
         }
     }
 }
@@ -341,15 +338,19 @@ __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_logits(ce_args a) {
         for (int j = 0; j < NT; j++) own |= lab[j] - block < 32u * MT ? 1u << j : 0u;
     });
     if constexpr (DT == ZS_F32 && !RAW) {
-        const int sw = ce_weight_shift(a);
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
-            const int back = -sw - a.row[tile.n_of(j)].sh;
+        for (int i = 0; i < MT; i++)
 #pragma unroll
-            for (int i = 0; i < MT; i++)
+            for (int q = 0; q < 4; q++) {
+                const int4 w = *(const int4*)(a.wsh + tile.m_of(i, q));
+                const int sw[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                for (int q = 0; q < 16; q++) c[i][j][q] = ldexpf(c[i][j][q], back);
-        }
+                for (int j = 0; j < NT; j++) {
+                    const int back = -a.row[tile.n_of(j)].sh;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) c[i][j][4 * q + k] = ldexpf(c[i][j][4 * q + k], back - sw[k]);
+                }
+            }
     }
     // The logits of the label's block, of which the row's loss and the block's gradient
     // are made: errors that the label's products have in common with the others' cancel
@@ -368,6 +369,26 @@ __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_logits(ce_args a) {
                     ce_store4<ZS_F32>(a.own, (uint64_t)tile.n_of(j) * (32 * MT) + (tile.m_of(i, q) - block), v, 4, true);
                 }
     const uint32_t sub = at.x * (T::BM / (32 * MT)) + T::wm();
+    constexpr bool LEAD = GRAD && DT == ZS_F32 && !RAW;
+    // The largest exponential over its id's power of two, by which the gradient's planes
+    // are scaled: 1 over the least of the block's powers, or half of that, where the others
+    // are at most twice it (as of most weights); else (0) each is looked at, which for all
+    // blocks took 118 us of 1024 rows' 1055 over 140910 x 869.
+    float over = 0.0f;
+    if constexpr (LEAD)
+        if (a.lead) {
+            uint32_t lo = ~0u, hi = 0u;
+#pragma unroll
+            for (uint32_t k = 0; k < 32u * MT; k += 64u) {
+                const uint32_t id = block + k + (uint32_t)zs_lane() % (32u * MT);
+                const uint32_t w = id < a.V ? (uint32_t)(a.wsh[id] + 1024) : ~0u;
+                lo = min(lo, w);
+                hi = max(hi, w == ~0u ? 0u : w);
+            }
+            lo = zs_wave_reduce(lo, [](uint32_t x, uint32_t y) { return min(x, y); });
+            hi = zs_wave_reduce(hi, [](uint32_t x, uint32_t y) { return max(x, y); });
+            if (hi <= lo + 1u && lo != ~0u) over = ldexpf(1.0f, 1024 - (int)lo);
+        }
     if (tile.m0 + T::BM > a.V) {
 #pragma unroll
         for (int i = 0; i < MT; i++)
@@ -424,6 +445,23 @@ __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_logits(ce_args a) {
                     if constexpr (GRAD) ce_store4<ZS_F32>(a.e, (uint64_t)tile.n_of(j) * a.Vp + tile.m_of(i, q), x, 4, true);
                 }
             part(j, 1.0f);
+            if constexpr (LEAD)
+                if (a.lead) {
+                    float lead = m > -INFINITY ? over : 0.0f;
+                    if (over == 0.0f) {
+#pragma unroll
+                        for (int i = 0; i < MT; i++)
+#pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                const int4 w = *(const int4*)(a.wsh + tile.m_of(i, q));
+                                const int sw[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                                for (int k = 0; k < 4; k++) lead = fmaxf(lead, ldexpf(ce_exp<DT>(c[i][j][4 * q + k] - m0), -sw[k]));
+                            }
+                        lead = fmaxf(lead, zs_lane_xor<32>(lead));
+                    }
+                    if (zs_lane() < 32) a.lead[(uint64_t)tile.n_of(j) * a.subs + sub] = lead;
+                }
         }
     }
 }
@@ -467,6 +505,14 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_loss(ce_args a) {
         const float g = a.row_grad[r * a.row_grad_stride];
         const double k1 = 1.0 + 2.0 * (double)a.zw * lse, bad = none ? NAN : g;
         const float f = (float)(bad * k1 / s);
+        float lead = 0.0f;   // (of the row's entries over their ids' powers of two, the largest)
+        if (DT == ZS_F32 && a.lead) {
+            if (in && id != label) lead = ldexpf(f * ce_exp<ZS_F32>(y - m0), -a.wsh[id]);
+            lead = fabsf(lead);
+            for (uint32_t k = t; k < a.subs; k += CE_NT)
+                if (k != own) lead = fmaxf(lead, fabsf(f * ce_exp<DT>(st[k].x - m0)) * a.lead[(uint64_t)i * a.subs + k]);
+            lead = block_max_f<CE_NT>(lead, shf);
+        }
         for (uint32_t k = t; k < a.subs; k += CE_NT) a.fac[(uint64_t)i * a.subs + k] = f * ce_exp<DT>(st[k].x - m0);
         if (t == 0u) {
             // g (k1 p - 1) at the label, at most g k1 rest / s at the others
@@ -476,7 +522,7 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_loss(ce_args a) {
             a.row[i].fix = fix;
             a.row[i].fac = f;
             a.row[i].m = m0;
-            a.row[i].sd = zs_split2_of(top);
+            if (DT == ZS_F32 && a.lead) a.row[i].sd = zs_split2_of(fmaxf(lead, none ? 0.0f : fabsf(ldexpf(fix, -a.wsh[label]))));
             if (DT == ZS_F16 && top < INFINITY) atomicMax(&a.st->amax[i & 63u], __float_as_uint(top));
         }
     }
@@ -531,7 +577,9 @@ __global__ __launch_bounds__(CE_NT) void zs_k_ce_grad(ce_args a) {
         if (a.dl2) {
             uint16_t p[8][2];
             const int sd = i < n ? a.row[i].sd : 0;
-            for (int k = 0; k < 8; k++) zs_split2(x[k], sd, p[k]);
+            const int4 u = *(const int4*)(a.wsh + v0), w = *(const int4*)(a.wsh + v0 + 4);
+            const int sw[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+            for (int k = 0; k < 8; k++) zs_split2(x[k], sd - sw[k], p[k]);
             for (int q = 0; q < 2; q++) {
                 hd_u4 o;
                 for (int k = 0; k < 4; k++) o[k] = (uint32_t)p[2 * k][q] | (uint32_t)p[2 * k + 1][q] << 16;
@@ -619,10 +667,9 @@ __global__ __launch_bounds__(CE_NT, 1) void zs_k_ce_dhidden(ce_args a) {
     tile.run(k0, all - k0 < p.steps ? all - k0 : p.steps, c);
     const float un = ldexpf(1.0f, -ce_shift<DT>(a));
     if constexpr (DT == ZS_F32 && !RAW) {
-        const int sw = ce_weight_shift(a);
 #pragma unroll
         for (int j = 0; j < NT; j++) {
-            const int back = -sw - a.row[tile.n_of(j)].sd;   // (rows past the last are not stored)
+            const int back = -a.row[tile.n_of(j)].sd;   // (rows past the last are not stored; ids' powers are in both operands)
 #pragma unroll
             for (int i = 0; i < MT; i++)
 #pragma unroll
@@ -785,8 +832,12 @@ template <int DT>
 static void ce_go(ce_args a, hipStream_t stream) {
     const dim3 wg(CE_NT);
     if (a.N > CE_SELF) hipLaunchKernelGGL(zs_k_ce_rows, dim3(1), dim3(1024), 0, stream, a);
-    if (DT == ZS_F32 && a.w) hipLaunchKernelGGL(zs_k_ce_max, dim3(CE_MAXIMA), wg, 0, stream, a);
-    if (a.w) hipLaunchKernelGGL(zs_k_ce_weight<DT>, dim3(8192, (a.V + 65535u) / 65536u), wg, 0, stream, a);
+    if constexpr (DT == ZS_F32) {
+        const uint32_t rows = a.Vp / (CE_NT / 64);
+        if (a.w) hipLaunchKernelGGL(zs_k_ce_split, dim3(rows < 8192u ? rows : 8192u), wg, 0, stream, a);
+    } else if (a.w) {
+        hipLaunchKernelGGL(zs_k_ce_weight<DT>, dim3(8192, (a.V + 65535u) / 65536u), wg, 0, stream, a);
+    }
     for (uint32_t p = 0; p < a.pieces; p++) {
         a.lo = p * a.R;
         a.first = p == 0u;
